@@ -69,6 +69,12 @@ SIGNATURES = {
     "cdclq_quantize_model": (I32, [P, ctypes.POINTER(CModelOpts), ctypes.POINTER(CModelReport)]),
     "cdclq_dequantize_packed": (I32, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p,
                                       ctypes.POINTER(ctypes.c_uint64)]),
+    "cdclq_operator_status": (I32, []),
+    "cdclq_linear_cross_entropy_workspace": (SZ, [SZ, SZ, SZ]),
+    "cdclq_linear_cross_entropy_device": (I32, [P, SZ, P, SZ, I32, SZ, SZ, SZ, P, P, P, P, SZ, P]),
+    "cdclq_linear_cross_entropy_backward_workspace": (SZ, [SZ, SZ, SZ, I32, I32]),
+    "cdclq_linear_cross_entropy_backward_device": (I32, [P, SZ, P, SZ, I32, SZ, SZ, SZ, P, P, P, P, SZ, P, SZ, P, SZ, P]),
+    "cdclq_align_rows_device": (I32, [P, SZ, SZ, SZ, P, SZ, P]),
     "cdclq_launch_count": (ctypes.c_uint64, []),
     "cdclq_last_run_profile": (I32, [ctypes.POINTER(CRunProfile)]),
     "cdclq_version": (ctypes.c_char_p, []),

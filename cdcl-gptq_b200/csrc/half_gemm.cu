@@ -1,0 +1,241 @@
+// half_gemm.cu - plans and launches the half-precision tensor-core product: tensor maps, tile width, K splits.
+#include <algorithm>
+#include <mutex>
+
+#include "half_gemm_launch.cuh"
+
+namespace cdclq {
+
+using namespace hg;
+
+int sm_count() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+// One word of mapped host memory: the host reads it without a synchronisation.
+static int* fail_word_host() {
+    static int* word = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
+            word = static_cast<int*>(p);
+            *word = 0;
+        } else {
+            cudaGetLastError();
+        }
+    });
+    return word;
+}
+
+int* device_fail_word() {
+    int* h = fail_word_host();
+    void* d = nullptr;
+    if (!h || cudaHostGetDevicePointer(&d, h, 0) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    return static_cast<int*>(d);
+}
+
+int check_fail_word(const char* what) {
+    int* h = fail_word_host();
+    if (!h) return set_error(CDCLQ_ERR_CUDA, std::string(what) + ": no mapped host memory (is there a CUDA device?)");
+    if (*(volatile int*)h) {
+        *(volatile int*)h = 0;
+        return set_error(CDCLQ_ERR_CUDA, std::string(what) + ": a pipeline wait of an earlier launch timed out (its outputs are incomplete)");
+    }
+    return 0;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+        else
+            cudaGetLastError();
+    });
+    return fn;
+}
+
+// Map of a 16-bit operand with boxes of 64 columns x box_rows rows (of one matrix of a batch when batched).
+static int encode(CUtensorMap* map, const HalfOperand& o, bool bf16, bool batched, int box_rows) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return set_error(CDCLQ_ERR_CUDA, "half product: cuTensorMapEncodeTiled is unavailable");
+    if ((reinterpret_cast<uintptr_t>(o.p) & 15) || (o.ld & 7) || (o.step & 7) || o.rows <= 0 || o.cols <= 0 || o.ld < o.cols)
+        return set_error(CDCLQ_ERR_ARG, "half product: operands need rows that start on 16 bytes");
+    cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.batch};
+    cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(o.step ? o.step : o.ld * o.rows) * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, batched ? 3 : 2,
+                     const_cast<void*>(o.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(CDCLQ_ERR_CUDA, "half product: tensor map encoding failed");
+    return 0;
+}
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
+    const bool store = form != HALF_STATS && form != HALF_GRAD;
+    const bool grouped = form == HALF_NT_GROUPED || form == HALF_NN_GROUPED;
+    const int64_t sms = sm_count(), tm = ceil_div(m, BM), nkb = ceil_div(k, KB);
+    HalfPlan p{256, 1, 0};
+    if (grouped) {
+        p.bn = 64;
+    } else {
+        // The least time of all waves, a wave costing its tile's columns and 32 for its start and end: 256 columns
+        // where they fill the SMs (a wider tile reads less through L2 for each product), narrower ones below that.
+        int64_t best = INT64_MAX;
+        for (int bn : {256, 128, 64}) {
+            if (bn == 64 && !store) break;
+            const int64_t cost = ceil_div(tm * ceil_div(n, bn), sms) * (bn + 32);
+            if (cost < best) {
+                best = cost;
+                p.bn = bn;
+            }
+        }
+    }
+    const int64_t tiles = tm * ceil_div(n, p.bn);
+    if (store && tiles * 2 <= sms && nkb >= 16) {
+        // too few tiles for the SMs: the K blocks of a tile over several items, eight blocks at least for each
+        p.splits = (int)std::min(sms / tiles, nkb / 8);
+        const int64_t per = ceil_div(nkb, p.splits);
+        p.splits = (int)ceil_div(nkb, per);
+    }
+    if (p.splits > 1) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
+    return p;
+}
+
+// out = alpha * (f32in + partial[0] + partial[1] + ...), splits in order; also or instead as f32.
+template <bool BF16>
+__global__ void __launch_bounds__(256) half_gemm_reduce_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
+                                                               int64_t ldp, const float* f32in, float* f32out, int64_t ldf,
+                                                               const float* alpha, uint16_t* out, int64_t ldo) {
+    const float a = alpha ? *alpha : 1.0f;
+    const int64_t total = m * ldp, stride = m * ldp;
+    for (int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 4; i < total; i += (int64_t)gridDim.x * blockDim.x * 4) {
+        const int64_t row = i / ldp;
+        const int col = (int)(i - row * ldp);
+        float4 s = make_float4(0, 0, 0, 0);
+        if (f32in) {
+            const float* src = f32in + row * ldf + col;
+            s.x = src[0];
+            if (col + 1 < n) s.y = src[1];
+            if (col + 2 < n) s.z = src[2];
+            if (col + 3 < n) s.w = src[3];
+        }
+        for (int k = 0; k < splits; k++) {
+            const float4 v = *reinterpret_cast<const float4*>(partial + k * stride + i);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        const float r[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (col + q >= n) break;
+            if (f32out) f32out[row * ldf + col + q] = r[q];
+            if (out) out[row * ldo + col + q] = hg::pack1<BF16>(r[q] * a);
+        }
+    }
+}
+
+int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
+    if (g.m <= 0 || g.n <= 0) return 0;
+    const bool a_mn = g.form == HALF_TN;
+    const bool b_mn = g.form == HALF_NN || g.form == HALF_TN || g.form == HALF_NN_EXTEND || g.form == HALF_NN_GROUPED;
+    const bool grouped = g.form == HALF_NT_GROUPED || g.form == HALF_NN_GROUPED;
+    const bool extend = (g.form == HALF_NT_EXTEND || g.form == HALF_NN_EXTEND) && g.adapters > 0;
+    if (g.m > 0x7fffff00 || g.n > 0x7fffff00 || g.k > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "half product: too large");
+    Maps maps{};
+    int rc;
+    if ((rc = encode(&maps.a, g.a, g.bf16, false, a_mn ? KB : BM))) return rc;
+    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : plan.bn))) return rc;
+    if (extend && (rc = encode(&maps.u, g.u, g.bf16, false, BM))) return rc;
+    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : plan.bn))) return rc;
+    Params p{};
+    p.m = (int)g.m;
+    p.n = (int)g.n;
+    p.nkb = (int)ceil_div(g.k, KB);
+    p.tiles_m = (int)ceil_div(g.m, BM);
+    p.tiles_n = (int)ceil_div(g.n, plan.bn);
+    if ((int64_t)p.tiles_m * p.tiles_n * plan.splits > 0x7fffffff) return set_error(CDCLQ_ERR_ARG, "half product: too many tiles");
+    p.ntiles = p.tiles_m * p.tiles_n;
+    p.splits = plan.splits;
+    p.kb_per_split = (int)ceil_div(p.nkb, plan.splits);
+    p.index = g.index;
+    p.adapters = (extend || grouped) ? g.adapters : 0;
+    p.rank = extend ? (int)g.u.cols : 0;
+    p.row_scale = g.row_scale;
+    p.target = g.target;
+    p.col0 = g.col0;
+    p.vocab = g.vocab;
+    p.stats = g.stats;
+    p.label_logit = g.label_logit;
+    p.lse = g.lse;
+    p.dloss = g.dloss;
+    p.gain = g.gain;
+    p.fail = device_fail_word();
+    if (!p.fail) return set_error(CDCLQ_ERR_CUDA, "half product: no mapped host memory (is there a CUDA device?)");
+    if (plan.splits > 1) {
+        p.f32out = g.partial;
+        p.ldf = ceil_div(g.n, 4) * 4;
+        p.split_stride = g.m * p.ldf;
+    } else {
+        p.out = g.out;
+        p.ldo = g.ldo;
+        p.out_vec = g.out && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo % 8 == 0;
+        p.f32out = g.f32out;
+        p.f32in = g.f32in;
+        p.ldf = g.ldf;
+        p.alpha = g.alpha;
+    }
+    rc = g.bf16 ? launch_form<true>(g.form, plan.bn, maps, p, st) : launch_form<false>(g.form, plan.bn, maps, p, st);
+    if (rc || plan.splits == 1) return rc;
+    const int64_t groups = ceil_div(g.m * p.ldf, 4 * 256);
+    const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 8);
+    auto kern = g.bf16 ? half_gemm_reduce_kernel<true> : half_gemm_reduce_kernel<false>;
+    CDCLQ_LAUNCH(kern, grid, 256, 0, st, g.partial, plan.splits, g.m, g.n, p.ldf, g.f32in, g.f32out, g.ldf, g.alpha,
+                 static_cast<uint16_t*>(g.out), g.ldo);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "half_gemm_reduce_kernel launch");
+}
+
+}  // namespace cdclq
+
+using namespace cdclq;
+
+extern "C" int cdclq_operator_status(void) { return check_fail_word("operator"); }
+
+namespace cdclq {
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t cols, int64_t lds,
+                                                         uint16_t* __restrict__ dst, int64_t ldd) {
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * ldd; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / ldd, c = i - r * ldd;
+        dst[i] = c < cols ? src[r * lds + c] : (uint16_t)0;
+    }
+}
+}  // namespace cdclq
+
+extern "C" int cdclq_align_rows_device(const void* src, size_t rows, size_t cols, size_t lds, void* dst, size_t ldd, void* stream) {
+    if (!rows || !cols) return 0;
+    if (!src || !dst || lds < cols || ldd < cols) return set_error(CDCLQ_ERR_ARG, "align_rows: null pointer, or rows overlap");
+    const int64_t blocks = ceil_div((int64_t)rows * (int64_t)ldd, 256);
+    CDCLQ_LAUNCH(align_rows_kernel, (unsigned)std::min<int64_t>(blocks, sm_count() * 16), 256, 0, static_cast<cudaStream_t>(stream),
+                 static_cast<const uint16_t*>(src), (int64_t)rows, (int64_t)cols, (int64_t)lds, static_cast<uint16_t*>(dst),
+                 (int64_t)ldd);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "align_rows_kernel launch");
+}

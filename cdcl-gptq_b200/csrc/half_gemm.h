@@ -1,0 +1,74 @@
+// half_gemm.h - host side of the half-precision tensor-core product (half_gemm.cuh) and what its callers share.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "cdclq.h"
+#include "common.cuh"
+
+namespace cdclq {
+
+// The forms of the product the operators use.
+enum HalfForm {
+    HALF_STATS,       // K-major x K-major, running softmax statistics of the rows
+    HALF_GRAD,        // K-major x K-major, softmax gradient
+    HALF_NN,          // K-major x MN-major, stored
+    HALF_TN,          // MN-major x MN-major, stored
+    HALF_NT_EXTEND,   // K-major x K-major plus the rows' adapters, stored
+    HALF_NN_EXTEND,   // K-major x MN-major plus the rows' adapters, stored
+    HALF_NT_GROUPED,  // K-major x the row's own K-major operand, stored
+    HALF_NN_GROUPED   // K-major x the row's own MN-major operand, stored
+};
+
+// A 16-bit operand: `rows` x `cols` (cols contiguous), `ld` elements from row to row, `batch` of them `step` elements apart.
+// Base, ld and step are whole multiples of 16 bytes.
+struct HalfOperand {
+    const void* p = nullptr;
+    int64_t rows = 0, cols = 0, ld = 0, batch = 1, step = 0;
+};
+
+struct HalfGemm {
+    HalfForm form;
+    bool bf16;
+    int64_t m, n, k;
+    HalfOperand a, b;            // b: unused in the grouped forms
+    HalfOperand u, x;            // extension: u (m x rank) times x[adapter]; grouped: x[adapter] is the second operand
+    const int* index = nullptr;  // the rows' adapters
+    int adapters = 0;
+    const float* row_scale = nullptr;
+    void* out = nullptr;         // 16-bit, ldo elements from row to row
+    int64_t ldo = 0;
+    float* f32out = nullptr;     // f32, ldf elements from row to row
+    const float* f32in = nullptr;
+    int64_t ldf = 0;
+    const float* alpha = nullptr;
+    const int64_t* target = nullptr;
+    int64_t col0 = 0, vocab = 0;
+    float2* stats = nullptr;
+    float* label_logit = nullptr;
+    const float *lse = nullptr, *dloss = nullptr, *gain = nullptr;
+    float* partial = nullptr;    // workspace of the split plan
+};
+
+// Tile columns and K splits of a product; partial_bytes of workspace when splits > 1.
+struct HalfPlan {
+    int bn, splits;
+    size_t partial_bytes;
+};
+HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);
+
+// Launches the product (and, when the plan splits K, the pass that adds the splits in order).
+int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st);
+
+// Number of SMs of the current device.
+int sm_count();
+// Device pointer of the host word that a kernel sets when one of its bounded waits ran out; null on failure.
+int* device_fail_word();
+// CDCLQ_OK, or the error left by an earlier launch whose wait ran out (reported once).
+int check_fail_word(const char* what);
+
+}  // namespace cdclq

@@ -22,17 +22,18 @@
 // Roles: warps 0-7 epilogue (warp w reads TMEM lanes 32(w%4).. and columns 128(w/4)..), warp 8 TMA producer,
 // warp 9 MMA issuer and TMEM owner.  Every wait on an mbarrier is bounded: on timeout the kernel records an error, leaves its loops,
 // waits (bounded) for its own copies and MMAs in flight, frees its tensor memory and returns.  No TMA multicast.
-#include <cuda.h>
-
 #include <mutex>
 #include <vector>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace cdclq {
 
 namespace syrk {
+
+using namespace tc;
 
 constexpr int BMP = 128;         // tile rows p (TMEM lanes)
 constexpr int BNQ = 256;         // tile columns q
@@ -51,48 +52,7 @@ constexpr int EPI_BYTES = EPI_WARPS * 2 * EPI_BUF_BYTES;  // two buffers per epi
 constexpr size_t smem_bytes(int ns) {
     return (size_t)ns * STAGE_BYTES + EPI_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 }
-constexpr int WAIT_LIMIT = 1 << 24;
 constexpr int TILE_BAND = 16;    // p blocks per band of the tile order
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-    asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(smem_u32(b)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait for the completion of the phase with the given parity; false (and the error flag set) on timeout.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* err) {
-    for (int it = 0; it < WAIT_LIMIT; it++) {
-        if (mbar_try(b, parity)) return true;
-        if ((it & 1023) == 1023 && *(volatile int*)err) return false;  // another role gave up
-    }
-    atomicExch(err, 1);
-    return false;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
 
 // Bulk f64 additions from shared memory into global memory, performed at L2 (round to nearest, as __dadd_rn).
 __device__ __forceinline__ void bulk_add_f64(double* gdst, uint32_t ssrc, uint32_t bytes) {
@@ -106,51 +66,6 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 // at most the most recent bulk group of this thread still reads its shared-memory source
 __device__ __forceinline__ void bulk_wait_read_le1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Shared-memory matrix descriptor of an MN-major operand with the 128-byte swizzle: 64-element (128-byte) atoms
-// along MN, `lbo` bytes apart; 8-token row groups along K, `sbo` bytes apart.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFF);
-    d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-    d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
-    d |= (uint64_t)1 << 46;  // descriptor version (sm_100)
-    d |= (uint64_t)2 << 61;  // 128-byte swizzle
-    return d;
-}
-
-// Instruction descriptor: D f32, A and B both bf16 (BF16) or both f16, both MN-major, M = 128, N = 256.
-template <bool BF16>
-__host__ __device__ constexpr uint32_t idesc() {
-    return (1u << 4) | ((BF16 ? 1u : 0u) << 7) | ((BF16 ? 1u : 0u) << 10) | (1u << 15) | (1u << 16) |
-           ((uint32_t)(BNQ >> 3) << 17) | ((uint32_t)(BMP >> 4) << 24);
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma_half(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc<BF16>()), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
 
 struct Params {
     double* h;
@@ -239,7 +154,7 @@ __global__ void __launch_bounds__(THREADS, 1) syrk_bf16_kernel(const __grid_cons
                             ok = false;
                             break;
                         }
-                        unsigned char* st = base + s * STAGE_BYTES;
+                        const uint32_t st = smem_u32(base) + s * STAGE_BYTES;
                         mbar_expect_tx(&full[s], STAGE_BYTES);
                         const int y = (int)(tok0 + (int64_t)kb * KB);
                         tma_load_2d(st, &tmap, p0, y, &full[s]);
@@ -284,8 +199,8 @@ __global__ void __launch_bounds__(THREADS, 1) syrk_bf16_kernel(const __grid_cons
                         const uint32_t sa = a_base + s * STAGE_BYTES, sb = sa + A_BYTES;
 #pragma unroll
                         for (int k = 0; k < KB / 16; k++)
-                            mma_half<BF16>(d, smem_desc(sa + k * 2048, BOX_BYTES, 1024), smem_desc(sb + k * 2048, BOX_BYTES, 1024),
-                                     (kb | k) != 0 ? 1u : 0u);
+                            mma_half(d, smem_desc(sa + k * 2048, BOX_BYTES, 1024), smem_desc(sb + k * 2048, BOX_BYTES, 1024),
+                                     idesc_half(BF16, true, true, BMP, BNQ), (kb | k) != 0 ? 1u : 0u);
                         mma_commit(&empty[s]);  // the stage is free once these MMAs have read it
                     }
                     if (!ok) break;

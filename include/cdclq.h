@@ -353,6 +353,38 @@ int cdclq_pack(const uint8_t* codes, size_t d_out, size_t n, size_t g, const uin
 int cdclq_unpack_dequant(const uint8_t* packed, size_t d_out, size_t n, size_t g, const uint8_t* gbits,
                          const uint32_t* perm, const float* scales, const float* zeros, float* out);
 
+/* ---- after the quantization: loss of a linear head ---------------------------------------------------- */
+
+/* No counterpart in the reference.  The operators below are asynchronous on `stream`, take device pointers and a
+ * workspace of the size their `_workspace` function gives (it may be reused by the next call on the same stream),
+ * and can be captured into a CUDA graph once each has run on the device.  A kernel whose bounded pipeline wait ran
+ * out ends without finishing its outputs; the next of these calls, or cdclq_operator_status, reports it
+ * (CDCLQ_ERR_CUDA). */
+
+/* CDCLQ_OK, or the error that an earlier operator left (reported once).  Synchronise first for a verdict on it. */
+int cdclq_operator_status(void);
+
+/* Softmax cross entropy of a linear head over v classes, without its logits z = h w^T:
+ *   lse[i] = log sum_c exp z[i][c],   loss[i] = lse[i] - z[i][target[i]]
+ * h: t x d, w: v x d, both f16 or bf16 (dtype CDCLQ_DTYPE_*), ldh / ldw elements from row to row; rows start on 16
+ * bytes.  A target outside [0, v) means no label: loss 0 (lse is still the row's).  loss, lse: f32. */
+size_t cdclq_linear_cross_entropy_workspace(size_t t, size_t d, size_t v);
+int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, const void* w, size_t ldw, int dtype, size_t t, size_t d,
+                                      size_t v, const int64_t* target, float* loss, float* lse, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+/* Its gradient for dloss (f32, one for each token), from the forward's lse:
+ *   g[i][c] = (exp(z[i][c] - lse[i]) - [c = target[i]]) dloss[i]   (0 without a label),  dh = g w,  dw = g^T h
+ * dh (t x d) and dw (v x d) have the inputs' type; either may be NULL.  What a token without a label holds in h,
+ * lse and dloss reaches neither. */
+size_t cdclq_linear_cross_entropy_backward_workspace(size_t t, size_t d, size_t v, int need_dh, int need_dw);
+int cdclq_linear_cross_entropy_backward_device(const void* h, size_t ldh, const void* w, size_t ldw, int dtype, size_t t,
+                                               size_t d, size_t v, const int64_t* target, const float* lse,
+                                               const float* dloss, void* dh, size_t lddh, void* dw, size_t lddw,
+                                               void* workspace, size_t workspace_bytes, void* stream);
+/* Copies `rows` x `cols` 16-bit elements, lds elements from row to row, to rows ldd elements apart (columns cols..ldd
+ * zero): the layout the operators need from a matrix whose rows do not start on 16 bytes. */
+int cdclq_align_rows_device(const void* src, size_t rows, size_t cols, size_t lds, void* dst, size_t ldd, void* stream);
+
 /* ---- runtime ---------------------------------------------------------------------------------------- */
 
 /* Device-side profile of the last quantize call made on this thread: elapsed times between CUDA events
