@@ -75,6 +75,10 @@ SIGNATURES = {
     "cdclq_linear_cross_entropy_backward_workspace": (SZ, [SZ, SZ, SZ, I32, I32]),
     "cdclq_linear_cross_entropy_backward_device": (I32, [P, SZ, P, SZ, I32, SZ, SZ, SZ, P, P, P, P, SZ, P, SZ, P, SZ, P]),
     "cdclq_align_rows_device": (I32, [P, SZ, SZ, SZ, P, SZ, P]),
+    "cdclq_checkpoint_save_device": (I32, [P, SZ, I32, SZ, SZ, P, P, P]),
+    "cdclq_checkpoint_restore_device": (I32, [P, P, SZ, SZ, P, SZ, I32, P]),
+    "cdclq_checkpoint_weight_grad_workspace": (SZ, [SZ, SZ, SZ]),
+    "cdclq_checkpoint_weight_grad_device": (I32, [P, SZ, I32, P, P, SZ, SZ, SZ, P, SZ, P, SZ, P]),
     "cdclq_launch_count": (ctypes.c_uint64, []),
     "cdclq_last_run_profile": (I32, [ctypes.POINTER(CRunProfile)]),
     "cdclq_version": (ctypes.c_char_p, []),

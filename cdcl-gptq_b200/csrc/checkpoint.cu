@@ -1,0 +1,260 @@
+// checkpoint.cu - activations kept in 8 bits between the forward and the backward pass.
+//
+//   s = max |x| / 127 over a block of 128 columns of a row      q = round(x / s), to nearest, ties to even      x^ = q s
+//
+// A block of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and is restored as NaN, so that an
+// overflow in the forward pass is not hidden.  q fits 8 signed bits, and the error is at most s / 2 for each value.
+// Saving and restoring are bound by memory: the 16-bit matrix once, the codes once.
+//
+// The weight gradient dW = dy^T x^ restores a piece of tokens at a time into a buffer that stays in L2 and multiplies it
+// on the tensor cores; pieces are added in f32.
+#include <algorithm>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "half_gemm.h"
+
+namespace cdclq {
+
+namespace {
+
+constexpr int BLOCK = 128;                  // columns of a scale
+constexpr size_t PIECE_BYTES = 32u << 20;   // restored tokens of the weight gradient
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
+
+template <int DT>
+struct Type;
+template <>
+struct Type<CDCLQ_DTYPE_F32> {
+    typedef float T;
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <>
+struct Type<CDCLQ_DTYPE_F16> {
+    typedef __half T;
+    static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Type<CDCLQ_DTYPE_BF16> {
+    typedef __nv_bfloat16 T;
+    static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+// One group of 16 lanes for each block of a row, 8 values a lane: one wide load of a 16-bit type.
+template <int DT, bool WIDE>
+__global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Type<DT>::T* __restrict__ x, int64_t ldx, int64_t t,
+                                                              int64_t d, int8_t* __restrict__ codes, float* __restrict__ scales) {
+    const int lane = threadIdx.x & 15;
+    const int64_t nb = (d + BLOCK - 1) / BLOCK, total = t * nb;
+    for (int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4; g < ((total + 1) & ~(int64_t)1);
+         g += ((int64_t)gridDim.x * blockDim.x) >> 4) {
+        const bool live = g < total;  // the warp's other half may have a block
+        const int64_t row = live ? g / nb : 0, b = live ? g - row * nb : 0;
+        const int64_t c = b * BLOCK + lane * 8;
+        const int n = live ? (int)max((int64_t)0, min((int64_t)8, d - c)) : 0;
+        const typename Type<DT>::T* src = x + row * ldx + c;
+        float v[8];
+        if (WIDE && n == 8) {
+            alignas(16) typename Type<DT>::T raw[8];
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(raw) / 16; i++) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(src)[i];
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = Type<DT>::up(raw[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = i < n ? Type<DT>::up(src[i]) : 0.0f;
+        }
+        float top = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            top = fmaxf(top, fabsf(v[i]));
+            bad |= !(fabsf(v[i]) < INFINITY);
+        }
+        if (bad) top = INFINITY;
+#pragma unroll
+        for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool finite = top < INFINITY;
+        const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
+        if (live && lane == 0) scales[g] = s;
+        alignas(8) int8_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float r = finite && s > 0.0f ? rintf(__fdiv_rn(v[i], s)) : 0.0f;
+            q[i] = (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
+        }
+        int8_t* dst = codes + row * d + c;
+        if (WIDE && n == 8) {
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(q);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < n) dst[i] = q[i];
+        }
+    }
+}
+
+// 8 values a thread.  ld: elements from row to row of the output; columns d..ld of it are left as they are.
+template <int DT, bool WIDE>
+__global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
+                                                                 int64_t t, int64_t d, typename Type<DT>::T* __restrict__ out,
+                                                                 int64_t ld) {
+    const int64_t d8 = (d + 7) / 8, nb = (d + BLOCK - 1) / BLOCK;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < t * d8; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t row = i / d8, c = (i - row * d8) * 8;
+        const float s = scales[row * nb + c / BLOCK];
+        alignas(16) typename Type<DT>::T r[8];
+        if (WIDE && c + 8 <= d) {
+            alignas(8) int8_t q[8];
+            *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(codes + row * d + c);
+#pragma unroll
+            for (int k = 0; k < 8; k++) r[k] = Type<DT>::down(__fmul_rn((float)q[k], s));
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(out + row * ld + c)[k] = reinterpret_cast<uint4*>(r)[k];
+        } else {
+            for (int k = 0; k < 8 && c + k < d; k++) out[row * ld + c + k] = Type<DT>::down(__fmul_rn((float)codes[row * d + c + k], s));
+        }
+    }
+}
+
+unsigned grid_of(int64_t blocks) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)sm_count() * 16)); }
+
+template <int DT>
+int save(const void* x, int64_t ldx, int64_t t, int64_t d, int8_t* codes, float* scales, cudaStream_t st) {
+    typedef typename Type<DT>::T T;
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * sizeof(T)) % 16 == 0 &&
+                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
+    const unsigned grid = grid_of(ceil_div(t * ceil_div(d, BLOCK), 16));
+    auto kern = wide ? checkpoint_save_kernel<DT, true> : checkpoint_save_kernel<DT, false>;
+    CDCLQ_LAUNCH(kern, grid, 256, 0, st, static_cast<const T*>(x), ldx, t, d, codes, scales);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "checkpoint_save_kernel launch");
+}
+
+template <int DT>
+int restore(const int8_t* codes, const float* scales, int64_t t, int64_t d, void* out, int64_t ld, cudaStream_t st) {
+    typedef typename Type<DT>::T T;
+    const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ld * sizeof(T)) % 16 == 0 &&
+                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
+    const unsigned grid = grid_of(ceil_div(t * ceil_div(d, 8), 256));
+    auto kern = wide ? checkpoint_restore_kernel<DT, true> : checkpoint_restore_kernel<DT, false>;
+    CDCLQ_LAUNCH(kern, grid, 256, 0, st, codes, scales, t, d, static_cast<T*>(out), ld);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "checkpoint_restore_kernel launch");
+}
+
+int restore_half(bool bf16, const int8_t* codes, const float* scales, int64_t t, int64_t d, void* out, int64_t ld, cudaStream_t st) {
+    return bf16 ? restore<CDCLQ_DTYPE_BF16>(codes, scales, t, d, out, ld, st)
+                : restore<CDCLQ_DTYPE_F16>(codes, scales, t, d, out, ld, st);
+}
+
+struct Grad {
+    int64_t rows, count;  // tokens of a piece, pieces
+    size_t acc, partial, total;
+};
+Grad grad_layout(int64_t t, int64_t d, int64_t n) {
+    Grad g{};
+    const int64_t ld = ceil_div(d, 8) * 8;
+    const int64_t most = std::max<int64_t>(64, (int64_t)(PIECE_BYTES / 2) / ld / 64 * 64);
+    g.count = ceil_div(t, most);
+    g.rows = ceil_div(ceil_div(t, g.count), 64) * 64;
+    g.count = ceil_div(t, g.rows);
+    size_t at = align_up((size_t)std::min(g.rows, t) * ld * 2);
+    g.acc = at;
+    if (g.count > 1) at += align_up((size_t)n * ceil_div(d, 4) * 4 * sizeof(float));
+    g.partial = at;
+    at += align_up(std::max(plan_half_gemm(HALF_TN, n, d, std::min(g.rows, t)).partial_bytes,
+                            plan_half_gemm(HALF_TN, n, d, t - (g.count - 1) * g.rows).partial_bytes));
+    g.total = at;
+    return g;
+}
+
+bool known(int dtype) { return dtype == CDCLQ_DTYPE_F32 || dtype == CDCLQ_DTYPE_F16 || dtype == CDCLQ_DTYPE_BF16; }
+
+}  // namespace
+
+}  // namespace cdclq
+
+using namespace cdclq;
+
+extern "C" int cdclq_checkpoint_save_device(const void* x, size_t ldx, int dtype, size_t t, size_t d, int8_t* codes, float* scales,
+                                            void* stream) {
+    if (!known(dtype)) return set_error(CDCLQ_ERR_ARG, "checkpoint_save: dtype must be f32, f16 or bf16");
+    if (!t || !d) return 0;
+    if (!x || !codes || !scales) return set_error(CDCLQ_ERR_ARG, "checkpoint_save: null pointer");
+    if (ldx < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_save: rows overlap");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == CDCLQ_DTYPE_F32) return save<CDCLQ_DTYPE_F32>(x, ldx, t, d, codes, scales, st);
+    if (dtype == CDCLQ_DTYPE_F16) return save<CDCLQ_DTYPE_F16>(x, ldx, t, d, codes, scales, st);
+    return save<CDCLQ_DTYPE_BF16>(x, ldx, t, d, codes, scales, st);
+}
+
+extern "C" int cdclq_checkpoint_restore_device(const int8_t* codes, const float* scales, size_t t, size_t d, void* out, size_t ldo,
+                                               int dtype, void* stream) {
+    if (!known(dtype)) return set_error(CDCLQ_ERR_ARG, "checkpoint_restore: dtype must be f32, f16 or bf16");
+    if (!t || !d) return 0;
+    if (!codes || !scales || !out) return set_error(CDCLQ_ERR_ARG, "checkpoint_restore: null pointer");
+    if (ldo < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_restore: rows overlap");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == CDCLQ_DTYPE_F32) return restore<CDCLQ_DTYPE_F32>(codes, scales, t, d, out, ldo, st);
+    return restore_half(dtype == CDCLQ_DTYPE_BF16, codes, scales, t, d, out, ldo, st);
+}
+
+extern "C" size_t cdclq_checkpoint_weight_grad_workspace(size_t t, size_t d, size_t n) {
+    return t && d && n ? grad_layout(t, d, n).total : 0;
+}
+
+extern "C" int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, int dtype, const int8_t* codes, const float* scales,
+                                                   size_t t, size_t d, size_t n, void* dw, size_t lddw, void* workspace,
+                                                   size_t workspace_bytes, void* stream) {
+    if (dtype != CDCLQ_DTYPE_F16 && dtype != CDCLQ_DTYPE_BF16)
+        return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: dtype must be f16 or bf16");
+    if (!d || !n) return 0;
+    if (!dw || lddw < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: null pointer, or rows overlap");
+    if (t > 0x7fffff00 || d > 0x7fffff00 || n > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: too large");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!t) {
+        CDCLQ_CUDA_TRY(cudaMemset2DAsync(dw, lddw * 2, 0, d * 2, n, st));
+        return 0;
+    }
+    if (!dy || !codes || !scales) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: null pointer");
+    if (lddy < n || lddy % 8 || (reinterpret_cast<uintptr_t>(dy) & 15))
+        return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: rows of dy must start on 16 bytes");
+    const Grad l = grad_layout(t, d, n);
+    if (!workspace || workspace_bytes < l.total) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: the workspace is too small");
+    int rc = check_fail_word("checkpoint_weight_grad");
+    if (rc) return rc;
+    char* ws = static_cast<char*>(workspace);
+    const bool bf16 = dtype == CDCLQ_DTYPE_BF16;
+    const int64_t ld = ceil_div(d, 8) * 8, nb = ceil_div(d, BLOCK);
+    for (int64_t i = 0; i < l.count; i++) {
+        const int64_t r0 = i * l.rows, rows = std::min<int64_t>(l.rows, (int64_t)t - r0);
+        if ((rc = restore_half(bf16, codes + r0 * d, scales + r0 * nb, rows, d, ws, ld, st))) return rc;
+        HalfGemm g{};
+        g.form = HALF_TN;
+        g.bf16 = bf16;
+        g.m = n, g.n = d, g.k = rows;
+        g.a.p = static_cast<const char*>(dy) + r0 * lddy * 2;
+        g.a.rows = rows, g.a.cols = n, g.a.ld = lddy;
+        g.b.p = ws;
+        g.b.rows = rows, g.b.cols = d, g.b.ld = ld;
+        g.ldf = ceil_div(d, 4) * 4;
+        float* acc = reinterpret_cast<float*>(ws + l.acc);
+        g.f32in = i ? acc : nullptr;
+        if (i + 1 < l.count) {
+            g.f32out = acc;
+        } else {
+            g.out = dw;
+            g.ldo = lddw;
+        }
+        g.partial = reinterpret_cast<float*>(ws + l.partial);
+        if ((rc = launch_half_gemm(g, plan_half_gemm(HALF_TN, n, d, rows), st))) return rc;
+    }
+    return 0;
+}

@@ -385,6 +385,23 @@ int cdclq_linear_cross_entropy_backward_device(const void* h, size_t ldh, const 
  * zero): the layout the operators need from a matrix whose rows do not start on 16 bytes. */
 int cdclq_align_rows_device(const void* src, size_t rows, size_t cols, size_t lds, void* dst, size_t ldd, void* stream);
 
+/* ---- after the quantization: activations in 8 bits ----------------------------------------------------- */
+
+/* x (t x d, any CDCLQ_DTYPE_*, ldx elements from row to row) as 8-bit codes (t x d) under one f32 scale for 128 columns
+ * of a row (t x ceil(d / 128)): scale = max |x| / 127, code = x / scale to the nearest whole number.  A block with a
+ * NaN or an infinity gets the scale NaN. */
+int cdclq_checkpoint_save_device(const void* x, size_t ldx, int dtype, size_t t, size_t d, int8_t* codes, float* scales,
+                                 void* stream);
+/* code * scale, rounded once to dtype. */
+int cdclq_checkpoint_restore_device(const int8_t* codes, const float* scales, size_t t, size_t d, void* out, size_t ldo,
+                                    int dtype, void* stream);
+/* dw (n x d) = dy^T x^ from the codes of x (t x d) and dy (t x n, f16 or bf16, rows start on 16 bytes); the restored
+ * values are rounded to dy's type, sums are f32, dw has dy's type. */
+size_t cdclq_checkpoint_weight_grad_workspace(size_t t, size_t d, size_t n);
+int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, int dtype, const int8_t* codes, const float* scales,
+                                        size_t t, size_t d, size_t n, void* dw, size_t lddw, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
 /* ---- runtime ---------------------------------------------------------------------------------------- */
 
 /* Device-side profile of the last quantize call made on this thread: elapsed times between CUDA events
