@@ -79,6 +79,37 @@ class CBatchLayer(ctypes.Structure):
     ]
 
 
+class CPackedLayer(ctypes.Structure):
+    """`cdclq_packed_layer` (include/cdclq.h)."""
+
+    _fields_ = [
+        ("d_out", ctypes.c_uint64),
+        ("d_in", ctypes.c_uint64),
+        ("group", ctypes.c_uint64),
+        ("groups", ctypes.c_uint64),
+        ("units", ctypes.c_uint64),
+        ("tile_words", ctypes.c_uint64),
+        ("max_bits", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("layout", ctypes.c_void_p),
+    ]
+
+
+class CAdapters(ctypes.Structure):
+    """`cdclq_adapters` (include/cdclq.h)."""
+
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("lda", ctypes.c_size_t),
+        ("ldb", ctypes.c_size_t),
+        ("scale", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("n", ctypes.c_size_t),
+        ("r", ctypes.c_size_t),
+    ]
+
+
 class CModelOpts(ctypes.Structure):
     """`cdclq_model_opts` (include/cdclq.h)."""
 

@@ -116,7 +116,7 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
         const int64_t per = ceil_div(nkb, p.splits);
         p.splits = (int)ceil_div(nkb, per);
     }
-    if (p.splits > 1) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
+    if (p.splits > 1 || grouped) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
     return p;
 }
 
@@ -178,7 +178,6 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.index = g.index;
     p.adapters = (extend || grouped) ? g.adapters : 0;
     p.rank = extend ? (int)g.u.cols : 0;
-    p.row_scale = g.row_scale;
     p.target = g.target;
     p.col0 = g.col0;
     p.vocab = g.vocab;
@@ -189,7 +188,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.gain = g.gain;
     p.fail = device_fail_word();
     if (!p.fail) return set_error(CDCLQ_ERR_CUDA, "half product: no mapped host memory (is there a CUDA device?)");
-    if (plan.splits > 1) {
+    if (plan.splits > 1 || grouped) {
         p.f32out = g.partial;
         p.ldf = ceil_div(g.n, 4) * 4;
         p.split_stride = g.m * p.ldf;
@@ -203,7 +202,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
         p.alpha = g.alpha;
     }
     rc = g.bf16 ? launch_form<true>(g.form, plan.bn, maps, p, st) : launch_form<false>(g.form, plan.bn, maps, p, st);
-    if (rc || plan.splits == 1) return rc;
+    if (rc || plan.splits == 1 || grouped) return rc;
     const int64_t groups = ceil_div(g.m * p.ldf, 4 * 256);
     const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 8);
     auto kern = g.bf16 ? half_gemm_reduce_kernel<true> : half_gemm_reduce_kernel<false>;

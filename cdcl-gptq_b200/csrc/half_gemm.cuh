@@ -60,7 +60,6 @@ struct Params {
     const float* f32in;        // added to the sums first, or null
     int64_t ldf, split_stride;
     const float* alpha;        // multiplies the sums on their way to `out`, or null
-    const float* row_scale;    // ROWS_GROUPED: factor of each adapter, or null
     // EPI_STATS, EPI_GRAD
     const int64_t* target;     // label of each row, relative to the whole vocabulary
     int64_t col0;              // the first column's place in the vocabulary
@@ -333,9 +332,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if constexpr (ROWS == ROWS_GROUPED) {
                     const int id = live ? P.index[row] : -1;
                     none = id < 0 || id >= P.adapters;
-                    if (!none && P.row_scale) factor = P.row_scale[id];
                 }
-                if (P.alpha) factor *= *P.alpha;
+                if (P.alpha) factor = *P.alpha;
             } else {
                 const int64_t t = live ? P.target[row] : -1;
                 const bool labelled = t >= 0 && t < P.vocab;

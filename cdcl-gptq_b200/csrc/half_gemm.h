@@ -20,8 +20,8 @@ enum HalfForm {
     HALF_TN,          // MN-major x MN-major, stored
     HALF_NT_EXTEND,   // K-major x K-major plus the rows' adapters, stored
     HALF_NN_EXTEND,   // K-major x MN-major plus the rows' adapters, stored
-    HALF_NT_GROUPED,  // K-major x the row's own K-major operand, stored
-    HALF_NN_GROUPED   // K-major x the row's own MN-major operand, stored
+    HALF_NT_GROUPED,  // K-major x the row's own K-major operand, the splits' f32 sums left in `partial`
+    HALF_NN_GROUPED   // K-major x the row's own MN-major operand, likewise
 };
 
 // A 16-bit operand: `rows` x `cols` (cols contiguous), `ld` elements from row to row, `batch` of them `step` elements apart.
@@ -39,7 +39,6 @@ struct HalfGemm {
     HalfOperand u, x;            // extension: u (m x rank) times x[adapter]; grouped: x[adapter] is the second operand
     const int* index = nullptr;  // the rows' adapters
     int adapters = 0;
-    const float* row_scale = nullptr;
     void* out = nullptr;         // 16-bit, ldo elements from row to row
     int64_t ldo = 0;
     float* f32out = nullptr;     // f32, ldf elements from row to row
@@ -54,7 +53,8 @@ struct HalfGemm {
     float* partial = nullptr;    // workspace of the split plan
 };
 
-// Tile columns and K splits of a product; partial_bytes of workspace when splits > 1.
+// Tile columns and K splits of a product; partial_bytes of workspace when splits > 1, and for the grouped forms.
+// Split s of row m is at partial + (s * m_total + m) * ld, ld = n rounded up to a multiple of 4.
 struct HalfPlan {
     int bn, splits;
     size_t partial_bytes;

@@ -402,6 +402,52 @@ int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, int dtype, 
                                         size_t t, size_t d, size_t n, void* dw, size_t lddw, void* workspace,
                                         size_t workspace_bytes, void* stream);
 
+/* ---- after the quantization: the packed projection and its adapters ------------------------------------ */
+
+/* A packed layer laid out once for products with activations (the fields are the library's). */
+typedef struct cdclq_packed_layer {
+    uint64_t d_out, d_in, group, groups;
+    uint64_t units, tile_words;
+    uint32_t max_bits, reserved;
+    void* layout; /* device buffer of cdclq_packed_layer_bytes, the caller's */
+} cdclq_packed_layer;
+
+/* Bytes of the layout of a layer (gbits on the host, one width for each group of `group` permuted columns; 0 = one
+ * group); 0 on a refused argument. */
+size_t cdclq_packed_layer_bytes(size_t d_out, size_t d_in, size_t group, const uint8_t* gbits);
+/* Lays out the tensors of the packed format (src/io.rs:244-270): qweight (d_out x row_bytes), scales_f16 and qzeros
+ * (d_out x groups), perm (d_in), all on the device; gbits on the host.  Synchronous: it refuses a perm that is no
+ * permutation and a zero point above its group's largest code.  The tensors are not needed afterwards. */
+int cdclq_packed_layer_build(const uint8_t* qweight, const void* scales_f16, const uint8_t* qzeros, const int32_t* perm,
+                             size_t d_out, size_t d_in, size_t group, const uint8_t* gbits, void* layout,
+                             size_t layout_bytes, cdclq_packed_layer* out, void* stream);
+
+/* Adapters of rank r: a (n x r x d_in, lda elements from row to row) and b (n x d_out x r, ldb), in the type of the
+ * call, rows on 16 bytes; scale (n, f32); index (one for each token; outside [0, n): the token has none). */
+typedef struct cdclq_adapters {
+    const void* a;
+    const void* b;
+    size_t lda, ldb;
+    const float* scale;
+    const int32_t* index;
+    size_t n, r;
+} cdclq_adapters;
+
+/* y (t x d_out) = x W^T + scale_i (x A_i^T) B_i^T for the adapter i of each token; u (t x r, may be NULL) = x A_i^T, 0
+ * without one, for the backward pass.  x: t x d_in, f16 or bf16, rows on 16 bytes.  ad may be NULL. */
+size_t cdclq_projection_forward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r);
+int cdclq_projection_forward_device(const cdclq_packed_layer* w, const void* x, size_t ldx, int dtype, size_t t,
+                                    const cdclq_adapters* ad, void* y, size_t ldy, void* u, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+/* The gradient for dy (t x d_out): v = scale_i dy B_i, dx (t x d_in) = dy W + v A_i, da (n x r x d_in) = sum over the
+ * adapter's tokens of v^T x, db (n x d_out x r) = scale_i sum dy^T u.  x is needed for da: in full, or (x NULL) as the
+ * checkpoint x_codes, x_scales.  u is needed for db.  dx, da and db may be NULL. */
+size_t cdclq_projection_backward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r, int need_dx);
+int cdclq_projection_backward_device(const cdclq_packed_layer* w, const void* dy, size_t lddy, int dtype, size_t t,
+                                     const cdclq_adapters* ad, const void* x, size_t ldx, const int8_t* x_codes,
+                                     const float* x_scales, const void* u, void* dx, size_t lddx, void* da, void* db,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- runtime ---------------------------------------------------------------------------------------- */
 
 /* Device-side profile of the last quantize call made on this thread: elapsed times between CUDA events
