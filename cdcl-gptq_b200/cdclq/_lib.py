@@ -6,7 +6,7 @@ raises.  Loading the library does not need a GPU; computing does (the C ABI retu
 import ctypes
 import os
 
-from .abi import CAdapters, CBatchInput, CBatchLayer, CConfig, CLayerStats, CModelOpts, CModelReport, CPackedLayer, CRunProfile
+from .abi import CBatchInput, CBatchLayer, CConfig, CLayerStats, CModelOpts, CModelReport, CRunProfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcdclq_cuda.so")
@@ -80,12 +80,12 @@ SIGNATURES = {
     "cdclq_checkpoint_weight_grad_workspace": (SZ, [SZ, SZ, SZ]),
     "cdclq_checkpoint_weight_grad_device": (I32, [P, SZ, I32, P, P, SZ, SZ, SZ, P, SZ, P, SZ, P]),
     "cdclq_packed_layer_bytes": (SZ, [SZ, SZ, SZ, P]),
-    "cdclq_packed_layer_build": (I32, [P, P, P, P, SZ, SZ, SZ, P, P, SZ, ctypes.POINTER(CPackedLayer), P]),
-    "cdclq_projection_forward_workspace": (SZ, [ctypes.POINTER(CPackedLayer), SZ, SZ, SZ]),
-    "cdclq_projection_forward_device": (I32, [ctypes.POINTER(CPackedLayer), P, SZ, I32, SZ, ctypes.POINTER(CAdapters), P, SZ,
+    "cdclq_packed_layer_build": (I32, [P, P, P, P, SZ, SZ, SZ, P, P, SZ, P, P]),
+    "cdclq_projection_forward_workspace": (SZ, [P, SZ, SZ, SZ]),
+    "cdclq_projection_forward_device": (I32, [P, P, SZ, I32, SZ, P, P, SZ,
                                               P, P, SZ, P]),
-    "cdclq_projection_backward_workspace": (SZ, [ctypes.POINTER(CPackedLayer), SZ, SZ, SZ, I32]),
-    "cdclq_projection_backward_device": (I32, [ctypes.POINTER(CPackedLayer), P, SZ, I32, SZ, ctypes.POINTER(CAdapters), P, SZ,
+    "cdclq_projection_backward_workspace": (SZ, [P, SZ, SZ, SZ, I32]),
+    "cdclq_projection_backward_device": (I32, [P, P, SZ, I32, SZ, P, P, SZ,
                                                P, P, P, P, SZ, P, P, P, SZ, P]),
     "cdclq_launch_count": (ctypes.c_uint64, []),
     "cdclq_last_run_profile": (I32, [ctypes.POINTER(CRunProfile)]),

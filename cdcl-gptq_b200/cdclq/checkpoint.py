@@ -9,7 +9,9 @@ multiple of it (ties to even), so it comes back within s / 2.  A block of zeros 
 NaN or an infinity comes back as NaN.  A checkpoint takes d + 4 ceil(d / 128) bytes a row: 52 % of a 16-bit matrix.
 The calls are asynchronous on `stream` (torch's current one if None).
 """
-from ._device import half_code, on, ptr, refuse, rows16, tensor, workspace
+import torch
+
+from ._device import Call, half_code, on_device_of, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 from .io import _dtype_code
 
@@ -19,12 +21,12 @@ BLOCK = 128
 class Checkpoint:
     """`codes` int8 t x d, `scales` float32 t x ceil(d / 128), and the type that restore() gives back."""
 
-    def __init__(self, codes, scales, dtype):
-        import torch
+    __slots__ = ("codes", "scales", "dtype")
 
-        tensor(codes, "codes", torch.int8, (None, None))
+    def __init__(self, codes, scales, dtype):
+        tensor(codes, "codes", 2, torch.int8)
         t, d = codes.shape
-        tensor(scales, "scales", torch.float32, (t, -(-d // BLOCK)), codes.device)
+        tensor(scales, "scales", 2, torch.float32, (t, -(-d // BLOCK)), codes.get_device())
         _dtype_code(torch, dtype)
         self.codes, self.scales, self.dtype = codes.contiguous(), scales.contiguous(), dtype
 
@@ -33,49 +35,49 @@ class Checkpoint:
         return self.codes.shape
 
 
+@on_device_of(0)
 def save(x, stream=None):
-    import torch
-
-    tensor(x, "x", shape=(None, None))
+    tensor(x, "x", 2)
     code = _dtype_code(torch, x.dtype)
     t, d = x.shape
-    with on(torch, x.device, stream) as call:
-        if d > 1 and x.stride(1) != 1 or t > 1 and x.stride(0) < d:
-            x = x.contiguous()
-        codes = torch.empty((t, d), dtype=torch.int8, device=x.device)
-        scales = torch.empty((t, -(-d // BLOCK)), dtype=torch.float32, device=x.device)
-        check(lib().cdclq_checkpoint_save_device(ptr(x), x.stride(0) if t > 1 else d, code, t, d, ptr(codes), ptr(scales),
-                                                 call.handle))
-        call.keep(x, codes, scales)
-        return Checkpoint(codes, scales, x.dtype)
+    call = Call(x, stream)
+    if d > 1 and x.stride(1) != 1 or t > 1 and x.stride(0) < d:
+        x = x.contiguous()
+    codes = torch.empty((t, d), dtype=torch.int8, device=x.device)
+    scales = torch.empty((t, -(-d // BLOCK)), dtype=torch.float32, device=x.device)
+    check(lib().cdclq_checkpoint_save_device(x.data_ptr(), x.stride(0) if t > 1 else d, code, t, d, codes.data_ptr(),
+                                             scales.data_ptr(), call.handle))
+    call.keep(x, codes, scales)
+    return Checkpoint(codes, scales, x.dtype)
 
 
+@on_device_of(0)
 def restore(c, stream=None):
-    import torch
-
     t, d = c.shape
-    with on(torch, c.codes.device, stream) as call:
-        out = torch.empty((t, d), dtype=c.dtype, device=c.codes.device)
-        check(lib().cdclq_checkpoint_restore_device(ptr(c.codes), ptr(c.scales), t, d, ptr(out), d,
-                                                    _dtype_code(torch, c.dtype), call.handle))
-        call.keep(c.codes, c.scales, out)
-        return out
+    call = Call(c.codes, stream)
+    out = torch.empty((t, d), dtype=c.dtype, device=c.codes.device)
+    check(lib().cdclq_checkpoint_restore_device(c.codes.data_ptr(), c.scales.data_ptr(), t, d, out.data_ptr(), d,
+                                                _dtype_code(torch, c.dtype), call.handle))
+    call.keep(c.codes, c.scales, out)
+    return out
 
 
+@on_device_of(0)
 def weight_grad(dy, c, stream=None):
     """dy^T x^ with the restored values rounded to dy's type, as the operand of the tensor cores."""
-    import torch
-
-    tensor(dy, "dy", shape=(c.shape[0], None), device=c.codes.device)
-    code = half_code(torch, dy.dtype, "dy")
-    (t, d), n = c.shape, dy.shape[1]
+    (t, d), codes = c.shape, c.codes
+    tensor(dy, "dy", 2, device=codes.get_device())
+    code = half_code(dy.dtype, "dy")
+    n = dy.shape[1]
+    tensor(dy, "dy", 2, shape=(t, n))
     if d == 0 or n == 0:
         refuse("weight_grad: no columns")
-    with on(torch, dy.device, stream) as call:
-        dw = torch.empty((n, d), dtype=dy.dtype, device=dy.device)
-        src, ld = rows16(torch, dy, call) if t else (dy, n)
-        ws = workspace(torch, lib().cdclq_checkpoint_weight_grad_workspace(t, d, n), dy.device, call)
-        check(lib().cdclq_checkpoint_weight_grad_device(ptr(src), ld, code, ptr(c.codes), ptr(c.scales), t, d, n, ptr(dw), d,
-                                                        ptr(ws), ws.numel(), call.handle))
-        call.keep(dy, c.codes, c.scales, dw)
-        return dw
+    call, L = Call(dy, stream), lib()
+    dw = torch.empty((n, d), dtype=dy.dtype, device=dy.device)
+    src, ld = rows16(dy, call) if t else (dy, n)
+    need = L.cdclq_checkpoint_weight_grad_workspace(t, d, n)
+    ws = workspace(need, dy, call)
+    check(L.cdclq_checkpoint_weight_grad_device(src.data_ptr(), ld, code, codes.data_ptr(), c.scales.data_ptr(), t, d, n,
+                                                dw.data_ptr(), d, ws.data_ptr(), need, call.handle))
+    call.keep(dy, codes, c.scales, dw)
+    return dw

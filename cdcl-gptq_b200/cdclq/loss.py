@@ -13,60 +13,63 @@ the vocabulary at a time.  Matrices whose rows do not start on 16 bytes are copi
 kept with padded rows: any row stride is taken as it is).  The calls are asynchronous on `stream` (torch's current one
 if None).
 """
-from ._device import half_code, on, ptr, refuse, rows16, tensor, workspace
+import torch
+
+from ._device import Call, half_code, on_device_of, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 
 
-def _head(torch, h, w, target):
-    tensor(h, "h", shape=(None, None))
-    code = half_code(torch, h.dtype, "h")
-    t, d = h.shape
-    tensor(w, "w", h.dtype, (None, d), h.device)
-    tensor(target, "target", torch.int64, (t,), h.device)
-    if d == 0 or w.shape[0] == 0:
+def _head(h, w, target):
+    tensor(h, "h", 2)
+    code = half_code(h.dtype, "h")
+    (t, d), dev = h.shape, h.get_device()
+    tensor(w, "w", 2, h.dtype, (w.shape[0], d) if w.dim() == 2 else (None, d), dev)
+    tensor(target, "target", 1, torch.int64, (t,), dev)
+    v = w.shape[0]
+    if d == 0 or v == 0:
         refuse("w: the head has no rows or no columns")
-    return code, t, d, w.shape[0]
+    return code, t, d, v
 
 
+@on_device_of(0)
 def linear_cross_entropy(h, w, target, stream=None):
     """(loss, lse), float32, one for each row of h."""
-    import torch
-
-    code, t, d, v = _head(torch, h, w, target)
-    with on(torch, h.device, stream) as call:
-        loss = torch.empty(t, dtype=torch.float32, device=h.device)
-        lse = torch.empty_like(loss)
-        if t == 0:
-            return loss, lse
-        target = target.contiguous()
-        hr, ldh = rows16(torch, h, call)
-        wr, ldw = rows16(torch, w, call)
-        ws = workspace(torch, lib().cdclq_linear_cross_entropy_workspace(t, d, v), h.device, call)
-        check(lib().cdclq_linear_cross_entropy_device(ptr(hr), ldh, ptr(wr), ldw, code, t, d, v, ptr(target), ptr(loss),
-                                                      ptr(lse), ptr(ws), ws.numel(), call.handle))
-        call.keep(h, w, target, loss, lse)
+    code, t, d, v = _head(h, w, target)
+    loss = torch.empty(t, dtype=torch.float32, device=h.device)
+    lse = torch.empty_like(loss)
+    if t == 0:
         return loss, lse
+    call, L = Call(h, stream), lib()
+    target = target.contiguous()
+    hr, ldh = rows16(h, call)
+    wr, ldw = rows16(w, call)
+    need = L.cdclq_linear_cross_entropy_workspace(t, d, v)
+    ws = workspace(need, h, call)
+    check(L.cdclq_linear_cross_entropy_device(hr.data_ptr(), ldh, wr.data_ptr(), ldw, code, t, d, v, target.data_ptr(),
+                                              loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, call.handle))
+    call.keep(h, w, target, loss, lse)
+    return loss, lse
 
 
+@on_device_of(0)
 def linear_cross_entropy_backward(h, w, target, lse, dloss, need_dh=True, need_dw=True, stream=None):
     """(dh, dw) for the gradient dloss of each token's loss; None in the place of one that is not needed."""
-    import torch
-
-    code, t, d, v = _head(torch, h, w, target)
-    tensor(lse, "lse", torch.float32, (t,), h.device)
-    tensor(dloss, "dloss", torch.float32, (t,), h.device)
-    with on(torch, h.device, stream) as call:
-        dh = torch.empty((t, d), dtype=h.dtype, device=h.device) if need_dh else None
-        dw = torch.empty((v, d), dtype=h.dtype, device=h.device) if need_dw else None
-        if t == 0 or not (need_dh or need_dw):
-            return dh, dw.zero_() if dw is not None else None
-        target, lse, dloss = target.contiguous(), lse.contiguous(), dloss.contiguous()
-        hr, ldh = rows16(torch, h, call)
-        wr, ldw = rows16(torch, w, call)
-        need = lib().cdclq_linear_cross_entropy_backward_workspace(t, d, v, need_dh, need_dw)
-        ws = workspace(torch, need, h.device, call)
-        check(lib().cdclq_linear_cross_entropy_backward_device(ptr(hr), ldh, ptr(wr), ldw, code, t, d, v, ptr(target),
-                                                               ptr(lse), ptr(dloss), ptr(dh), d, ptr(dw), d, ptr(ws),
-                                                               ws.numel(), call.handle))
-        call.keep(h, w, target, lse, dloss, dh, dw)
-        return dh, dw
+    code, t, d, v = _head(h, w, target)
+    dev = h.get_device()
+    tensor(lse, "lse", 1, torch.float32, (t,), dev)
+    tensor(dloss, "dloss", 1, torch.float32, (t,), dev)
+    dh = torch.empty((t, d), dtype=h.dtype, device=h.device) if need_dh else None
+    dw = torch.empty((v, d), dtype=h.dtype, device=h.device) if need_dw else None
+    if t == 0 or not (need_dh or need_dw):
+        return dh, dw.zero_() if dw is not None else None
+    call, L = Call(h, stream), lib()
+    target, lse, dloss = target.contiguous(), lse.contiguous(), dloss.contiguous()
+    hr, ldh = rows16(h, call)
+    wr, ldw = rows16(w, call)
+    need = L.cdclq_linear_cross_entropy_backward_workspace(t, d, v, need_dh, need_dw)
+    ws = workspace(need, h, call)
+    check(L.cdclq_linear_cross_entropy_backward_device(
+        hr.data_ptr(), ldh, wr.data_ptr(), ldw, code, t, d, v, target.data_ptr(), lse.data_ptr(), dloss.data_ptr(),
+        dh.data_ptr() if need_dh else None, d, dw.data_ptr() if need_dw else None, d, ws.data_ptr(), need, call.handle))
+    call.keep(h, w, target, lse, dloss, dh, dw)
+    return dh, dw

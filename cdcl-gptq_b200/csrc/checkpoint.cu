@@ -46,93 +46,137 @@ struct Type<CDCLQ_DTYPE_BF16> {
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// One group of 16 lanes for each block of a row, 8 values a lane: one wide load of a 16-bit type.
+// x / s to the nearest whole number, for |x| <= 127 s (1 + 2^-23).  x * (1 / s) is within 127 * 2^-22 of the quotient, so it
+// rounds to the same number unless it lies within 2^-13 of a half; there the division decides.
+__device__ __forceinline__ float nearest(float x, float s, float inv) {
+    const float p = x * inv, r = rintf(p);
+    if (fabsf(fabsf(p - r) - 0.5f) < 1.0f / 8192.0f) return rintf(__fdiv_rn(x, s));
+    return r;
+}
+
+// 16 lanes to a block of 128 columns, 8 values a lane: one wide load of a 16-bit type.  A CTA has 16 such groups: `across`
+// of them (a power of two) side by side along a row, 16 / across rows; it takes the rows UNROLL at a time.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Type<DT>::T* __restrict__ x, int64_t ldx, int64_t t,
-                                                              int64_t d, int8_t* __restrict__ codes, float* __restrict__ scales) {
-    const int lane = threadIdx.x & 15;
-    const int64_t nb = (d + BLOCK - 1) / BLOCK, total = t * nb;
-    for (int64_t g = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4; g < ((total + 1) & ~(int64_t)1);
-         g += ((int64_t)gridDim.x * blockDim.x) >> 4) {
-        const bool live = g < total;  // the warp's other half may have a block
-        const int64_t row = live ? g / nb : 0, b = live ? g - row * nb : 0;
-        const int64_t c = b * BLOCK + lane * 8;
-        const int n = live ? (int)max((int64_t)0, min((int64_t)8, d - c)) : 0;
-        const typename Type<DT>::T* src = x + row * ldx + c;
-        float v[8];
-        if (WIDE && n == 8) {
-            alignas(16) typename Type<DT>::T raw[8];
+                                                              int64_t d, int across, int8_t* __restrict__ codes,
+                                                              float* __restrict__ scales) {
+    typedef typename Type<DT>::T T;
+    constexpr int UNROLL = 2;
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int64_t nb = (d + BLOCK - 1) / BLOCK;
+    const int64_t b = (int64_t)blockIdx.x * across + (group & (across - 1));
+    const int64_t c = b * BLOCK + lane * 8;
+    const int down = 16 / across;
+    const int n = (int)max((int64_t)0, min((int64_t)8, d - c));
+    // every thread of a warp walks the same number of rows (the shuffles need them all)
+    for (int64_t r0 = (int64_t)blockIdx.y * down * UNROLL; r0 < t; r0 += (int64_t)gridDim.y * down * UNROLL) {
+        alignas(16) T raw[UNROLL][8];
+        int64_t row[UNROLL];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(raw) / 16; i++) reinterpret_cast<uint4*>(raw)[i] = reinterpret_cast<const uint4*>(src)[i];
+        for (int k = 0; k < UNROLL; k++) {
+            row[k] = r0 + k * down + group / across;
+            const int m = row[k] < t ? n : 0;
+            const T* src = x + row[k] * ldx + c;
+            if (WIDE && m == 8) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = Type<DT>::up(raw[i]);
-        } else {
+                for (int i = 0; i < (int)sizeof(raw[0]) / 16; i++) reinterpret_cast<uint4*>(raw[k])[i] = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = i < n ? Type<DT>::up(src[i]) : 0.0f;
+                for (int i = 0; i < 8; i++) raw[k][i] = i < m ? src[i] : Type<DT>::down(0.0f);
+            }
         }
-        float top = 0.0f;
-        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            top = fmaxf(top, fabsf(v[i]));
-            bad |= !(fabsf(v[i]) < INFINITY);
-        }
-        if (bad) top = INFINITY;
+        for (int k = 0; k < UNROLL; k++) {
+            float v[8], top = 0.0f;
+            bool fine = true;
 #pragma unroll
-        for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool finite = top < INFINITY;
-        const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
-        if (live && lane == 0) scales[g] = s;
-        alignas(8) int8_t q[8];
+            for (int i = 0; i < 8; i++) {
+                v[i] = Type<DT>::up(raw[k][i]);
+                top = fmaxf(top, fabsf(v[i]));
+                fine &= fabsf(v[i]) < INFINITY;
+            }
+            if (!fine) top = INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float r = finite && s > 0.0f ? rintf(__fdiv_rn(v[i], s)) : 0.0f;
-            q[i] = (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
-        }
-        int8_t* dst = codes + row * d + c;
-        if (WIDE && n == 8) {
-            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(q);
-        } else {
+            for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const bool finite = top < INFINITY;
+            const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
+            const bool normal = finite && s >= 1.1754944e-38f;  // 1 / s is then finite
+            const float inv = normal ? __fdiv_rn(1.0f, s) : 0.0f;
+            alignas(8) int8_t q[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < n) dst[i] = q[i];
+            for (int i = 0; i < 8; i++) {
+                float r = 0.0f;
+                if (normal)
+                    r = nearest(v[i], s, inv);
+                else if (finite && s > 0.0f)
+                    r = rintf(__fdiv_rn(v[i], s));
+                q[i] = (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
+            }
+            if (row[k] >= t || n == 0) continue;
+            if (lane == 0) scales[row[k] * nb + b] = s;
+            int8_t* dst = codes + row[k] * d + c;
+            if (WIDE && n == 8) {
+                *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(q);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (i < n) dst[i] = q[i];
+            }
         }
     }
 }
 
-// 8 values a thread.  ld: elements from row to row of the output; columns d..ld of it are left as they are.
+// 16 values a thread; a CTA has `across` (a power of two) threads along a row.  ld: elements from row to row of the output;
+// columns d..ld of it are left as they are.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
-                                                                 int64_t t, int64_t d, typename Type<DT>::T* __restrict__ out,
+                                                                 int64_t t, int64_t d, int across, typename Type<DT>::T* __restrict__ out,
                                                                  int64_t ld) {
-    const int64_t d8 = (d + 7) / 8, nb = (d + BLOCK - 1) / BLOCK;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < t * d8; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / d8, c = (i - row * d8) * 8;
+    typedef typename Type<DT>::T T;
+    const int64_t nb = (d + BLOCK - 1) / BLOCK;
+    const int64_t c = ((int64_t)blockIdx.x * across + (threadIdx.x & (across - 1))) * 16;
+    if (c >= d) return;
+    const int down = 256 / across;
+    for (int64_t row = (int64_t)blockIdx.y * down + threadIdx.x / across; row < t; row += (int64_t)gridDim.y * down) {
         const float s = scales[row * nb + c / BLOCK];
-        alignas(16) typename Type<DT>::T r[8];
-        if (WIDE && c + 8 <= d) {
-            alignas(8) int8_t q[8];
-            *reinterpret_cast<uint2*>(q) = *reinterpret_cast<const uint2*>(codes + row * d + c);
+        const int8_t* src = codes + row * d + c;
+        T* dst = out + row * ld + c;
+        if (WIDE && c + 16 <= d) {
+            alignas(16) int8_t q[16];
+            alignas(16) T r[16];
+            *reinterpret_cast<uint4*>(q) = __ldcs(reinterpret_cast<const uint4*>(src));
 #pragma unroll
-            for (int k = 0; k < 8; k++) r[k] = Type<DT>::down(__fmul_rn((float)q[k], s));
+            for (int k = 0; k < 16; k++) r[k] = Type<DT>::down(__fmul_rn((float)q[k], s));
 #pragma unroll
-            for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(out + row * ld + c)[k] = reinterpret_cast<uint4*>(r)[k];
+            for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<uint4*>(r)[k];
         } else {
-            for (int k = 0; k < 8 && c + k < d; k++) out[row * ld + c + k] = Type<DT>::down(__fmul_rn((float)codes[row * d + c + k], s));
+            for (int k = 0; k < 16 && c + k < d; k++) dst[k] = Type<DT>::down(__fmul_rn((float)src[k], s));
         }
     }
 }
 
-unsigned grid_of(int64_t blocks) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)sm_count() * 16)); }
+int power_of_two(int64_t want, int most) {
+    int p = 1;
+    while (p < most && p < want) p *= 2;
+    return p;
+}
+
+// Rows' CTAs: enough for 32 to an SM over the whole grid, at most what a grid's second dimension holds.
+unsigned grid_rows(int64_t rows, int64_t columns) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>({rows, ceil_div((int64_t)sm_count() * 32, columns), 65535}));
+}
 
 template <int DT>
 int save(const void* x, int64_t ldx, int64_t t, int64_t d, int8_t* codes, float* scales, cudaStream_t st) {
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * sizeof(T)) % 16 == 0 &&
                       (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
-    const unsigned grid = grid_of(ceil_div(t * ceil_div(d, BLOCK), 16));
+    const int64_t nb = ceil_div(d, BLOCK);
+    const int across = power_of_two(nb, 16);
+    const int64_t gx = ceil_div(nb, across);
     auto kern = wide ? checkpoint_save_kernel<DT, true> : checkpoint_save_kernel<DT, false>;
-    CDCLQ_LAUNCH(kern, grid, 256, 0, st, static_cast<const T*>(x), ldx, t, d, codes, scales);
+    CDCLQ_LAUNCH(kern, dim3((unsigned)gx, grid_rows(ceil_div(t, 2 * (16 / across)), gx)), 256, 0, st, static_cast<const T*>(x), ldx, t, d,
+                 across, codes, scales);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "checkpoint_save_kernel launch");
 }
@@ -141,10 +185,12 @@ template <int DT>
 int restore(const int8_t* codes, const float* scales, int64_t t, int64_t d, void* out, int64_t ld, cudaStream_t st) {
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ld * sizeof(T)) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
-    const unsigned grid = grid_of(ceil_div(t * ceil_div(d, 8), 256));
+                      (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && d % 16 == 0;
+    const int across = power_of_two(ceil_div(d, 16), 256);
+    const int64_t gx = ceil_div(d, 16 * across);
     auto kern = wide ? checkpoint_restore_kernel<DT, true> : checkpoint_restore_kernel<DT, false>;
-    CDCLQ_LAUNCH(kern, grid, 256, 0, st, codes, scales, t, d, static_cast<T*>(out), ld);
+    CDCLQ_LAUNCH(kern, dim3((unsigned)gx, grid_rows(ceil_div(t, 256 / across), gx)), 256, 0, st, codes, scales, t, d, across,
+                 static_cast<T*>(out), ld);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "checkpoint_restore_kernel launch");
 }

@@ -1,5 +1,6 @@
 // half_gemm.cu - plans and launches the half-precision tensor-core product: tensor maps, tile width, K splits.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "half_gemm_launch.cuh"
@@ -9,9 +10,15 @@ namespace cdclq {
 using namespace hg;
 
 int sm_count() {
+    static std::atomic<int> known[64];  // of each device
     int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return sms;
+    }
+    if (dev < 64 && known[dev].load(std::memory_order_relaxed)) return known[dev].load(std::memory_order_relaxed);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) cudaGetLastError();
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 

@@ -64,6 +64,25 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);
 // Launches the product (and, when the plan splits K, the pass that adds the splits in order).
 int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st);
 
+// Launches a kernel that may start while the one before it in the stream still runs; it waits for that one's results itself
+// (griddepcontrol.wait).
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e == cudaSuccess ? 0 : cuda_error(e, what);
+}
+
 // Number of SMs of the current device.
 int sm_count();
 // Device pointer of the host word that a kernel sets when one of its bounded waits ran out; null on failure.

@@ -19,38 +19,44 @@ namespace cdclq {
 namespace {
 
 constexpr size_t GRAD_BYTES = 256u << 20;  // one piece of g
-constexpr int JOIN_ROWS = 32, JOIN_PARTS = 16;
+constexpr int JOIN_ROWS = 8, JOIN_PARTS = 64;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Joins the (maximum, sum) pairs of a row's column tiles: 32 rows x 16 threads that each take every 16th pair.
+// Joins the (maximum, sum) pairs of a row's column tiles: 8 rows x 64 threads that each take every 64th pair, four loads
+// in flight.  A pair's maximum is -inf where its logits all are; its sum is then 0, or NaN with a NaN among them.
+__device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    if (top == -INFINITY) return make_float2(top, a.y + b.y);
+    return make_float2(top, (a.x == -INFINITY ? a.y : a.y * expf(a.x - top)) + (b.x == -INFINITY ? b.y : b.y * expf(b.x - top)));
+}
 __global__ void __launch_bounds__(JOIN_ROWS* JOIN_PARTS)
 loss_join_kernel(const float2* __restrict__ stats, int parts, int t, int64_t vocab, const int64_t* __restrict__ target,
                  const float* __restrict__ label_logit, float* loss, float* lse) {
     __shared__ float2 s[JOIN_PARTS][JOIN_ROWS];
     const int tx = threadIdx.x % JOIN_ROWS, ty = threadIdx.x / JOIN_ROWS;
     const int row = blockIdx.x * JOIN_ROWS + tx;
-    float top = -INFINITY, sum = 0.0f;
+    float2 mine = make_float2(-INFINITY, 0.0f);
     if (row < t) {
-#pragma unroll 4
-        for (int p = ty; p < parts; p += JOIN_PARTS) {
-            const float2 v = stats[(int64_t)p * t + row];
-            const float hi = fmaxf(top, v.x);
-            const float ref = hi == -INFINITY ? 0.0f : hi;
-            sum = (top == -INFINITY ? sum : sum * expf(top - ref)) + (v.x == -INFINITY ? v.y : v.y * expf(v.x - ref));
-            top = hi;
+        for (int p = ty; p < parts; p += 4 * JOIN_PARTS) {
+            float2 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                v[q] = p + q * JOIN_PARTS < parts ? stats[(int64_t)(p + q * JOIN_PARTS) * t + row] : make_float2(-INFINITY, 0.0f);
+            mine = join_pairs(mine, join_pairs(join_pairs(v[0], v[1]), join_pairs(v[2], v[3])));
         }
     }
-    s[ty][tx] = make_float2(top, sum);
+    s[ty][tx] = mine;
     __syncthreads();
+#pragma unroll
+    for (int o = JOIN_PARTS / 2; o; o >>= 1) {
+        if (ty < o) s[ty][tx] = join_pairs(s[ty][tx], s[ty + o][tx]);
+        __syncthreads();
+    }
     if (ty == 0 && row < t) {
-        for (int q = 0; q < JOIN_PARTS; q++) top = fmaxf(top, s[q][tx].x);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float all = 0.0f;
-        for (int q = 0; q < JOIN_PARTS; q++)
-            all += s[q][tx].x == -INFINITY ? s[q][tx].y : s[q][tx].y * expf(s[q][tx].x - ref);
-        const float l = ref + logf(all);
+        const float2 all = s[0][tx];
+        const float l = (all.x == -INFINITY ? 0.0f : all.x) + logf(all.y);
         const int64_t label = target[row];
         lse[row] = l;
         loss[row] = (label >= 0 && label < vocab) ? l - label_logit[row] : 0.0f;

@@ -9,6 +9,7 @@
 
 #include "half_gemm.h"
 #include "packed.h"
+#include "tcgen05.cuh"
 
 namespace cdclq {
 
@@ -80,25 +81,6 @@ __host__ __device__ constexpr int plane_bits(int bits, int p) {
     const int second = rest >= 4 ? 4 : rest >= 2 ? 2 : 1;
     if (p == 1) return second;
     return rest - second;
-}
-
-// Code of k-step `ks`, column pair `pair` (0..3: see PackedUnit's lanes), member `odd`, from a lane's words `stride` apart.
-template <typename Words>
-__device__ __forceinline__ uint32_t code_at(Words w, int stride, int bits, int ks, int pair, int odd) {
-    uint32_t code = 0;
-    int shift = 0;
-#pragma unroll
-    for (int p = 0; p < 3; p++) {
-        const int pb = plane_bits(bits, p);
-        if (pb == 0) break;
-        const int slot = ks * 4 + pair;                  // of the unit's 16 pairs
-        const int per = pb == 4 ? 4 : pb == 2 ? 8 : 16;  // pairs in a word of the plane
-        const uint32_t v = w[(slot / per) * stride];
-        code |= ((v >> (pb * (slot % per) + 16 * odd)) & ((1u << pb) - 1u)) << shift;
-        w += pb * stride;
-        shift += pb;
-    }
-    return code;
 }
 
 // One thread for each word of the layout.  `column` still holds permuted places here.
@@ -182,52 +164,145 @@ __device__ __forceinline__ float half_value(uint16_t v) {
     return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
-// A row tile's 16 rows in the original column order: its codes are staged in shared memory (their places are a permutation),
-// a thread takes two columns so that a warp writes 128 bytes along a row.
+// ---------------------------------------------------------------------------------------------------------------------
+// Expansion to a 16-bit matrix in the original column order.
+
+// A pair of small whole numbers (16 bits each) as f16 or bf16, minus a zero point, exactly: the numbers go into the low
+// bits of a float whose last place is 1 (f16 1024, bf16 128), and the same offset plus the zero point comes off.
 template <bool BF16>
-__global__ void __launch_bounds__(512) packed_expand_kernel(const PackedView W, int staged, uint16_t* __restrict__ out, int64_t ldw,
-                                                            int pairs_wide) {
-    extern __shared__ uint32_t words[];
-    const int tile = blockIdx.x;
-    const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
-    if (staged) {
-        for (int i = threadIdx.x * 4; i < W.tile_words * 32; i += blockDim.x * 4)
-            *reinterpret_cast<uint4*>(words + i) = *reinterpret_cast<const uint4*>(codes + i);
-        __syncthreads();
+__device__ __forceinline__ uint32_t minus_zero(uint32_t q, uint32_t offset_zero) {
+    if constexpr (BF16) {
+        const uint32_t v = q | 0x43004300u;
+        __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&offset_zero));
+        return *reinterpret_cast<uint32_t*>(&r);
+    } else {
+        const uint32_t v = q | 0x64006400u;
+        __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&offset_zero));
+        return *reinterpret_cast<uint32_t*>(&r);
     }
-    const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
-    const int rows = min(16, W.d_out - tile * 16);
-    const int c_step = gridDim.y * blockDim.x * 2;
-    for (int c = (blockIdx.y * blockDim.x + threadIdx.x) * 2; c < W.d_in; c += c_step) {
-        const int n = min(2, W.d_in - c);
-        uint32_t res[16];
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pair_of(float v) {
+    const uint32_t h = half_bits<BF16>(v);
+    return h | h << 16;
+}
+// What minus_zero (or, for 8 bits in bf16, decode_pair) takes off for a zero point.
+template <bool BF16, int BITS>
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
+    return pair_of<BF16>((float)z + (BF16 ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f));
+}
+
+// Code minus zero point, exactly, of pair p (0..3) of a k-step: rows l / 4 (even pairs) and l / 4 + 8.  For 8 bits in bf16,
+// which holds whole numbers to 256 only, the two nibbles are brought in one by one.
+template <bool BF16, int BITS>
+__device__ __forceinline__ uint32_t decode_pair(const uint32_t (&w)[BITS], int ks, int p, uint32_t zero) {
+    const int slot = ks * 4 + p;
+    if constexpr (BITS == 8 && BF16) {
+        const uint32_t lo = (w[slot / 4] >> (4 * (slot % 4))) & 0x000f000fu, hi = (w[4 + slot / 4] >> (4 * (slot % 4))) & 0x000f000fu;
+        const uint32_t h = hi | 0x45004500u, h0 = 0x45004500u;  // 2048 + 16 hi, 2048
+        const uint32_t l = lo | 0x43004300u, l0 = 0x43004300u;  // 128 + lo, 128
+        typedef __nv_bfloat162 B2;
+        const B2 high = __hsub2(*reinterpret_cast<const B2*>(&h), *reinterpret_cast<const B2*>(&h0));
+        const B2 low = __hsub2(*reinterpret_cast<const B2*>(&l), *reinterpret_cast<const B2*>(&l0));
+        B2 r = __hadd2(__hsub2(high, *reinterpret_cast<const B2*>(&zero)), low);
+        return *reinterpret_cast<uint32_t*>(&r);
+    } else {
+        uint32_t q = 0;
+        int at = 0, shift = 0;
 #pragma unroll
-        for (int r = 0; r < 16; r++) res[r] = 0;
-        for (int e = 0; e < n; e++) {
-            const int p = W.place[c + e];
-            const PackedUnit u = W.unit[p >> 6];
-            const int ks = (p >> 4) & 3, k = p & 15;
-            const uint32_t* gs = grid + (int64_t)u.group[ks] * 16;
-            const int first = (int)u.word * 32 + ((k & 7) >> 1);
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int at = first + (r & 7) * 4, pair = (k >> 3) * 2 + (r >> 3);
-                const uint32_t q = staged ? code_at(words + at, 32, u.bits, ks, pair, k & 1) : code_at(codes + at, 32, u.bits, ks, pair, k & 1);
-                const uint32_t sz = gs[r];
-                const float v = __fmul_rn(__half2float(__ushort_as_half((uint16_t)sz)), (float)((int)q - (int)(sz >> 16)));
-                res[r] |= (uint32_t)half_bits<BF16>(v) << (16 * e);
+        for (int plane = 0; plane < 3; plane++) {
+            const int pb = plane_bits(BITS, plane);
+            if (pb) {
+                const int per = 16 / pb;
+                const uint32_t m = (1u << pb) - 1u;
+                q |= ((w[at + slot / per] >> (pb * (slot % per))) & (m | m << 16)) << shift;
+                at += pb;
+                shift += pb;
             }
         }
-        uint16_t* dst = out + (int64_t)tile * 16 * ldw + c;
+        return minus_zero<BF16>(q, zero);
+    }
+}
+
+// scale * (code - zero point), rounded once: the product of an 11-bit and an 8-bit significand is exact in f32, and f16's
+// own product is that product rounded.
+template <bool BF16>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) {
+    if constexpr (BF16) {
+        const float s = __half2float(__ushort_as_half((uint16_t)scale_f16));
+        __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(d << 16) * s, __uint_as_float(d & 0xffff0000u) * s);
+        return *reinterpret_cast<uint32_t*>(&r);
+    } else {
+        const uint32_t ss = scale_f16 | scale_f16 << 16;
+        __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&d), *reinterpret_cast<const __half2*>(&ss));
+        return *reinterpret_cast<uint32_t*>(&r);
+    }
+}
+
+constexpr int EXPAND_WARPS = 16;
+
+template <bool BF16, int BITS>
+__device__ __forceinline__ void expand_unit(const PackedView& W, const PackedUnit& u, int ui, const uint32_t* __restrict__ codes,
+                                            const uint32_t* __restrict__ grid, int lane, int half, int row, bool live,
+                                            uint16_t* rows, int ld) {
+    uint32_t w[BITS];
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            if (r >= rows) break;
-            if (pairs_wide && n == 2) {
-                *reinterpret_cast<uint32_t*>(dst + r * ldw) = res[r];
-            } else {
-                dst[r * ldw] = (uint16_t)res[r];
-                if (n == 2) dst[r * ldw + 1] = (uint16_t)(res[r] >> 16);
+    for (int i = 0; i < BITS; i++) w[i] = codes[(u.word + i) * 32 + lane];
+    const int2* column = reinterpret_cast<const int2*>(W.column + ui * 64) + (lane & 3);
+    uint32_t sz = 0, zero = 0;
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) {
+        if (ks == 0 || u.group[ks] != u.group[ks - 1]) {
+            sz = grid[(int64_t)u.group[ks] * 16 + half * 8 + lane / 4];
+            zero = zero_pair<BF16, BITS>(sz >> 16);
+        }
+#pragma unroll
+        for (int hi = 0; hi < 2; hi++) {
+            const int2 c = column[ks * 8 + hi * 4];
+            const uint32_t v = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, hi * 2 + half, zero), sz & 0xffffu);
+            if (live) {
+                if (c.x >= 0) rows[row * ld + c.x] = (uint16_t)v;
+                if (c.y >= 0) rows[row * ld + c.y] = (uint16_t)(v >> 16);
             }
+        }
+    }
+}
+
+// A CTA expands `R` of a tile's 16 rows (R = 8 unless the rows do not fit): warps decode unit by unit into rows in shared
+// memory, at their original columns, and the CTA writes whole rows out.  Bound by the 16-bit rows written; the scattered
+// 2-byte stores cost about two shared-memory cycles each, rows being four banks apart.
+template <bool BF16>
+__global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, int R, int ld, uint16_t* __restrict__ out,
+                                                                          int64_t ldw, int wide) {
+    extern __shared__ __align__(16) uint16_t rows[];
+    const int parts = 16 / R, tile = blockIdx.x / parts, first = (blockIdx.x % parts) * R;  // rows first .. first + R of the tile
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half = first >> 3, row = lane / 4 - (first & 7);
+    const bool live = row >= 0 && row < R;
+    const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
+    const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
+    for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
+        const PackedUnit u = W.unit[ui];
+        switch (u.bits) {
+            case 2: expand_unit<BF16, 2>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            case 3: expand_unit<BF16, 3>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            case 4: expand_unit<BF16, 4>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            case 5: expand_unit<BF16, 5>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            case 6: expand_unit<BF16, 6>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            case 7: expand_unit<BF16, 7>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+            default: expand_unit<BF16, 8>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+        }
+    }
+    __syncthreads();
+    const int rows_here = min(R, W.d_out - tile * 16 - first);
+    for (int r = 0; r < rows_here; r++) {
+        uint16_t* dst = out + ((int64_t)tile * 16 + first + r) * ldw;
+        const uint16_t* src = rows + r * ld;
+        if (wide) {  // ldw is d_in rounded up to 8; what lies past d_in is written along
+            for (int c = threadIdx.x * 8; c < W.d_in; c += EXPAND_WARPS * 32 * 8)
+                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        } else {
+            for (int c = threadIdx.x; c < W.d_in; c += EXPAND_WARPS * 32) dst[c] = src[c];
         }
     }
 }
@@ -251,14 +326,15 @@ PackedView packed_view(const cdclq_packed_layer& w) {
 }
 
 int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, cudaStream_t st) {
-    const size_t bytes = (size_t)w.tile_words * 32 * 4;
-    const int staged = bytes <= 200 * 1024;
+    // rows 4 banks apart (16 bytes past a multiple of 128), whole 16-byte pieces
+    const int64_t ld = ceil_div(w.d_in, 64) * 64 + 8;
+    int R = 8;
+    while (R > 1 && R * ld * 2 > 220 * 1024) R /= 2;
+    if (R * ld * 2 > 220 * 1024) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
     auto kern = bf16 ? packed_expand_kernel<true> : packed_expand_kernel<false>;
-    if (staged) CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    const int pairs_wide = ldw % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
-    // few row tiles: their columns over several CTAs
-    const int chunks = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(sm_count() * 2, w.tiles), ceil_div(w.d_in, 1024)));
-    CDCLQ_LAUNCH(kern, dim3(w.tiles, chunks), 512, staged ? bytes : 0, st, w, staged, static_cast<uint16_t*>(out), ldw, pairs_wide);
+    CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+    const int wide = ldw % 8 == 0 && ldw >= ceil_div(w.d_in, 8) * 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    CDCLQ_LAUNCH(kern, w.tiles * (16 / R), EXPAND_WARPS * 32, (size_t)(R * ld * 2), st, w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "packed_expand_kernel launch");
 }
@@ -268,7 +344,11 @@ int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw,
 
 namespace {
 
+using namespace tc;
+
 constexpr int DEC_WARPS = 8;
+constexpr int DEC_CODES = 72 * 1024;  // codes of a CTA's rows in shared memory at a time: three CTAs to an SM
+constexpr int DEC_GRID = 16 * 1024;   // scales and zero points of its rows, where they fit
 
 // First launch: x in the tensor instruction's order (its columns gathered through the permutation, padding zero), and
 // u_t = A_i x_t, one warp for each (token, rank).
@@ -276,48 +356,47 @@ template <bool BF16>
 __global__ void __launch_bounds__(256) packed_tokens_kernel(const PackedView W, const uint16_t* __restrict__ x, int64_t ldx, int t,
                                                             int token_tiles, uint2* __restrict__ xf, int frag_blocks,
                                                             const AdapterArgs ad, float* __restrict__ u32, uint16_t* __restrict__ u16) {
-    if ((int)blockIdx.x < frag_blocks) {
-        const int total = W.units * 4 * token_tiles * 32;
-        const int i = blockIdx.x * 256 + threadIdx.x;
-        if (i >= total) return;
-        const int lane = i & 31, nt = (i >> 5) % token_tiles, step = (i >> 5) / token_tiles;
-        const int tok = nt * 8 + lane / 4;
-        uint32_t v[4];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if ((int)blockIdx.x >= frag_blocks) {
+        const int w = (blockIdx.x - frag_blocks) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+        if (w >= t * ad.r) return;
+        const int tok = w / ad.r, r = w - tok * ad.r, id = ad.index[tok];
+        float s = 0.0f;
+        if (id >= 0 && id < ad.n) {
+            const uint16_t* a = static_cast<const uint16_t*>(ad.a) + ((int64_t)id * ad.r + r) * ad.lda;
+            const uint16_t* xr = x + tok * ldx;
+            float p[8] = {};
+            int c = lane * 8;
+#pragma unroll 4
+            for (; c + 8 <= W.d_in; c += 256) {
+                const uint4 av = *reinterpret_cast<const uint4*>(a + c), xv = *reinterpret_cast<const uint4*>(xr + c);
+                const uint32_t aw[4] = {av.x, av.y, av.z, av.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int c = W.column[step * 16 + (lane & 3) * 2 + (q & 1) + (q >> 1) * 8];
-            v[q] = (tok < t && c >= 0) ? x[tok * ldx + c] : 0;
+                for (int q = 0; q < 4; q++) {
+                    p[2 * q] = fmaf(half_value<BF16>((uint16_t)aw[q]), half_value<BF16>((uint16_t)xw[q]), p[2 * q]);
+                    p[2 * q + 1] = fmaf(half_value<BF16>((uint16_t)(aw[q] >> 16)), half_value<BF16>((uint16_t)(xw[q] >> 16)), p[2 * q + 1]);
+                }
+            }
+            for (; c < W.d_in; c++) p[0] = fmaf(half_value<BF16>(a[c]), half_value<BF16>(xr[c]), p[0]);  // one lane's last columns
+            s = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         }
-        xf[i] = make_uint2(v[0] | v[1] << 16, v[2] | v[3] << 16);
+        if (lane == 0) {
+            u32[w] = s;
+            if (u16) u16[w] = half_bits<BF16>(s);
+        }
         return;
     }
-    const int w = (blockIdx.x - frag_blocks) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (w >= t * ad.r) return;
-    const int tok = w / ad.r, r = w - tok * ad.r, id = ad.index[tok];
-    float s = 0.0f;
-    if (id >= 0 && id < ad.n) {
-        const uint16_t* a = static_cast<const uint16_t*>(ad.a) + ((int64_t)id * ad.r + r) * ad.lda;
-        const uint16_t* xr = x + tok * ldx;
-        float p[8] = {};
-        int c = lane * 8;
-        for (; c + 8 <= W.d_in; c += 256) {
-            const uint4 av = *reinterpret_cast<const uint4*>(a + c), xv = *reinterpret_cast<const uint4*>(xr + c);
-            const uint32_t aw[4] = {av.x, av.y, av.z, av.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                p[2 * q] = fmaf(half_value<BF16>((uint16_t)aw[q]), half_value<BF16>((uint16_t)xw[q]), p[2 * q]);
-                p[2 * q + 1] = fmaf(half_value<BF16>((uint16_t)(aw[q] >> 16)), half_value<BF16>((uint16_t)(xw[q] >> 16)), p[2 * q + 1]);
-            }
-        }
-        for (; c < W.d_in; c++) p[0] = fmaf(half_value<BF16>(a[c]), half_value<BF16>(xr[c]), p[0]);  // one lane's last columns
-        s = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    }
-    if (lane == 0) {
-        u32[w] = s;
-        if (u16) u16[w] = half_bits<BF16>(s);
-    }
+    const int i = blockIdx.x * 256 + threadIdx.x, total = W.units * 4 * token_tiles * 32;
+    if (i >= total) return;
+    const int lane = i & 31, nt = (i >> 5) % token_tiles, step = (i >> 5) / token_tiles;
+    const int tok = nt * 8 + lane / 4;
+    const int2* column = reinterpret_cast<const int2*>(W.column + step * 16) + (lane & 3);
+    const int2 c0 = column[0], c1 = column[4];
+    const uint16_t* xr = x + (int64_t)min(tok, t - 1) * ldx;
+    const uint32_t a = c0.x >= 0 ? xr[c0.x] : 0, b = c0.y >= 0 ? xr[c0.y] : 0, c = c1.x >= 0 ? xr[c1.x] : 0, d = c1.y >= 0 ? xr[c1.y] : 0;
+    xf[i] = tok < t ? make_uint2(a | b << 16, c | d << 16) : make_uint2(0, 0);
 }
 
 template <bool BF16>
@@ -332,138 +411,141 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// A pair of small whole numbers (16 bits each) as f16 or bf16, minus a zero point, exactly: the numbers go into the low
-// bits of a float whose last place is 1 (f16 1024, bf16 128), and the same offset plus the zero point comes off.
-template <bool BF16>
-__device__ __forceinline__ uint32_t minus_zero(uint32_t q, uint32_t offset_zero) {
-    if constexpr (BF16) {
-        const uint32_t v = q | 0x43004300u;
-        __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&offset_zero));
-        return *reinterpret_cast<uint32_t*>(&r);
-    } else {
-        const uint32_t v = q | 0x64006400u;
-        __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&offset_zero));
-        return *reinterpret_cast<uint32_t*>(&r);
-    }
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pair_of(float v) {
-    const uint32_t h = half_bits<BF16>(v);
-    return h | h << 16;
-}
-
-// The code minus zero point pairs of one k-step for the tensor instruction: rows l / 4 (even pairs) and l / 4 + 8.
-// zero[]: the rows' zero points as pairs, with the offset of minus_zero; for 8 bits in bf16, which holds whole numbers to
-// 256 only, the two nibbles are brought in one by one.
-template <bool BF16, int BITS>
-__device__ __forceinline__ void decode_step(const uint32_t (&w)[BITS], int ks, const uint32_t (&zero)[2], uint32_t (&a)[4]) {
+// One unit of RT row tiles times NT token tiles.  codes, grid: the first tile's (shared memory, or for grid global);
+// `tile_codes` and `tile_grid` words to the next tile.
+template <bool BF16, int BITS, int NT, int RT>
+__device__ __forceinline__ void decode_unit(const uint16_t (&group)[4], const uint32_t* codes, int tile_codes, const uint32_t* grid,
+                                            int tile_grid, const uint2* __restrict__ xf, int lane, float (&acc)[RT][NT][4]) {
+    uint2 x[4][NT];
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-        const int slot = ks * 4 + p;
-        if constexpr (BITS == 8 && BF16) {
-            const uint32_t lo = (w[slot / 4] >> (4 * (slot % 4))) & 0x000f000fu, hi = (w[4 + slot / 4] >> (4 * (slot % 4))) & 0x000f000fu;
-            const uint32_t h = hi | 0x45004500u;           // 2048 + 16 hi
-            const uint32_t base = 0x45004500u;             // 2048
-            __nv_bfloat162 high = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), *reinterpret_cast<const __nv_bfloat162*>(&base));
-            const uint32_t l = lo | 0x43004300u, lbase = 0x43004300u;
-            __nv_bfloat162 low = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&l), *reinterpret_cast<const __nv_bfloat162*>(&lbase));
-            __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero[p & 1]);  // the zero point itself
-            __nv_bfloat162 r = __hadd2(__hsub2(high, z), low);
-            a[p] = *reinterpret_cast<uint32_t*>(&r);
-        } else {
-            uint32_t q = 0;
-            int at = 0, shift = 0;
+    for (int ks = 0; ks < 4; ks++)
 #pragma unroll
-            for (int plane = 0; plane < 3; plane++) {
-                const int pb = plane_bits(BITS, plane);
-                if (pb) {
-                    const int per = 16 / pb;
-                    const uint32_t m = (1u << pb) - 1u;
-                    q |= ((w[at + slot / per] >> (pb * (slot % per))) & (m | m << 16)) << shift;
-                    at += pb;
-                    shift += pb;
+        for (int n = 0; n < NT; n++) x[ks][n] = xf[(ks * NT + n) * 32 + lane];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        uint32_t w[BITS];
+#pragma unroll
+        for (int i = 0; i < BITS; i++) w[i] = codes[rt * tile_codes + i * 32 + lane];
+        float part[NT][4], scale[2] = {};
+        uint32_t zero[2] = {};
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            if (ks == 0 || group[ks] != group[ks - 1]) {
+                const uint32_t* g = grid + rt * tile_grid + group[ks] * 16 + lane / 4;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t sz = g[h * 8];
+                    scale[h] = __half2float(__ushort_as_half((uint16_t)sz));
+                    zero[h] = zero_pair<BF16, BITS>(sz >> 16);
                 }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) part[n][i] = 0.0f;
             }
-            a[p] = minus_zero<BF16>(q, zero[p & 1]);
+            uint32_t a[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
+            if (ks == 3 || group[ks + 1] != group[ks]) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(scale[i >> 1], part[n][i], acc[rt][n][i]);
+            }
         }
     }
 }
 
-template <bool BF16, int BITS, int NT>
-__device__ __forceinline__ void decode_unit(const PackedView& W, const PackedUnit& u, const uint32_t* __restrict__ codes,
-                                            const uint32_t* __restrict__ grid, const uint2* __restrict__ xf, int lane,
-                                            float (&acc)[NT][4]) {
-    uint32_t w[BITS];
-#pragma unroll
-    for (int i = 0; i < BITS; i++) w[i] = codes[(u.word + i) * 32 + lane];
-    float part[NT][4];
-    uint32_t zero[2];
-    float scale[2];
-#pragma unroll
-    for (int ks = 0; ks < 4; ks++) {
-        if (ks == 0 || u.group[ks] != u.group[ks - 1]) {
-            const uint32_t* g = grid + (int64_t)u.group[ks] * 16 + lane / 4;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t sz = g[h * 8];
-                scale[h] = __half2float(__ushort_as_half((uint16_t)sz));
-                const float offset = BF16 ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f;
-                zero[h] = pair_of<BF16>((float)(sz >> 16) + offset);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) part[n][i] = 0.0f;
-        }
-        uint32_t a[4];
-        decode_step<BF16, BITS>(w, ks, zero, a);
-#pragma unroll
-        for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, xf[(ks * NT + n) * 32 + lane]);
-        if (ks == 3 || u.group[ks + 1] != u.group[ks]) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[n][i] = fmaf(scale[i >> 1], part[n][i], acc[n][i]);
-        }
-    }
-}
+struct DecodeArgs {
+    const uint2* xf;
+    const float* u32;
+    uint16_t* y;
+    int64_t ldy;
+    int t;
+    int chunk_units;  // units of a pass through shared memory
+    int grid_staged;
+    int* fail;
+};
 
-// Second launch: a CTA for each 16 rows, its warps over the units.  The scale of a (row, group) multiplies the group's f32
-// sum, so the codes minus their zero points enter the tensor instruction exactly and no weight is rounded.
-// Bound by the codes' bytes; mma.sync because M = 16 rows and a few tokens leave tcgen05's 128 rows empty.
-template <bool BF16, int NT>
-__global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const PackedView W, const uint2* __restrict__ xf, int t,
-                                                                       const AdapterArgs ad, const float* __restrict__ u32,
-                                                                       uint16_t* __restrict__ y, int64_t ldy) {
-    __shared__ float sums[DEC_WARPS][16][NT * 8 + 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.x;
+// Second launch: a CTA for RT * 16 rows, its warps over the units.  Bulk copies bring the rows' codes and grid into shared
+// memory before the first launch has finished (they do not depend on it).  The scale of a (row, group) multiplies the
+// group's f32 sum, so the codes minus their zero points enter the tensor instruction exactly and no weight is rounded.
+// Bound by the codes' bytes; mma.sync because 16 rows and a few tokens leave most of tcgen05's 128 rows empty.
+template <bool BF16, int NT, int RT>
+__global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const PackedView W, const AdapterArgs ad, const DecodeArgs P) {
+    extern __shared__ __align__(128) uint32_t stage[];
+    __shared__ float sums[DEC_WARPS][RT * 16][NT * 8 + 1];
+    __shared__ uint64_t ready;
+    __shared__ int flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.x * RT, tiles = min(RT, W.tiles - tile);
     const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
     const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
-    float acc[NT][4];
+    const int tile_codes = P.chunk_units * W.max_bits * 32;  // words
+    uint32_t* grid_s = stage + RT * tile_codes;
+    // units u0 .. u1 of every tile of the CTA
+    auto fetch = [&](int u0, int u1, bool with_grid) {
+        const uint32_t w0 = W.unit[u0].word, w1 = u1 < W.units ? W.unit[u1].word : (uint32_t)W.tile_words;
+        const uint32_t bytes = (w1 - w0) * 128, gbytes = with_grid ? (uint32_t)(tiles * W.groups * 64) : 0;
+        mbar_expect_tx(&ready, tiles * bytes + gbytes);
+        for (int i = 0; i < tiles; i++)
+            bulk_load(smem_u32(stage + i * tile_codes), codes + ((int64_t)i * W.tile_words + w0) * 32, bytes, &ready);
+        if (gbytes) bulk_load(smem_u32(grid_s), grid, gbytes, &ready);
+    };
+    if (threadIdx.x == 0) {
+        mbar_init(&ready, 1);
+        flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fetch(0, min(W.units, P.chunk_units), P.grid_staged);
+    }
+    float acc[RT][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][i] = 0.0f;
-    for (int ui = warp; ui < W.units; ui += DEC_WARPS) {
-        const PackedUnit u = W.unit[ui];
-        const uint2* xu = xf + (int64_t)ui * 4 * NT * 32;
-        switch (u.bits) {
-            case 2: decode_unit<BF16, 2, NT>(W, u, codes, grid, xu, lane, acc); break;
-            case 3: decode_unit<BF16, 3, NT>(W, u, codes, grid, xu, lane, acc); break;
-            case 4: decode_unit<BF16, 4, NT>(W, u, codes, grid, xu, lane, acc); break;
-            case 5: decode_unit<BF16, 5, NT>(W, u, codes, grid, xu, lane, acc); break;
-            case 6: decode_unit<BF16, 6, NT>(W, u, codes, grid, xu, lane, acc); break;
-            case 7: decode_unit<BF16, 7, NT>(W, u, codes, grid, xu, lane, acc); break;
-            default: decode_unit<BF16, 8, NT>(W, u, codes, grid, xu, lane, acc); break;
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[r][n][i] = 0.0f;
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t* g = P.grid_staged ? grid_s : grid;
+    for (int u0 = 0, pass = 0; u0 < W.units; u0 += P.chunk_units, pass++) {
+        const int u1 = min(W.units, u0 + P.chunk_units);
+        if (pass) {
+            __syncthreads();  // every warp is done with the last units
+            if (threadIdx.x == 0) fetch(u0, u1, false);
+        }
+        if (!mbar_wait(&ready, pass & 1, &flag)) break;
+        const uint32_t w0 = W.unit[u0].word;
+        for (int ui = u0 + warp; ui < u1; ui += DEC_WARPS) {
+            const PackedUnit u = W.unit[ui];
+            const uint2* xu = P.xf + (int64_t)ui * 4 * NT * 32;
+            const uint32_t* c = stage + (u.word - w0) * 32;
+            const int tg = W.groups * 16;
+            switch (u.bits) {
+                case 2: decode_unit<BF16, 2, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                case 3: decode_unit<BF16, 3, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                case 4: decode_unit<BF16, 4, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                case 5: decode_unit<BF16, 5, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                case 6: decode_unit<BF16, 6, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                case 7: decode_unit<BF16, 7, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+                default: decode_unit<BF16, 8, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+            }
         }
     }
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+    for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) sums[warp][lane / 4 + (i >> 1) * 8][n * 8 + (lane & 3) * 2 + (i & 1)] = acc[n][i];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sums[warp][r * 16 + lane / 4 + (i >> 1) * 8][n * 8 + (lane & 3) * 2 + (i & 1)] = acc[r][n][i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * t; i += DEC_WARPS * 32) {
-        const int r = i & 15, tok = i >> 4, row = tile * 16 + r;
+    if (threadIdx.x == 0 && flag) {
+        *(volatile int*)P.fail = 1;
+        __threadfence_system();
+    }
+    for (int i = threadIdx.x; i < RT * 16 * P.t; i += DEC_WARPS * 32) {
+        const int r = i % (RT * 16), tok = i / (RT * 16), row = tile * 16 + r;
         if (row >= W.d_out) continue;
         float s = 0.0f;
 #pragma unroll
@@ -471,41 +553,69 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const Pac
         const int id = ad.n > 0 ? ad.index[tok] : -1;
         if (id >= 0 && id < ad.n) {
             const uint16_t* b = static_cast<const uint16_t*>(ad.b) + ((int64_t)id * W.d_out + row) * ad.ldb;
+            const float* u = P.u32 + tok * ad.r;
             float v = 0.0f;
-            for (int k = 0; k < ad.r; k++) v = fmaf(half_value<BF16>(b[k]), u32[tok * ad.r + k], v);
+            int k = 0;
+            for (; k + 8 <= ad.r; k += 8) {
+                const uint4 q = *reinterpret_cast<const uint4*>(b + k);
+                const uint32_t bw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    v = fmaf(half_value<BF16>((uint16_t)bw[j]), u[k + 2 * j], v);
+                    v = fmaf(half_value<BF16>((uint16_t)(bw[j] >> 16)), u[k + 2 * j + 1], v);
+                }
+            }
+            for (; k < ad.r; k++) v = fmaf(half_value<BF16>(b[k]), u[k], v);
             s = fmaf(ad.scale[id], v, s);
         }
-        y[tok * ldy + row] = half_bits<BF16>(s);
+        P.y[tok * P.ldy + row] = half_bits<BF16>(s);
     }
 }
 
-}  // namespace
-
-static int token_tiles(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
-
-size_t packed_decode_workspace(const PackedView& w, int t, int rank) {
-    return align_up((size_t)w.units * 4 * token_tiles(t) * 32 * sizeof(uint2)) + align_up((size_t)t * rank * sizeof(float));
+template <bool BF16, int NT, int RT>
+int decode_rows(const PackedView& w, const AdapterArgs& ad, DecodeArgs p, cudaStream_t st) {
+    const int unit_bytes = RT * w.max_bits * 128;
+    p.chunk_units = std::max(1, std::min(w.units, DEC_CODES / unit_bytes));
+    p.grid_staged = RT * w.groups * 64 <= DEC_GRID;
+    const size_t smem = (size_t)p.chunk_units * unit_bytes + (p.grid_staged ? (size_t)RT * w.groups * 64 : 0);
+    auto kern = packed_decode_kernel<BF16, NT, RT>;
+    CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DEC_CODES + DEC_GRID));
+    return launch_dependent(kern, dim3((unsigned)ceil_div(w.tiles, RT)), dim3(DEC_WARPS * 32), smem, st, "packed_decode_kernel launch", w, ad, p);
 }
 
+int token_tiles(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
+
 template <bool BF16>
-static int decode(const PackedView& w, const void* x, int64_t ldx, int t, const AdapterArgs& ad, void* y, int64_t ldy, void* u,
-                  void* workspace, cudaStream_t st) {
+int decode(const PackedView& w, const void* x, int64_t ldx, int t, const AdapterArgs& ad, void* y, int64_t ldy, void* u,
+           void* workspace, cudaStream_t st) {
     const int nt = token_tiles(t);
     uint2* xf = static_cast<uint2*>(workspace);
+    DecodeArgs p{};
+    p.xf = xf;
     float* u32 = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up((size_t)w.units * 4 * nt * 32 * sizeof(uint2)));
+    p.u32 = u32;
+    p.y = static_cast<uint16_t*>(y);
+    p.ldy = ldy;
+    p.t = t;
+    p.fail = device_fail_word();
+    if (!p.fail) return set_error(CDCLQ_ERR_CUDA, "projection_forward: no mapped host memory (is there a CUDA device?)");
     const int frag_blocks = (int)ceil_div((int64_t)w.units * 4 * nt * 32, 256);
     const int dot_blocks = ad.n > 0 ? (int)ceil_div((int64_t)t * ad.r, 8) : 0;
     CDCLQ_LAUNCH((packed_tokens_kernel<BF16>), frag_blocks + dot_blocks, 256, 0, st, w, static_cast<const uint16_t*>(x), ldx, t, nt, xf,
                  frag_blocks, ad, u32, static_cast<uint16_t*>(u));
-    uint16_t* out = static_cast<uint16_t*>(y);
-    if (nt == 1)
-        CDCLQ_LAUNCH((packed_decode_kernel<BF16, 1>), w.tiles, DEC_WARPS * 32, 0, st, w, xf, t, ad, u32, out, ldy);
-    else if (nt == 2)
-        CDCLQ_LAUNCH((packed_decode_kernel<BF16, 2>), w.tiles, DEC_WARPS * 32, 0, st, w, xf, t, ad, u32, out, ldy);
-    else
-        CDCLQ_LAUNCH((packed_decode_kernel<BF16, 4>), w.tiles, DEC_WARPS * 32, 0, st, w, xf, t, ad, u32, out, ldy);
     cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : cuda_error(e, "packed_decode_kernel launch");
+    if (e != cudaSuccess) return cuda_error(e, "packed_tokens_kernel launch");
+    // two row tiles to a CTA halve the tokens' bytes that it reads through L2, where that still leaves two CTAs to an SM
+    const bool two = w.tiles >= 4 * sm_count();
+    if (nt == 1) return two ? decode_rows<BF16, 1, 2>(w, ad, p, st) : decode_rows<BF16, 1, 1>(w, ad, p, st);
+    if (nt == 2) return two ? decode_rows<BF16, 2, 2>(w, ad, p, st) : decode_rows<BF16, 2, 1>(w, ad, p, st);
+    return two ? decode_rows<BF16, 4, 2>(w, ad, p, st) : decode_rows<BF16, 4, 1>(w, ad, p, st);
+}
+
+}  // namespace
+
+size_t packed_decode_workspace(const PackedView& w, int t, int rank) {
+    return align_up((size_t)w.units * 4 * token_tiles(t) * 32 * sizeof(uint2)) + align_up((size_t)t * rank * sizeof(float));
 }
 
 int launch_packed_decode(const PackedView& w, bool bf16, const void* x, int64_t ldx, int t, const AdapterArgs& ad, void* y,

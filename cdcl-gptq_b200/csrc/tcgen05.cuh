@@ -63,6 +63,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// Untiled copy into shared memory: both addresses and the size are whole multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // Shared-memory matrix descriptor with the 128-byte swizzle.  MN-major: 64-element (128-byte) atoms along MN `lbo`
 // bytes apart, 8-row groups along K `sbo` bytes apart.  K-major: 8-row groups along MN `sbo` bytes apart (`lbo` unused).
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
