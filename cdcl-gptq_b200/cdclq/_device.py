@@ -8,7 +8,9 @@ from .abi import CDCLQ_ERR_ARG
 from .io import DTYPE_BF16, DTYPE_F16
 
 HALF = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent from a torch built without CUDA
+# absent from a torch built without CUDA
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def refuse(msg):
@@ -47,7 +49,7 @@ def on_device_of(position):
             x = args[position] if len(args) > position else None
             if not isinstance(x, torch.Tensor):
                 x = getattr(x, "codes", None)  # a Checkpoint
-            if x is not None and x.is_cuda and x.get_device() != torch.cuda.current_device():
+            if x is not None and x.is_cuda and x.get_device() != _current_device():
                 with torch.cuda.device(x.device):
                     return f(*args, **kw)
             return f(*args, **kw)

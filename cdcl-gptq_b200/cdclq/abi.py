@@ -90,7 +90,7 @@ class CPackedLayer(ctypes.Structure):
         ("units", ctypes.c_uint64),
         ("tile_words", ctypes.c_uint64),
         ("max_bits", ctypes.c_uint32),
-        ("reserved", ctypes.c_uint32),
+        ("bits", ctypes.c_uint32),
         ("layout", ctypes.c_void_p),
     ]
 

@@ -77,6 +77,14 @@ class PackedProjection:
         return self._layout.numel()
 
 
+def _matrix(x, call):
+    """The rows of an n x rows x columns tensor, as rows16 gives them."""
+    n, rows, cols = x.shape
+    if cols % 8 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, cols
+    return rows16(x.reshape(-1, cols), call)
+
+
 class _Adapters:
     """The adapters of one call, checked and in the layout the kernels read."""
 
@@ -102,8 +110,8 @@ class _Adapters:
             return
         if r == 0:
             refuse("a: the rank must be > 0")
-        ar, lda = rows16(a.reshape(-1, d_in), call)
-        br, ldb = rows16(b.reshape(-1, r), call)
+        ar, lda = _matrix(a, call)
+        br, ldb = _matrix(b, call)
         scale, index = scale.contiguous(), index.contiguous()
         self.held = (a, b, ar, br, scale, index)
         self.c = CAdapters(ar.data_ptr(), br.data_ptr(), lda, ldb, scale.data_ptr(), index.data_ptr(), n, r)

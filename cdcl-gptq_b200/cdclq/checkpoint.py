@@ -11,7 +11,7 @@ The calls are asynchronous on `stream` (torch's current one if None).
 """
 import torch
 
-from ._device import Call, half_code, on_device_of, refuse, rows16, tensor, workspace
+from ._device import HALF, Call, half_code, on_device_of, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 from .io import _dtype_code
 
@@ -30,35 +30,48 @@ class Checkpoint:
         _dtype_code(torch, dtype)
         self.codes, self.scales, self.dtype = codes.contiguous(), scales.contiguous(), dtype
 
+    @classmethod
+    def _made(cls, codes, scales, dtype):
+        c = cls.__new__(cls)
+        c.codes, c.scales, c.dtype = codes, scales, dtype
+        return c
+
     @property
     def shape(self):
         return self.codes.shape
 
 
+def _code(dt):
+    code = HALF.get(dt)
+    return _dtype_code(torch, dt) if code is None else code
+
+
 @on_device_of(0)
 def save(x, stream=None):
     tensor(x, "x", 2)
-    code = _dtype_code(torch, x.dtype)
+    code = _code(x.dtype)
     t, d = x.shape
     call = Call(x, stream)
-    if d > 1 and x.stride(1) != 1 or t > 1 and x.stride(0) < d:
-        x = x.contiguous()
+    ld, step = x.stride()
+    if d > 1 and step != 1 or t > 1 and ld < d:
+        x, ld = x.contiguous(), d
     codes = torch.empty((t, d), dtype=torch.int8, device=x.device)
     scales = torch.empty((t, -(-d // BLOCK)), dtype=torch.float32, device=x.device)
-    check(lib().cdclq_checkpoint_save_device(x.data_ptr(), x.stride(0) if t > 1 else d, code, t, d, codes.data_ptr(),
-                                             scales.data_ptr(), call.handle))
+    check(lib().cdclq_checkpoint_save_device(x.data_ptr(), ld if t > 1 else d, code, t, d, codes.data_ptr(), scales.data_ptr(),
+                                             call.handle))
     call.keep(x, codes, scales)
-    return Checkpoint(codes, scales, x.dtype)
+    return Checkpoint._made(codes, scales, x.dtype)
 
 
 @on_device_of(0)
 def restore(c, stream=None):
-    t, d = c.shape
-    call = Call(c.codes, stream)
-    out = torch.empty((t, d), dtype=c.dtype, device=c.codes.device)
-    check(lib().cdclq_checkpoint_restore_device(c.codes.data_ptr(), c.scales.data_ptr(), t, d, out.data_ptr(), d,
-                                                _dtype_code(torch, c.dtype), call.handle))
-    call.keep(c.codes, c.scales, out)
+    codes, scales = c.codes, c.scales
+    t, d = codes.shape
+    call = Call(codes, stream)
+    out = torch.empty((t, d), dtype=c.dtype, device=codes.device)
+    check(lib().cdclq_checkpoint_restore_device(codes.data_ptr(), scales.data_ptr(), t, d, out.data_ptr(), d, _code(c.dtype),
+                                                call.handle))
+    call.keep(codes, scales, out)
     return out
 
 

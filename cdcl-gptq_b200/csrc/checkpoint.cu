@@ -46,22 +46,38 @@ struct Type<CDCLQ_DTYPE_BF16> {
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// x / s to the nearest whole number, for |x| <= 127 s (1 + 2^-23).  x * (1 / s) is within 127 * 2^-22 of the quotient, so it
-// rounds to the same number unless it lies within 2^-13 of a half; there the division decides.
-__device__ __forceinline__ float nearest(float x, float s, float inv) {
-    const float p = x * inv, r = rintf(p);
-    if (fabsf(fabsf(p - r) - 0.5f) < 1.0f / 8192.0f) return rintf(__fdiv_rn(x, s));
-    return r;
+// The absolute values' largest bits over 8 values: as whole numbers they order like the values, infinities and NaN above.
+__device__ __forceinline__ uint32_t top_bits(const float (&raw)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(raw[i]) & 0x7fffffffu);
+    return m;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const T (&raw)[8]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    return max(m & 0xffffu, m >> 16);
+}
+__device__ __forceinline__ float value_of_bits(uint32_t b, const float*) { return __uint_as_float(b); }
+__device__ __forceinline__ float value_of_bits(uint32_t b, const __half*) { return __half2float(__ushort_as_half((uint16_t)b)); }
+__device__ __forceinline__ float value_of_bits(uint32_t b, const __nv_bfloat16*) { return __uint_as_float(b << 16); }
 
 // 16 lanes to a block of 128 columns, 8 values a lane: one wide load of a 16-bit type.  A CTA has 16 such groups: `across`
-// of them (a power of two) side by side along a row, 16 / across rows; it takes the rows UNROLL at a time.
+// of them (a power of two) side by side along a row, 16 / across rows; it takes two such sets of rows at a time.
+//
+// Rounding x / s: p = x * (1 / s) is within 127 * 2^-23 of the quotient, so it rounds to the same number unless it lies
+// within 2^-15 of a half; a thread with such a value divides.  Adding 1.5 * 2^23 rounds p to the nearest whole number, ties
+// to even, and leaves it in the sum's low byte.  |p| <= 127 (1 + 2^-22), so no code is out of range.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Type<DT>::T* __restrict__ x, int64_t ldx, int64_t t,
                                                               int64_t d, int across, int8_t* __restrict__ codes,
                                                               float* __restrict__ scales) {
     typedef typename Type<DT>::T T;
     constexpr int UNROLL = 2;
+    constexpr float MAGIC = 12582912.0f;
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
     const int64_t b = (int64_t)blockIdx.x * across + (group & (across - 1));
@@ -77,9 +93,10 @@ __global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Typ
             row[k] = r0 + k * down + group / across;
             const int m = row[k] < t ? n : 0;
             const T* src = x + row[k] * ldx + c;
-            if (WIDE && m == 8) {
+            if (WIDE) {
 #pragma unroll
-                for (int i = 0; i < (int)sizeof(raw[0]) / 16; i++) reinterpret_cast<uint4*>(raw[k])[i] = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+                for (int i = 0; i < (int)sizeof(raw[0]) / 16; i++)
+                    reinterpret_cast<uint4*>(raw[k])[i] = m ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) raw[k][i] = i < m ? src[i] : Type<DT>::down(0.0f);
@@ -87,40 +104,39 @@ __global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Typ
         }
 #pragma unroll
         for (int k = 0; k < UNROLL; k++) {
-            float v[8], top = 0.0f;
-            bool fine = true;
+            uint32_t bits = top_bits(raw[k]);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[i] = Type<DT>::up(raw[k][i]);
-                top = fmaxf(top, fabsf(v[i]));
-                fine &= fabsf(v[i]) < INFINITY;
-            }
-            if (!fine) top = INFINITY;
-#pragma unroll
-            for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 8; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+            const float top = value_of_bits(bits, static_cast<const T*>(nullptr));
             const bool finite = top < INFINITY;
             const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
             const bool normal = finite && s >= 1.1754944e-38f;  // 1 / s is then finite
             const float inv = normal ? __fdiv_rn(1.0f, s) : 0.0f;
-            alignas(8) int8_t q[8];
+            uint32_t q[8];
+            float near = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                float r = 0.0f;
-                if (normal)
-                    r = nearest(v[i], s, inv);
-                else if (finite && s > 0.0f)
-                    r = rintf(__fdiv_rn(v[i], s));
-                q[i] = (int8_t)fminf(fmaxf(r, -127.0f), 127.0f);
+                const float p = normal ? Type<DT>::up(raw[k][i]) * inv : 0.0f;
+                const float m = p + MAGIC;
+                near = fmaxf(near, fabsf(p - (m - MAGIC)));
+                q[i] = __float_as_uint(m);
+            }
+            if (near > 0.5f - 1.0f / 32768.0f || (finite && !normal && s > 0.0f)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    q[i] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(Type<DT>::up(raw[k][i]), s)), -127.0f), 127.0f);
             }
             if (row[k] >= t || n == 0) continue;
             if (lane == 0) scales[row[k] * nb + b] = s;
             int8_t* dst = codes + row[k] * d + c;
-            if (WIDE && n == 8) {
-                *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(q);
+            if (WIDE) {
+                const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+                *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (i < n) dst[i] = q[i];
+                    if (i < n) dst[i] = (int8_t)q[i];
             }
         }
     }

@@ -38,15 +38,8 @@ static int* fail_word_host() {
     return word;
 }
 
-int* device_fail_word() {
-    int* h = fail_word_host();
-    void* d = nullptr;
-    if (!h || cudaHostGetDevicePointer(&d, h, 0) != cudaSuccess) {
-        cudaGetLastError();
-        return nullptr;
-    }
-    return static_cast<int*>(d);
-}
+// Unified addressing: the word has the same address on every device.
+int* device_fail_word() { return fail_word_host(); }
 
 int check_fail_word(const char* what) {
     int* h = fail_word_host();

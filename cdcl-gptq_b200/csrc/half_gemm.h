@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -81,6 +82,20 @@ int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t sm
     g_launches.fetch_add(1, std::memory_order_relaxed);
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? 0 : cuda_error(e, what);
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once for each device; `done` is the kernel's own record.
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done, const char* what) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_error(e, what);
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return cuda_error(e, what);
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
 }
 
 // Number of SMs of the current device.

@@ -14,7 +14,8 @@ struct Maps {
 template <bool BF16, bool AMN, bool BMN, int BN, int ROWS, int EPI>
 static int launch_one(const Maps& maps, const Params& p, cudaStream_t st) {
     auto kern = half_gemm_kernel<BF16, AMN, BMN, BN, ROWS, EPI>;
-    CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes()));
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_smem(kern, smem_bytes(), done, "half_gemm_kernel shared memory")) return rc;
     const int64_t items = (int64_t)p.ntiles * p.splits;
     const int sms = sm_count();
     CDCLQ_LAUNCH(kern, (unsigned)(items < sms ? items : sms), THREADS, smem_bytes(), st, maps.a, maps.b, maps.u, maps.x, p);

@@ -36,14 +36,15 @@ Sections sections(uint64_t d_out, uint64_t d_in, uint64_t groups, uint64_t units
 
 // The units of a layer; false when the groups' widths are not 2..8.
 bool plan_units(size_t d_in, size_t g, const uint8_t* gbits, std::vector<PackedUnit>* unit, std::vector<int>* column,
-                uint64_t* units, uint64_t* tile_words, int* max_bits) {
+                uint64_t* units, uint64_t* tile_words, int* max_bits, int* min_bits) {
     const size_t ng = (d_in + g - 1) / g;
     uint64_t n = 0, words = 0;
-    int most = 0;
+    int most = 0, least = 8;
     for (size_t i = 0; i < ng;) {
         const int bits = gbits[i];
         if (bits < 2 || bits > 8) return false;
         most = std::max(most, bits);
+        least = std::min(least, bits);
         size_t steps = 0;
         for (; i < ng && gbits[i] == bits; i++) {
             const size_t c0 = i * g, width = std::min(g, d_in - c0);
@@ -69,6 +70,7 @@ bool plan_units(size_t d_in, size_t g, const uint8_t* gbits, std::vector<PackedU
     *units = n;
     *tile_words = words;
     *max_bits = most;
+    *min_bits = least;
     return true;
 }
 
@@ -186,10 +188,12 @@ __device__ __forceinline__ uint32_t pair_of(float v) {
     const uint32_t h = half_bits<BF16>(v);
     return h | h << 16;
 }
-// What minus_zero (or, for 8 bits in bf16, decode_pair) takes off for a zero point.
+// What minus_zero (or, for 8 bits in bf16, decode_pair) takes off for the zero point of a grid word: its 16 high bits are
+// the zero point, which lies in the low bits of the offset's significand.
 template <bool BF16, int BITS>
-__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
-    return pair_of<BF16>((float)z + (BF16 ? (BITS == 8 ? 0.0f : 128.0f) : 1024.0f));
+__device__ __forceinline__ uint32_t zero_pair(uint32_t scale_zero) {
+    if constexpr (BF16 && BITS == 8) return pair_of<BF16>((float)(scale_zero >> 16));
+    return __byte_perm(scale_zero | (BF16 ? 0x43000000u : 0x64000000u), 0, 0x3232);
 }
 
 // Code minus zero point, exactly, of pair p (0..3) of a k-step: rows l / 4 (even pairs) and l / 4 + 8.  For 8 bits in bf16,
@@ -239,58 +243,71 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) 
     }
 }
 
-constexpr int EXPAND_WARPS = 16;
+constexpr int EXPAND_WARPS = 8;
 
-template <bool BF16, int BITS>
+// The unit's codes of one half of the tile's rows, scaled, to the rows' columns; padding goes to column `trash`.
+template <bool BF16, int BITS, bool ALL>
 __device__ __forceinline__ void expand_unit(const PackedView& W, const PackedUnit& u, int ui, const uint32_t* __restrict__ codes,
-                                            const uint32_t* __restrict__ grid, int lane, int half, int row, bool live,
-                                            uint16_t* rows, int ld) {
+                                            const uint32_t* __restrict__ grid, int lane, int half, bool live, uint16_t* row,
+                                            uint32_t trash) {
     uint32_t w[BITS];
+    int2 c[8];
+    const int2* column = reinterpret_cast<const int2*>(W.column + ui * 64) + (lane & 3);
 #pragma unroll
     for (int i = 0; i < BITS; i++) w[i] = codes[(u.word + i) * 32 + lane];
-    const int2* column = reinterpret_cast<const int2*>(W.column + ui * 64) + (lane & 3);
-    uint32_t sz = 0, zero = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = column[i * 4];
+    const uint32_t* g = grid + half * 8 + lane / 4;
+    const bool one = u.group[0] == u.group[3];
+    uint32_t sz = g[(int64_t)u.group[0] * 16], zero = zero_pair<BF16, BITS>(sz);
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
-        if (ks == 0 || u.group[ks] != u.group[ks - 1]) {
-            sz = grid[(int64_t)u.group[ks] * 16 + half * 8 + lane / 4];
-            zero = zero_pair<BF16, BITS>(sz >> 16);
+        if (ks > 0 && !one) {
+            sz = g[(int64_t)u.group[ks] * 16];
+            zero = zero_pair<BF16, BITS>(sz);
         }
 #pragma unroll
         for (int hi = 0; hi < 2; hi++) {
-            const int2 c = column[ks * 8 + hi * 4];
-            const uint32_t v = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, hi * 2 + half, zero), sz & 0xffffu);
-            if (live) {
-                if (c.x >= 0) rows[row * ld + c.x] = (uint16_t)v;
-                if (c.y >= 0) rows[row * ld + c.y] = (uint16_t)(v >> 16);
+            const uint32_t lower = decode_pair<BF16, BITS>(w, ks, hi * 2, zero), upper = decode_pair<BF16, BITS>(w, ks, hi * 2 + 1, zero);
+            const uint32_t v = scaled_pair<BF16>(half ? upper : lower, sz & 0xffffu);
+            const int2 at = c[ks * 2 + hi];
+            if (ALL || live) {
+                row[min((uint32_t)at.x, trash)] = (uint16_t)v;
+                row[min((uint32_t)at.y, trash)] = (uint16_t)(v >> 16);
             }
         }
     }
 }
 
-// A CTA expands `R` of a tile's 16 rows (R = 8 unless the rows do not fit): warps decode unit by unit into rows in shared
-// memory, at their original columns, and the CTA writes whole rows out.  Bound by the 16-bit rows written; the scattered
-// 2-byte stores cost about two shared-memory cycles each, rows being four banks apart.
-template <bool BF16>
+// A CTA expands `R` of a tile's 16 rows (R = 8, ALL, unless the rows do not fit): warps decode unit by unit into rows in
+// shared memory, at their original columns, and the CTA writes whole rows out.  BITS: the width of every group, or 0 where
+// they differ.  Bound by the 16-bit rows written and by issuing the scattered 2-byte stores, rows being four banks apart.
+template <bool BF16, int BITS, bool ALL>
 __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, int R, int ld, uint16_t* __restrict__ out,
                                                                           int64_t ldw, int wide) {
     extern __shared__ __align__(16) uint16_t rows[];
     const int parts = 16 / R, tile = blockIdx.x / parts, first = (blockIdx.x % parts) * R;  // rows first .. first + R of the tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = first >> 3, row = lane / 4 - (first & 7);
-    const bool live = row >= 0 && row < R;
+    const int half = first >> 3, r0 = lane / 4 - (first & 7);
+    const bool live = r0 >= 0 && r0 < R;
+    uint16_t* row = rows + (live ? r0 : 0) * ld;
+    const uint32_t trash = ld - 1;
     const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
     const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
     for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
         const PackedUnit u = W.unit[ui];
-        switch (u.bits) {
-            case 2: expand_unit<BF16, 2>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            case 3: expand_unit<BF16, 3>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            case 4: expand_unit<BF16, 4>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            case 5: expand_unit<BF16, 5>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            case 6: expand_unit<BF16, 6>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            case 7: expand_unit<BF16, 7>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
-            default: expand_unit<BF16, 8>(W, u, ui, codes, grid, lane, half, row, live, rows, ld); break;
+        if constexpr (BITS) {
+            expand_unit<BF16, BITS, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash);
+        } else {
+            switch (u.bits) {
+                case 2: expand_unit<BF16, 2, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 3: expand_unit<BF16, 3, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 4: expand_unit<BF16, 4, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 5: expand_unit<BF16, 5, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 6: expand_unit<BF16, 6, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 7: expand_unit<BF16, 7, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                default: expand_unit<BF16, 8, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+            }
         }
     }
     __syncthreads();
@@ -299,11 +316,35 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
         uint16_t* dst = out + ((int64_t)tile * 16 + first + r) * ldw;
         const uint16_t* src = rows + r * ld;
         if (wide) {  // ldw is d_in rounded up to 8; what lies past d_in is written along
+#pragma unroll 4
             for (int c = threadIdx.x * 8; c < W.d_in; c += EXPAND_WARPS * 32 * 8)
                 *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
         } else {
             for (int c = threadIdx.x; c < W.d_in; c += EXPAND_WARPS * 32) dst[c] = src[c];
         }
+    }
+}
+
+template <bool BF16, int BITS>
+int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, cudaStream_t st) {
+    static std::atomic<uint64_t> done_all{0}, done_some{0};
+    auto kern = R == 8 ? packed_expand_kernel<BF16, BITS, true> : packed_expand_kernel<BF16, BITS, false>;
+    if (int rc = allow_smem(kern, 220 * 1024, R == 8 ? done_all : done_some, "packed_expand_kernel shared memory")) return rc;
+    CDCLQ_LAUNCH(kern, w.tiles * (16 / R), EXPAND_WARPS * 32, (size_t)(R * ld * 2), st, w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "packed_expand_kernel launch");
+}
+
+// The widths of configurations that quantize every group alike have a kernel of their own; the others share one that
+// branches by unit.
+template <bool BF16>
+int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, cudaStream_t st) {
+    switch (w.bits) {
+        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, st);
+        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, st);
+        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, st);
+        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, st);
+        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, st);
     }
 }
 
@@ -317,6 +358,7 @@ PackedView packed_view(const cdclq_packed_layer& w) {
     v.tiles = (v.d_out + 15) / 16;
     v.tile_words = (int)w.tile_words;
     v.max_bits = (int)w.max_bits;
+    v.bits = (int)w.bits;
     v.unit = reinterpret_cast<const PackedUnit*>(base + s.unit);
     v.column = reinterpret_cast<const int*>(base + s.column);
     v.place = reinterpret_cast<const int*>(base + s.place);
@@ -331,12 +373,8 @@ int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw,
     int R = 8;
     while (R > 1 && R * ld * 2 > 220 * 1024) R /= 2;
     if (R * ld * 2 > 220 * 1024) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
-    auto kern = bf16 ? packed_expand_kernel<true> : packed_expand_kernel<false>;
-    CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
     const int wide = ldw % 8 == 0 && ldw >= ceil_div(w.d_in, 8) * 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    CDCLQ_LAUNCH(kern, w.tiles * (16 / R), EXPAND_WARPS * 32, (size_t)(R * ld * 2), st, w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : cuda_error(e, "packed_expand_kernel launch");
+    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, st) : expand_any<false>(w, R, ld, out, ldw, wide, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -351,38 +389,54 @@ constexpr int DEC_CODES = 72 * 1024;  // codes of a CTA's rows in shared memory 
 constexpr int DEC_GRID = 16 * 1024;   // scales and zero points of its rows, where they fit
 
 // First launch: x in the tensor instruction's order (its columns gathered through the permutation, padding zero), and
-// u_t = A_i x_t, one warp for each (token, rank).
+// u_t = A_i x_t, some warps for each (token, rank).
 template <bool BF16>
 __global__ void __launch_bounds__(256) packed_tokens_kernel(const PackedView W, const uint16_t* __restrict__ x, int64_t ldx, int t,
-                                                            int token_tiles, uint2* __restrict__ xf, int frag_blocks,
+                                                            int token_tiles, uint2* __restrict__ xf, int frag_blocks, int cut,
                                                             const AdapterArgs ad, float* __restrict__ u32, uint16_t* __restrict__ u16) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if ((int)blockIdx.x >= frag_blocks) {
-        const int w = (blockIdx.x - frag_blocks) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-        if (w >= t * ad.r) return;
-        const int tok = w / ad.r, r = w - tok * ad.r, id = ad.index[tok];
+        // `cut` warps (a power of two) to a product, each with 2048 neighbouring columns at a time
+        __shared__ float part[8];
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int w = (blockIdx.x - frag_blocks) * (8 / cut) + warp / cut;
+        const int tok = w / ad.r, r = w - tok * ad.r, id = w < t * ad.r ? ad.index[tok] : -1;
         float s = 0.0f;
         if (id >= 0 && id < ad.n) {
             const uint16_t* a = static_cast<const uint16_t*>(ad.a) + ((int64_t)id * ad.r + r) * ad.lda;
             const uint16_t* xr = x + tok * ldx;
             float p[8] = {};
-            int c = lane * 8;
-#pragma unroll 4
-            for (; c + 8 <= W.d_in; c += 256) {
-                const uint4 av = *reinterpret_cast<const uint4*>(a + c), xv = *reinterpret_cast<const uint4*>(xr + c);
-                const uint32_t aw[4] = {av.x, av.y, av.z, av.w}, xw[4] = {xv.x, xv.y, xv.z, xv.w};
+            for (int c0 = (warp & (cut - 1)) * 2048; c0 < W.d_in; c0 += cut * 2048) {
+                uint4 av[8], xv[8];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    p[2 * q] = fmaf(half_value<BF16>((uint16_t)aw[q]), half_value<BF16>((uint16_t)xw[q]), p[2 * q]);
-                    p[2 * q + 1] = fmaf(half_value<BF16>((uint16_t)(aw[q] >> 16)), half_value<BF16>((uint16_t)(xw[q] >> 16)), p[2 * q + 1]);
+                for (int k = 0; k < 8; k++) {
+                    const int c = c0 + k * 256 + lane * 8;
+                    av[k] = xv[k] = make_uint4(0, 0, 0, 0);
+                    if (c + 8 <= W.d_in) {
+                        av[k] = *reinterpret_cast<const uint4*>(a + c);
+                        xv[k] = *reinterpret_cast<const uint4*>(xr + c);
+                    } else {
+                        for (int q = c; q < W.d_in; q++) p[0] = fmaf(half_value<BF16>(a[q]), half_value<BF16>(xr[q]), p[0]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t aw[4] = {av[k].x, av[k].y, av[k].z, av[k].w}, xw[4] = {xv[k].x, xv[k].y, xv[k].z, xv[k].w};
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        p[2 * q] = fmaf(half_value<BF16>((uint16_t)aw[q]), half_value<BF16>((uint16_t)xw[q]), p[2 * q]);
+                        p[2 * q + 1] = fmaf(half_value<BF16>((uint16_t)(aw[q] >> 16)), half_value<BF16>((uint16_t)(xw[q] >> 16)), p[2 * q + 1]);
+                    }
                 }
             }
-            for (; c < W.d_in; c++) p[0] = fmaf(half_value<BF16>(a[c]), half_value<BF16>(xr[c]), p[0]);  // one lane's last columns
             s = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
             for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         }
-        if (lane == 0) {
+        if (lane == 0) part[warp] = s;
+        __syncthreads();
+        if (lane == 0 && (warp & (cut - 1)) == 0 && w < t * ad.r) {
+            for (int k = 1; k < cut; k++) s += part[warp + k];
             u32[w] = s;
             if (u16) u16[w] = half_bits<BF16>(s);
         }
@@ -414,45 +468,53 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // One unit of RT row tiles times NT token tiles.  codes, grid: the first tile's (shared memory, or for grid global);
 // `tile_codes` and `tile_grid` words to the next tile.
 template <bool BF16, int BITS, int NT, int RT>
-__device__ __forceinline__ void decode_unit(const uint16_t (&group)[4], const uint32_t* codes, int tile_codes, const uint32_t* grid,
+__device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t* codes, int tile_codes, const uint32_t* grid,
                                             int tile_grid, const uint2* __restrict__ xf, int lane, float (&acc)[RT][NT][4]) {
     uint2 x[4][NT];
 #pragma unroll
     for (int ks = 0; ks < 4; ks++)
 #pragma unroll
         for (int n = 0; n < NT; n++) x[ks][n] = xf[(ks * NT + n) * 32 + lane];
+    const bool one = u.group[0] == u.group[3];  // one column group: its four k-steps share a scale
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         uint32_t w[BITS];
 #pragma unroll
         for (int i = 0; i < BITS; i++) w[i] = codes[rt * tile_codes + i * 32 + lane];
-        float part[NT][4], scale[2] = {};
-        uint32_t zero[2] = {};
+        const uint32_t* g = grid + rt * tile_grid + lane / 4;
+        if (one) {
+            const uint32_t s0 = g[u.group[0] * 16], s1 = g[u.group[0] * 16 + 8];
+            const uint32_t zero[2] = {zero_pair<BF16, BITS>(s0), zero_pair<BF16, BITS>(s1)};
+            float part[NT][4] = {};
 #pragma unroll
-        for (int ks = 0; ks < 4; ks++) {
-            if (ks == 0 || group[ks] != group[ks - 1]) {
-                const uint32_t* g = grid + rt * tile_grid + group[ks] * 16 + lane / 4;
+            for (int ks = 0; ks < 4; ks++) {
+                uint32_t a[4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t sz = g[h * 8];
-                    scale[h] = __half2float(__ushort_as_half((uint16_t)sz));
-                    zero[h] = zero_pair<BF16, BITS>(sz >> 16);
-                }
+                for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) part[n][i] = 0.0f;
+                for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
             }
-            uint32_t a[4];
+            const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
 #pragma unroll
-            for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
-            if (ks == 3 || group[ks + 1] != group[ks]) {
+                for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(i < 2 ? f0 : f1, part[n][i], acc[rt][n][i]);
+        } else {
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+            for (int ks = 0; ks < 4; ks++) {
+                const uint32_t s0 = g[u.group[ks] * 16], s1 = g[u.group[ks] * 16 + 8];
+                const uint32_t zero[2] = {zero_pair<BF16, BITS>(s0), zero_pair<BF16, BITS>(s1)};
+                const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
+                uint32_t a[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(scale[i >> 1], part[n][i], acc[rt][n][i]);
+                for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float part[4] = {};
+                    mma16816<BF16>(part, a, x[ks][n]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(i < 2 ? f0 : f1, part[i], acc[rt][n][i]);
+                }
             }
         }
     }
@@ -473,7 +535,7 @@ struct DecodeArgs {
 // memory before the first launch has finished (they do not depend on it).  The scale of a (row, group) multiplies the
 // group's f32 sum, so the codes minus their zero points enter the tensor instruction exactly and no weight is rounded.
 // Bound by the codes' bytes; mma.sync because 16 rows and a few tokens leave most of tcgen05's 128 rows empty.
-template <bool BF16, int NT, int RT>
+template <bool BF16, int BITS, int NT, int RT>
 __global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const PackedView W, const AdapterArgs ad, const DecodeArgs P) {
     extern __shared__ __align__(128) uint32_t stage[];
     __shared__ float sums[DEC_WARPS][RT * 16][NT * 8 + 1];
@@ -522,14 +584,18 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const Pac
             const uint2* xu = P.xf + (int64_t)ui * 4 * NT * 32;
             const uint32_t* c = stage + (u.word - w0) * 32;
             const int tg = W.groups * 16;
-            switch (u.bits) {
-                case 2: decode_unit<BF16, 2, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                case 3: decode_unit<BF16, 3, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                case 4: decode_unit<BF16, 4, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                case 5: decode_unit<BF16, 5, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                case 6: decode_unit<BF16, 6, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                case 7: decode_unit<BF16, 7, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
-                default: decode_unit<BF16, 8, NT, RT>(u.group, c, tile_codes, g, tg, xu, lane, acc); break;
+            if constexpr (BITS) {
+                decode_unit<BF16, BITS, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc);
+            } else {
+                switch (u.bits) {
+                    case 2: decode_unit<BF16, 2, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    case 3: decode_unit<BF16, 3, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    case 4: decode_unit<BF16, 4, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    case 5: decode_unit<BF16, 5, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    case 6: decode_unit<BF16, 6, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    case 7: decode_unit<BF16, 7, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                    default: decode_unit<BF16, 8, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+                }
             }
         }
     }
@@ -572,15 +638,25 @@ __global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const Pac
     }
 }
 
-template <bool BF16, int NT, int RT>
+template <bool BF16, int BITS, int NT, int RT>
 int decode_rows(const PackedView& w, const AdapterArgs& ad, DecodeArgs p, cudaStream_t st) {
     const int unit_bytes = RT * w.max_bits * 128;
     p.chunk_units = std::max(1, std::min(w.units, DEC_CODES / unit_bytes));
     p.grid_staged = RT * w.groups * 64 <= DEC_GRID;
     const size_t smem = (size_t)p.chunk_units * unit_bytes + (p.grid_staged ? (size_t)RT * w.groups * 64 : 0);
-    auto kern = packed_decode_kernel<BF16, NT, RT>;
-    CDCLQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DEC_CODES + DEC_GRID));
+    auto kern = packed_decode_kernel<BF16, BITS, NT, RT>;
+    static std::atomic<uint64_t> done{0};
+    if (int rc = allow_smem(kern, DEC_CODES + DEC_GRID, done, "packed_decode_kernel shared memory")) return rc;
     return launch_dependent(kern, dim3((unsigned)ceil_div(w.tiles, RT)), dim3(DEC_WARPS * 32), smem, st, "packed_decode_kernel launch", w, ad, p);
+}
+
+template <bool BF16, int BITS>
+int decode_width(const PackedView& w, const AdapterArgs& ad, const DecodeArgs& p, int nt, cudaStream_t st) {
+    // two row tiles to a CTA halve the tokens' bytes that it reads through L2, where that still leaves two CTAs to an SM
+    const bool two = w.tiles >= 4 * sm_count();
+    if (nt == 1) return two ? decode_rows<BF16, BITS, 1, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 1, 1>(w, ad, p, st);
+    if (nt == 2) return two ? decode_rows<BF16, BITS, 2, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 2, 1>(w, ad, p, st);
+    return two ? decode_rows<BF16, BITS, 4, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 4, 1>(w, ad, p, st);
 }
 
 int token_tiles(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
@@ -600,16 +676,20 @@ int decode(const PackedView& w, const void* x, int64_t ldx, int t, const Adapter
     p.fail = device_fail_word();
     if (!p.fail) return set_error(CDCLQ_ERR_CUDA, "projection_forward: no mapped host memory (is there a CUDA device?)");
     const int frag_blocks = (int)ceil_div((int64_t)w.units * 4 * nt * 32, 256);
-    const int dot_blocks = ad.n > 0 ? (int)ceil_div((int64_t)t * ad.r, 8) : 0;
+    int cut = 1;
+    while (cut < 8 && cut * 2048 < w.d_in) cut *= 2;
+    const int dot_blocks = ad.n > 0 ? (int)ceil_div((int64_t)t * ad.r * cut, 8) : 0;
     CDCLQ_LAUNCH((packed_tokens_kernel<BF16>), frag_blocks + dot_blocks, 256, 0, st, w, static_cast<const uint16_t*>(x), ldx, t, nt, xf,
-                 frag_blocks, ad, u32, static_cast<uint16_t*>(u));
+                 frag_blocks, cut, ad, u32, static_cast<uint16_t*>(u));
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_error(e, "packed_tokens_kernel launch");
-    // two row tiles to a CTA halve the tokens' bytes that it reads through L2, where that still leaves two CTAs to an SM
-    const bool two = w.tiles >= 4 * sm_count();
-    if (nt == 1) return two ? decode_rows<BF16, 1, 2>(w, ad, p, st) : decode_rows<BF16, 1, 1>(w, ad, p, st);
-    if (nt == 2) return two ? decode_rows<BF16, 2, 2>(w, ad, p, st) : decode_rows<BF16, 2, 1>(w, ad, p, st);
-    return two ? decode_rows<BF16, 4, 2>(w, ad, p, st) : decode_rows<BF16, 4, 1>(w, ad, p, st);
+    switch (w.bits) {
+        case 2: return decode_width<BF16, 2>(w, ad, p, nt, st);
+        case 3: return decode_width<BF16, 3>(w, ad, p, nt, st);
+        case 4: return decode_width<BF16, 4>(w, ad, p, nt, st);
+        case 8: return decode_width<BF16, 8>(w, ad, p, nt, st);
+        default: return decode_width<BF16, 0>(w, ad, p, nt, st);
+    }
 }
 
 }  // namespace
@@ -635,11 +715,12 @@ static int plan_layer(size_t d_out, size_t d_in, size_t group, const uint8_t* gb
     const size_t g = group < d_in ? group : d_in;
     if ((d_in + g - 1) / g > 65535) return set_error(CDCLQ_ERR_ARG, "packed layer: more than 65535 column groups");
     uint64_t units = 0, words = 0;
-    int most = 0;
-    if (!plan_units(d_in, g, gbits, unit, column, &units, &words, &most))
+    int most = 0, least = 0;
+    if (!plan_units(d_in, g, gbits, unit, column, &units, &words, &most, &least))
         return set_error(CDCLQ_ERR_CONFIG, "packed layer: group widths must be in 2..=8 bits");
     w->d_out = d_out, w->d_in = d_in, w->group = g, w->groups = (d_in + g - 1) / g;
     w->units = units, w->tile_words = words, w->max_bits = (uint32_t)most;
+    w->bits = most == least ? (uint32_t)most : 0;
     return 0;
 }
 

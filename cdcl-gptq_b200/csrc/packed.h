@@ -26,6 +26,7 @@ struct PackedView {
     int d_out, d_in, groups, units, tiles;
     int tile_words;            // words of a row tile, in units of 32 lanes
     int max_bits;
+    int bits;                  // the width of every group, 0 where they differ
     const PackedUnit* unit;    // [units]
     const int* column;         // [64 * units]: original column of a padded place, -1 for padding
     const int* place;          // [d_in]: padded place of an original column

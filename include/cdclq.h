@@ -408,7 +408,7 @@ int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, int dtype, 
 typedef struct cdclq_packed_layer {
     uint64_t d_out, d_in, group, groups;
     uint64_t units, tile_words;
-    uint32_t max_bits, reserved;
+    uint32_t max_bits, bits;
     void* layout; /* device buffer of cdclq_packed_layer_bytes, the caller's */
 } cdclq_packed_layer;
 
