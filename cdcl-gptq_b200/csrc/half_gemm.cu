@@ -92,27 +92,27 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
     const bool store = form != HALF_STATS && form != HALF_GRAD;
     const bool grouped = form == HALF_NT_GROUPED || form == HALF_NN_GROUPED;
-    const int64_t sms = sm_count(), tm = ceil_div(m, BM), nkb = ceil_div(k, KB);
-    HalfPlan p{256, 1, 0};
-    if (grouped) {
-        p.bn = 64;
-    } else {
-        // The least time of all waves, a wave costing its tile's columns and 32 for its start and end: 256 columns
-        // where they fill the SMs (a wider tile reads less through L2 for each product), narrower ones below that.
+    const int64_t sms = sm_count(), nkb = ceil_div(k, KB);
+    HalfPlan p{1, 64, 1, 0};
+    if (!grouped) {
+        // The least time of all waves: a wave costs its tile's columns, more for what a smaller tile reads through L2, and 16
+        // columns' time for its start and end.
+        static const struct { int cg, bn, cost; } tiles[] = {{2, 256, 256 + 16}, {2, 128, 152 + 16}, {1, 128, 176 + 16}, {1, 64, 110 + 16}};
         int64_t best = INT64_MAX;
-        for (int bn : {256, 128, 64}) {
-            if (bn == 64 && !store) break;
-            const int64_t cost = ceil_div(tm * ceil_div(n, bn), sms) * (bn + 32);
+        for (const auto& c : tiles) {
+            if (c.bn == 64 && !store) break;
+            const int64_t cost = ceil_div(ceil_div(m, c.cg * BM) * ceil_div(n, c.bn), sms / c.cg) * c.cost;
             if (cost < best) {
                 best = cost;
-                p.bn = bn;
+                p.cg = c.cg;
+                p.bn = c.bn;
             }
         }
     }
-    const int64_t tiles = tm * ceil_div(n, p.bn);
-    if (store && tiles * 2 <= sms && nkb >= 16) {
+    const int64_t tiles = ceil_div(m, p.cg * BM) * ceil_div(n, p.bn), slots = sms / p.cg;
+    if (store && tiles * 2 <= slots && nkb >= 16) {
         // too few tiles for the SMs: the K blocks of a tile over several items, eight blocks at least for each
-        p.splits = (int)std::min(sms / tiles, nkb / 8);
+        p.splits = (int)std::min(slots / tiles, nkb / 8);
         const int64_t per = ceil_div(nkb, p.splits);
         p.splits = (int)ceil_div(nkb, per);
     }
@@ -162,14 +162,14 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     Maps maps{};
     int rc;
     if ((rc = encode(&maps.a, g.a, g.bf16, false, a_mn ? KB : BM))) return rc;
-    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : plan.bn))) return rc;
+    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : plan.bn / plan.cg))) return rc;
     if (extend && (rc = encode(&maps.u, g.u, g.bf16, false, BM))) return rc;
-    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : plan.bn))) return rc;
+    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : plan.bn / plan.cg))) return rc;
     Params p{};
     p.m = (int)g.m;
     p.n = (int)g.n;
     p.nkb = (int)ceil_div(g.k, KB);
-    p.tiles_m = (int)ceil_div(g.m, BM);
+    p.tiles_m = (int)ceil_div(g.m, plan.cg * BM);
     p.tiles_n = (int)ceil_div(g.n, plan.bn);
     if ((int64_t)p.tiles_m * p.tiles_n * plan.splits > 0x7fffffff) return set_error(CDCLQ_ERR_ARG, "half product: too many tiles");
     p.ntiles = p.tiles_m * p.tiles_n;
@@ -201,7 +201,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
         p.ldf = g.ldf;
         p.alpha = g.alpha;
     }
-    rc = g.bf16 ? launch_form<true>(g.form, plan.bn, maps, p, st) : launch_form<false>(g.form, plan.bn, maps, p, st);
+    rc = g.bf16 ? launch_form<true>(g.form, plan.cg, plan.bn, maps, p, st) : launch_form<false>(g.form, plan.cg, plan.bn, maps, p, st);
     if (rc || plan.splits == 1 || grouped) return rc;
     const int64_t groups = ceil_div(g.m * p.ldf, 4 * 256);
     const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 8);

@@ -4,7 +4,10 @@
 //
 // One persistent kernel, specialised at compile time on
 //   AMN, BMN   whether an operand is contiguous along its rows' index (MN-major) or along k (K-major)
-//   BN         tile columns (128 rows x BN columns): 256 where that fills the SMs, else 128 or 64
+//   CG, BN     a tile is 128 CG rows x BN columns.  CG = 2: a pair of CTAs shares it, each with half of A's and half of
+//              B's rows in its shared memory and half of D's rows in its tensor memory, so that a product of 256 x 256
+//              reads 64 bytes a clock and SM through L2 (96 with CG = 1 and 128 x 256).  CG = 1, narrow, where there are
+//              few tiles
 //   ROWS       what the adapters of the rows do (see RowMode)
 //   EPI        what becomes of a finished tile (see Epilogue)
 // TMA brings 64-deep K blocks into a ring of 128-byte-swizzled stages, one thread issues the MMAs, and eight warps
@@ -19,7 +22,7 @@ namespace hg {
 
 using namespace tc;
 
-constexpr int BM = 128;            // tile rows = tensor-memory lanes
+constexpr int BM = 128;            // tile rows of a CTA = tensor-memory lanes
 constexpr int KB = 64;             // K block: 128 bytes of a 16-bit type
 constexpr int EPI_WARPS = 8;       // two per lane quadrant, each with half of the tile's columns
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
@@ -28,9 +31,16 @@ constexpr int STAGE_WORDS = 32 * 33;  // one epilogue warp's transposition buffe
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int BAND = 16;           // row blocks per band of the tile order: a wave's operands stay in L2
 
-__host__ __device__ constexpr int b_bytes(int bn) { return bn * KB * 2; }
-__host__ __device__ constexpr int stages(int bn) { return RING_BYTES / (A_BYTES + b_bytes(bn)); }
-__host__ __device__ constexpr size_t smem_bytes() { return RING_BYTES + EPI_WARPS * STAGE_WORDS * 4 + 1024 /* alignment */ + 256 /* barriers */; }
+// Each sum of at most this many K blocks leaves tensor memory and is added up in registers (EPI_STATS): the tensor core
+// cuts its f32 sums off instead of rounding them, which over 4096 products moved a loss of 10 by 1e-5; 1024 at a time
+// keep it within a few 1e-6.
+constexpr int STATS_KB = 16;
+
+__host__ __device__ constexpr int b_bytes(int cg, int bn) { return bn / cg * KB * 2; }
+__host__ __device__ constexpr int stages(int cg, int bn) { return RING_BYTES / (A_BYTES + b_bytes(cg, bn)); }
+__host__ __device__ constexpr size_t smem_bytes() {
+    return RING_BYTES + EPI_WARPS * STAGE_WORDS * 4 + 1024 /* alignment */ + 256 /* barriers */;
+}
 
 // How the adapter of each row (index[m]; none if outside [0, adapters)) takes part.
 enum RowMode {
@@ -102,23 +112,27 @@ __device__ __forceinline__ void item_coords(const Params& P, int item, int& mb, 
     mb = band * BAND + t - nb * rows;
 }
 
-// The adapters of a tile's 128 rows, lowest first; a warp holds four rows in each lane.
+// The adapters of a tile's 128 CG rows, lowest first; a warp holds 4 CG rows in each lane.
+template <int CG>
 struct RowAdapters {
     static constexpr int NONE = 0x7fffffff;
-    int id[4];
+    int id[4 * CG];
     __device__ __forceinline__ void load(const Params& P, int m0, int lane) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
+        for (int q = 0; q < 4 * CG; q++) {
             const int row = m0 + 32 * q + lane;
             const int v = (row < P.m && P.adapters > 0) ? P.index[row] : -1;
             id[q] = (v >= 0 && v < P.adapters) ? v : NONE;
         }
     }
     // the next adapter and the lanes that are not its rows; NONE after the last
-    __device__ __forceinline__ int next(uint32_t (&off)[4]) {
-        const int cur = __reduce_min_sync(0xffffffffu, min(min(id[0], id[1]), min(id[2], id[3])));
+    __device__ __forceinline__ int next(uint32_t (&off)[4 * CG]) {
+        int least = id[0];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
+        for (int q = 1; q < 4 * CG; q++) least = min(least, id[q]);
+        const int cur = __reduce_min_sync(0xffffffffu, least);
+#pragma unroll
+        for (int q = 0; q < 4 * CG; q++) {
             const bool mine = id[q] == cur;
             off[q] = ~__ballot_sync(0xffffffffu, mine);
             if (mine) id[q] = NONE;
@@ -127,24 +141,25 @@ struct RowAdapters {
     }
 };
 
-template <bool BF16, bool AMN, bool BMN, int BN, int ROWS, int EPI>
+template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_x, const Params P) {
-    constexpr int NS = stages(BN);
-    constexpr int B_BYTES = b_bytes(BN);
-    constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    constexpr int NS = stages(CG, BN);
+    constexpr int STAGE_BYTES = A_BYTES + b_bytes(CG, BN);
+    constexpr int BC = BN / CG;  // B's rows in this CTA
     constexpr uint32_t TMEM_COLS = 2 * BN;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* turn = reinterpret_cast<float*>(base + RING_BYTES);
-    uint64_t* full = reinterpret_cast<uint64_t*>(turn + EPI_WARPS * STAGE_WORDS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + EPI_WARPS * STAGE_WORDS);  // of the pair's first CTA
     uint64_t* empty = full + NS;
     uint64_t* accf = empty + NS;
-    uint64_t* acce = accf + 2;
+    uint64_t* acce = accf + 2;  // of the pair's first CTA
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
     int* flag = reinterpret_cast<int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 2 ? (int)cluster_rank() : 0;
 
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
@@ -153,61 +168,76 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], EPI_WARPS * 32);
+            mbar_init(&acce[b], CG * EPI_WARPS);
         }
         *flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == EPI_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
+    if (warp == EPI_WARPS + 1) tmem_alloc<CG>(tmem_slot, TMEM_COLS);
     fence_before();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int items = P.ntiles * P.splits;
+    const int step = gridDim.x / CG, first = blockIdx.x / CG;
     const uint32_t ring = smem_u32(base);
 
     if (warp == EPI_WARPS) {
         // ---------------- TMA producer: the whole warp walks the items, lane 0 waits and issues
         int ctr = 0;
         bool ok = true;
-        // waits for the next stage and announces its bytes; returns its address (0 when a wait ran out)
-        auto stage = [&](uint64_t*& bar) -> uint32_t {
+        // waits for the next stage and, in the first CTA, announces the pair's bytes; returns its address
+        auto stage = [&](uint32_t& bar) -> uint32_t {
             const int s = ctr % NS;
             if (ctr >= NS && !mbar_wait(&empty[s], ((ctr / NS) - 1) & 1, flag)) {
                 ok = false;
                 return 0;
             }
-            bar = &full[s];
-            mbar_expect_tx(bar, STAGE_BYTES);
+            bar = smem_u32(&full[s]);
+            if constexpr (CG == 2) bar = first_cta(bar);
+            if (rank == 0) mbar_expect_tx(&full[s], CG * STAGE_BYTES);
             ctr++;
             return ring + s * STAGE_BYTES;
         };
-        auto load_a = [&](uint32_t dst, int m0, int kb, uint64_t* bar) {
+        auto load2 = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+            if constexpr (CG == 2)
+                tma_load_2d_pair(dst, map, x, y, bar);
+            else
+                tma_load_2d(dst, map, x, y, bar);
+        };
+        auto load3 = [&](uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+            if constexpr (CG == 2)
+                tma_load_3d_pair(dst, map, x, y, z, bar);
+            else
+                tma_load_3d(dst, map, x, y, z, bar);
+        };
+        auto load_a = [&](uint32_t dst, int m0, int kb, uint32_t bar) {
             if constexpr (AMN) {
 #pragma unroll
-                for (int h = 0; h < BM / 64; h++) tma_load_2d(dst + h * (64 * KB * 2), &map_a, m0 + 64 * h, kb * KB, bar);
+                for (int h = 0; h < BM / 64; h++) load2(dst + h * (64 * KB * 2), &map_a, m0 + 64 * h, kb * KB, bar);
             } else {
-                tma_load_2d(dst, &map_a, kb * KB, m0, bar);
+                load2(dst, &map_a, kb * KB, m0, bar);
             }
         };
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        for (int item = first; item < items && ok; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
-            const int m0 = mb * BM, n0 = nb * BN;
+            const int m0 = (mb * CG + rank) * BM, n0 = nb * BN + rank * BC;
             const int kb0 = split * P.kb_per_split, kb1 = min(P.nkb, kb0 + P.kb_per_split);
             if constexpr (ROWS != ROWS_GROUPED) {
                 if (lane == 0) {
                     for (int kb = kb0; kb < kb1; kb++) {
-                        uint64_t* bar;
+                        uint32_t bar;
                         const uint32_t st = stage(bar);
                         if (!ok) break;
                         load_a(st, m0, kb, bar);
                         if constexpr (BMN) {
 #pragma unroll
-                            for (int h = 0; h < BN / 64; h++)
-                                tma_load_2d(st + A_BYTES + h * (64 * KB * 2), &map_b, n0 + 64 * h, kb * KB, bar);
+                            for (int h = 0; h < BC / 64; h++)
+                                load2(st + A_BYTES + h * (64 * KB * 2), &map_b, n0 + 64 * h, kb * KB, bar);
                         } else {
-                            tma_load_2d(st + A_BYTES, &map_b, kb * KB, n0, bar);
+                            load2(st + A_BYTES, &map_b, kb * KB, n0, bar);
                         }
                     }
                 }
@@ -215,27 +245,27 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             if constexpr (ROWS != ROWS_PLAIN) {
                 if (ROWS == ROWS_EXTEND && split != P.splits - 1) continue;  // the last split extends
-                RowAdapters who;
-                who.load(P, m0, lane);
-                uint32_t off[4];
-                for (int j = who.next(off); j != RowAdapters::NONE && ok; j = who.next(off)) {
+                RowAdapters<CG> who;
+                who.load(P, mb * CG * BM, lane);
+                uint32_t off[4 * CG];
+                for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
                     if (lane == 0) {
                         const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                         const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
                         for (int kb = e0; kb < e1; kb++) {
-                            uint64_t* bar;
+                            uint32_t bar;
                             const uint32_t st = stage(bar);
                             if (!ok) break;
                             if constexpr (ROWS == ROWS_GROUPED)
                                 load_a(st, m0, kb, bar);
                             else
-                                tma_load_2d(st, &map_u, kb * KB, m0, bar);
+                                load2(st, &map_u, kb * KB, m0, bar);
                             if constexpr (BMN) {
 #pragma unroll
-                                for (int h = 0; h < BN / 64; h++)
-                                    tma_load_3d(st + A_BYTES + h * (64 * KB * 2), &map_x, n0 + 64 * h, kb * KB, j, bar);
+                                for (int h = 0; h < BC / 64; h++)
+                                    load3(st + A_BYTES + h * (64 * KB * 2), &map_x, n0 + 64 * h, kb * KB, j, bar);
                             } else {
-                                tma_load_3d(st + A_BYTES, &map_x, kb * KB, n0, j, bar);
+                                load3(st + A_BYTES, &map_x, kb * KB, n0, j, bar);
                             }
                         }
                     }
@@ -243,15 +273,17 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
             }
         }
-        // copies still in flight land before the CTA leaves (bounded)
+        // the last stages have been read before the pair leaves, so nothing is on its way to either CTA; where the MMA
+        // issuer gave up, the copies in flight land (bounded)
         if (lane == 0)
-            for (int k = (ctr > NS ? ctr - NS : 0); k < ctr; k++) mbar_wait(&full[k % NS], (k / NS) & 1, flag);
+            for (int k = (ctr > NS ? ctr - NS : 0); k < ctr; k++)
+                if (!mbar_wait(&empty[k % NS], (k / NS) & 1, flag) && rank == 0) mbar_wait(&full[k % NS], (k / NS) & 1, flag);
     } else if (warp == EPI_WARPS + 1) {
-        // ---------------- MMA issuer
+        // ---------------- MMA issuer, of the pair's first CTA
         int ctr = 0, acc = 0;
-        bool ok = true;
+        bool ok = rank == 0;
         // the MMAs of one stage: `ks` steps of 16; A is MN-major only where `amn`
-        auto multiply = [&](uint32_t d, bool amn, int ks, bool fresh, const uint32_t (&off)[4], bool rows) {
+        auto multiply = [&](uint32_t d, bool amn, int ks, bool fresh, const uint32_t (&off)[4 * CG], bool rows) {
             const int s = ctr % NS;
             if (!mbar_wait(&full[s], (ctr / NS) & 1, flag)) {
                 ok = false;
@@ -264,27 +296,43 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (k < ks) {
                     const uint64_t da = amn ? smem_desc(sa + k * 2048, 64 * KB * 2, 1024) : smem_desc(sa + k * 32, 16, 1024);
                     const uint64_t db = BMN ? smem_desc(sb + k * 2048, 64 * KB * 2, 1024) : smem_desc(sb + k * 32, 16, 1024);
-                    const uint32_t id = idesc_half(BF16, amn, BMN, BM, BN);
+                    const uint32_t id = idesc_half(BF16, amn, BMN, CG * BM, BN);
                     if (rows)
                         mma_half_rows(d, da, db, id, (fresh && k == 0) ? 0u : 1u, off);
                     else
-                        mma_half(d, da, db, id, (fresh && k == 0) ? 0u : 1u);
+                        mma_half<CG>(d, da, db, id, (fresh && k == 0) ? 0u : 1u);
                 }
             }
-            mma_commit(&empty[s]);  // the stage is free once these MMAs have read it
+            mma_commit<CG>(&empty[s]);  // the stage is free once these MMAs have read it
             ctr++;
         };
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        // accumulator `acc & 1`, once its last contents have been read
+        auto accumulator = [&]() -> uint32_t {
+            if (lane == 0 && acc >= 2 && !mbar_wait(&acce[acc & 1], ((acc / 2) - 1) & 1, flag)) ok = false;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            fence_after();
+            return tmem_base + (uint32_t)((acc & 1) * BN);
+        };
+        for (int item = first; item < items && ok; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
             const int kb0 = split * P.kb_per_split, kb1 = min(P.nkb, kb0 + P.kb_per_split);
-            const int b = acc & 1;
-            const uint32_t d = tmem_base + (uint32_t)(b * BN);
-            if (lane == 0 && acc >= 2 && !mbar_wait(&acce[b], ((acc / 2) - 1) & 1, flag)) ok = false;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            uint32_t off[4 * CG] = {};
+            if constexpr (EPI == EPI_STATS) {
+                for (int c0 = kb0; c0 < kb1 && ok; c0 += STATS_KB) {
+                    const uint32_t d = accumulator();
+                    if (!ok) break;
+                    if (lane == 0) {
+                        for (int kb = c0; kb < min(kb1, c0 + STATS_KB) && ok; kb++) multiply(d, AMN, KB / 16, kb == c0, off, false);
+                        mma_commit<CG>(&accf[acc & 1]);
+                    }
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    acc++;
+                }
+                continue;
+            }
+            const uint32_t d = accumulator();
             if (!ok) break;
-            fence_after();
-            uint32_t off[4] = {0, 0, 0, 0};
             if constexpr (ROWS != ROWS_GROUPED) {
                 if (lane == 0)
                     for (int kb = kb0; kb < kb1 && ok; kb++) multiply(d, AMN, KB / 16, kb == kb0, off, false);
@@ -292,9 +340,9 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             if constexpr (ROWS != ROWS_PLAIN) {
                 if (ROWS == ROWS_GROUPED || split == P.splits - 1) {
-                    RowAdapters who;
-                    who.load(P, mb * BM, lane);
-                    for (int j = who.next(off); j != RowAdapters::NONE && ok; j = who.next(off)) {
+                    RowAdapters<CG> who;
+                    who.load(P, mb * CG * BM, lane);
+                    for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
                         if (lane == 0) {
                             const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                             const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
@@ -309,7 +357,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 }
             }
-            if (lane == 0) mma_commit(&accf[b]);  // accumulator b is complete (or tracks what was issued)
+            if (lane == 0) mma_commit<CG>(&accf[acc & 1]);  // the accumulator is complete (or tracks what was issued)
             acc++;
         }
         // every issued MMA has completed before the tensor memory is released (bounded)
@@ -319,13 +367,84 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int quad = warp & 3, half = warp >> 2;
         float* buf = turn + warp * STAGE_WORDS;
         int acc = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x, acc++) {
+        // the accumulator has been read: tell the MMA issuer
+        auto release = [&](int b) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2)
+                    mbar_arrive_cluster(first_cta(smem_u32(&acce[b])));
+                else
+                    mbar_arrive(&acce[b]);
+            }
+        };
+        for (int item = first; item < items; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
-            const int b = acc & 1, row0 = mb * BM + quad * 32, row = row0 + lane;
+            const int row0 = (mb * CG + rank) * BM + quad * 32, row = row0 + lane;
             const bool live = row < P.m;
+            if constexpr (EPI == EPI_STATS) {
+                const int64_t t = live ? P.target[row] : -1;
+                const int64_t label = (t >= 0 && t < P.vocab) ? t - P.col0 : -1;  // relative to this piece's column 0
+                const int chunks = (P.nkb + STATS_KB - 1) / STATS_KB;
+                float z[BN / 64][32];
+                bool ok = true;
+                for (int c = 0; c < chunks; c++, acc++) {
+                    if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
+                        ok = false;
+                        break;
+                    }
+                    fence_after();
+#pragma unroll
+                    for (int q = 0; q < BN / 64; q++) {
+                        float v[32];
+                        tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)((acc & 1) * BN + half * (BN / 2) + q * 32), v);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) z[q][i] = c ? z[q][i] + v[i] : v[i];
+                    }
+                    release(acc & 1);
+                }
+                if (!ok) break;
+                const int c0 = nb * BN + half * (BN / 2), cols = min(BN / 2, P.n - c0);
+                float top = -INFINITY, sum = 0.0f;
+                if (cols == BN / 2) {
+#pragma unroll
+                    for (int q = 0; q < BN / 64; q++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) top = fmaxf(top, z[q][i]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < BN / 64; q++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            if (q * 32 + i >= cols) z[q][i] = -INFINITY;
+                            top = fmaxf(top, z[q][i]);
+                        }
+                }
+                // exp2((z - top) log2 e); a row of -inf alone keeps sum 0
+                constexpr float L2E = 1.4426950408889634f;
+                const float ref = top == -INFINITY ? 0.0f : top;
+                const int64_t at = label - c0;
+#pragma unroll
+                for (int q = 0; q < BN / 64; q++) {
+                    if (at >= q * 32 && at < q * 32 + 32) {
+                        float mine = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (q * 32 + i == at) mine = z[q][i];
+                        if (at < cols) P.label_logit[row] = mine;
+                    }
+                    float part = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) part += exp2f((z[q][i] - ref) * L2E);
+                    sum += part;
+                }
+                if (live) P.stats[(int64_t)(nb * 2 + half) * P.m + row] = make_float2(top, sum);
+                continue;
+            }
+            const int b = acc & 1;
             // what the row's epilogue needs, read while the MMAs run
-            float factor = 1.0f, lse = 0.0f, dl = 0.0f, top = -INFINITY, sum = 0.0f;
+            float factor = 1.0f, lse = 0.0f, dl = 0.0f;
             int64_t label = -1;  // relative to this piece's column 0
             bool none = false;
             if constexpr (EPI == EPI_STORE) {
@@ -336,19 +455,17 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (P.alpha) factor = *P.alpha;
             } else {
                 const int64_t t = live ? P.target[row] : -1;
-                const bool labelled = t >= 0 && t < P.vocab;
-                label = labelled ? t - P.col0 : -1;
-                if constexpr (EPI == EPI_GRAD) {
-                    none = !labelled;
-                    if (labelled) {
-                        lse = P.lse[row];
-                        dl = P.dloss[row];
-                        if (P.gain) dl *= *P.gain;
-                    }
+                none = !(t >= 0 && t < P.vocab);
+                if (!none) {
+                    label = t - P.col0;
+                    lse = P.lse[row];
+                    dl = P.dloss[row];
+                    if (P.gain) dl *= *P.gain;
                 }
             }
             if (!mbar_wait(&accf[b], (acc / 2) & 1, flag)) break;
             fence_after();
+            acc++;
 #pragma unroll 1
             for (int cb = half * (BN / 64); cb < (half + 1) * (BN / 64); cb++) {
                 const int c0 = nb * BN + cb * 32;
@@ -356,30 +473,6 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN + cb * 32), v);
                 if (c0 >= P.n || row0 >= P.m) continue;
                 const int cols = min(32, P.n - c0);
-                if constexpr (EPI == EPI_STATS) {
-                    float hi = top;
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (i < cols) hi = fmaxf(hi, v[i]);
-                    // exp2((v - hi) log2 e); a row of -inf alone keeps sum 0
-                    constexpr float L2E = 1.4426950408889634f;
-                    const float ref = hi == -INFINITY ? 0.0f : hi;
-                    float part = sum * exp2f((top - ref) * L2E);
-                    if (top == -INFINITY) part = sum;
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (i < cols) part += exp2f((v[i] - ref) * L2E);
-                    sum = part;
-                    top = hi;
-                    if (label >= c0 && label < c0 + cols) {
-                        float mine = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (c0 + i == label) mine = v[i];
-                        P.label_logit[row] = mine;
-                    }
-                    continue;
-                }
                 if constexpr (EPI == EPI_GRAD) {
                     constexpr float L2E = 1.4426950408889634f;
 #pragma unroll
@@ -433,19 +526,16 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     __syncwarp();
                 }
             }
-            if constexpr (EPI == EPI_STATS) {
-                if (live) P.stats[(int64_t)(nb * 2 + half) * P.m + row] = make_float2(top, sum);
-            }
-            fence_before();
-            mbar_arrive(&acce[b]);
+            release(b);
         }
     }
 
-    // teardown: every role is done with the tensor memory
+    // teardown: every role of the pair is done with the tensor memory, the stages and the barriers
     fence_before();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
     fence_after();
-    if (warp == EPI_WARPS + 1) tmem_free(tmem_base, TMEM_COLS);
+    if (warp == EPI_WARPS + 1) tmem_free<CG>(tmem_base, TMEM_COLS);
     if (tid == 0 && *(volatile int*)flag) {
         *(volatile int*)P.fail = 1;
         __threadfence_system();

@@ -54,10 +54,10 @@ struct HalfGemm {
     float* partial = nullptr;    // workspace of the split plan
 };
 
-// Tile columns and K splits of a product; partial_bytes of workspace when splits > 1, and for the grouped forms.
+// Tile (cg CTAs of 128 rows, bn columns) and K splits of a product; partial_bytes of workspace when splits > 1, and for the grouped forms.
 // Split s of row m is at partial + (s * m_total + m) * ld, ld = n rounded up to a multiple of 4.
 struct HalfPlan {
-    int bn, splits;
+    int cg, bn, splits;
     size_t partial_bytes;
 };
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);

@@ -157,11 +157,11 @@ __global__ void __launch_bounds__(THREADS, 1) syrk_bf16_kernel(const __grid_cons
                         const uint32_t st = smem_u32(base) + s * STAGE_BYTES;
                         mbar_expect_tx(&full[s], STAGE_BYTES);
                         const int y = (int)(tok0 + (int64_t)kb * KB);
-                        tma_load_2d(st, &tmap, p0, y, &full[s]);
-                        tma_load_2d(st + BOX_BYTES, &tmap, p0 + 64, y, &full[s]);
+                        tma_load_2d(st, &tmap, p0, y, smem_u32(&full[s]));
+                        tma_load_2d(st + BOX_BYTES, &tmap, p0 + 64, y, smem_u32(&full[s]));
 #pragma unroll
                         for (int h = 0; h < 4; h++)
-                            tma_load_2d(st + A_BYTES + h * BOX_BYTES, &tmap, q0 + 64 * h, y, &full[s]);
+                            tma_load_2d(st + A_BYTES + h * BOX_BYTES, &tmap, q0 + 64 * h, y, smem_u32(&full[s]));
                     }
                 }
             }
