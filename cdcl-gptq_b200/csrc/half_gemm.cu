@@ -110,7 +110,12 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
         }
     }
     const int64_t tiles = ceil_div(m, p.cg * BM) * ceil_div(n, p.bn), slots = sms / p.cg;
-    if (store && tiles * 2 <= slots && nkb >= 16) {
+    if (grouped) {
+        // a tile's work grows with its adapters: two items to an SM, four K blocks at least for each
+        p.splits = (int)std::max<int64_t>(1, std::min(2 * slots / tiles, nkb / 4));
+        const int64_t per = ceil_div(nkb, p.splits);
+        p.splits = (int)ceil_div(nkb, per);
+    } else if (store && tiles * 2 <= slots && nkb >= 16) {
         // too few tiles for the SMs: the K blocks of a tile over several items, eight blocks at least for each
         p.splits = (int)std::min(slots / tiles, nkb / 8);
         const int64_t per = ceil_div(nkb, p.splits);
@@ -119,6 +124,8 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
     if (p.splits > 1 || grouped) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
     return p;
 }
+
+int64_t half_stats_parts(const HalfPlan& plan, int64_t n) { return STATS_PARTS * ceil_div(n, plan.bn); }
 
 // out = alpha * (f32in + partial[0] + partial[1] + ...), splits in order; also or instead as f32.
 template <bool BF16>

@@ -24,9 +24,8 @@ using namespace tc;
 
 constexpr int BM = 128;            // tile rows of a CTA = tensor-memory lanes
 constexpr int KB = 64;             // K block: 128 bytes of a 16-bit type
-constexpr int EPI_WARPS = 8;       // two per lane quadrant, each with half of the tile's columns
-constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int A_BYTES = BM * KB * 2;
+constexpr int GROUP = 4;           // ROWS_GROUPED: adapters of a pass over K
 constexpr int STAGE_WORDS = 32 * 33;  // one epilogue warp's transposition buffer, in floats
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int BAND = 16;           // row blocks per band of the tile order: a wave's operands stay in L2
@@ -37,10 +36,6 @@ constexpr int BAND = 16;           // row blocks per band of the tile order: a w
 constexpr int STATS_KB = 16;
 
 __host__ __device__ constexpr int b_bytes(int cg, int bn) { return bn / cg * KB * 2; }
-__host__ __device__ constexpr int stages(int cg, int bn) { return RING_BYTES / (A_BYTES + b_bytes(cg, bn)); }
-__host__ __device__ constexpr size_t smem_bytes() {
-    return RING_BYTES + EPI_WARPS * STAGE_WORDS * 4 + 1024 /* alignment */ + 256 /* barriers */;
-}
 
 // How the adapter of each row (index[m]; none if outside [0, adapters)) takes part.
 enum RowMode {
@@ -53,6 +48,19 @@ enum Epilogue {
     EPI_STATS = 1,  // running maximum and sum of exp of each row, and the label's logit
     EPI_GRAD = 2    // (softmax - onehot) * dloss as a 16-bit matrix
 };
+
+// Epilogue warps: two per lane quadrant, each with half of the tile's columns; four, with a quarter, where a thread holds
+// its columns' sums in registers.
+__host__ __device__ constexpr int epi_warps(int epi) { return epi == EPI_STATS ? 16 : 8; }
+__host__ __device__ constexpr int threads(int epi) { return (epi_warps(epi) + 2) * 32; }
+__host__ __device__ constexpr int stage_bytes(int cg, int bn, int rows) {
+    return A_BYTES + (rows == ROWS_GROUPED ? GROUP : 1) * b_bytes(cg, bn);
+}
+__host__ __device__ constexpr size_t smem_bytes(int epi) {
+    return RING_BYTES + (epi == EPI_STATS ? 0 : epi_warps(epi) * STAGE_WORDS * 4) + 1024 /* alignment */ + 256 /* barriers */;
+}
+// Parts of a tile's columns for which EPI_STATS keeps a (maximum, sum) pair of each row.
+constexpr int STATS_PARTS = epi_warps(EPI_STATS) / 4;
 
 struct Params {
     int m, n, nkb;             // rows, columns, K blocks
@@ -74,7 +82,7 @@ struct Params {
     const int64_t* target;     // label of each row, relative to the whole vocabulary
     int64_t col0;              // the first column's place in the vocabulary
     int64_t vocab;
-    float2* stats;             // [2 * tiles_n][m]: maximum, sum of exp(v - maximum)
+    float2* stats;             // [STATS_PARTS * tiles_n][m]: maximum, sum of exp(v - maximum)
     float* label_logit;        // [m]
     const float* lse;          // [m]
     const float* dloss;        // [m]
@@ -142,17 +150,19 @@ struct RowAdapters {
 };
 
 template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(threads(EPI), 1)
 half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_x, const Params P) {
-    constexpr int NS = stages(CG, BN);
-    constexpr int STAGE_BYTES = A_BYTES + b_bytes(CG, BN);
+    constexpr int EPI_WARPS = epi_warps(EPI);
+    constexpr int B_BYTES = b_bytes(CG, BN);
+    constexpr int STAGE_BYTES = stage_bytes(CG, BN, ROWS);
+    constexpr int NS = RING_BYTES / STAGE_BYTES;
     constexpr int BC = BN / CG;  // B's rows in this CTA
     constexpr uint32_t TMEM_COLS = 2 * BN;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* turn = reinterpret_cast<float*>(base + RING_BYTES);
-    uint64_t* full = reinterpret_cast<uint64_t*>(turn + EPI_WARPS * STAGE_WORDS);  // of the pair's first CTA
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + (EPI == EPI_STATS ? 0 : EPI_WARPS * STAGE_WORDS));  // of the pair's first CTA
     uint64_t* empty = full + NS;
     uint64_t* accf = empty + NS;
     uint64_t* acce = accf + 2;  // of the pair's first CTA
@@ -188,7 +198,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int ctr = 0;
         bool ok = true;
         // waits for the next stage and, in the first CTA, announces the pair's bytes; returns its address
-        auto stage = [&](uint32_t& bar) -> uint32_t {
+        auto stage = [&](uint32_t& bar, uint32_t bytes) -> uint32_t {
             const int s = ctr % NS;
             if (ctr >= NS && !mbar_wait(&empty[s], ((ctr / NS) - 1) & 1, flag)) {
                 ok = false;
@@ -196,7 +206,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             bar = smem_u32(&full[s]);
             if constexpr (CG == 2) bar = first_cta(bar);
-            if (rank == 0) mbar_expect_tx(&full[s], CG * STAGE_BYTES);
+            if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
             ctr++;
             return ring + s * STAGE_BYTES;
         };
@@ -229,7 +239,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (lane == 0) {
                     for (int kb = kb0; kb < kb1; kb++) {
                         uint32_t bar;
-                        const uint32_t st = stage(bar);
+                        const uint32_t st = stage(bar, A_BYTES + B_BYTES);
                         if (!ok) break;
                         load_a(st, m0, kb, bar);
                         if constexpr (BMN) {
@@ -248,24 +258,37 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 RowAdapters<CG> who;
                 who.load(P, mb * CG * BM, lane);
                 uint32_t off[4 * CG];
-                for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
+                constexpr int MOST = ROWS == ROWS_GROUPED ? GROUP : 1;
+                int j[MOST];
+                for (j[0] = who.next(off); j[0] != RowAdapters<CG>::NONE && ok; j[0] = who.next(off)) {
+                    int count = 1;
+#pragma unroll
+                    for (int q = 1; q < MOST; q++) {
+                        j[q] = who.next(off);
+                        count += j[q] != RowAdapters<CG>::NONE;
+                    }
                     if (lane == 0) {
                         const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                         const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
                         for (int kb = e0; kb < e1; kb++) {
                             uint32_t bar;
-                            const uint32_t st = stage(bar);
+                            const uint32_t st = stage(bar, A_BYTES + count * B_BYTES);
                             if (!ok) break;
                             if constexpr (ROWS == ROWS_GROUPED)
                                 load_a(st, m0, kb, bar);
                             else
                                 load2(st, &map_u, kb * KB, m0, bar);
-                            if constexpr (BMN) {
 #pragma unroll
-                                for (int h = 0; h < BC / 64; h++)
-                                    load3(st + A_BYTES + h * (64 * KB * 2), &map_x, n0 + 64 * h, kb * KB, j, bar);
-                            } else {
-                                load3(st + A_BYTES, &map_x, kb * KB, n0, j, bar);
+                            for (int q = 0; q < MOST; q++) {
+                                if (q >= count) break;
+                                const uint32_t sb = st + A_BYTES + q * B_BYTES;
+                                if constexpr (BMN) {
+#pragma unroll
+                                    for (int h = 0; h < BC / 64; h++)
+                                        load3(sb + h * (64 * KB * 2), &map_x, n0 + 64 * h, kb * KB, j[q], bar);
+                                } else {
+                                    load3(sb, &map_x, kb * KB, n0, j[q], bar);
+                                }
                             }
                         }
                     }
@@ -282,29 +305,43 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // ---------------- MMA issuer, of the pair's first CTA
         int ctr = 0, acc = 0;
         bool ok = rank == 0;
-        // the MMAs of one stage: `ks` steps of 16; A is MN-major only where `amn`
-        auto multiply = [&](uint32_t d, bool amn, int ks, bool fresh, const uint32_t (&off)[4 * CG], bool rows) {
+        // waits for the next stage; returns its address (0 when the wait ran out)
+        auto stage = [&]() -> uint32_t {
             const int s = ctr % NS;
             if (!mbar_wait(&full[s], (ctr / NS) & 1, flag)) {
                 ok = false;
-                return;
+                return 0;
             }
             fence_after();
-            const uint32_t sa = ring + s * STAGE_BYTES, sb = sa + A_BYTES;
+            return ring + s * STAGE_BYTES;
+        };
+        // the MMAs of one operand pair: `ks` steps of 16; A is MN-major only where `amn`; with `off`, of some rows only
+        auto multiply = [&](uint32_t d, uint32_t sa, uint32_t sb, bool amn, int ks, bool fresh, const uint32_t (*off)[4 * CG]) {
 #pragma unroll
             for (int k = 0; k < KB / 16; k++) {
                 if (k < ks) {
                     const uint64_t da = amn ? smem_desc(sa + k * 2048, 64 * KB * 2, 1024) : smem_desc(sa + k * 32, 16, 1024);
                     const uint64_t db = BMN ? smem_desc(sb + k * 2048, 64 * KB * 2, 1024) : smem_desc(sb + k * 32, 16, 1024);
                     const uint32_t id = idesc_half(BF16, amn, BMN, CG * BM, BN);
-                    if (rows)
-                        mma_half_rows(d, da, db, id, (fresh && k == 0) ? 0u : 1u, off);
+                    if (off)
+                        mma_half_rows(d, da, db, id, (fresh && k == 0) ? 0u : 1u, *off);
                     else
                         mma_half<CG>(d, da, db, id, (fresh && k == 0) ? 0u : 1u);
                 }
             }
-            mma_commit<CG>(&empty[s]);  // the stage is free once these MMAs have read it
+        };
+        // the stage is free once the MMAs issued so far have read it
+        auto done = [&]() {
+            mma_commit<CG>(&empty[ctr % NS]);
             ctr++;
+        };
+        auto plain = [&](uint32_t d, int k0, int k1) {
+            for (int kb = k0; kb < k1; kb++) {
+                const uint32_t sa = stage();
+                if (!ok) break;
+                multiply(d, sa, sa + A_BYTES, AMN, KB / 16, kb == k0, nullptr);
+                done();
+            }
         };
         // accumulator `acc & 1`, once its last contents have been read
         auto accumulator = [&]() -> uint32_t {
@@ -317,13 +354,12 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
             const int kb0 = split * P.kb_per_split, kb1 = min(P.nkb, kb0 + P.kb_per_split);
-            uint32_t off[4 * CG] = {};
             if constexpr (EPI == EPI_STATS) {
                 for (int c0 = kb0; c0 < kb1 && ok; c0 += STATS_KB) {
                     const uint32_t d = accumulator();
                     if (!ok) break;
                     if (lane == 0) {
-                        for (int kb = c0; kb < min(kb1, c0 + STATS_KB) && ok; kb++) multiply(d, AMN, KB / 16, kb == c0, off, false);
+                        plain(d, c0, min(kb1, c0 + STATS_KB));
                         mma_commit<CG>(&accf[acc & 1]);
                     }
                     ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -334,23 +370,34 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const uint32_t d = accumulator();
             if (!ok) break;
             if constexpr (ROWS != ROWS_GROUPED) {
-                if (lane == 0)
-                    for (int kb = kb0; kb < kb1 && ok; kb++) multiply(d, AMN, KB / 16, kb == kb0, off, false);
+                if (lane == 0) plain(d, kb0, kb1);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
             }
             if constexpr (ROWS != ROWS_PLAIN) {
                 if (ROWS == ROWS_GROUPED || split == P.splits - 1) {
                     RowAdapters<CG> who;
                     who.load(P, mb * CG * BM, lane);
-                    for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
+                    constexpr int MOST = ROWS == ROWS_GROUPED ? GROUP : 1;
+                    uint32_t off[MOST][4 * CG];
+                    while (ok && who.next(off[0]) != RowAdapters<CG>::NONE) {
+                        int count = 1;
+#pragma unroll
+                        for (int q = 1; q < MOST; q++) count += who.next(off[q]) != RowAdapters<CG>::NONE;
                         if (lane == 0) {
                             const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                             const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
-                            for (int kb = e0; kb < e1 && ok; kb++) {
-                                if constexpr (ROWS == ROWS_GROUPED)
-                                    multiply(d, AMN, KB / 16, kb == kb0, off, true);
-                                else
-                                    multiply(d, false, min(KB / 16, (P.rank - kb * KB + 15) / 16), false, off, true);
+                            for (int kb = e0; kb < e1; kb++) {
+                                const uint32_t sa = stage();
+                                if (!ok) break;
+#pragma unroll
+                                for (int q = 0; q < MOST; q++) {
+                                    if (q >= count) break;
+                                    if constexpr (ROWS == ROWS_GROUPED)
+                                        multiply(d, sa, sa + A_BYTES + q * B_BYTES, AMN, KB / 16, kb == kb0, &off[q]);
+                                    else
+                                        multiply(d, sa, sa + A_BYTES, false, min(KB / 16, (P.rank - kb * KB + 15) / 16), false, &off[0]);
+                                }
+                                done();
                             }
                         }
                         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -363,9 +410,9 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // every issued MMA has completed before the tensor memory is released (bounded)
         if (lane == 0 && acc > 0) mbar_wait(&accf[(acc - 1) & 1], ((acc - 1) / 2) & 1, flag);
     } else {
-        // ---------------- epilogue: warps 0..7; lanes 32 * (warp % 4) .., columns BN / 2 * (warp / 4) ..
+        // ---------------- epilogue: lanes 32 * (warp % 4) .., columns BN / 2 (BN / 4) * (warp / 4) ..
         const int quad = warp & 3, half = warp >> 2;
-        float* buf = turn + warp * STAGE_WORDS;
+        [[maybe_unused]] float* buf = turn + warp * STAGE_WORDS;
         int acc = 0;
         // the accumulator has been read: tell the MMA issuer
         auto release = [&](int b) {
@@ -387,7 +434,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const int64_t t = live ? P.target[row] : -1;
                 const int64_t label = (t >= 0 && t < P.vocab) ? t - P.col0 : -1;  // relative to this piece's column 0
                 const int chunks = (P.nkb + STATS_KB - 1) / STATS_KB;
-                float z[BN / 64][32];
+                constexpr int PB = BN / (32 * STATS_PARTS);  // blocks of 32 columns of a part
+                float z[PB][32];
                 bool ok = true;
                 for (int c = 0; c < chunks; c++, acc++) {
                     if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
@@ -396,25 +444,25 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                     fence_after();
 #pragma unroll
-                    for (int q = 0; q < BN / 64; q++) {
-                        float v[32];
-                        tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)((acc & 1) * BN + half * (BN / 2) + q * 32), v);
+                    for (int q = 0; q < PB * 2; q++) {
+                        float v[16];
+                        tmem_ld16(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)((acc & 1) * BN + half * (PB * 32) + q * 16), v);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) z[q][i] = c ? z[q][i] + v[i] : v[i];
+                        for (int i = 0; i < 16; i++) z[q / 2][q % 2 * 16 + i] = c ? z[q / 2][q % 2 * 16 + i] + v[i] : v[i];
                     }
                     release(acc & 1);
                 }
                 if (!ok) break;
-                const int c0 = nb * BN + half * (BN / 2), cols = min(BN / 2, P.n - c0);
+                const int c0 = nb * BN + half * (PB * 32), cols = min(PB * 32, P.n - c0);
                 float top = -INFINITY, sum = 0.0f;
-                if (cols == BN / 2) {
+                if (cols == PB * 32) {
 #pragma unroll
-                    for (int q = 0; q < BN / 64; q++)
+                    for (int q = 0; q < PB; q++)
 #pragma unroll
                         for (int i = 0; i < 32; i++) top = fmaxf(top, z[q][i]);
                 } else {
 #pragma unroll
-                    for (int q = 0; q < BN / 64; q++)
+                    for (int q = 0; q < PB; q++)
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
                             if (q * 32 + i >= cols) z[q][i] = -INFINITY;
@@ -426,7 +474,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const float ref = top == -INFINITY ? 0.0f : top;
                 const int64_t at = label - c0;
 #pragma unroll
-                for (int q = 0; q < BN / 64; q++) {
+                for (int q = 0; q < PB; q++) {
                     if (at >= q * 32 && at < q * 32 + 32) {
                         float mine = 0.0f;
 #pragma unroll
@@ -439,7 +487,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     for (int i = 0; i < 32; i++) part += exp2f((z[q][i] - ref) * L2E);
                     sum += part;
                 }
-                if (live) P.stats[(int64_t)(nb * 2 + half) * P.m + row] = make_float2(top, sum);
+                if (live) P.stats[(int64_t)(nb * STATS_PARTS + half) * P.m + row] = make_float2(top, sum);
                 continue;
             }
             const int b = acc & 1;

@@ -62,6 +62,9 @@ struct HalfPlan {
 };
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);
 
+// (maximum, sum) pairs that the statistics form leaves for each row.
+int64_t half_stats_parts(const HalfPlan& plan, int64_t n);
+
 // Launches the product (and, when the plan splits K, the pass that adds the splits in order).
 int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st);
 

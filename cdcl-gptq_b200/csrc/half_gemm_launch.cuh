@@ -15,13 +15,13 @@ template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
 static int launch_one(const Maps& maps, const Params& p, cudaStream_t st) {
     auto kern = half_gemm_kernel<BF16, AMN, BMN, CG, BN, ROWS, EPI>;
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_smem(kern, smem_bytes(), done, "half_gemm_kernel shared memory")) return rc;
+    if (int rc = allow_smem(kern, smem_bytes(EPI), done, "half_gemm_kernel shared memory")) return rc;
     const int64_t items = (int64_t)p.ntiles * p.splits;
     const int most = sm_count() / CG;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(CG * (items < most ? items : most)));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem_bytes();
+    cfg.blockDim = dim3(threads(EPI));
+    cfg.dynamicSmemBytes = smem_bytes(EPI);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;

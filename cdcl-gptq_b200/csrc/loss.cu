@@ -180,8 +180,7 @@ using namespace cdclq;
 
 extern "C" size_t cdclq_linear_cross_entropy_workspace(size_t t, size_t d, size_t v) {
     if (!t || !d || !v) return 0;
-    const int64_t tiles = ceil_div(v, plan_half_gemm(HALF_STATS, t, v, d).bn);
-    return align_up(sizeof(float2) * 2 * tiles * t) + align_up(sizeof(float) * t);
+    return align_up(sizeof(float2) * half_stats_parts(plan_half_gemm(HALF_STATS, t, v, d), v) * t) + align_up(sizeof(float) * t);
 }
 
 extern "C" int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, const void* w, size_t ldw, int dtype, size_t t,
@@ -202,7 +201,7 @@ extern "C" int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, cons
     g.target = target;
     g.vocab = v;
     const HalfPlan plan = plan_half_gemm(HALF_STATS, t, v, d);
-    const int parts = (int)(2 * ceil_div(v, plan.bn));
+    const int parts = (int)half_stats_parts(plan, v);
     g.stats = static_cast<float2*>(workspace);
     g.label_logit = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(sizeof(float2) * parts * t));
     if ((rc = launch_half_gemm(g, plan, st))) return rc;
