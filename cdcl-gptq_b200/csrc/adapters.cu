@@ -29,31 +29,11 @@ __device__ __forceinline__ uint16_t half_bits(float v) {
     return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// The f32 sums of a grouped product, splits in order: u16 = sum, su16 = scale of the row's adapter times sum (either may be
-// null; ldu and lds elements from row to row).
-template <bool BF16>
-__global__ void __launch_bounds__(256) rank_finish_kernel(const float* __restrict__ partial, int splits, int t, int r, int ldp,
-                                                          const int* __restrict__ index, int n, const float* __restrict__ scale,
-                                                          uint16_t* __restrict__ u16, int ldu, uint16_t* __restrict__ su16, int lds) {
-    const int64_t total = (int64_t)t * r;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / r;
-        const int c = (int)(i - row * r);
-        float s = 0.0f;
-        for (int k = 0; k < splits; k++) s += partial[((int64_t)k * t + row) * ldp + c];
-        if (u16) u16[row * ldu + c] = half_bits<BF16>(s);
-        if (su16) {
-            const int id = index[row];
-            su16[row * lds + c] = half_bits<BF16>((id >= 0 && id < n) ? scale[id] * s : 0.0f);
-        }
-    }
-}
-
-// Each adapter's tokens in ascending order, one CTA an adapter: start[i] = tokens of lower adapters.
-__global__ void __launch_bounds__(1024) token_lists_kernel(const int* __restrict__ index, int t, int n, int* __restrict__ start,
-                                                           int* __restrict__ order) {
+// Each adapter's tokens in ascending order, one CTA (1024 threads) an adapter: start[i] = tokens of lower adapters.
+__device__ __forceinline__ void token_list(const int* __restrict__ index, int t, int n, int id, int* __restrict__ start,
+                                           int* __restrict__ order) {
     __shared__ int below[32], mine[32];
-    const int id = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int lower = 0;
     for (int i = threadIdx.x; i < t; i += 1024) {
         const int v = index[i];
@@ -83,13 +63,56 @@ __global__ void __launch_bounds__(1024) token_lists_kernel(const int* __restrict
     if (id == n - 1 && threadIdx.x == 0) start[n] = at;
 }
 
+struct FinishArgs {
+    const float* partial;  // [split][t][ldp], or null
+    int splits, t, r, ldp;
+    const int* index;
+    int n;
+    const float* scale;
+    uint16_t* u16;         // the sums, rounded, or null
+    int64_t ldu;
+    uint16_t* su16;        // scale of the row's adapter times the sums, rounded, or null
+    int64_t lds;
+    float* su32;           // the same, not rounded, [t][r], or null
+    int* start;            // the adapters' token lists, or null
+    int* order;
+};
+
+// The f32 sums of a grouped product, splits in order; and, in its first n CTAs, the token lists that the gradients need.
+template <bool BF16>
+__global__ void __launch_bounds__(1024) rank_finish_kernel(const FinishArgs P) {
+    const int lists = P.start ? P.n : 0;
+    if ((int)blockIdx.x < lists) {
+        token_list(P.index, P.t, P.n, blockIdx.x, P.start, P.order);
+        return;
+    }
+    if (!P.partial) return;
+    const int64_t total = (int64_t)P.t * P.r;
+    for (int64_t i = (blockIdx.x - lists) * (int64_t)1024 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - lists) * 1024) {
+        const int64_t row = i / P.r;
+        const int c = (int)(i - row * P.r);
+        float s = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < P.splits; k++) s += P.partial[((int64_t)k * P.t + row) * P.ldp + c];
+        if (P.u16) P.u16[row * P.ldu + c] = half_bits<BF16>(s);
+        if (P.su16 || P.su32) {
+            const int id = P.index[row];
+            const float v = (id >= 0 && id < P.n) ? P.scale[id] * s : 0.0f;
+            if (P.su16) P.su16[row * P.lds + c] = half_bits<BF16>(v);
+            if (P.su32) P.su32[i] = v;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 // Outer products of an adapter's tokens: out[c][k] = factor * sum_t wide[t][c] narrow[t][k], c over the wide matrix'
-// columns, k over the rank.  Work item: 128 columns of c, one adapter, up to OUTER_CHUNK of its tokens.  An adapter of one
-// chunk writes its result; the chunks of others go to f32 slots that a second kernel adds in order.  Tokens are gathered by
-// list into shared memory (transposed into fragments by ldmatrix); a token past the chunk's end is a row of zeros.
+// columns, k over the rank: dA (wide = x, narrow = v) and dB (wide = dy, narrow = u) in one launch.  Work item: 128 columns,
+// 64 ranks, one adapter, a chunk of its tokens.  An adapter of one chunk writes its result; the chunks of others go to f32
+// slots that a second kernel adds in order.  Tokens are gathered by list into a ring in shared memory (asynchronous copies;
+// a checkpoint's codes through registers) and transposed into fragments by ldmatrix; what lies past the chunk is zero.
+// v is f32: it enters as the sum of two 16-bit numbers, so that dA is rounded where it is written and nowhere before.
 // Bound by reading `wide`: the rank is small, so mma.sync keeps up with memory.
-constexpr int OUTER_COLS = 128, OUTER_TOK = 32, OUTER_CHUNK = 512, OUTER_RANK = 64;
+constexpr int OUTER_COLS = 128, OUTER_TOK = 32, OUTER_MOST = 512, OUTER_RANK = 64, OUTER_STAGES = 4;
 
 struct OuterArgs {
     const uint16_t* wide;      // [t][ldw] 16-bit, or null:
@@ -97,197 +120,301 @@ struct OuterArgs {
     const float* scales;       // [t][ceil(cols / 128)]
     int64_t ldw;
     int cols;
-    const uint16_t* narrow;    // [t][ldn]
-    int64_t ldn;
-    int r, n, t;
+    int wide16;                // its rows can be read 16 bytes at a time
+    const uint16_t* narrow;    // [t][r] 16-bit, or null:
+    const float* narrow32;     // [t][r]
+    const float* factor;       // [n] or null
+    uint16_t* out;             // dA: [n][r][cols], dB: [n][cols][r]
+    int by_rank;               // the rank is the last index (dB)
+    float* slots;              // [slot][r * cols], in the output's order
+    int tiles;                 // column tiles; 0: not wanted
+};
+struct OuterPair {
+    OuterArgs a, b;
+    int r, n, t, chunk;
     const int* start;          // [n + 1]
     const int* order;
-    const float* factor;       // [n] or null
-    uint16_t* out;             // element (i, c, k) at i * out_i + c * out_c + k * out_k
-    int64_t out_i, out_c, out_k;
-    float* slots;              // [slot][r rounded up to 64][cols]
-    int slot_rank;
 };
 
-// The chunk items of all adapters in order; item -> (adapter, chunk).  slot: the item's place among those of adapters with
-// several chunks.
-__device__ __forceinline__ bool outer_item(const OuterArgs& P, int item, int& id, int& chunk, int& chunks, int& slot) {
+// Item -> (adapter, chunk, its chunks); slot: the item's place among those of adapters with several chunks.  A warp looks
+// at 32 adapters at a time.
+__device__ __forceinline__ bool outer_item(const OuterPair& P, int item, int lane, int& id, int& chunk, int& chunks, int& slot) {
     int at = 0, s = 0;
-    for (id = 0; id < P.n; id++) {
-        const int count = P.start[id + 1] - P.start[id];
-        chunks = max(1, (count + OUTER_CHUNK - 1) / OUTER_CHUNK);
-        if (item < at + chunks) {
-            chunk = item - at;
-            slot = s + chunk;
+    for (int base = 0; base < P.n; base += 32) {
+        const int i = base + lane;
+        const int mine = i < P.n ? max(1, (P.start[i + 1] - P.start[i] + P.chunk - 1) / P.chunk) : 0;
+        const int many = mine > 1 ? mine : 0;
+        int sum = mine, msum = many;  // inclusive prefix sums
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o), w = __shfl_up_sync(0xffffffffu, msum, o);
+            if (lane >= o) sum += v, msum += w;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, item < at + sum && i < P.n);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            id = base + l;
+            chunks = __shfl_sync(0xffffffffu, mine, l);
+            chunk = item - at - (__shfl_sync(0xffffffffu, sum, l) - chunks);
+            slot = s + __shfl_sync(0xffffffffu, msum - many, l) + chunk;
             return true;
         }
-        at += chunks;
-        if (chunks > 1) s += chunks;
+        at += __shfl_sync(0xffffffffu, sum, 31);
+        s += __shfl_sync(0xffffffffu, msum, 31);
     }
     return false;
 }
 
-template <bool BF16, bool CODES>
-__global__ void __launch_bounds__(256) outer_kernel(const OuterArgs P) {
-    // rows of 128 + 8 and 64 + 8 halves: 16-byte pieces of eight rows fall into different banks
-    __shared__ __align__(16) uint16_t wide[2][OUTER_TOK][OUTER_COLS + 8];
-    __shared__ __align__(16) uint16_t narrow[2][OUTER_TOK][OUTER_RANK + 8];
-    __shared__ int which[4];
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "r"(live ? 16 : 0)
+                 : "memory");
+}
+
+// rows of 128 + 8 and 64 + 8 halves: 16-byte pieces of eight rows fall into different banks
+struct OuterStage {
+    uint16_t wide[OUTER_TOK][OUTER_COLS + 8];
+    uint16_t high[OUTER_TOK][OUTER_RANK + 8];
+    uint16_t low[OUTER_TOK][OUTER_RANK + 8];
+};
+
+template <bool BF16>
+__device__ __forceinline__ float half_value(uint16_t v) {
+    return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// NARROW32: the narrow factor is f32 and enters as high + low.
+template <bool BF16, bool CODES, bool NARROW32>
+__device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& Q, OuterStage* ring, const int* list, int count, int id,
+                                           int chunks, int slot, int tile, int k0) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) {
-        int id = 0, chunk = 0, chunks = 0, slot = 0;
-        which[0] = outer_item(P, blockIdx.y, id, chunk, chunks, slot) ? id : -1;
-        which[1] = chunk, which[2] = chunks, which[3] = slot;
-    }
-    __syncthreads();
-    const int id = which[0], chunk = which[1], chunks = which[2], slot = which[3];
-    if (id < 0) return;
-    const int c0 = blockIdx.x * OUTER_COLS, k0 = blockIdx.z * OUTER_RANK;
-    const int first = P.start[id] + chunk * OUTER_CHUNK, last = min(P.start[id + 1], first + OUTER_CHUNK);
-    const int ranks = min(OUTER_RANK, P.r - k0);
-    const int nb = (P.cols + 127) / 128;
+    const int c0 = tile * OUTER_COLS, ranks = min(OUTER_RANK, P.r - k0);
+    const int nb = (Q.cols + 127) / 128, steps = (count + OUTER_TOK - 1) / OUTER_TOK;
+    const int row = tid >> 3, part = tid & 7, c = c0 + part * 16;  // wide: 8 threads a token, 16 columns each
     float acc[8][4];
 #pragma unroll
     for (int j = 0; j < 8; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
 
-    auto load = [&](int b, int at) {
-        // wide: 8 threads a token, 16 columns each; narrow: 8 columns each
-        const int row = tid >> 3, part = tid & 7, k = at + row;
-        const int tok = k < last ? P.order[k] : -1;
-        float s = 1.0f;
-        uint16_t* dst = &wide[b][row][part * 16];
-        const int c = c0 + part * 16;
+    // registers of the stage being fetched: a thread's 8 ranks of its token, and its 16 codes
+    float nv[8];
+    uint4 qv = make_uint4(0, 0, 0, 0);
+    auto fetch = [&](int s) {
+        const int k = s * OUTER_TOK + row;
+        const int tok = k < count ? list[k] : -1;
+        OuterStage& st = ring[s % OUTER_STAGES];
+        float f = 1.0f;
         if constexpr (CODES) {
-            if (tok >= 0) s = P.scales[(int64_t)tok * nb + c0 / 128];
-            const int8_t* src = P.codes + (int64_t)(tok < 0 ? 0 : tok) * P.cols + c;
-            alignas(16) uint16_t v[16];
-            if (tok >= 0 && c + 16 <= P.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+            if (tok >= 0) f = Q.scales[(int64_t)tok * nb + tile];
+            const int8_t* src = Q.codes + (int64_t)max(tok, 0) * Q.cols + c;
+            if (tok >= 0 && Q.wide16 && c + 16 <= Q.cols) {
+                qv = *reinterpret_cast<const uint4*>(src);
+            } else {
                 alignas(16) int8_t q[16];
-                *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(src);
 #pragma unroll
-                for (int i = 0; i < 16; i++) v[i] = half_bits<BF16>((float)q[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i++) v[i] = (tok >= 0 && c + i < P.cols) ? half_bits<BF16>((float)src[i]) : (uint16_t)0;
+                for (int i = 0; i < 16; i++) q[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (int8_t)0;
+                qv = *reinterpret_cast<uint4*>(q);
             }
-            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<uint4*>(v)[0];
-            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<uint4*>(v)[1];
         } else {
-            const uint16_t* src = P.wide + (int64_t)(tok < 0 ? 0 : tok) * P.ldw + c;
-            if (tok >= 0 && c + 16 <= P.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<const uint4*>(src)[0];
-                reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<const uint4*>(src)[1];
+            const uint16_t* src = Q.wide + (int64_t)max(tok, 0) * Q.ldw + c;
+            uint16_t* dst = &st.wide[row][part * 16];
+            if (Q.wide16) {
+                copy16(dst, tok >= 0 && c + 8 <= Q.cols ? src : Q.wide, tok >= 0 && c + 8 <= Q.cols);
+                copy16(dst + 8, tok >= 0 && c + 16 <= Q.cols ? src + 8 : Q.wide, tok >= 0 && c + 16 <= Q.cols);
             } else {
-                for (int i = 0; i < 16; i++) dst[i] = (tok >= 0 && c + i < P.cols) ? src[i] : (uint16_t)0;
+                for (int i = 0; i < 16; i++) dst[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (uint16_t)0;
             }
         }
-        const uint16_t* nsrc = P.narrow + (int64_t)(tok < 0 ? 0 : tok) * P.ldn + k0 + part * 8;
-        uint16_t* ndst = &narrow[b][row][part * 8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            uint16_t v = (tok >= 0 && part * 8 + i < ranks) ? nsrc[i] : (uint16_t)0;
+            const bool in = tok >= 0 && part * 8 + i < ranks;
+            const int64_t at = (int64_t)max(tok, 0) * P.r + k0 + part * 8 + i;
+            nv[i] = 0.0f;
+            if (in) nv[i] = NARROW32 ? Q.narrow32[at] : half_value<BF16>(Q.narrow[at]);
+            // a checkpoint's values are code * scale, one scale for these 128 columns: it joins the narrow factor, so that
+            // the codes enter the tensor instruction exactly
             if constexpr (CODES) {
-                // a checkpoint's values are code * scale, one scale for these 128 columns: it joins the narrow factor, so
-                // that the codes enter the tensor instruction exactly
-                const float f = BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-                v = tok >= 0 ? half_bits<BF16>(f * s) : (uint16_t)0;
+                if (in) nv[i] *= f;
             }
-            ndst[i] = v;
         }
     };
-
-    int b = 0;
-    if (first < last) load(0, first);
-    __syncthreads();
-    for (int at = first; at < last; at += OUTER_TOK, b ^= 1) {
-        if (at + OUTER_TOK < last) load(b ^ 1, at + OUTER_TOK);
+    // what fetch() left in registers goes to its stage
+    auto put = [&](int s) {
+        OuterStage& st = ring[s % OUTER_STAGES];
+        alignas(16) uint16_t h[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            h[i] = half_bits<BF16>(nv[i]);
+            const float high = half_value<BF16>(h[i]);
+            l[i] = half_bits<BF16>(fabsf(high) < INFINITY ? nv[i] - high : 0.0f);  // an infinity is all in the high part
+        }
+        *reinterpret_cast<uint4*>(&st.high[row][part * 8]) = *reinterpret_cast<uint4*>(h);
+        if constexpr (NARROW32) *reinterpret_cast<uint4*>(&st.low[row][part * 8]) = *reinterpret_cast<uint4*>(l);
+        if constexpr (CODES) {
+            alignas(16) int8_t q[16];
+            alignas(16) uint16_t v[16];
+            *reinterpret_cast<uint4*>(q) = qv;
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = half_bits<BF16>((float)q[i]);
+            uint16_t* dst = &st.wide[row][part * 16];
+            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<uint4*>(v)[0];
+            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<uint4*>(v)[1];
+        }
+    };
+#pragma unroll 1
+    for (int s = 0; s < OUTER_STAGES - 1; s++) {
+        if (s < steps) {
+            fetch(s);
+            put(s);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+#pragma unroll 1
+    for (int s = 0; s < steps; s++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(OUTER_STAGES - 2) : "memory");
+        __syncthreads();  // stage s is there, and stage s - 1 has been used by every warp
+        const int next = s + OUTER_STAGES - 1;
+        if (next < steps) fetch(next);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const OuterStage& st = ring[s % OUTER_STAGES];
         const int m0 = warp * 16;
 #pragma unroll
         for (int kk = 0; kk < OUTER_TOK; kk += 16) {
             // A (16 columns x 16 tokens) from token rows: transposed 8 x 8 pieces
             uint32_t a[4];
-            const uint32_t pa = (uint32_t)__cvta_generic_to_shared(&wide[b][kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + ((lane >> 3) & 1) * 8]);
+            const uint32_t pa = (uint32_t)__cvta_generic_to_shared(&st.wide[kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + ((lane >> 3) & 1) * 8]);
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                          : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                         : "r"(pa));
+                         : "r"(pa)
+                         : "memory");
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 if (j * 8 >= ranks) break;
                 uint32_t q0, q1;
-                const uint32_t pb = (uint32_t)__cvta_generic_to_shared(&narrow[b][kk + (lane & 15)][j * 8]);
-                asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(q0), "=r"(q1) : "r"(pb));
-                if constexpr (BF16)
-                    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                                 : "+f"(acc[j][0]), "+f"(acc[j][1]), "+f"(acc[j][2]), "+f"(acc[j][3])
-                                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(q0), "r"(q1));
-                else
-                    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                                 : "+f"(acc[j][0]), "+f"(acc[j][1]), "+f"(acc[j][2]), "+f"(acc[j][3])
-                                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(q0), "r"(q1));
+                const uint32_t ph = (uint32_t)__cvta_generic_to_shared(&st.high[kk + (lane & 15)][j * 8]);
+                asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(q0), "=r"(q1) : "r"(ph) : "memory");
+                mma16816<BF16>(acc[j], a, q0, q1);
+                if constexpr (NARROW32) {
+                    const uint32_t pl = (uint32_t)__cvta_generic_to_shared(&st.low[kk + (lane & 15)][j * 8]);
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(q0), "=r"(q1) : "r"(pl) : "memory");
+                    mma16816<BF16>(acc[j], a, q0, q1);
+                }
             }
         }
-        __syncthreads();
+        if (next < steps) put(next);  // its stage was used last by step s - 1
     }
-    const float f = (chunks == 1 && P.factor) ? P.factor[id] : 1.0f;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const bool whole = chunks == 1;
+    const float f = (whole && Q.factor) ? Q.factor[id] : 1.0f;
+    const int64_t base = (int64_t)(whole ? id : slot) * P.r * Q.cols;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int c = c0 + warp * 16 + lane / 4 + (i >> 1) * 8, k = j * 8 + (lane & 3) * 2 + (i & 1);
-            if (k >= ranks || c >= P.cols) continue;
-            if (chunks == 1)
-                P.out[id * P.out_i + c * P.out_c + (k0 + k) * P.out_k] = half_bits<BF16>(acc[j][i] * f);
+            const int cc = c0 + warp * 16 + lane / 4 + (i >> 1) * 8, k = k0 + j * 8 + (lane & 3) * 2 + (i & 1);
+            if (k >= P.r || j * 8 >= ranks || cc >= Q.cols) continue;
+            const int64_t at = base + (Q.by_rank ? (int64_t)cc * P.r + k : (int64_t)k * Q.cols + cc);
+            if (whole)
+                Q.out[at] = half_bits<BF16>(acc[j][i] * f);
             else
-                P.slots[((int64_t)slot * P.slot_rank + k0 + k) * P.cols + c] = acc[j][i];
+                Q.slots[at] = acc[j][i];
         }
     }
 }
 
-// The adapters of several chunks: out = factor * (slot 0 + slot 1 + ...).
-template <bool BF16>
-__global__ void __launch_bounds__(256) outer_finish_kernel(const OuterArgs P) {
-    const int id = blockIdx.y;
-    int slot = 0;
-    for (int i = 0; i < id; i++) {
-        const int chunks = (P.start[i + 1] - P.start[i] + OUTER_CHUNK - 1) / OUTER_CHUNK;
-        if (chunks > 1) slot += chunks;
+template <bool BF16, bool CODES>
+__global__ void __launch_bounds__(256) outer_kernel(const OuterPair P) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    OuterStage* ring = reinterpret_cast<OuterStage*>(smem);
+    __shared__ int list[OUTER_MOST];
+    __shared__ int which[4];
+    if (threadIdx.x < 32) {
+        int id = 0, chunk = 0, chunks = 0, slot = 0;
+        const bool any = outer_item(P, blockIdx.y, threadIdx.x, id, chunk, chunks, slot);
+        if (threadIdx.x == 0) which[0] = any ? id : -1, which[1] = chunk, which[2] = chunks, which[3] = slot;
     }
-    const int chunks = (P.start[id + 1] - P.start[id] + OUTER_CHUNK - 1) / OUTER_CHUNK;
+    __syncthreads();
+    const int id = which[0], chunks = which[2], slot = which[3];
+    if (id < 0) return;
+    const int first = P.start[id] + which[1] * P.chunk, count = max(0, min(P.start[id + 1] - first, P.chunk));
+    for (int i = threadIdx.x; i < count; i += 256) list[i] = P.order[first + i];
+    __syncthreads();
+    const int k0 = blockIdx.z * OUTER_RANK;
+    if ((int)blockIdx.x < P.a.tiles)
+        outer_tile<BF16, CODES, true>(P, P.a, ring, list, count, id, chunks, slot, blockIdx.x, k0);
+    else
+        outer_tile<BF16, false, false>(P, P.b, ring, list, count, id, chunks, slot, blockIdx.x - P.a.tiles, k0);
+}
+
+// The adapters of several chunks: out = factor * (slot 0 + slot 1 + ...), four neighbouring values a thread.
+template <bool BF16>
+__global__ void __launch_bounds__(256) outer_finish_kernel(const OuterPair P) {
+    const OuterArgs& Q = blockIdx.z ? P.b : P.a;
+    if (!Q.tiles) return;
+    const int id = blockIdx.y;
+    __shared__ int before;
+    if (threadIdx.x < 32) {
+        int s = 0;
+        for (int i = threadIdx.x; i < id; i += 32) {
+            const int chunks = (P.start[i + 1] - P.start[i] + P.chunk - 1) / P.chunk;
+            s += chunks > 1 ? chunks : 0;
+        }
+        s = __reduce_add_sync(0xffffffffu, s);
+        if (threadIdx.x == 0) before = s;
+    }
+    __syncthreads();
+    const int chunks = (P.start[id + 1] - P.start[id] + P.chunk - 1) / P.chunk;
     if (chunks <= 1) return;
-    const float f = P.factor ? P.factor[id] : 1.0f;
-    const int64_t total = (int64_t)P.r * P.cols;
+    const float f = Q.factor ? Q.factor[id] : 1.0f;
+    const int64_t total = (int64_t)P.r * Q.cols;
+    const float* src = Q.slots + before * total;
+    uint16_t* out = Q.out + id * total;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        // neighbouring threads along the output's contiguous index
-        const int64_t k = P.out_k == 1 ? i % P.r : i / P.cols, c = P.out_k == 1 ? i / P.r : i % P.cols;
         float s = 0.0f;
-        for (int q = 0; q < chunks; q++) s += P.slots[((int64_t)(slot + q) * P.slot_rank + k) * P.cols + c];
-        P.out[id * P.out_i + c * P.out_c + k * P.out_k] = half_bits<BF16>(s * f);
+#pragma unroll 4
+        for (int q = 0; q < chunks; q++) s += src[q * total + i];
+        out[i] = half_bits<BF16>(s * f);
     }
 }
 
-// Slots of adapters with several chunks: each such adapter has over OUTER_CHUNK tokens, so chunks <= 2 tokens / OUTER_CHUNK.
-int64_t outer_slots(int64_t t) { return 2 * t / OUTER_CHUNK; }
+// Tokens of a chunk: as many as leave three CTAs to an SM over both products' column tiles, 128 at least.
+int outer_chunk(int64_t t, int64_t tiles, int64_t r) {
+    int chunk = OUTER_MOST;
+    while (chunk > 128 && ceil_div(t, chunk) * tiles * ceil_div(r, OUTER_RANK) < 3 * sm_count()) chunk /= 2;
+    return chunk;
+}
+// Slots of adapters with several chunks: each such adapter has over `chunk` tokens, so it has fewer than 2 tokens / chunk.
+int64_t outer_slots(int64_t t, int chunk) { return 2 * t / chunk; }
 
-size_t outer_bytes(int64_t t, int64_t cols, int64_t r) { return (size_t)outer_slots(t) * ceil_div(r, 64) * 64 * cols * sizeof(float); }
-
-int launch_outer(bool bf16, const OuterArgs& p, cudaStream_t st) {
+int launch_outer(bool bf16, const OuterPair& p, cudaStream_t st) {
     // an adapter without tokens still writes its zeros: one item each
-    const int64_t items = ceil_div(p.t, OUTER_CHUNK) + p.n;
+    const int64_t items = ceil_div(p.t, p.chunk) + p.n, tiles = p.a.tiles + p.b.tiles;
     if (items > 65535) return set_error(CDCLQ_ERR_ARG, "adapters: too many tokens or adapters for one call");
-    const dim3 grid((unsigned)ceil_div(p.cols, OUTER_COLS), (unsigned)items, (unsigned)ceil_div(p.r, OUTER_RANK));
-    if (p.codes) {
-        auto kern = bf16 ? outer_kernel<true, true> : outer_kernel<false, true>;
-        CDCLQ_LAUNCH(kern, grid, 256, 0, st, p);
-    } else {
-        auto kern = bf16 ? outer_kernel<true, false> : outer_kernel<false, false>;
-        CDCLQ_LAUNCH(kern, grid, 256, 0, st, p);
-    }
-    if (outer_slots(p.t) > 0) {
-        const unsigned gx = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div((int64_t)p.r * p.cols, 1024), sm_count() * 4));
-        auto kern = bf16 ? outer_finish_kernel<true> : outer_finish_kernel<false>;
-        CDCLQ_LAUNCH(kern, dim3(gx, p.n), 256, 0, st, p);
+    const dim3 grid((unsigned)tiles, (unsigned)items, (unsigned)ceil_div(p.r, OUTER_RANK));
+    const size_t smem = OUTER_STAGES * sizeof(OuterStage);
+    static std::atomic<uint64_t> done[4];
+    const int which = (bf16 ? 2 : 0) + (p.a.codes ? 1 : 0);
+    auto kern = bf16 ? (p.a.codes ? outer_kernel<true, true> : outer_kernel<true, false>)
+                     : (p.a.codes ? outer_kernel<false, true> : outer_kernel<false, false>);
+    if (int rc = allow_smem(kern, smem, done[which], "outer_kernel shared memory")) return rc;
+    CDCLQ_LAUNCH(kern, grid, 256, smem, st, p);
+    if (outer_slots(p.t, p.chunk) > 0) {
+        const int64_t most = (int64_t)p.r * std::max(p.a.cols, p.b.cols);
+        const unsigned gx = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(most, 256), sm_count() * 4));
+        auto fin = bf16 ? outer_finish_kernel<true> : outer_finish_kernel<false>;
+        CDCLQ_LAUNCH(fin, dim3(gx, p.n, 2), 256, 0, st, p);
     }
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "adapters' outer products launch");
@@ -326,7 +453,7 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
 }
 
 struct BackwardLayout {
-    size_t expanded = 0, ranked = 0, partial = 0, start = 0, order = 0, slots = 0, total = 0;
+    size_t expanded = 0, ranked = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
 };
 BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r, bool need_dx) {
     BackwardLayout l;
@@ -341,7 +468,12 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
         partial = std::max(partial, plan_half_gemm(HALF_NN_GROUPED, t, r, w.d_out).partial_bytes);
         l.start = s.take((size_t)(n + 1) * sizeof(int));
         l.order = s.take((size_t)t * sizeof(int));
-        l.slots = s.take(outer_bytes(t, std::max(w.d_in, w.d_out), r));
+        l.ranked32 = s.take((size_t)t * r * sizeof(float));
+        // the chunk is longer where only one of the two is wanted
+        const int chunk = outer_chunk(t, ceil_div(w.d_in, OUTER_COLS) + ceil_div(w.d_out, OUTER_COLS), r);
+        const size_t slots = (size_t)outer_slots(t, std::min(chunk, outer_chunk(t, ceil_div(std::min(w.d_in, w.d_out), OUTER_COLS), r)));
+        l.slots_a = s.take(slots * r * w.d_in * sizeof(float));
+        l.slots_b = s.take(slots * r * w.d_out * sizeof(float));
     }
     l.partial = s.take(partial);
     l.total = s.at;
@@ -376,13 +508,18 @@ int check_call(const char* what, const cdclq_packed_layer* w, int dtype, size_t 
     return check_fail_word(what);
 }
 
-// The f32 sums of a grouped product, turned into u and scale * u.
-int finish_rank(bool bf16, const HalfGemm& g, const HalfPlan& plan, const float* scale, void* u, int64_t ldu, void* su, int64_t lds,
-                cudaStream_t st) {
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(g.m * g.n, 256), sm_count() * 8);
+// The f32 sums of a grouped product (none where g.partial is null), and the adapters' token lists.
+int finish_rank(bool bf16, const HalfGemm& g, const HalfPlan& plan, FinishArgs f, cudaStream_t st) {
+    f.partial = g.partial;
+    f.splits = plan.splits;
+    f.t = (int)g.m, f.r = (int)g.n, f.ldp = (int)(ceil_div(g.n, 4) * 4);
+    f.index = g.index;
+    f.n = g.adapters;
+    const int64_t sums = g.partial ? std::max<int64_t>(1, std::min<int64_t>(ceil_div(g.m * g.n, 1024), sm_count() * 2)) : 0;
+    const unsigned grid = (unsigned)(sums + (f.start ? f.n : 0));
+    if (!grid) return 0;
     auto kern = bf16 ? rank_finish_kernel<true> : rank_finish_kernel<false>;
-    CDCLQ_LAUNCH(kern, grid, 256, 0, st, g.partial, plan.splits, (int)g.m, (int)g.n, (int)(ceil_div(g.n, 4) * 4), g.index, g.adapters, scale,
-                 static_cast<uint16_t*>(u), (int)ldu, static_cast<uint16_t*>(su), (int)lds);
+    CDCLQ_LAUNCH(kern, grid, 1024, 0, st, f);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "rank_finish_kernel launch");
 }
@@ -431,7 +568,13 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         g.partial = partial;
         const HalfPlan plan = plan_half_gemm(HALF_NT_GROUPED, t, r, v.d_in);
         if ((rc = launch_half_gemm(g, plan, st))) return rc;
-        if ((rc = finish_rank(bf16, g, plan, ad->scale, u, r, ws + l.ranked, ldr, st))) return rc;
+        FinishArgs f{};
+        f.scale = ad->scale;
+        f.u16 = static_cast<uint16_t*>(u);
+        f.ldu = r;
+        f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
+        f.lds = ldr;
+        if ((rc = finish_rank(bf16, g, plan, f, st))) return rc;
     }
     if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;
     HalfGemm g{};
@@ -482,7 +625,7 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
     const bool bf16 = dtype == CDCLQ_DTYPE_BF16;
     const int64_t ldw = ceil_div(v.d_in, 8) * 8, ldr = ceil_div(r, 8) * 8;
     float* partial = reinterpret_cast<float*>(ws + l.partial);
-    if (n && (dx || da)) {
+    if (n) {
         HalfGemm g{};
         g.form = HALF_NN_GROUPED;
         g.bf16 = bf16;
@@ -491,10 +634,21 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         g.x = operand(ad->b, v.d_out, r, ad->ldb, n);
         g.index = ad->index;
         g.adapters = (int)n;
-        g.partial = partial;
         const HalfPlan plan = plan_half_gemm(HALF_NN_GROUPED, t, r, v.d_out);
-        if ((rc = launch_half_gemm(g, plan, st))) return rc;
-        if ((rc = finish_rank(bf16, g, plan, ad->scale, nullptr, 0, ws + l.ranked, ldr, st))) return rc;
+        FinishArgs f{};
+        if (dx || da) {
+            g.partial = partial;
+            if ((rc = launch_half_gemm(g, plan, st))) return rc;
+            f.scale = ad->scale;
+            if (dx) f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
+            f.lds = ldr;
+            if (da) f.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+        }
+        if (da || db) {
+            f.start = reinterpret_cast<int*>(ws + l.start);
+            f.order = reinterpret_cast<int*>(ws + l.order);
+        }
+        if ((rc = finish_rank(bf16, g, plan, f, st))) return rc;
     }
     if (dx) {
         if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;
@@ -516,39 +670,34 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         if ((rc = launch_half_gemm(g, plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out), st))) return rc;
     }
     if (!n || !(da || db)) return 0;
-    OuterArgs o{};
+    OuterPair o{};
     o.r = (int)r, o.n = (int)n, o.t = (int)t;
     o.start = reinterpret_cast<const int*>(ws + l.start);
     o.order = reinterpret_cast<const int*>(ws + l.order);
-    o.slots = reinterpret_cast<float*>(ws + l.slots);
-    o.slot_rank = (int)(ceil_div(r, 64) * 64);
-    CDCLQ_LAUNCH(token_lists_kernel, (unsigned)n, 1024, 0, st, ad->index, (int)t, (int)n, reinterpret_cast<int*>(ws + l.start),
-                 reinterpret_cast<int*>(ws + l.order));
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_error(e, "token_lists_kernel launch");
     if (da) {
-        OuterArgs p = o;
-        p.wide = static_cast<const uint16_t*>(x);
-        if (!x) p.codes = x_codes, p.scales = x_scales;
-        p.ldw = ldx;
-        p.cols = v.d_in;
-        p.narrow = reinterpret_cast<const uint16_t*>(ws + l.ranked);
-        p.ldn = ldr;
-        p.out = static_cast<uint16_t*>(da);
-        p.out_i = r * v.d_in, p.out_c = 1, p.out_k = v.d_in;
-        if ((rc = launch_outer(bf16, p, st))) return rc;
+        o.a.wide = static_cast<const uint16_t*>(x);
+        if (!x) o.a.codes = x_codes, o.a.scales = x_scales;
+        o.a.ldw = ldx;
+        o.a.cols = v.d_in;
+        o.a.wide16 = x ? ldx % 8 == 0 && v.d_in % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0
+                       : v.d_in % 16 == 0 && (reinterpret_cast<uintptr_t>(x_codes) & 15) == 0;
+        o.a.narrow32 = reinterpret_cast<const float*>(ws + l.ranked32);
+        o.a.out = static_cast<uint16_t*>(da);
+        o.a.slots = reinterpret_cast<float*>(ws + l.slots_a);
+        o.a.tiles = (int)ceil_div(v.d_in, OUTER_COLS);
     }
     if (db) {
-        OuterArgs p = o;
-        p.wide = static_cast<const uint16_t*>(dy);
-        p.ldw = lddy;
-        p.cols = v.d_out;
-        p.narrow = static_cast<const uint16_t*>(u);
-        p.ldn = r;
-        p.factor = ad->scale;
-        p.out = static_cast<uint16_t*>(db);
-        p.out_i = r * v.d_out, p.out_c = r, p.out_k = 1;
-        if ((rc = launch_outer(bf16, p, st))) return rc;
+        o.b.wide = static_cast<const uint16_t*>(dy);
+        o.b.ldw = lddy;
+        o.b.cols = v.d_out;
+        o.b.wide16 = v.d_out % 8 == 0;  // the rows start on 16 bytes
+        o.b.narrow = static_cast<const uint16_t*>(u);
+        o.b.factor = ad->scale;
+        o.b.out = static_cast<uint16_t*>(db);
+        o.b.by_rank = 1;
+        o.b.slots = reinterpret_cast<float*>(ws + l.slots_b);
+        o.b.tiles = (int)ceil_div(v.d_out, OUTER_COLS);
     }
-    return 0;
+    o.chunk = outer_chunk(t, o.a.tiles + o.b.tiles, r);
+    return launch_outer(bf16, o, st);
 }

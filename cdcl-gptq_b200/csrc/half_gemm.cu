@@ -89,37 +89,38 @@ static int encode(CUtensorMap* map, const HalfOperand& o, bool bf16, bool batche
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The plan of least estimated time, in clocks.  A K block of a tile costs a CTA its MMAs (128 columns: 256 clocks, shared by
+// a pair) or its operands' way through L2, at 48 bytes a clock and SM (measured over 64 x 512 KB tiles of 256 x 256: 47),
+// whichever is longer; an item 1500 for its start and end; splitting K the f32 sums' way out and back and a launch.
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
     const bool store = form != HALF_STATS && form != HALF_GRAD;
     const bool grouped = form == HALF_NT_GROUPED || form == HALF_NN_GROUPED;
     const int64_t sms = sm_count(), nkb = ceil_div(k, KB);
     HalfPlan p{1, 64, 1, 0};
-    if (!grouped) {
-        // The least time of all waves: a wave costs its tile's columns, more for what a smaller tile reads through L2, and 16
-        // columns' time for its start and end.
-        static const struct { int cg, bn, cost; } tiles[] = {{2, 256, 256 + 16}, {2, 128, 152 + 16}, {1, 128, 176 + 16}, {1, 64, 110 + 16}};
-        int64_t best = INT64_MAX;
-        for (const auto& c : tiles) {
-            if (c.bn == 64 && !store) break;
-            const int64_t cost = ceil_div(ceil_div(m, c.cg * BM) * ceil_div(n, c.bn), sms / c.cg) * c.cost;
-            if (cost < best) {
-                best = cost;
-                p.cg = c.cg;
-                p.bn = c.bn;
-            }
-        }
-    }
-    const int64_t tiles = ceil_div(m, p.cg * BM) * ceil_div(n, p.bn), slots = sms / p.cg;
     if (grouped) {
         // a tile's work grows with its adapters: two items to an SM, four K blocks at least for each
-        p.splits = (int)std::max<int64_t>(1, std::min(2 * slots / tiles, nkb / 4));
-        const int64_t per = ceil_div(nkb, p.splits);
-        p.splits = (int)ceil_div(nkb, per);
-    } else if (store && tiles * 2 <= slots && nkb >= 16) {
-        // too few tiles for the SMs: the K blocks of a tile over several items, eight blocks at least for each
-        p.splits = (int)std::min(slots / tiles, nkb / 8);
-        const int64_t per = ceil_div(nkb, p.splits);
-        p.splits = (int)ceil_div(nkb, per);
+        const int64_t tiles = ceil_div(m, BM) * ceil_div(n, p.bn);
+        p.splits = (int)std::max<int64_t>(1, std::min(2 * sms / tiles, nkb / 4));
+        p.splits = (int)ceil_div(nkb, ceil_div(nkb, p.splits));
+    } else {
+        static const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
+        double best = 1e300;
+        for (const auto& s : shapes) {
+            if (s.bn == 64 && !store) break;
+            const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
+            const double block = std::max(2.0 * s.bn, (BM + s.bn / s.cg) * KB * 2 / 48.0);
+            const int64_t most = store ? std::max<int64_t>(1, std::min(slots / tiles, nkb / 8)) : 1;
+            for (int64_t want = 1; want <= most; want++) {
+                const int64_t per = ceil_div(nkb, want), splits = ceil_div(nkb, per);
+                if (splits != want) continue;
+                double cost = (double)ceil_div(tiles * splits, slots) * (per * block + 1500.0);
+                if (splits > 1) cost += 6000.0 + (splits + 1.0) * m * n * 4.0 / 2000.0;
+                if (cost < best) {
+                    best = cost;
+                    p.cg = s.cg, p.bn = s.bn, p.splits = (int)splits;
+                }
+            }
+        }
     }
     if (p.splits > 1 || grouped) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
     return p;

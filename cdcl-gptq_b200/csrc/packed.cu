@@ -243,7 +243,7 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) 
     }
 }
 
-constexpr int EXPAND_WARPS = 8;
+constexpr int EXPAND_WARPS = 16;
 
 // The unit's codes of one half of the tile's rows, scaled, to the rows' columns; padding goes to column `trash`.
 template <bool BF16, int BITS, bool ALL>
@@ -294,8 +294,10 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
     const uint32_t trash = ld - 1;
     const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
     const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
+    PackedUnit next = W.unit[min(warp, W.units - 1)];
     for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
-        const PackedUnit u = W.unit[ui];
+        const PackedUnit u = next;
+        next = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
         if constexpr (BITS) {
             expand_unit<BF16, BITS, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash);
         } else {
