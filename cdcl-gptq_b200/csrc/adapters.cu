@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(1024) rank_finish_kernel(const FinishArgs P) {
 // a checkpoint's codes through registers) and transposed into fragments by ldmatrix; what lies past the chunk is zero.
 // v is f32: it enters as the sum of two 16-bit numbers, so that dA is rounded where it is written and nowhere before.
 // Bound by reading `wide`: the rank is small, so mma.sync keeps up with memory.
-constexpr int OUTER_COLS = 128, OUTER_TOK = 32, OUTER_MOST = 512, OUTER_RANK = 64, OUTER_STAGES = 4;
+constexpr int OUTER_COLS = 128, OUTER_TOK = 32, OUTER_MOST = 1024, OUTER_RANK = 64, OUTER_STAGES = 4;
 
 struct OuterArgs {
     const uint16_t* wide;      // [t][ldw] 16-bit, or null:
@@ -202,11 +202,15 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
     const int c0 = tile * OUTER_COLS, ranks = min(OUTER_RANK, P.r - k0);
     const int nb = (Q.cols + 127) / 128, steps = (count + OUTER_TOK - 1) / OUTER_TOK;
     const int row = tid >> 3, part = tid & 7, c = c0 + part * 16;  // wide: 8 threads a token, 16 columns each
-    float acc[8][4];
+    // a warp's share: 32 columns, one half of a stage's tokens; the halves are added at the end
+    const int m0 = (warp & 3) * 32, kk = (warp >> 2) * 16;
+    float acc[2][8][4];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+    for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[m][j][i] = 0.0f;
 
     // registers of the stage being fetched: a thread's 8 ranks of its token, and its 16 codes
     float nv[8];
@@ -289,48 +293,61 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         if (next < steps) fetch(next);
         asm volatile("cp.async.commit_group;" ::: "memory");
         const OuterStage& st = ring[s % OUTER_STAGES];
-        const int m0 = warp * 16;
+        // A (16 columns x 16 tokens, twice) from token rows: transposed 8 x 8 pieces
+        uint32_t a[2][4];
 #pragma unroll
-        for (int kk = 0; kk < OUTER_TOK; kk += 16) {
-            // A (16 columns x 16 tokens) from token rows: transposed 8 x 8 pieces
-            uint32_t a[4];
-            const uint32_t pa = (uint32_t)__cvta_generic_to_shared(&st.wide[kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + ((lane >> 3) & 1) * 8]);
+        for (int m = 0; m < 2; m++) {
+            const uint32_t pa = (uint32_t)__cvta_generic_to_shared(
+                &st.wide[kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + m * 16 + ((lane >> 3) & 1) * 8]);
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                         : "=r"(a[m][0]), "=r"(a[m][1]), "=r"(a[m][2]), "=r"(a[m][3])
                          : "r"(pa)
                          : "memory");
+        }
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (j * 8 >= ranks) break;
-                uint32_t q0, q1;
-                const uint32_t ph = (uint32_t)__cvta_generic_to_shared(&st.high[kk + (lane & 15)][j * 8]);
-                asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(q0), "=r"(q1) : "r"(ph) : "memory");
-                mma16816<BF16>(acc[j], a, q0, q1);
-                if constexpr (NARROW32) {
-                    const uint32_t pl = (uint32_t)__cvta_generic_to_shared(&st.low[kk + (lane & 15)][j * 8]);
-                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(q0), "=r"(q1) : "r"(pl) : "memory");
-                    mma16816<BF16>(acc[j], a, q0, q1);
+        for (int j = 0; j < 8; j += 2) {
+            if (j * 8 >= ranks) break;
+#pragma unroll
+            for (int low = 0; low < (NARROW32 ? 2 : 1); low++) {
+                uint32_t q[4];  // ranks j * 8 .. + 8, and the next 8
+                const uint32_t pb = (uint32_t)__cvta_generic_to_shared(&(low ? st.low : st.high)[kk + (lane & 15)][j * 8 + (lane >> 4) * 8]);
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                             : "r"(pb)
+                             : "memory");
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    mma16816<BF16>(acc[m][j], a[m], q[0], q[1]);
+                    mma16816<BF16>(acc[m][j + 1], a[m], q[2], q[3]);
                 }
             }
         }
         if (next < steps) put(next);  // its stage was used last by step s - 1
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // the second half's sums, through the ring's memory: 64 floats of each of 128 threads
+    float* turn = reinterpret_cast<float*>(ring);
+    if (warp >= 4) {
+#pragma unroll
+        for (int q = 0; q < 64; q++) turn[q * 128 + (tid & 127)] = acc[q / 32][q / 4 % 8][q % 4];
+    }
+    __syncthreads();
+    if (warp >= 4) return;
     const bool whole = chunks == 1;
     const float f = (whole && Q.factor) ? Q.factor[id] : 1.0f;
     const int64_t base = (int64_t)(whole ? id : slot) * P.r * Q.cols;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int cc = c0 + warp * 16 + lane / 4 + (i >> 1) * 8, k = k0 + j * 8 + (lane & 3) * 2 + (i & 1);
-            if (k >= P.r || j * 8 >= ranks || cc >= Q.cols) continue;
-            const int64_t at = base + (Q.by_rank ? (int64_t)cc * P.r + k : (int64_t)k * Q.cols + cc);
-            if (whole)
-                Q.out[at] = half_bits<BF16>(acc[j][i] * f);
-            else
-                Q.slots[at] = acc[j][i];
-        }
+    for (int q = 0; q < 64; q++) {
+        const int m = q / 32, j = q / 4 % 8, i = q % 4;
+        const float v = acc[m][j][i] + turn[q * 128 + tid];
+        const int cc = c0 + m0 + m * 16 + lane / 4 + (i >> 1) * 8, k = k0 + j * 8 + (lane & 3) * 2 + (i & 1);
+        if (k >= P.r || j * 8 >= ranks || cc >= Q.cols) continue;
+        const int64_t at = base + (Q.by_rank ? (int64_t)cc * P.r + k : (int64_t)k * Q.cols + cc);
+        if (whole)
+            Q.out[at] = half_bits<BF16>(v * f);
+        else
+            Q.slots[at] = v;
     }
 }
 
@@ -389,10 +406,10 @@ __global__ void __launch_bounds__(256) outer_finish_kernel(const OuterPair P) {
     }
 }
 
-// Tokens of a chunk: as many as leave three CTAs to an SM over both products' column tiles, 128 at least.
+// Tokens of a chunk: as many as leave two CTAs to an SM over both products' column tiles, 128 at least.
 int outer_chunk(int64_t t, int64_t tiles, int64_t r) {
     int chunk = OUTER_MOST;
-    while (chunk > 128 && ceil_div(t, chunk) * tiles * ceil_div(r, OUTER_RANK) < 3 * sm_count()) chunk /= 2;
+    while (chunk > 128 && ceil_div(t, chunk) * tiles * ceil_div(r, OUTER_RANK) < 2 * sm_count()) chunk /= 2;
     return chunk;
 }
 // Slots of adapters with several chunks: each such adapter has over `chunk` tokens, so it has fewer than 2 tokens / chunk.

@@ -107,6 +107,7 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
         double best = 1e300;
         for (const auto& s : shapes) {
             if (s.bn == 64 && !store) break;
+            if (s.cg == 2 && m <= BM) continue;  // the second CTA's rows would be empty
             const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
             const double block = std::max(2.0 * s.bn, (BM + s.bn / s.cg) * KB * 2 / 48.0);
             const int64_t most = store ? std::max<int64_t>(1, std::min(slots / tiles, nkb / 8)) : 1;

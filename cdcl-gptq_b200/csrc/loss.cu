@@ -19,21 +19,23 @@ namespace cdclq {
 namespace {
 
 constexpr size_t GRAD_BYTES = 256u << 20;  // one piece of g
-constexpr int JOIN_ROWS = 8, JOIN_PARTS = 64;
+constexpr int JOIN_THREADS = 512;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Joins the (maximum, sum) pairs of a row's column tiles: 8 rows x 64 threads that each take every 64th pair, four loads
-// in flight.  A pair's maximum is -inf where its logits all are; its sum is then 0, or NaN with a NaN among them.
+// Joins the (maximum, sum) pairs of a row's column tiles: ROWS rows to a CTA, a row's threads each with every (threads to a
+// row)-th pair, four loads in flight.  32 rows read whole lines; 8 where that leaves SMs idle.  A pair's maximum is -inf where its logits all are; its sum is then 0, or NaN with a NaN among them.
 __device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
     const float top = fmaxf(a.x, b.x);
     if (top == -INFINITY) return make_float2(top, a.y + b.y);
     return make_float2(top, (a.x == -INFINITY ? a.y : a.y * expf(a.x - top)) + (b.x == -INFINITY ? b.y : b.y * expf(b.x - top)));
 }
-__global__ void __launch_bounds__(JOIN_ROWS* JOIN_PARTS)
+template <int JOIN_ROWS>
+__global__ void __launch_bounds__(JOIN_THREADS)
 loss_join_kernel(const float2* __restrict__ stats, int parts, int t, int64_t vocab, const int64_t* __restrict__ target,
                  const float* __restrict__ label_logit, float* loss, float* lse) {
+    constexpr int JOIN_PARTS = JOIN_THREADS / JOIN_ROWS;
     __shared__ float2 s[JOIN_PARTS][JOIN_ROWS];
     const int tx = threadIdx.x % JOIN_ROWS, ty = threadIdx.x / JOIN_ROWS;
     const int row = blockIdx.x * JOIN_ROWS + tx;
@@ -205,8 +207,10 @@ extern "C" int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, cons
     g.stats = static_cast<float2*>(workspace);
     g.label_logit = reinterpret_cast<float*>(static_cast<char*>(workspace) + align_up(sizeof(float2) * parts * t));
     if ((rc = launch_half_gemm(g, plan, st))) return rc;
-    CDCLQ_LAUNCH(loss_join_kernel, (unsigned)ceil_div(t, JOIN_ROWS), JOIN_ROWS * JOIN_PARTS, 0, st, g.stats, parts, (int)t,
-                 (int64_t)v, target, g.label_logit, loss, lse);
+    const int rows = t >= 32 * (size_t)sm_count() ? 32 : 8;
+    auto join = rows == 32 ? loss_join_kernel<32> : loss_join_kernel<8>;
+    CDCLQ_LAUNCH(join, (unsigned)ceil_div(t, rows), JOIN_THREADS, 0, st, g.stats, parts, (int)t, (int64_t)v, target, g.label_logit, loss,
+                 lse);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "loss_join_kernel launch");
 }

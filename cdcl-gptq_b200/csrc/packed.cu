@@ -2,6 +2,7 @@
 // expansion to a 16-bit matrix, and the product with a few tokens.
 #include <algorithm>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 #include <cuda_bf16.h>
@@ -247,17 +248,20 @@ constexpr int EXPAND_WARPS = 16;
 
 // The unit's codes of one half of the tile's rows, scaled, to the rows' columns; padding goes to column `trash`.
 template <bool BF16, int BITS, bool ALL>
-__device__ __forceinline__ void expand_unit(const PackedView& W, const PackedUnit& u, int ui, const uint32_t* __restrict__ codes,
-                                            const uint32_t* __restrict__ grid, int lane, int half, bool live, uint16_t* row,
-                                            uint32_t trash) {
-    uint32_t w[BITS];
+__device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[BITS], const int2* __restrict__ column,
+                                            const uint32_t* __restrict__ g, int half, bool live, uint16_t* row, uint32_t trash) {
     int2 c[8];
-    const int2* column = reinterpret_cast<const int2*>(W.column + ui * 64) + (lane & 3);
-#pragma unroll
-    for (int i = 0; i < BITS; i++) w[i] = codes[(u.word + i) * 32 + lane];
 #pragma unroll
     for (int i = 0; i < 8; i++) c[i] = column[i * 4];
-    const uint32_t* g = grid + half * 8 + lane / 4;
+    // the upper rows' codes follow the lower rows' in every plane
+    int at = 0;
+#pragma unroll
+    for (int plane = 0; plane < 3; plane++) {
+        const int pb = plane_bits(BITS, plane);
+#pragma unroll
+        for (int i = 0; i < pb; i++) w[at + i] >>= half * pb;
+        at += pb;
+    }
     const bool one = u.group[0] == u.group[3];
     uint32_t sz = g[(int64_t)u.group[0] * 16], zero = zero_pair<BF16, BITS>(sz);
 #pragma unroll
@@ -268,12 +272,11 @@ __device__ __forceinline__ void expand_unit(const PackedView& W, const PackedUni
         }
 #pragma unroll
         for (int hi = 0; hi < 2; hi++) {
-            const uint32_t lower = decode_pair<BF16, BITS>(w, ks, hi * 2, zero), upper = decode_pair<BF16, BITS>(w, ks, hi * 2 + 1, zero);
-            const uint32_t v = scaled_pair<BF16>(half ? upper : lower, sz & 0xffffu);
-            const int2 at = c[ks * 2 + hi];
+            const uint32_t v = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, hi * 2, zero), sz & 0xffffu);
+            const int2 to = c[ks * 2 + hi];
             if (ALL || live) {
-                row[min((uint32_t)at.x, trash)] = (uint16_t)v;
-                row[min((uint32_t)at.y, trash)] = (uint16_t)(v >> 16);
+                row[min((uint32_t)to.x, trash)] = (uint16_t)v;
+                row[min((uint32_t)to.y, trash)] = (uint16_t)(v >> 16);
             }
         }
     }
@@ -294,21 +297,42 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
     const uint32_t trash = ld - 1;
     const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
     const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
-    PackedUnit next = W.unit[min(warp, W.units - 1)];
-    for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
-        const PackedUnit u = next;
-        next = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
-        if constexpr (BITS) {
-            expand_unit<BF16, BITS, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash);
-        } else {
+    const uint32_t* g = grid + half * 8 + lane / 4;
+    const int2* columns = reinterpret_cast<const int2*>(W.column) + (lane & 3);
+    if constexpr (BITS) {
+        // the next unit's codes are on their way while this one is decoded
+        uint32_t ahead[BITS];
+        PackedUnit u = W.unit[min(warp, W.units - 1)];
+#pragma unroll
+        for (int i = 0; i < BITS; i++) ahead[i] = codes[(u.word + i) * 32 + lane];
+        for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
+            const PackedUnit here = u;
+            uint32_t w[BITS];
+#pragma unroll
+            for (int i = 0; i < BITS; i++) w[i] = ahead[i];
+            u = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
+#pragma unroll
+            for (int i = 0; i < BITS; i++) ahead[i] = codes[(u.word + i) * 32 + lane];
+            expand_unit<BF16, BITS, ALL>(here, w, columns + ui * 32, g, half, live, row, trash);
+        }
+    } else {
+        auto unit = [&](auto width, const PackedUnit& u, int ui) {
+            constexpr int B = decltype(width)::value;
+            uint32_t w[B];
+#pragma unroll
+            for (int i = 0; i < B; i++) w[i] = codes[(u.word + i) * 32 + lane];
+            expand_unit<BF16, B, ALL>(u, w, columns + ui * 32, g, half, live, row, trash);
+        };
+        for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
+            const PackedUnit u = W.unit[ui];
             switch (u.bits) {
-                case 2: expand_unit<BF16, 2, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                case 3: expand_unit<BF16, 3, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                case 4: expand_unit<BF16, 4, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                case 5: expand_unit<BF16, 5, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                case 6: expand_unit<BF16, 6, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                case 7: expand_unit<BF16, 7, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
-                default: expand_unit<BF16, 8, ALL>(W, u, ui, codes, grid, lane, half, live, row, trash); break;
+                case 2: unit(std::integral_constant<int, 2>(), u, ui); break;
+                case 3: unit(std::integral_constant<int, 3>(), u, ui); break;
+                case 4: unit(std::integral_constant<int, 4>(), u, ui); break;
+                case 5: unit(std::integral_constant<int, 5>(), u, ui); break;
+                case 6: unit(std::integral_constant<int, 6>(), u, ui); break;
+                case 7: unit(std::integral_constant<int, 7>(), u, ui); break;
+                default: unit(std::integral_constant<int, 8>(), u, ui); break;
             }
         }
     }
@@ -386,9 +410,9 @@ namespace {
 
 using namespace tc;
 
-constexpr int DEC_WARPS = 8;
-constexpr int DEC_CODES = 72 * 1024;  // codes of a CTA's rows in shared memory at a time: three CTAs to an SM
-constexpr int DEC_GRID = 16 * 1024;   // scales and zero points of its rows, where they fit
+constexpr int DEC_GROUPS = 8, DEC_WARPS = 16, DEC_THREADS = DEC_WARPS * 32;
+// shared memory: two slots of codes (at least one row tile of 8 bits), sums, the units' table, the grid
+constexpr int DEC_RING = 160 * 1024, DEC_SUMS = 44 * 1024, DEC_TABLE = 4 * 1024, DEC_SMEM = 226 * 1024;
 
 // First launch: x in the tensor instruction's order (its columns gathered through the permutation, padding zero), and
 // u_t = A_i x_t, some warps for each (token, rank).
@@ -467,56 +491,46 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-// One unit of RT row tiles times NT token tiles.  codes, grid: the first tile's (shared memory, or for grid global);
-// `tile_codes` and `tile_grid` words to the next tile.
-template <bool BF16, int BITS, int NT, int RT>
-__device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t* codes, int tile_codes, const uint32_t* grid,
-                                            int tile_grid, const uint2* __restrict__ xf, int lane, float (&acc)[RT][NT][4]) {
-    uint2 x[4][NT];
+// One unit of a row tile times NT token tiles.  codes: the unit's words; grid: the tile's, one word for each (group, row).
+template <bool BF16, int BITS, int NT>
+__device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t* codes, const uint32_t* grid, const uint2 (&x)[4][NT],
+                                            int lane, float (&acc)[NT][4]) {
+    uint32_t w[BITS];
 #pragma unroll
-    for (int ks = 0; ks < 4; ks++)
+    for (int i = 0; i < BITS; i++) w[i] = codes[i * 32 + lane];
+    const uint32_t* g = grid + lane / 4;
+    if (u.group[0] == u.group[3]) {  // one column group: its four k-steps share a scale
+        const uint32_t s0 = g[u.group[0] * 16], s1 = g[u.group[0] * 16 + 8];
+        const uint32_t zero[2] = {zero_pair<BF16, BITS>(s0), zero_pair<BF16, BITS>(s1)};
+        float part[NT][4] = {};
 #pragma unroll
-        for (int n = 0; n < NT; n++) x[ks][n] = xf[(ks * NT + n) * 32 + lane];
-    const bool one = u.group[0] == u.group[3];  // one column group: its four k-steps share a scale
+        for (int ks = 0; ks < 4; ks++) {
+            uint32_t a[4];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        uint32_t w[BITS];
+            for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
 #pragma unroll
-        for (int i = 0; i < BITS; i++) w[i] = codes[rt * tile_codes + i * 32 + lane];
-        const uint32_t* g = grid + rt * tile_grid + lane / 4;
-        if (one) {
-            const uint32_t s0 = g[u.group[0] * 16], s1 = g[u.group[0] * 16 + 8];
+            for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
+        }
+        const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[n][i] = fmaf(i < 2 ? f0 : f1, part[n][i], acc[n][i]);
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            const uint32_t s0 = g[u.group[ks] * 16], s1 = g[u.group[ks] * 16 + 8];
             const uint32_t zero[2] = {zero_pair<BF16, BITS>(s0), zero_pair<BF16, BITS>(s1)};
-            float part[NT][4] = {};
-#pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                uint32_t a[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
-#pragma unroll
-                for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
-            }
             const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
+            uint32_t a[4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(i < 2 ? f0 : f1, part[n][i], acc[rt][n][i]);
-        } else {
+            for (int n = 0; n < NT; n++) {
+                float part[4] = {};
+                mma16816<BF16>(part, a, x[ks][n]);
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++) {
-                const uint32_t s0 = g[u.group[ks] * 16], s1 = g[u.group[ks] * 16 + 8];
-                const uint32_t zero[2] = {zero_pair<BF16, BITS>(s0), zero_pair<BF16, BITS>(s1)};
-                const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
-                uint32_t a[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float part[4] = {};
-                    mma16816<BF16>(part, a, x[ks][n]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[rt][n][i] = fmaf(i < 2 ? f0 : f1, part[i], acc[rt][n][i]);
-                }
+                for (int i = 0; i < 4; i++) acc[n][i] = fmaf(i < 2 ? f0 : f1, part[i], acc[n][i]);
             }
         }
     }
@@ -528,137 +542,169 @@ struct DecodeArgs {
     uint16_t* y;
     int64_t ldy;
     int t;
-    int chunk_units;  // units of a pass through shared memory
-    int grid_staged;
+    int tiles;        // row tiles of a CTA
+    int pass_tiles;   // of them at a time
+    int table_staged; // the units' table in shared memory
+    int grid_staged;  // the grid of all the CTA's row tiles in shared memory
     int* fail;
 };
 
-// Second launch: a CTA for RT * 16 rows, its warps over the units.  Bulk copies bring the rows' codes and grid into shared
-// memory before the first launch has finished (they do not depend on it).  The scale of a (row, group) multiplies the
-// group's f32 sum, so the codes minus their zero points enter the tensor instruction exactly and no weight is rounded.
+// Units of a pass through shared memory: DEC_GROUPS groups of warps with DEC_UNITS units each, whose tokens stay in registers
+// for all the row tiles.
+__host__ __device__ constexpr int dec_units(int nt) { return nt == 4 ? 2 : 4; }
+__host__ __device__ constexpr int dec_chunk(int nt) { return DEC_GROUPS * dec_units(nt); }
+// Sums of a group of warps: [row tile of the pass][token][16 rows + 1].
+__host__ __device__ constexpr int dec_sums(int nt) { return nt * 8 * 17; }
+
+// Second launch: one CTA to an SM, each with its share of the row tiles.  Bulk copies bring a chunk of the units' codes for
+// all row tiles of a pass into one of two slots, the first two before the first launch has finished (they do not depend on
+// it): at 4 bits a layer of 4096 x 11008 is then in flight at once.  Warp w has the units of group w % 8 and the row tiles of
+// parity w / 8; a token's bytes cross L2 once for all rows of a CTA.  The scale of a (row, group) multiplies the group's f32
+// sum, so the codes minus their zero points enter the tensor instruction exactly and no weight is rounded.
 // Bound by the codes' bytes; mma.sync because 16 rows and a few tokens leave most of tcgen05's 128 rows empty.
-template <bool BF16, int BITS, int NT, int RT>
-__global__ void __launch_bounds__(DEC_WARPS * 32) packed_decode_kernel(const PackedView W, const AdapterArgs ad, const DecodeArgs P) {
-    extern __shared__ __align__(128) uint32_t stage[];
-    __shared__ float sums[DEC_WARPS][RT * 16][NT * 8 + 1];
-    __shared__ uint64_t ready;
+template <bool BF16, int BITS, int NT>
+__global__ void __launch_bounds__(DEC_THREADS, 1) packed_decode_kernel(const PackedView W, const AdapterArgs ad, const DecodeArgs P) {
+    extern __shared__ __align__(128) uint32_t smem[];
+    constexpr int UNITS = dec_units(NT), CHUNK = dec_chunk(NT), TOK = NT * 8;
+    __shared__ uint64_t ready[2];
     __shared__ int flag;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile = blockIdx.x * RT, tiles = min(RT, W.tiles - tile);
-    const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
-    const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
-    const int tile_codes = P.chunk_units * W.max_bits * 32;  // words
-    uint32_t* grid_s = stage + RT * tile_codes;
-    // units u0 .. u1 of every tile of the CTA
-    auto fetch = [&](int u0, int u1, bool with_grid) {
-        const uint32_t w0 = W.unit[u0].word, w1 = u1 < W.units ? W.unit[u1].word : (uint32_t)W.tile_words;
-        const uint32_t bytes = (w1 - w0) * 128, gbytes = with_grid ? (uint32_t)(tiles * W.groups * 64) : 0;
-        mbar_expect_tx(&ready, tiles * bytes + gbytes);
-        for (int i = 0; i < tiles; i++)
-            bulk_load(smem_u32(stage + i * tile_codes), codes + ((int64_t)i * W.tile_words + w0) * 32, bytes, &ready);
-        if (gbytes) bulk_load(smem_u32(grid_s), grid, gbytes, &ready);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp % DEC_GROUPS, parity = warp / DEC_GROUPS;
+    const int tile0 = blockIdx.x * P.tiles, tiles = min(P.tiles, W.tiles - tile0);
+    const int chunks = (W.units + CHUNK - 1) / CHUNK, passes = (tiles + P.pass_tiles - 1) / P.pass_tiles, fills = chunks * passes;
+    const int tile_words = CHUNK * W.max_bits * 32, slot_words = P.pass_tiles * tile_words;
+    uint32_t* table_s = smem + 2 * slot_words;
+    uint32_t* grid_s = table_s + (P.table_staged ? W.units * 4 : 0);
+    float* sums = reinterpret_cast<float*>(grid_s + (P.grid_staged ? P.tiles * W.groups * 16 : 0));
+    const uint32_t* grid = P.grid_staged ? grid_s : W.grid + (int64_t)tile0 * W.groups * 16;
+    const PackedUnit* table = P.table_staged ? reinterpret_cast<const PackedUnit*>(table_s) : W.unit;
+    auto word_of = [&](int u) -> uint32_t { return u >= W.units ? (uint32_t)W.tile_words : BITS ? (uint32_t)(u * BITS) : W.unit[u].word; };
+    auto fetch = [&](int f, uint32_t more) {
+        const int t0 = f / chunks * P.pass_tiles, n = min(P.pass_tiles, tiles - t0), u0 = f % chunks * CHUNK;
+        const uint32_t w0 = word_of(u0), bytes = (word_of(u0 + CHUNK) - w0) * 128;
+        mbar_expect_tx(&ready[f & 1], n * bytes + more);
+        for (int i = 0; i < n; i++)
+            bulk_load(smem_u32(smem + (f & 1) * slot_words + i * tile_words), W.codes + ((int64_t)(tile0 + t0 + i) * W.tile_words + w0) * 32,
+                      bytes, &ready[f & 1]);
     };
     if (threadIdx.x == 0) {
-        mbar_init(&ready, 1);
+        mbar_init(&ready[0], 1);
+        mbar_init(&ready[1], 1);
         flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fetch(0, min(W.units, P.chunk_units), P.grid_staged);
+        const uint32_t tb = P.table_staged ? W.units * 16 : 0, gb = P.grid_staged ? tiles * W.groups * 64 : 0;
+        fetch(0, tb + gb);
+        if (tb) bulk_load(smem_u32(table_s), W.unit, tb, &ready[0]);
+        if (gb) bulk_load(smem_u32(grid_s), W.grid + (int64_t)tile0 * W.groups * 16, gb, &ready[0]);
+        if (fills > 1) fetch(1, 0);
     }
-    float acc[RT][NT][4];
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[r][n][i] = 0.0f;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t* g = P.grid_staged ? grid_s : grid;
-    for (int u0 = 0, pass = 0; u0 < W.units; u0 += P.chunk_units, pass++) {
-        const int u1 = min(W.units, u0 + P.chunk_units);
-        if (pass) {
-            __syncthreads();  // every warp is done with the last units
-            if (threadIdx.x == 0) fetch(u0, u1, false);
-        }
-        if (!mbar_wait(&ready, pass & 1, &flag)) break;
-        const uint32_t w0 = W.unit[u0].word;
-        for (int ui = u0 + warp; ui < u1; ui += DEC_WARPS) {
-            const PackedUnit u = W.unit[ui];
-            const uint2* xu = P.xf + (int64_t)ui * 4 * NT * 32;
-            const uint32_t* c = stage + (u.word - w0) * 32;
-            const int tg = W.groups * 16;
-            if constexpr (BITS) {
-                decode_unit<BF16, BITS, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc);
-            } else {
-                switch (u.bits) {
-                    case 2: decode_unit<BF16, 2, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    case 3: decode_unit<BF16, 3, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    case 4: decode_unit<BF16, 4, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    case 5: decode_unit<BF16, 5, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    case 6: decode_unit<BF16, 6, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    case 7: decode_unit<BF16, 7, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
-                    default: decode_unit<BF16, 8, NT, RT>(u, c, tile_codes, g, tg, xu, lane, acc); break;
+    for (int f = 0; f < fills; f++) {
+        const int t0 = f / chunks * P.pass_tiles, n = min(P.pass_tiles, tiles - t0), c = f % chunks;
+        const int u0 = c * CHUNK + group * UNITS;
+        uint2 x[UNITS][4][NT];
+#pragma unroll
+        for (int q = 0; q < UNITS; q++)
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+                for (int k = 0; k < NT; k++)
+                    x[q][ks][k] = u0 + q < W.units ? P.xf[((int64_t)((u0 + q) * 4 + ks) * NT + k) * 32 + lane] : make_uint2(0, 0);
+        if (!mbar_wait(&ready[f & 1], (f >> 1) & 1, &flag)) break;
+        const uint32_t w0 = word_of(c * CHUNK);
+        for (int tl = parity; tl < n; tl += DEC_WARPS / DEC_GROUPS) {
+            const uint32_t* codes = smem + (f & 1) * slot_words + tl * tile_words;
+            const uint32_t* g = grid + (t0 + tl) * W.groups * 16;
+            float acc[NT][4];
+            float* mine = sums + (group * P.pass_tiles + tl) * dec_sums(NT) + (lane & 3) * 34 + lane / 4;
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[k][i] = c ? mine[(k * 8 + (i & 1)) * 17 + (i >> 1) * 8] : 0.0f;
+#pragma unroll
+            for (int q = 0; q < UNITS; q++) {
+                if (u0 + q >= W.units) break;
+                const PackedUnit u = table[u0 + q];
+                const uint32_t* cw = codes + (u.word - w0) * 32;
+                if constexpr (BITS) {
+                    decode_unit<BF16, BITS, NT>(u, cw, g, x[q], lane, acc);
+                } else {
+                    switch (u.bits) {
+                        case 2: decode_unit<BF16, 2, NT>(u, cw, g, x[q], lane, acc); break;
+                        case 3: decode_unit<BF16, 3, NT>(u, cw, g, x[q], lane, acc); break;
+                        case 4: decode_unit<BF16, 4, NT>(u, cw, g, x[q], lane, acc); break;
+                        case 5: decode_unit<BF16, 5, NT>(u, cw, g, x[q], lane, acc); break;
+                        case 6: decode_unit<BF16, 6, NT>(u, cw, g, x[q], lane, acc); break;
+                        case 7: decode_unit<BF16, 7, NT>(u, cw, g, x[q], lane, acc); break;
+                        default: decode_unit<BF16, 8, NT>(u, cw, g, x[q], lane, acc); break;
+                    }
                 }
             }
+#pragma unroll
+            for (int k = 0; k < NT; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[(k * 8 + (i & 1)) * 17 + (i >> 1) * 8] = acc[k][i];
         }
+        __syncthreads();  // the slot is free, the sums are there
+        if (threadIdx.x == 0 && f + 2 < fills) fetch(f + 2, 0);
+        if (c + 1 < chunks) continue;
+        for (int i = threadIdx.x; i < n * 16 * P.t; i += DEC_THREADS) {
+            const int r = i & 15, tl = i / 16 % n, tok = i / 16 / n, row = (tile0 + t0 + tl) * 16 + r;
+            if (row >= W.d_out) continue;
+            float s = 0.0f;
+#pragma unroll
+            for (int q = 0; q < DEC_GROUPS; q++) s += sums[(q * P.pass_tiles + tl) * dec_sums(NT) + tok * 17 + r];
+            const int id = ad.n > 0 ? ad.index[tok] : -1;
+            if (id >= 0 && id < ad.n) {
+                const uint16_t* b = static_cast<const uint16_t*>(ad.b) + ((int64_t)id * W.d_out + row) * ad.ldb;
+                const float* u = P.u32 + tok * ad.r;
+                float v = 0.0f;
+                int k = 0;
+                for (; k + 8 <= ad.r; k += 8) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(b + k);
+                    const uint32_t bw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        v = fmaf(half_value<BF16>((uint16_t)bw[j]), u[k + 2 * j], v);
+                        v = fmaf(half_value<BF16>((uint16_t)(bw[j] >> 16)), u[k + 2 * j + 1], v);
+                    }
+                }
+                for (; k < ad.r; k++) v = fmaf(half_value<BF16>(b[k]), u[k], v);
+                s = fmaf(ad.scale[id], v, s);
+            }
+            P.y[tok * P.ldy + row] = half_bits<BF16>(s);
+        }
+        __syncthreads();  // the sums may be written again
     }
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sums[warp][r * 16 + lane / 4 + (i >> 1) * 8][n * 8 + (lane & 3) * 2 + (i & 1)] = acc[r][n][i];
-    __syncthreads();
     if (threadIdx.x == 0 && flag) {
         *(volatile int*)P.fail = 1;
         __threadfence_system();
     }
-    for (int i = threadIdx.x; i < RT * 16 * P.t; i += DEC_WARPS * 32) {
-        const int r = i % (RT * 16), tok = i / (RT * 16), row = tile * 16 + r;
-        if (row >= W.d_out) continue;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < DEC_WARPS; w++) s += sums[w][r][tok];
-        const int id = ad.n > 0 ? ad.index[tok] : -1;
-        if (id >= 0 && id < ad.n) {
-            const uint16_t* b = static_cast<const uint16_t*>(ad.b) + ((int64_t)id * W.d_out + row) * ad.ldb;
-            const float* u = P.u32 + tok * ad.r;
-            float v = 0.0f;
-            int k = 0;
-            for (; k + 8 <= ad.r; k += 8) {
-                const uint4 q = *reinterpret_cast<const uint4*>(b + k);
-                const uint32_t bw[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    v = fmaf(half_value<BF16>((uint16_t)bw[j]), u[k + 2 * j], v);
-                    v = fmaf(half_value<BF16>((uint16_t)(bw[j] >> 16)), u[k + 2 * j + 1], v);
-                }
-            }
-            for (; k < ad.r; k++) v = fmaf(half_value<BF16>(b[k]), u[k], v);
-            s = fmaf(ad.scale[id], v, s);
-        }
-        P.y[tok * P.ldy + row] = half_bits<BF16>(s);
-    }
 }
 
-template <bool BF16, int BITS, int NT, int RT>
-int decode_rows(const PackedView& w, const AdapterArgs& ad, DecodeArgs p, cudaStream_t st) {
-    const int unit_bytes = RT * w.max_bits * 128;
-    p.chunk_units = std::max(1, std::min(w.units, DEC_CODES / unit_bytes));
-    p.grid_staged = RT * w.groups * 64 <= DEC_GRID;
-    const size_t smem = (size_t)p.chunk_units * unit_bytes + (p.grid_staged ? (size_t)RT * w.groups * 64 : 0);
-    auto kern = packed_decode_kernel<BF16, BITS, NT, RT>;
+template <bool BF16, int BITS, int NT>
+int decode_tokens(const PackedView& w, const AdapterArgs& ad, DecodeArgs p, cudaStream_t st) {
+    // as many row tiles at a time as the two slots and the sums hold
+    const int tile_bytes = dec_chunk(NT) * w.max_bits * 128, sum_bytes = DEC_GROUPS * dec_sums(NT) * 4;
+    p.tiles = (int)ceil_div(w.tiles, sm_count());
+    const int most = std::max(1, std::min(DEC_RING / (2 * tile_bytes), DEC_SUMS / sum_bytes));
+    p.pass_tiles = (int)ceil_div(p.tiles, ceil_div(p.tiles, most));
+    size_t smem = (size_t)p.pass_tiles * (2 * tile_bytes + sum_bytes);
+    p.table_staged = w.units * 16 <= DEC_TABLE;
+    if (p.table_staged) smem += (size_t)w.units * 16;
+    p.grid_staged = smem + (size_t)p.tiles * w.groups * 64 <= DEC_SMEM;
+    if (p.grid_staged) smem += (size_t)p.tiles * w.groups * 64;
+    auto kern = packed_decode_kernel<BF16, BITS, NT>;
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_smem(kern, DEC_CODES + DEC_GRID, done, "packed_decode_kernel shared memory")) return rc;
-    return launch_dependent(kern, dim3((unsigned)ceil_div(w.tiles, RT)), dim3(DEC_WARPS * 32), smem, st, "packed_decode_kernel launch", w, ad, p);
+    if (int rc = allow_smem(kern, DEC_SMEM, done, "packed_decode_kernel shared memory")) return rc;
+    return launch_dependent(kern, dim3((unsigned)ceil_div(w.tiles, p.tiles)), dim3(DEC_THREADS), smem, st, "packed_decode_kernel launch",
+                            w, ad, p);
 }
 
 template <bool BF16, int BITS>
 int decode_width(const PackedView& w, const AdapterArgs& ad, const DecodeArgs& p, int nt, cudaStream_t st) {
-    // two row tiles to a CTA halve the tokens' bytes that it reads through L2, where that still leaves two CTAs to an SM
-    const bool two = w.tiles >= 4 * sm_count();
-    if (nt == 1) return two ? decode_rows<BF16, BITS, 1, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 1, 1>(w, ad, p, st);
-    if (nt == 2) return two ? decode_rows<BF16, BITS, 2, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 2, 1>(w, ad, p, st);
-    return two ? decode_rows<BF16, BITS, 4, 2>(w, ad, p, st) : decode_rows<BF16, BITS, 4, 1>(w, ad, p, st);
+    if (nt == 1) return decode_tokens<BF16, BITS, 1>(w, ad, p, st);
+    return nt == 2 ? decode_tokens<BF16, BITS, 2>(w, ad, p, st) : decode_tokens<BF16, BITS, 4>(w, ad, p, st);
 }
 
 int token_tiles(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : 4; }
