@@ -49,10 +49,10 @@ def on_device_of(position):
             x = args[position] if len(args) > position else None
             if not isinstance(x, torch.Tensor):
                 x = getattr(x, "codes", None)  # a Checkpoint
-            if x is not None and x.is_cuda and x.get_device() != _current_device():
-                with torch.cuda.device(x.device):
-                    return f(*args, **kw)
-            return f(*args, **kw)
+            if x is None or not x.is_cuda or x.get_device() == _current_device():
+                return f(*args, **kw)
+            with torch.cuda.device(x.device):
+                return f(*args, **kw)
 
         return g
 

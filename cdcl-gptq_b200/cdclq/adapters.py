@@ -17,7 +17,7 @@ import ctypes
 
 import torch
 
-from ._device import Call, half_code, on_device_of, refuse, rows16, tensor, workspace
+from ._device import HALF, Call, half_code, on_device_of, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 from .abi import CAdapters, CPackedLayer
 from .checkpoint import Checkpoint
@@ -77,12 +77,25 @@ class PackedProjection:
         return self._layout.numel()
 
 
-def _matrix(x, call):
+def _matrix(x, cols, call):
     """The rows of an n x rows x columns tensor, as rows16 gives them."""
-    n, rows, cols = x.shape
     if cols % 8 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
         return x, cols
     return rows16(x.reshape(-1, cols), call)
+
+
+def _refuse_adapters(w, like, a, b, scale, index, t):
+    """The message for adapters that do not fit."""
+    if a is None or b is None or scale is None or index is None:
+        refuse("adapters: a, b, scale and index go together")
+    dev = like.get_device()
+    tensor(a, "a", 3, like.dtype, None, dev)
+    n, r = a.shape[:2]
+    tensor(a, "a", 3, shape=(n, r, w.d_in))
+    tensor(b, "b", 3, like.dtype, (n, w.d_out, r), dev)
+    tensor(scale, "scale", 1, torch.float32, (n,), dev)
+    tensor(index, "index", 1, torch.int32, (t,), dev)
+    refuse("a: the rank must be > 0")
 
 
 class _Adapters:
@@ -93,25 +106,21 @@ class _Adapters:
     def __init__(self, w, like, a, b, scale, index, t, call):
         self.n = self.r = 0
         self.ref, self.held = None, ()
-        if a is None or b is None or scale is None or index is None:
-            if not (a is None and b is None and scale is None and index is None):
-                refuse("adapters: a, b, scale and index go together")
+        if a is None and b is None and scale is None and index is None:
             return
-        dev = like.get_device()
-        tensor(a, "a", 3, like.dtype, None, dev)
+        dev, dt = like.get_device(), like.dtype
+        if a is None or b is None or scale is None or index is None or a.dim() != 3:
+            _refuse_adapters(w, like, a, b, scale, index, t)
         n, r, d_in = a.shape
-        if d_in != w.d_in:
-            tensor(a, "a", 3, shape=(n, r, w.d_in))
-        tensor(b, "b", 3, like.dtype, (n, w.d_out, r), dev)
-        tensor(scale, "scale", 1, torch.float32, (n,), dev)
-        tensor(index, "index", 1, torch.int32, (t,), dev)
+        if not (d_in == w.d_in and r and b.shape == (n, w.d_out, r) and scale.shape == (n,) and index.shape == (t,) and a.dtype is dt
+                and b.dtype is dt and scale.dtype is torch.float32 and index.dtype is torch.int32 and a.get_device() == dev
+                and b.get_device() == dev and scale.get_device() == dev and index.get_device() == dev):
+            _refuse_adapters(w, like, a, b, scale, index, t)
         self.n, self.r = n, r
         if n == 0:
             return
-        if r == 0:
-            refuse("a: the rank must be > 0")
-        ar, lda = _matrix(a, call)
-        br, ldb = _matrix(b, call)
+        ar, lda = _matrix(a, d_in, call)
+        br, ldb = _matrix(b, r, call)
         scale, index = scale.contiguous(), index.contiguous()
         self.held = (a, b, ar, br, scale, index)
         self.c = CAdapters(ar.data_ptr(), br.data_ptr(), lda, ldb, scale.data_ptr(), index.data_ptr(), n, r)
@@ -121,12 +130,13 @@ class _Adapters:
 def _projection(w, x, what, backward):
     if not isinstance(w, PackedProjection):
         refuse("w: need a PackedProjection")
-    tensor(x, what, 2, device=w.device.index)
-    code = half_code(x.dtype, what)
-    t, cols = x.shape
-    if cols != (w.d_out if backward else w.d_in):
-        tensor(x, what, 2, shape=(t, w.d_out if backward else w.d_in))
-    return code, t
+    cols = w.d_out if backward else w.d_in
+    code = HALF.get(x.dtype)
+    if code is None or x.get_device() != w.device.index or x.dim() != 2 or x.shape[1] != cols:
+        tensor(x, what, 2, device=w.device.index)
+        half_code(x.dtype, what)
+        tensor(x, what, 2, shape=(x.shape[0], cols))
+    return code, x.shape[0]
 
 
 @on_device_of(0)
@@ -135,8 +145,8 @@ def forward(x, w, a=None, b=None, scale=None, index=None, keep=False, stream=Non
     code, t = _projection(w, x, "x", False)
     call, L = Call(x, stream), lib()
     ad = _Adapters(w, x, a, b, scale, index, t, call)
-    y = torch.empty((t, w.d_out), dtype=x.dtype, device=x.device)
-    u = torch.empty((t, ad.r), dtype=x.dtype, device=x.device) if keep else None
+    y = x.new_empty((t, w.d_out))
+    u = x.new_empty((t, ad.r)) if keep else None
     if t:
         xr, ldx = rows16(x, call)
         need = L.cdclq_projection_forward_workspace(w._ref, t, ad.n, ad.r)
@@ -157,7 +167,7 @@ def backward(dy, x, u, w, a, b, scale, index, need_dx=True, need_da=True, need_d
     code, t = _projection(w, dy, "dy", True)
     call, L, dev = Call(dy, stream), lib(), dy.get_device()
     ad = _Adapters(w, dy, a, b, scale, index, t, call)
-    new = lambda need, shape: torch.empty(shape, dtype=dy.dtype, device=dy.device) if need else None  # noqa: E731
+    new = lambda need, shape: dy.new_empty(shape) if need else None  # noqa: E731
     dx = new(need_dx, (t, w.d_in))
     da = new(need_da and a is not None, (ad.n, ad.r, w.d_in))
     db = new(need_db and a is not None, (ad.n, w.d_out, ad.r))

@@ -48,7 +48,8 @@ def _code(dt):
 
 @on_device_of(0)
 def save(x, stream=None):
-    tensor(x, "x", 2)
+    if x.dim() != 2 or not x.is_cuda:
+        tensor(x, "x", 2)
     code = _code(x.dtype)
     t, d = x.shape
     call = Call(x, stream)
@@ -86,7 +87,7 @@ def weight_grad(dy, c, stream=None):
     if d == 0 or n == 0:
         refuse("weight_grad: no columns")
     call, L = Call(dy, stream), lib()
-    dw = torch.empty((n, d), dtype=dy.dtype, device=dy.device)
+    dw = dy.new_empty((n, d))
     src, ld = rows16(dy, call) if t else (dy, n)
     need = L.cdclq_checkpoint_weight_grad_workspace(t, d, n)
     ws = workspace(need, dy, call)

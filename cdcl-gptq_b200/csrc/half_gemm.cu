@@ -103,10 +103,10 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
         p.splits = (int)std::max<int64_t>(1, std::min(2 * sms / tiles, nkb / 4));
         p.splits = (int)ceil_div(nkb, ceil_div(nkb, p.splits));
     } else {
-        static const struct { int cg, bn; } shapes[] = {{2, 256}, {2, 128}, {1, 128}, {1, 64}};
+        static const struct { int cg, bn; } shapes[] = {{2, 512}, {2, 256}, {2, 128}, {1, 128}, {1, 64}};
         double best = 1e300;
         for (const auto& s : shapes) {
-            if (s.bn == 64 && !store) break;
+            if ((s.bn == 64 && !store) || (s.bn == 512 && form == HALF_STATS)) continue;
             if (s.cg == 2 && m <= BM) continue;  // the second CTA's rows would be empty
             const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
             const double block = std::max(2.0 * s.bn, (BM + s.bn / s.cg) * KB * 2 / 48.0);
@@ -171,9 +171,9 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     Maps maps{};
     int rc;
     if ((rc = encode(&maps.a, g.a, g.bf16, false, a_mn ? KB : BM))) return rc;
-    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : plan.bn / plan.cg))) return rc;
+    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
     if (extend && (rc = encode(&maps.u, g.u, g.bf16, false, BM))) return rc;
-    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : plan.bn / plan.cg))) return rc;
+    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
     Params p{};
     p.m = (int)g.m;
     p.n = (int)g.n;

@@ -6,12 +6,14 @@
 //   AMN, BMN   whether an operand is contiguous along its rows' index (MN-major) or along k (K-major)
 //   CG, BN     a tile is 128 CG rows x BN columns.  CG = 2: a pair of CTAs shares it, each with half of A's and half of
 //              B's rows in its shared memory and half of D's rows in its tensor memory, so that a product of 256 x 256
-//              reads 64 bytes a clock and SM through L2 (96 with CG = 1 and 128 x 256).  CG = 1, narrow, where there are
-//              few tiles
+//              reads 64 bytes a clock and SM through L2 (96 with CG = 1 and 128 x 256), one of 256 x 512 48; 47 is what
+//              L2 was measured to give.  CG = 1, narrow, where there are few tiles
 //   ROWS       what the adapters of the rows do (see RowMode)
 //   EPI        what becomes of a finished tile (see Epilogue)
-// TMA brings 64-deep K blocks into a ring of 128-byte-swizzled stages, one thread issues the MMAs, and eight warps
-// work on the finished accumulator while the next tile's MMAs fill the other one.
+// TMA brings 64-deep K blocks into a ring of 128-byte-swizzled stages, one thread issues the MMAs, and sixteen warps take
+// a finished accumulator into registers and work on it while the next MMAs run.  Tensor memory holds two accumulators of
+// up to 256 columns: two tiles' in turn, or the halves of a tile of 512, where the next tile's first MMAs go to the half
+// that is free first.
 #pragma once
 
 #include "common.cuh"
@@ -26,8 +28,11 @@ constexpr int BM = 128;            // tile rows of a CTA = tensor-memory lanes
 constexpr int KB = 64;             // K block: 128 bytes of a 16-bit type
 constexpr int A_BYTES = BM * KB * 2;
 constexpr int GROUP = 4;           // ROWS_GROUPED: adapters of a pass over K
-constexpr int STAGE_WORDS = 32 * 33;  // one epilogue warp's transposition buffer, in floats
+constexpr int EPI_WARPS = 16;      // four per lane quadrant, each with a quarter of the accumulator's columns
+constexpr int THREADS = (EPI_WARPS + 2) * 32;
+constexpr int TURN_BYTES = 32 * 64;   // one epilogue warp's transposition buffer: 64 bytes of each of its 32 rows
 constexpr int RING_BYTES = 192 * 1024;
+constexpr int LEAD = 2;            // tiles of 512: stages whose MMAs go to the first half before the second half's
 constexpr int BAND = 16;           // row blocks per band of the tile order: a wave's operands stay in L2
 
 // Each sum of at most this many K blocks leaves tensor memory and is added up in registers (EPI_STATS): the tensor core
@@ -49,18 +54,14 @@ enum Epilogue {
     EPI_GRAD = 2    // (softmax - onehot) * dloss as a 16-bit matrix
 };
 
-// Epilogue warps: two per lane quadrant, each with half of the tile's columns; four, with a quarter, where a thread holds
-// its columns' sums in registers.
-__host__ __device__ constexpr int epi_warps(int epi) { return epi == EPI_STATS ? 16 : 8; }
-__host__ __device__ constexpr int threads(int epi) { return (epi_warps(epi) + 2) * 32; }
 __host__ __device__ constexpr int stage_bytes(int cg, int bn, int rows) {
     return A_BYTES + (rows == ROWS_GROUPED ? GROUP : 1) * b_bytes(cg, bn);
 }
-__host__ __device__ constexpr size_t smem_bytes(int epi) {
-    return RING_BYTES + (epi == EPI_STATS ? 0 : epi_warps(epi) * STAGE_WORDS * 4) + 1024 /* alignment */ + 256 /* barriers */;
+__host__ __device__ constexpr size_t smem_bytes() {
+    return RING_BYTES + EPI_WARPS * TURN_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 }
 // Parts of a tile's columns for which EPI_STATS keeps a (maximum, sum) pair of each row.
-constexpr int STATS_PARTS = epi_warps(EPI_STATS) / 4;
+constexpr int STATS_PARTS = EPI_WARPS / 4;
 
 struct Params {
     int m, n, nkb;             // rows, columns, K blocks
@@ -150,19 +151,22 @@ struct RowAdapters {
 };
 
 template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
-__global__ void __launch_bounds__(threads(EPI), 1)
+__global__ void __launch_bounds__(THREADS, 1)
 half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_x, const Params P) {
-    constexpr int EPI_WARPS = epi_warps(EPI);
+    constexpr bool WIDE = BN == 512;
+    constexpr int AC = WIDE ? 256 : BN;  // columns of an accumulator
     constexpr int B_BYTES = b_bytes(CG, BN);
     constexpr int STAGE_BYTES = stage_bytes(CG, BN, ROWS);
     constexpr int NS = RING_BYTES / STAGE_BYTES;
-    constexpr int BC = BN / CG;  // B's rows in this CTA
-    constexpr uint32_t TMEM_COLS = 2 * BN;
+    constexpr int BC = AC / CG;  // B's rows of an accumulator in this CTA
+    constexpr int HALF_BYTES = BC * KB * 2;
+    constexpr uint32_t TMEM_COLS = 2 * AC;
+    static_assert(!WIDE || (CG == 2 && ROWS != ROWS_GROUPED && EPI != EPI_STATS), "tiles of 512 columns");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* turn = reinterpret_cast<float*>(base + RING_BYTES);
-    uint64_t* full = reinterpret_cast<uint64_t*>(turn + (EPI == EPI_STATS ? 0 : EPI_WARPS * STAGE_WORDS));  // of the pair's first CTA
+    unsigned char* turn = base + RING_BYTES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(turn + EPI_WARPS * TURN_BYTES);  // of the pair's first CTA
     uint64_t* empty = full + NS;
     uint64_t* accf = empty + NS;
     uint64_t* acce = accf + 2;  // of the pair's first CTA
@@ -242,12 +246,16 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         const uint32_t st = stage(bar, A_BYTES + B_BYTES);
                         if (!ok) break;
                         load_a(st, m0, kb, bar);
-                        if constexpr (BMN) {
 #pragma unroll
-                            for (int h = 0; h < BC / 64; h++)
-                                load2(st + A_BYTES + h * (64 * KB * 2), &map_b, n0 + 64 * h, kb * KB, bar);
-                        } else {
-                            load2(st + A_BYTES, &map_b, kb * KB, n0, bar);
+                        for (int w = 0; w < BN / AC; w++) {
+                            const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
+                            if constexpr (BMN) {
+#pragma unroll
+                                for (int h = 0; h < BC / 64; h++)
+                                    load2(sb + h * (64 * KB * 2), &map_b, n0 + w * AC + 64 * h, kb * KB, bar);
+                            } else {
+                                load2(sb, &map_b, kb * KB, n0 + w * AC, bar);
+                            }
                         }
                     }
                 }
@@ -281,13 +289,16 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                             for (int q = 0; q < MOST; q++) {
                                 if (q >= count) break;
-                                const uint32_t sb = st + A_BYTES + q * B_BYTES;
-                                if constexpr (BMN) {
 #pragma unroll
-                                    for (int h = 0; h < BC / 64; h++)
-                                        load3(sb + h * (64 * KB * 2), &map_x, n0 + 64 * h, kb * KB, j[q], bar);
-                                } else {
-                                    load3(sb, &map_x, kb * KB, n0, j[q], bar);
+                                for (int w = 0; w < BN / AC; w++) {
+                                    const uint32_t sb = st + A_BYTES + q * B_BYTES + w * HALF_BYTES;
+                                    if constexpr (BMN) {
+#pragma unroll
+                                        for (int h = 0; h < BC / 64; h++)
+                                            load3(sb + h * (64 * KB * 2), &map_x, n0 + w * AC + 64 * h, kb * KB, j[q], bar);
+                                    } else {
+                                        load3(sb, &map_x, kb * KB, n0 + w * AC, j[q], bar);
+                                    }
                                 }
                             }
                         }
@@ -305,10 +316,10 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // ---------------- MMA issuer, of the pair's first CTA
         int ctr = 0, acc = 0;
         bool ok = rank == 0;
-        // waits for the next stage; returns its address (0 when the wait ran out)
-        auto stage = [&]() -> uint32_t {
-            const int s = ctr % NS;
-            if (!mbar_wait(&full[s], (ctr / NS) & 1, flag)) {
+        // waits for stage `c`; returns its address (0 when the wait ran out)
+        auto stage = [&](int c) -> uint32_t {
+            const int s = c % NS;
+            if (!mbar_wait(&full[s], (c / NS) & 1, flag)) {
                 ok = false;
                 return 0;
             }
@@ -322,7 +333,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (k < ks) {
                     const uint64_t da = amn ? smem_desc(sa + k * 2048, 64 * KB * 2, 1024) : smem_desc(sa + k * 32, 16, 1024);
                     const uint64_t db = BMN ? smem_desc(sb + k * 2048, 64 * KB * 2, 1024) : smem_desc(sb + k * 32, 16, 1024);
-                    const uint32_t id = idesc_half(BF16, amn, BMN, CG * BM, BN);
+                    const uint32_t id = idesc_half(BF16, amn, BMN, CG * BM, AC);
                     if (off)
                         mma_half_rows(d, da, db, id, (fresh && k == 0) ? 0u : 1u, *off);
                     else
@@ -335,20 +346,50 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             mma_commit<CG>(&empty[ctr % NS]);
             ctr++;
         };
+        // the K blocks k0 .. k1 into accumulator d
         auto plain = [&](uint32_t d, int k0, int k1) {
             for (int kb = k0; kb < k1; kb++) {
-                const uint32_t sa = stage();
+                const uint32_t sa = stage(ctr);
                 if (!ok) break;
                 multiply(d, sa, sa + A_BYTES, AMN, KB / 16, kb == k0, nullptr);
                 done();
             }
         };
-        // accumulator `acc & 1`, once its last contents have been read
+        // the same into both halves of a tile of 512; the second is waited for after the first stages' MMAs into the first
+        auto plain_wide = [&](int item_no, int k0, int k1) {
+            const int lead = min(LEAD, k1 - k0);
+            for (int q = 0; q < lead; q++) {
+                const uint32_t sa = stage(ctr + q);
+                if (!ok) return;
+                multiply(tmem_base, sa, sa + A_BYTES, AMN, KB / 16, q == 0, nullptr);
+            }
+            if (item_no > 0 && !mbar_wait(&acce[1], (item_no - 1) & 1, flag)) {
+                ok = false;
+                return;
+            }
+            fence_after();
+            for (int kb = k0; kb < k1; kb++) {
+                const uint32_t sa = stage(ctr);
+                if (!ok) return;
+                if (kb >= k0 + lead) multiply(tmem_base, sa, sa + A_BYTES, AMN, KB / 16, false, nullptr);
+                multiply(tmem_base + AC, sa, sa + A_BYTES + HALF_BYTES, AMN, KB / 16, kb == k0, nullptr);
+                done();
+            }
+        };
+        // accumulator `acc & 1` (of a tile of 512: the first half), once its last contents have been read
         auto accumulator = [&]() -> uint32_t {
-            if (lane == 0 && acc >= 2 && !mbar_wait(&acce[acc & 1], ((acc / 2) - 1) & 1, flag)) ok = false;
+            const int b = WIDE ? 0 : acc & 1, use = WIDE ? acc : acc / 2;
+            if (lane == 0 && use > 0 && !mbar_wait(&acce[b], (use - 1) & 1, flag)) ok = false;
             ok = __shfl_sync(0xffffffffu, ok, 0);
             fence_after();
-            return tmem_base + (uint32_t)((acc & 1) * BN);
+            return tmem_base + (uint32_t)(b * AC);
+        };
+        auto finished = [&]() {
+            if (lane == 0) {
+                mma_commit<CG>(&accf[WIDE ? 0 : acc & 1]);  // the accumulator is complete (or tracks what was issued)
+                if (WIDE) mma_commit<CG>(&accf[1]);
+            }
+            acc++;
         };
         for (int item = first; item < items && ok; item += step) {
             int mb, nb, split;
@@ -358,19 +399,21 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 for (int c0 = kb0; c0 < kb1 && ok; c0 += STATS_KB) {
                     const uint32_t d = accumulator();
                     if (!ok) break;
-                    if (lane == 0) {
-                        plain(d, c0, min(kb1, c0 + STATS_KB));
-                        mma_commit<CG>(&accf[acc & 1]);
-                    }
+                    if (lane == 0) plain(d, c0, min(kb1, c0 + STATS_KB));
                     ok = __shfl_sync(0xffffffffu, ok, 0);
-                    acc++;
+                    finished();
                 }
                 continue;
             }
             const uint32_t d = accumulator();
             if (!ok) break;
             if constexpr (ROWS != ROWS_GROUPED) {
-                if (lane == 0) plain(d, kb0, kb1);
+                if (lane == 0) {
+                    if constexpr (WIDE)
+                        plain_wide(acc, kb0, kb1);
+                    else
+                        plain(d, kb0, kb1);
+                }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
             }
             if constexpr (ROWS != ROWS_PLAIN) {
@@ -387,15 +430,19 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                             const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
                             for (int kb = e0; kb < e1; kb++) {
-                                const uint32_t sa = stage();
+                                const uint32_t sa = stage(ctr);
                                 if (!ok) break;
+                                if constexpr (ROWS == ROWS_GROUPED) {
 #pragma unroll
-                                for (int q = 0; q < MOST; q++) {
-                                    if (q >= count) break;
-                                    if constexpr (ROWS == ROWS_GROUPED)
+                                    for (int q = 0; q < MOST; q++) {
+                                        if (q >= count) break;
                                         multiply(d, sa, sa + A_BYTES + q * B_BYTES, AMN, KB / 16, kb == kb0, &off[q]);
-                                    else
-                                        multiply(d, sa, sa + A_BYTES, false, min(KB / 16, (P.rank - kb * KB + 15) / 16), false, &off[0]);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int w = 0; w < BN / AC; w++)
+                                        multiply(d + w * AC, sa, sa + A_BYTES + w * HALF_BYTES, false,
+                                                 min(KB / 16, (P.rank - kb * KB + 15) / 16), false, &off[0]);
                                 }
                                 done();
                             }
@@ -404,15 +451,25 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                 }
             }
-            if (lane == 0) mma_commit<CG>(&accf[acc & 1]);  // the accumulator is complete (or tracks what was issued)
-            acc++;
+            finished();
         }
         // every issued MMA has completed before the tensor memory is released (bounded)
-        if (lane == 0 && acc > 0) mbar_wait(&accf[(acc - 1) & 1], ((acc - 1) / 2) & 1, flag);
+        if (lane == 0 && acc > 0) {
+            if (WIDE)
+                mbar_wait(&accf[1], (acc - 1) & 1, flag);
+            else
+                mbar_wait(&accf[(acc - 1) & 1], ((acc - 1) / 2) & 1, flag);
+        }
     } else {
-        // ---------------- epilogue: lanes 32 * (warp % 4) .., columns BN / 2 (BN / 4) * (warp / 4) ..
-        const int quad = warp & 3, half = warp >> 2;
-        [[maybe_unused]] float* buf = turn + warp * STAGE_WORDS;
+        // ---------------- epilogue: lanes 32 * (warp % 4) .., quarter warp / 4 of the accumulator's columns
+        constexpr int COLS = AC / 4;  // a thread's: 64, 32 or 16 of one row
+        const int quad = warp & 3, part = warp >> 2;
+        // A thread holds one row, so 32 rows' pieces of 64 bytes are turned in shared memory: a warp then reads or writes whole
+        // sectors, eight rows at a time (piece by piece of 16 bytes and row, a tile's stores took 8000 clocks).  Chunk c of
+        // row r lies at c ^ (r / 2) % 4: neither side meets a bank twice.
+        [[maybe_unused]] unsigned char* buf = turn + warp * TURN_BYTES;
+        [[maybe_unused]] auto chunk = [&](int r, int c) { return reinterpret_cast<uint4*>(buf + r * 64 + ((c ^ (r >> 1)) & 3) * 16); };
+        const uint32_t mine = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * COLS);
         int acc = 0;
         // the accumulator has been read: tell the MMA issuer
         auto release = [&](int b) {
@@ -425,18 +482,17 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     mbar_arrive(&acce[b]);
             }
         };
-        for (int item = first; item < items; item += step) {
+        bool ok = true;
+        for (int item = first; item < items && ok; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
             const int row0 = (mb * CG + rank) * BM + quad * 32, row = row0 + lane;
             const bool live = row < P.m;
+            float z[COLS];
             if constexpr (EPI == EPI_STATS) {
                 const int64_t t = live ? P.target[row] : -1;
                 const int64_t label = (t >= 0 && t < P.vocab) ? t - P.col0 : -1;  // relative to this piece's column 0
                 const int chunks = (P.nkb + STATS_KB - 1) / STATS_KB;
-                constexpr int PB = BN / (32 * STATS_PARTS);  // blocks of 32 columns of a part
-                float z[PB][32];
-                bool ok = true;
                 for (int c = 0; c < chunks; c++, acc++) {
                     if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
                         ok = false;
@@ -444,53 +500,43 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     }
                     fence_after();
 #pragma unroll
-                    for (int q = 0; q < PB * 2; q++) {
+                    for (int q = 0; q < COLS; q += 16) {
                         float v[16];
-                        tmem_ld16(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)((acc & 1) * BN + half * (PB * 32) + q * 16), v);
+                        tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) z[q / 2][q % 2 * 16 + i] = c ? z[q / 2][q % 2 * 16 + i] + v[i] : v[i];
+                        for (int i = 0; i < 16; i++) z[q + i] = c ? z[q + i] + v[i] : v[i];
                     }
                     release(acc & 1);
                 }
                 if (!ok) break;
-                const int c0 = nb * BN + half * (PB * 32), cols = min(PB * 32, P.n - c0);
+                const int c0 = nb * BN + part * COLS, cols = min(COLS, P.n - c0);
                 float top = -INFINITY, sum = 0.0f;
-                if (cols == PB * 32) {
 #pragma unroll
-                    for (int q = 0; q < PB; q++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) top = fmaxf(top, z[q][i]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < PB; q++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            if (q * 32 + i >= cols) z[q][i] = -INFINITY;
-                            top = fmaxf(top, z[q][i]);
-                        }
+                for (int i = 0; i < COLS; i++) {
+                    if (i >= cols) z[i] = -INFINITY;
+                    top = fmaxf(top, z[i]);
                 }
                 // exp2((z - top) log2 e); a row of -inf alone keeps sum 0
                 constexpr float L2E = 1.4426950408889634f;
                 const float ref = top == -INFINITY ? 0.0f : top;
                 const int64_t at = label - c0;
 #pragma unroll
-                for (int q = 0; q < PB; q++) {
-                    if (at >= q * 32 && at < q * 32 + 32) {
-                        float mine = 0.0f;
+                for (int q = 0; q < COLS; q += 16) {
+                    if (at >= q && at < q + 16 && at < cols) {
+                        float own = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (q * 32 + i == at) mine = z[q][i];
-                        if (at < cols) P.label_logit[row] = mine;
+                        for (int i = 0; i < 16; i++)
+                            if (q + i == at) own = z[q + i];
+                        P.label_logit[row] = own;
                     }
-                    float part = 0.0f;
+                    float some = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) part += exp2f((z[q][i] - ref) * L2E);
-                    sum += part;
+                    for (int i = 0; i < 16; i++) some += exp2f((z[q + i] - ref) * L2E);
+                    sum += some;
                 }
-                if (live) P.stats[(int64_t)(nb * STATS_PARTS + half) * P.m + row] = make_float2(top, sum);
+                if (live) P.stats[(int64_t)(nb * STATS_PARTS + part) * P.m + row] = make_float2(top, sum);
                 continue;
             }
-            const int b = acc & 1;
             // what the row's epilogue needs, read while the MMAs run
             float factor = 1.0f, lse = 0.0f, dl = 0.0f;
             int64_t label = -1;  // relative to this piece's column 0
@@ -511,70 +557,100 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     if (P.gain) dl *= *P.gain;
                 }
             }
-            if (!mbar_wait(&accf[b], (acc / 2) & 1, flag)) break;
-            fence_after();
-            acc++;
 #pragma unroll 1
-            for (int cb = half * (BN / 64); cb < (half + 1) * (BN / 64); cb++) {
-                const int c0 = nb * BN + cb * 32;
-                float v[32];
-                tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * BN + cb * 32), v);
-                if (c0 >= P.n || row0 >= P.m) continue;
-                const int cols = min(32, P.n - c0);
+            for (int w = 0; w < BN / AC; w++, acc++) {
+                if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
+                    ok = false;
+                    break;
+                }
+                fence_after();
+#pragma unroll
+                for (int q = 0; q < COLS; q += 16) tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), *reinterpret_cast<float(*)[16]>(&z[q]));
+                release(acc & 1);
+                const int first_col = nb * BN + w * AC + part * COLS;
+                const int rows = min(32, P.m - row0);
+                if (rows <= 0) continue;
                 if constexpr (EPI == EPI_GRAD) {
                     constexpr float L2E = 1.4426950408889634f;
+                    const int at = (label >= first_col && label < first_col + COLS) ? (int)(label - first_col) : -1;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        float p = exp2f((v[i] - lse) * L2E);
-                        if (c0 + i == label) p -= 1.0f;
-                        v[i] = none ? 0.0f : p * dl;
+                    for (int i = 0; i < COLS; i++) {
+                        float p = exp2f((z[i] - lse) * L2E);
+                        if (i == at) p -= 1.0f;
+                        z[i] = none ? 0.0f : p * dl;
                     }
-                }
-                if constexpr (EPI == EPI_STORE) {
-                    if (P.f32in && live) {
-                        const float* src = P.f32in + (int64_t)row * P.ldf + c0;
+                } else {
+                    if (P.f32in || P.f32out) {
+                        // 16 columns of f32 at a time
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (i < cols) v[i] += src[i];
-                    }
+                        for (int q = 0; q < COLS; q += 16) {
+                            const int c0 = first_col + q, cols = min(16, P.n - c0);
+                            if (cols <= 0) break;
+                            if (P.f32in) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = (ROWS == ROWS_GROUPED && none) ? 0.0f : v[i] * factor;
-                    if (P.f32out && live) {
-                        float* dst = P.f32out + (int64_t)split * P.split_stride + (int64_t)row * P.ldf + c0;
-                        if (cols == 32) {
+                                for (int i = 0; i < 4; i++) {
+                                    const int r = i * 8 + lane / 4, c = (lane & 3) * 4;
+                                    const float* src = P.f32in + (int64_t)(row0 + r) * P.ldf + c0 + c;
+                                    float4 f = make_float4(0, 0, 0, 0);
+                                    if (r < rows && c < cols) f = *reinterpret_cast<const float4*>(src);  // ldf is a multiple of 4
+                                    *reinterpret_cast<float4*>(chunk(r, lane & 3)) = f;
+                                }
+                                __syncwarp();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<float4*>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        } else {
+                                for (int i = 0; i < 4; i++) {
+                                    const float4 f = *reinterpret_cast<const float4*>(chunk(lane, i));
+                                    z[q + 4 * i] += f.x, z[q + 4 * i + 1] += f.y, z[q + 4 * i + 2] += f.z, z[q + 4 * i + 3] += f.w;
+                                }
+                                __syncwarp();
+                            }
+                            if (P.f32out) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (i < cols) dst[i] = v[i];
+                                for (int i = 0; i < 4; i++)
+                                    *reinterpret_cast<float4*>(chunk(lane, i)) =
+                                        (ROWS == ROWS_GROUPED && none) ? make_float4(0, 0, 0, 0)
+                                                                       : make_float4(z[q + 4 * i], z[q + 4 * i + 1], z[q + 4 * i + 2], z[q + 4 * i + 3]);
+                                __syncwarp();
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const int r = i * 8 + lane / 4, c = (lane & 3) * 4;
+                                    float* dst = P.f32out + (int64_t)split * P.split_stride + (int64_t)(row0 + r) * P.ldf + c0 + c;
+                                    if (r < rows && c < cols) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(chunk(r, lane & 3));
+                                }
+                                __syncwarp();
+                            }
                         }
                     }
                     if (!P.out) continue;
+#pragma unroll
+                    for (int i = 0; i < COLS; i++) z[i] *= factor;
                 }
-                uint16_t* out = reinterpret_cast<uint16_t*>(P.out);
-                if (P.out_vec && cols == 32) {
-                    if (live) {
-                        uint16_t* dst = out + (int64_t)row * P.ldo + c0;
+                // 32 columns of 16 bits at a time (16 where the thread has no more)
+                constexpr int PIECE = COLS < 32 ? COLS : 32, CH = PIECE / 8;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-                            *reinterpret_cast<uint4*>(dst + i) =
-                                make_uint4(pack2<BF16>(v[i], v[i + 1]), pack2<BF16>(v[i + 2], v[i + 3]),
-                                           pack2<BF16>(v[i + 4], v[i + 5]), pack2<BF16>(v[i + 6], v[i + 7]));
+                for (int q = 0; q < COLS; q += PIECE) {
+                    const int c0 = first_col + q, cols = min(PIECE, P.n - c0);
+                    if (cols <= 0) break;
+#pragma unroll
+                    for (int i = 0; i < CH; i++) {
+                        const float* v = &z[q + 8 * i];
+                        *chunk(lane, i) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
                     }
-                } else {
-                    // rows that start anywhere: turned in shared memory so that a warp writes along one row
-#pragma unroll
-                    for (int i = 0; i < 32; i++) buf[lane * 33 + i] = v[i];
                     __syncwarp();
-                    const int rows = min(32, P.m - row0);
-                    for (int r = 0; r < rows; r++)
-                        if (lane < cols) out[(int64_t)(row0 + r) * P.ldo + c0 + lane] = pack1<BF16>(buf[r * 33 + lane]);
+                    uint16_t* out = reinterpret_cast<uint16_t*>(P.out);
+                    if (P.out_vec && cols == PIECE) {
+#pragma unroll
+                        for (int i = 0; i < CH; i++) {
+                            const int r = i * (32 / CH) + lane / CH, c = lane % CH;
+                            if (r < rows) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + r) * P.ldo + c0 + c * 8) = *chunk(r, c);
+                        }
+                    } else {
+                        // rows that start anywhere: a warp writes along one row
+                        for (int r = 0; r < rows; r++)
+                            if (lane < cols) out[(int64_t)(row0 + r) * P.ldo + c0 + lane] = reinterpret_cast<const uint16_t*>(chunk(r, lane / 8))[lane & 7];
+                    }
                     __syncwarp();
                 }
             }
-            release(b);
         }
     }
 

@@ -15,13 +15,13 @@ template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
 static int launch_one(const Maps& maps, const Params& p, cudaStream_t st) {
     auto kern = half_gemm_kernel<BF16, AMN, BMN, CG, BN, ROWS, EPI>;
     static std::atomic<uint64_t> done{0};
-    if (int rc = allow_smem(kern, smem_bytes(EPI), done, "half_gemm_kernel shared memory")) return rc;
+    if (int rc = allow_smem(kern, smem_bytes(), done, "half_gemm_kernel shared memory")) return rc;
     const int64_t items = (int64_t)p.ntiles * p.splits;
     const int most = sm_count() / CG;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(CG * (items < most ? items : most)));
-    cfg.blockDim = dim3(threads(EPI));
-    cfg.dynamicSmemBytes = smem_bytes(EPI);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem_bytes();
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -39,6 +39,9 @@ static int launch_tile(int cg, int bn, const Maps& maps, const Params& p, cudaSt
     if constexpr (ROWS == ROWS_GROUPED) {
         return launch_one<BF16, AMN, BMN, 1, 64, ROWS, EPI>(maps, p, st);
     } else {
+        if constexpr (EPI != EPI_STATS) {
+            if (bn == 512) return launch_one<BF16, AMN, BMN, 2, 512, ROWS, EPI>(maps, p, st);
+        }
         if (cg == 2 && bn == 256) return launch_one<BF16, AMN, BMN, 2, 256, ROWS, EPI>(maps, p, st);
         if (cg == 2) return launch_one<BF16, AMN, BMN, 2, 128, ROWS, EPI>(maps, p, st);
         if (bn == 128) return launch_one<BF16, AMN, BMN, 1, 128, ROWS, EPI>(maps, p, st);
