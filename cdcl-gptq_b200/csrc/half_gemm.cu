@@ -89,9 +89,10 @@ static int encode(CUtensorMap* map, const HalfOperand& o, bool bf16, bool batche
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The plan of least estimated time, in clocks.  A K block of a tile costs a CTA its MMAs (128 columns: 256 clocks, shared by
-// a pair) or its operands' way through L2, at 48 bytes a clock and SM (measured over 64 x 512 KB tiles of 256 x 256: 47),
-// whichever is longer; an item 1500 for its start and end; splitting K the f32 sums' way out and back and a launch.
+// The plan of least estimated time, in clocks, from what was measured on products of 2048..8191 rows: what a K block of 64
+// costs a tile (512 clocks of MMAs for 256 x 256; its operands' way through L2 for the narrower ones), and what an item costs
+// beside (filling the pipeline; a tile of 512 is not taken out of tensor memory while the next one's MMAs run at full rate).
+// Splitting K adds the f32 sums' way out and back, and a launch.
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
     const bool store = form != HALF_STATS && form != HALF_GRAD;
     const bool grouped = form == HALF_NT_GROUPED || form == HALF_NN_GROUPED;
@@ -103,18 +104,18 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
         p.splits = (int)std::max<int64_t>(1, std::min(2 * sms / tiles, nkb / 4));
         p.splits = (int)ceil_div(nkb, ceil_div(nkb, p.splits));
     } else {
-        static const struct { int cg, bn; } shapes[] = {{2, 512}, {2, 256}, {2, 128}, {1, 128}, {1, 64}};
+        static const struct { int cg, bn, block, item; } shapes[] = {
+            {2, 512, 1060, 6000}, {2, 256, 630, 3000}, {2, 128, 450, 3000}, {1, 128, 560, 2500}, {1, 64, 430, 2000}};
         double best = 1e300;
         for (const auto& s : shapes) {
             if ((s.bn == 64 && !store) || (s.bn == 512 && form == HALF_STATS)) continue;
             if (s.cg == 2 && m <= BM) continue;  // the second CTA's rows would be empty
             const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
-            const double block = std::max(2.0 * s.bn, (BM + s.bn / s.cg) * KB * 2 / 48.0);
             const int64_t most = store ? std::max<int64_t>(1, std::min(slots / tiles, nkb / 8)) : 1;
             for (int64_t want = 1; want <= most; want++) {
                 const int64_t per = ceil_div(nkb, want), splits = ceil_div(nkb, per);
                 if (splits != want) continue;
-                double cost = (double)ceil_div(tiles * splits, slots) * (per * block + 1500.0);
+                double cost = (double)ceil_div(tiles * splits, slots) * ((double)per * s.block + s.item);
                 if (splits > 1) cost += 6000.0 + (splits + 1.0) * m * n * 4.0 / 2000.0;
                 if (cost < best) {
                     best = cost;

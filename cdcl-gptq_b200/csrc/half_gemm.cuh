@@ -314,66 +314,79 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (!mbar_wait(&empty[k % NS], (k / NS) & 1, flag) && rank == 0) mbar_wait(&full[k % NS], (k / NS) & 1, flag);
     } else if (warp == EPI_WARPS + 1) {
         // ---------------- MMA issuer, of the pair's first CTA
-        int ctr = 0, acc = 0;
+        int acc = 0;
         bool ok = rank == 0;
-        // waits for stage `c`; returns its address (0 when the wait ran out)
-        auto stage = [&](int c) -> uint32_t {
-            const int s = c % NS;
-            if (!mbar_wait(&full[s], (c / NS) & 1, flag)) {
+        int slot = 0;        // of the next stage
+        uint32_t phase = 0;  // parity of its barrier
+        // the next stage's operands are there (false: the wait ran out); a look at the barrier may have shown it already
+        auto arrived = [&](bool seen) -> bool {
+            if (!seen && !mbar_wait(&full[slot], phase, flag)) {
                 ok = false;
-                return 0;
+                return false;
             }
             fence_after();
-            return ring + s * STAGE_BYTES;
+            return true;
         };
-        // the MMAs of one operand pair: `ks` steps of 16; A is MN-major only where `amn`; with `off`, of some rows only
-        auto multiply = [&](uint32_t d, uint32_t sa, uint32_t sb, bool amn, int ks, bool fresh, const uint32_t (*off)[4 * CG]) {
+        auto advance = [&](int& s, uint32_t& p) {
+            if (++s == NS) s = 0, p ^= 1;
+        };
+        // the stage is free once the MMAs issued so far have read it; a look at the next one while they run
+        auto done = [&]() -> bool {
+            mma_commit<CG>(&empty[slot]);
+            advance(slot, phase);
+            return mbar_try(&full[slot], phase);
+        };
+        // descriptors of the first stage's operands; a stage, a half and a step of 16 further are added to their addresses
+        constexpr uint64_t A_STEP = (AMN ? 2048 : 32) >> 4, B_STEP = (BMN ? 2048 : 32) >> 4;
+        const uint64_t desc_a = AMN ? smem_desc(ring, 64 * KB * 2, 1024) : smem_desc(ring, 16, 1024);
+        const uint64_t desc_u = smem_desc(ring, 16, 1024);  // the extension's first operand is K-major
+        const uint64_t desc_b = BMN ? smem_desc(ring + A_BYTES, 64 * KB * 2, 1024) : smem_desc(ring + A_BYTES, 16, 1024);
+        constexpr uint32_t ID = idesc_half(BF16, AMN, BMN, CG * BM, AC), ID_U = idesc_half(BF16, false, BMN, CG * BM, AC);
+        // the four MMAs of a stage's operands into d
+        auto multiply = [&](uint32_t d, int s, int half, bool fresh) {
+            const uint64_t da = desc_a + (uint64_t)(s * (STAGE_BYTES >> 4)), db = desc_b + (uint64_t)(s * (STAGE_BYTES >> 4) + half * (HALF_BYTES >> 4));
 #pragma unroll
-            for (int k = 0; k < KB / 16; k++) {
-                if (k < ks) {
-                    const uint64_t da = amn ? smem_desc(sa + k * 2048, 64 * KB * 2, 1024) : smem_desc(sa + k * 32, 16, 1024);
-                    const uint64_t db = BMN ? smem_desc(sb + k * 2048, 64 * KB * 2, 1024) : smem_desc(sb + k * 32, 16, 1024);
-                    const uint32_t id = idesc_half(BF16, amn, BMN, CG * BM, AC);
-                    if (off)
-                        mma_half_rows(d, da, db, id, (fresh && k == 0) ? 0u : 1u, *off);
-                    else
-                        mma_half<CG>(d, da, db, id, (fresh && k == 0) ? 0u : 1u);
-                }
-            }
+            for (int k = 0; k < KB / 16; k++) mma_half<CG>(d, da + k * A_STEP, db + k * B_STEP, ID, (fresh && k == 0) ? 0u : 1u);
         };
-        // the stage is free once the MMAs issued so far have read it
-        auto done = [&]() {
-            mma_commit<CG>(&empty[ctr % NS]);
-            ctr++;
+        // `ks` of them for some rows only; at: 16-byte units from the stage's second operand
+        auto multiply_rows = [&](uint32_t d, int s, int at, bool u, int ks, bool fresh, const uint32_t (&off)[4 * CG]) {
+            const uint64_t da = (u ? desc_u : desc_a) + (uint64_t)(s * (STAGE_BYTES >> 4)), db = desc_b + (uint64_t)(s * (STAGE_BYTES >> 4) + at);
+#pragma unroll
+            for (int k = 0; k < KB / 16; k++)
+                if (k < ks) mma_half_rows(d, da + k * (u ? 2 : A_STEP), db + k * B_STEP, u ? ID_U : ID, (fresh && k == 0) ? 0u : 1u, off);
         };
         // the K blocks k0 .. k1 into accumulator d
         auto plain = [&](uint32_t d, int k0, int k1) {
+            bool seen = false;
             for (int kb = k0; kb < k1; kb++) {
-                const uint32_t sa = stage(ctr);
-                if (!ok) break;
-                multiply(d, sa, sa + A_BYTES, AMN, KB / 16, kb == k0, nullptr);
-                done();
+                if (!arrived(seen)) break;
+                multiply(d, slot, 0, kb == k0);
+                seen = done();
             }
         };
         // the same into both halves of a tile of 512; the second is waited for after the first stages' MMAs into the first
         auto plain_wide = [&](int item_no, int k0, int k1) {
             const int lead = min(LEAD, k1 - k0);
+            const int slot0 = slot;
+            const uint32_t phase0 = phase;
             for (int q = 0; q < lead; q++) {
-                const uint32_t sa = stage(ctr + q);
-                if (!ok) return;
-                multiply(tmem_base, sa, sa + A_BYTES, AMN, KB / 16, q == 0, nullptr);
+                if (!arrived(false)) return;
+                multiply(tmem_base, slot, 0, q == 0);
+                advance(slot, phase);
             }
+            slot = slot0;
+            phase = phase0;
             if (item_no > 0 && !mbar_wait(&acce[1], (item_no - 1) & 1, flag)) {
                 ok = false;
                 return;
             }
             fence_after();
+            bool seen = true;
             for (int kb = k0; kb < k1; kb++) {
-                const uint32_t sa = stage(ctr);
-                if (!ok) return;
-                if (kb >= k0 + lead) multiply(tmem_base, sa, sa + A_BYTES, AMN, KB / 16, false, nullptr);
-                multiply(tmem_base + AC, sa, sa + A_BYTES + HALF_BYTES, AMN, KB / 16, kb == k0, nullptr);
-                done();
+                if (!arrived(seen)) return;
+                if (kb >= k0 + lead) multiply(tmem_base, slot, 0, false);
+                multiply(tmem_base + AC, slot, 1, kb == k0);
+                seen = done();
             }
         };
         // accumulator `acc & 1` (of a tile of 512: the first half), once its last contents have been read
@@ -430,19 +443,18 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
                             const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
                             for (int kb = e0; kb < e1; kb++) {
-                                const uint32_t sa = stage(ctr);
-                                if (!ok) break;
+                                if (!arrived(false)) break;
                                 if constexpr (ROWS == ROWS_GROUPED) {
 #pragma unroll
                                     for (int q = 0; q < MOST; q++) {
                                         if (q >= count) break;
-                                        multiply(d, sa, sa + A_BYTES + q * B_BYTES, AMN, KB / 16, kb == kb0, &off[q]);
+                                        multiply_rows(d, slot, q * (B_BYTES >> 4), false, KB / 16, kb == kb0, off[q]);
                                     }
                                 } else {
 #pragma unroll
                                     for (int w = 0; w < BN / AC; w++)
-                                        multiply(d + w * AC, sa, sa + A_BYTES + w * HALF_BYTES, false,
-                                                 min(KB / 16, (P.rank - kb * KB + 15) / 16), false, &off[0]);
+                                        multiply_rows(d + w * AC, slot, w * (HALF_BYTES >> 4), true,
+                                                      min(KB / 16, (P.rank - kb * KB + 15) / 16), false, off[0]);
                                 }
                                 done();
                             }
@@ -482,14 +494,31 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     mbar_arrive(&acce[b]);
             }
         };
+        // writes `cols` of `piece` columns from c0 of the rows in the buffer
+        [[maybe_unused]] auto put_rows = [&](int piece, int c0, int cols, int rows, int row0) {
+            uint16_t* out = reinterpret_cast<uint16_t*>(P.out);
+            const int ch = piece / 8;
+            if (P.out_vec && cols == piece) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = i * (32 / ch) + lane / ch, c = lane % ch;
+                    if (i < ch && r < rows) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + r) * P.ldo + c0 + c * 8) = *chunk(r, c);
+                }
+            } else {
+                // rows that start anywhere: a warp writes along one row
+                for (int r = 0; r < rows; r++)
+                    if (lane < cols) out[(int64_t)(row0 + r) * P.ldo + c0 + lane] = reinterpret_cast<const uint16_t*>(chunk(r, lane / 8))[lane & 7];
+            }
+            __syncwarp();
+        };
         bool ok = true;
         for (int item = first; item < items && ok; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
             const int row0 = (mb * CG + rank) * BM + quad * 32, row = row0 + lane;
             const bool live = row < P.m;
-            float z[COLS];
             if constexpr (EPI == EPI_STATS) {
+                float z[COLS];
                 const int64_t t = live ? P.target[row] : -1;
                 const int64_t label = (t >= 0 && t < P.vocab) ? t - P.col0 : -1;  // relative to this piece's column 0
                 const int chunks = (P.nkb + STATS_KB - 1) / STATS_KB;
@@ -557,35 +586,25 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     if (P.gain) dl *= *P.gain;
                 }
             }
-#pragma unroll 1
-            for (int w = 0; w < BN / AC; w++, acc++) {
-                if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
-                    ok = false;
-                    break;
-                }
+            const int rows = min(32, P.m - row0);
+            // waits for the accumulator of the tile's half `w` (or the whole tile)
+            auto complete = [&]() -> bool {
+                if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) ok = false;
                 fence_after();
-#pragma unroll
-                for (int q = 0; q < COLS; q += 16) tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), *reinterpret_cast<float(*)[16]>(&z[q]));
-                release(acc & 1);
-                const int first_col = nb * BN + w * AC + part * COLS;
-                const int rows = min(32, P.m - row0);
-                if (rows <= 0) continue;
-                if constexpr (EPI == EPI_GRAD) {
-                    constexpr float L2E = 1.4426950408889634f;
-                    const int at = (label >= first_col && label < first_col + COLS) ? (int)(label - first_col) : -1;
-#pragma unroll
-                    for (int i = 0; i < COLS; i++) {
-                        float p = exp2f((z[i] - lse) * L2E);
-                        if (i == at) p -= 1.0f;
-                        z[i] = none ? 0.0f : p * dl;
-                    }
-                } else {
-                    if (P.f32in || P.f32out) {
-                        // 16 columns of f32 at a time
-#pragma unroll
+                return ok;
+            };
+            if constexpr (EPI == EPI_STORE) {
+                if (P.f32in || P.f32out) {
+                    // f32 sums, 16 columns at a time
+#pragma unroll 1
+                    for (int w = 0; w < BN / AC; w++, acc++) {
+                        if (!complete()) break;
+#pragma unroll 1
                         for (int q = 0; q < COLS; q += 16) {
-                            const int c0 = first_col + q, cols = min(16, P.n - c0);
-                            if (cols <= 0) break;
+                            float z[16];
+                            tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), z);
+                            const int c0 = nb * BN + w * AC + part * COLS + q, cols = min(16, P.n - c0);
+                            if (cols <= 0 || rows <= 0) continue;
                             if (P.f32in) {
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
@@ -599,16 +618,16 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
                                     const float4 f = *reinterpret_cast<const float4*>(chunk(lane, i));
-                                    z[q + 4 * i] += f.x, z[q + 4 * i + 1] += f.y, z[q + 4 * i + 2] += f.z, z[q + 4 * i + 3] += f.w;
+                                    z[4 * i] += f.x, z[4 * i + 1] += f.y, z[4 * i + 2] += f.z, z[4 * i + 3] += f.w;
                                 }
                                 __syncwarp();
                             }
                             if (P.f32out) {
 #pragma unroll
                                 for (int i = 0; i < 4; i++)
-                                    *reinterpret_cast<float4*>(chunk(lane, i)) =
-                                        (ROWS == ROWS_GROUPED && none) ? make_float4(0, 0, 0, 0)
-                                                                       : make_float4(z[q + 4 * i], z[q + 4 * i + 1], z[q + 4 * i + 2], z[q + 4 * i + 3]);
+                                    *reinterpret_cast<float4*>(chunk(lane, i)) = (ROWS == ROWS_GROUPED && none)
+                                                                                     ? make_float4(0, 0, 0, 0)
+                                                                                     : make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
                                 __syncwarp();
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
@@ -618,37 +637,63 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                 }
                                 __syncwarp();
                             }
+                            if (P.out) {
+#pragma unroll
+                                for (int i = 0; i < 2; i++)
+                                    *chunk(lane, i) = make_uint4(pack2<BF16>(z[8 * i] * factor, z[8 * i + 1] * factor),
+                                                                 pack2<BF16>(z[8 * i + 2] * factor, z[8 * i + 3] * factor),
+                                                                 pack2<BF16>(z[8 * i + 4] * factor, z[8 * i + 5] * factor),
+                                                                 pack2<BF16>(z[8 * i + 6] * factor, z[8 * i + 7] * factor));
+                                __syncwarp();
+                                put_rows(16, c0, cols, rows, row0);
+                            }
+                        }
+                        release(acc & 1);
+                    }
+                    continue;
+                }
+            }
+            // A tile of 512 leaves tensor memory as 16-bit numbers, both halves, before any is written: all CTAs finish their
+            // tiles at about the same time, and 64 KB a half then wait 3000 clocks for L2.
+            uint32_t packed[BN / AC][COLS / 2];
+#pragma unroll
+            for (int w = 0; w < BN / AC; w++, acc++) {
+                if (!complete()) break;
+                const int first_col = nb * BN + w * AC + part * COLS;
+#pragma unroll
+                for (int q = 0; q < COLS; q += 16) {
+                    float z[16];
+                    tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), z);
+                    if constexpr (EPI == EPI_GRAD) {
+                        constexpr float L2E = 1.4426950408889634f;
+                        const int c0 = first_col + q, at = (label >= c0 && label < c0 + 16) ? (int)(label - c0) : -1;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            float p = exp2f((z[i] - lse) * L2E);
+                            if (i == at) p -= 1.0f;
+                            z[i] = none ? 0.0f : p * dl;
                         }
                     }
-                    if (!P.out) continue;
 #pragma unroll
-                    for (int i = 0; i < COLS; i++) z[i] *= factor;
+                    for (int i = 0; i < 8; i++) packed[w][q / 2 + i] = pack2<BF16>(z[2 * i] * factor, z[2 * i + 1] * factor);
                 }
-                // 32 columns of 16 bits at a time (16 where the thread has no more)
-                constexpr int PIECE = COLS < 32 ? COLS : 32, CH = PIECE / 8;
+                release(acc & 1);
+            }
+            if (!ok || rows <= 0 || !P.out) continue;
+#pragma unroll
+            for (int w = 0; w < BN / AC; w++) {
+                // 32 columns at a time (16 where the thread has no more)
+                constexpr int PIECE = COLS < 32 ? COLS : 32;
 #pragma unroll
                 for (int q = 0; q < COLS; q += PIECE) {
-                    const int c0 = first_col + q, cols = min(PIECE, P.n - c0);
+                    const int c0 = nb * BN + w * AC + part * COLS + q, cols = min(PIECE, P.n - c0);
                     if (cols <= 0) break;
 #pragma unroll
-                    for (int i = 0; i < CH; i++) {
-                        const float* v = &z[q + 8 * i];
-                        *chunk(lane, i) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
-                    }
+                    for (int i = 0; i < PIECE / 8; i++)
+                        *chunk(lane, i) = make_uint4(packed[w][q / 2 + 4 * i], packed[w][q / 2 + 4 * i + 1], packed[w][q / 2 + 4 * i + 2],
+                                                     packed[w][q / 2 + 4 * i + 3]);
                     __syncwarp();
-                    uint16_t* out = reinterpret_cast<uint16_t*>(P.out);
-                    if (P.out_vec && cols == PIECE) {
-#pragma unroll
-                        for (int i = 0; i < CH; i++) {
-                            const int r = i * (32 / CH) + lane / CH, c = lane % CH;
-                            if (r < rows) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + r) * P.ldo + c0 + c * 8) = *chunk(r, c);
-                        }
-                    } else {
-                        // rows that start anywhere: a warp writes along one row
-                        for (int r = 0; r < rows; r++)
-                            if (lane < cols) out[(int64_t)(row0 + r) * P.ldo + c0 + lane] = reinterpret_cast<const uint16_t*>(chunk(r, lane / 8))[lane & 7];
-                    }
-                    __syncwarp();
+                    put_rows(PIECE, c0, cols, rows, row0);
                 }
             }
         }
