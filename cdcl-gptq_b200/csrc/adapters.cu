@@ -29,6 +29,17 @@ __device__ __forceinline__ uint16_t half_bits(float v) {
     return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
+template <bool BF16>
+__device__ __forceinline__ float half_value(uint16_t v) {
+    return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
+}
+// v - h, rounded: with h = v rounded, h + rest has twice the significand.  An infinity is all in h.
+template <bool BF16>
+__device__ __forceinline__ uint16_t rest_bits(float v, uint16_t h) {
+    const float high = half_value<BF16>(h);
+    return half_bits<BF16>(fabsf(high) < INFINITY ? v - high : 0.0f);
+}
+
 // Each adapter's tokens in ascending order, one CTA (1024 threads) an adapter: start[i] = tokens of lower adapters.
 __device__ __forceinline__ void token_list(const int* __restrict__ index, int t, int n, int id, int* __restrict__ start,
                                            int* __restrict__ order) {
@@ -72,6 +83,7 @@ struct FinishArgs {
     uint16_t* u16;         // the sums, rounded, or null
     int64_t ldu;
     uint16_t* su16;        // scale of the row's adapter times the sums, rounded, or null
+    uint16_t* rest16;      // what the rounding took off, rounded, or null
     int64_t lds;
     float* su32;           // the same, not rounded, [t][r], or null
     int* start;            // the adapters' token lists, or null
@@ -98,7 +110,9 @@ __global__ void __launch_bounds__(1024) rank_finish_kernel(const FinishArgs P) {
         if (P.su16 || P.su32) {
             const int id = P.index[row];
             const float v = (id >= 0 && id < P.n) ? P.scale[id] * s : 0.0f;
-            if (P.su16) P.su16[row * P.lds + c] = half_bits<BF16>(v);
+            const uint16_t h = half_bits<BF16>(v);
+            if (P.su16) P.su16[row * P.lds + c] = h;
+            if (P.rest16) P.rest16[row * P.lds + c] = rest_bits<BF16>(v, h);
             if (P.su32) P.su32[i] = v;
         }
     }
@@ -121,8 +135,11 @@ struct OuterArgs {
     int64_t ldw;
     int cols;
     int wide16;                // its rows can be read 16 bytes at a time
-    const uint16_t* narrow;    // [t][r] 16-bit, or null:
+    const uint16_t* narrow;    // [t][ldn] 16-bit, and
+    const uint16_t* rest;      // what is added to it, or null; with codes both are null:
     const float* narrow32;     // [t][r]
+    int64_t ldn;
+    int narrow16;              // its rows can be read 16 bytes at a time
     const float* factor;       // [n] or null
     uint16_t* out;             // dA: [n][r][cols], dB: [n][cols][r]
     int by_rank;               // the rank is the last index (dB)
@@ -179,10 +196,6 @@ struct OuterStage {
 };
 
 template <bool BF16>
-__device__ __forceinline__ float half_value(uint16_t v) {
-    return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-}
-template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (BF16)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -194,14 +207,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// NARROW32: the narrow factor is f32 and enters as high + low.
-template <bool BF16, bool CODES, bool NARROW32>
+// LOW: the narrow factor is high + low.
+template <bool BF16, bool CODES, bool LOW>
 __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& Q, OuterStage* ring, const int* list, int count, int id,
                                            int chunks, int slot, int tile, int k0) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c0 = tile * OUTER_COLS, ranks = min(OUTER_RANK, P.r - k0);
-    const int nb = (Q.cols + 127) / 128, steps = (count + OUTER_TOK - 1) / OUTER_TOK;
-    const int row = tid >> 3, part = tid & 7, c = c0 + part * 16;  // wide: 8 threads a token, 16 columns each
+    const int steps = (count + OUTER_TOK - 1) / OUTER_TOK;
+    const int row = tid >> 3, part = tid & 7, c = c0 + part * 16;  // 8 threads a token, with 16 columns and 8 ranks each
+    const int in = min(8, ranks - part * 8);                       // of this thread's ranks
     // a warp's share: 32 columns, one half of a stage's tokens; the halves are added at the end
     const int m0 = (warp & 3) * 32, kk = (warp >> 2) * 16;
     float acc[2][8][4];
@@ -212,85 +226,102 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
 #pragma unroll
             for (int i = 0; i < 4; i++) acc[m][j][i] = 0.0f;
 
-    // registers of the stage being fetched: a thread's 8 ranks of its token, and its 16 codes
+    auto token = [&](int s) {
+        const int k = s * OUTER_TOK + row;
+        return k < count ? list[k] : -1;
+    };
+    // 16-bit matrices: copies on their way to stage s
+    auto copy = [&](int s) {
+        const int tok = token(s);
+        OuterStage& st = ring[s % OUTER_STAGES];
+        const uint16_t* src = Q.wide + (int64_t)max(tok, 0) * Q.ldw + c;
+        uint16_t* dst = &st.wide[row][part * 16];
+        if (Q.wide16) {
+            const bool first = tok >= 0 && c + 8 <= Q.cols, second = tok >= 0 && c + 16 <= Q.cols;
+            copy16(dst, first ? src : Q.wide, first);
+            copy16(dst + 8, second ? src + 8 : Q.wide, second);
+        } else {
+            for (int i = 0; i < 16; i++) dst[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (uint16_t)0;
+        }
+        const int64_t at = (int64_t)max(tok, 0) * Q.ldn + k0 + part * 8;
+        uint16_t* high = &st.high[row][part * 8];
+        uint16_t* low = &st.low[row][part * 8];
+        if (Q.narrow16 && (in <= 0 || in == 8)) {
+            const bool live = tok >= 0 && in > 0;
+            copy16(high, live ? Q.narrow + at : Q.wide, live);
+            if constexpr (LOW) copy16(low, live ? Q.rest + at : Q.wide, live);
+        } else {
+            for (int i = 0; i < 8; i++) {
+                high[i] = (tok >= 0 && i < in) ? Q.narrow[at + i] : (uint16_t)0;
+                if constexpr (LOW) low[i] = (tok >= 0 && i < in) ? Q.rest[at + i] : (uint16_t)0;
+            }
+        }
+    };
+    // a checkpoint: a thread's 16 codes and 8 ranks of its token, through registers
     float nv[8];
     uint4 qv = make_uint4(0, 0, 0, 0);
     auto fetch = [&](int s) {
-        const int k = s * OUTER_TOK + row;
-        const int tok = k < count ? list[k] : -1;
-        OuterStage& st = ring[s % OUTER_STAGES];
-        float f = 1.0f;
-        if constexpr (CODES) {
-            if (tok >= 0) f = Q.scales[(int64_t)tok * nb + tile];
-            const int8_t* src = Q.codes + (int64_t)max(tok, 0) * Q.cols + c;
-            if (tok >= 0 && Q.wide16 && c + 16 <= Q.cols) {
-                qv = *reinterpret_cast<const uint4*>(src);
-            } else {
-                alignas(16) int8_t q[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) q[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (int8_t)0;
-                qv = *reinterpret_cast<uint4*>(q);
-            }
+        const int tok = token(s);
+        const float f = tok >= 0 ? Q.scales[(int64_t)tok * ((Q.cols + 127) / 128) + tile] : 0.0f;
+        const int8_t* src = Q.codes + (int64_t)max(tok, 0) * Q.cols + c;
+        if (tok >= 0 && Q.wide16 && c + 16 <= Q.cols) {
+            qv = *reinterpret_cast<const uint4*>(src);
         } else {
-            const uint16_t* src = Q.wide + (int64_t)max(tok, 0) * Q.ldw + c;
-            uint16_t* dst = &st.wide[row][part * 16];
-            if (Q.wide16) {
-                copy16(dst, tok >= 0 && c + 8 <= Q.cols ? src : Q.wide, tok >= 0 && c + 8 <= Q.cols);
-                copy16(dst + 8, tok >= 0 && c + 16 <= Q.cols ? src + 8 : Q.wide, tok >= 0 && c + 16 <= Q.cols);
-            } else {
-                for (int i = 0; i < 16; i++) dst[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (uint16_t)0;
-            }
-        }
+            alignas(16) int8_t q[16];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const bool in = tok >= 0 && part * 8 + i < ranks;
-            const int64_t at = (int64_t)max(tok, 0) * P.r + k0 + part * 8 + i;
-            nv[i] = 0.0f;
-            if (in) nv[i] = NARROW32 ? Q.narrow32[at] : half_value<BF16>(Q.narrow[at]);
-            // a checkpoint's values are code * scale, one scale for these 128 columns: it joins the narrow factor, so that
-            // the codes enter the tensor instruction exactly
-            if constexpr (CODES) {
-                if (in) nv[i] *= f;
-            }
+            for (int i = 0; i < 16; i++) q[i] = (tok >= 0 && c + i < Q.cols) ? src[i] : (int8_t)0;
+            qv = *reinterpret_cast<uint4*>(q);
         }
+        // a checkpoint's values are code * scale, one scale for these 128 columns: it joins the narrow factor, so that the
+        // codes enter the tensor instruction exactly
+        const float* v = Q.narrow32 + (int64_t)max(tok, 0) * P.r + k0 + part * 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++) nv[i] = (tok >= 0 && i < in) ? v[i] * f : 0.0f;
     };
-    // what fetch() left in registers goes to its stage
     auto put = [&](int s) {
         OuterStage& st = ring[s % OUTER_STAGES];
-        alignas(16) uint16_t h[8], l[8];
+        alignas(16) uint16_t h[8], l[8], w[16];
+        alignas(16) int8_t q[16];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             h[i] = half_bits<BF16>(nv[i]);
-            const float high = half_value<BF16>(h[i]);
-            l[i] = half_bits<BF16>(fabsf(high) < INFINITY ? nv[i] - high : 0.0f);  // an infinity is all in the high part
+            l[i] = rest_bits<BF16>(nv[i], h[i]);
         }
         *reinterpret_cast<uint4*>(&st.high[row][part * 8]) = *reinterpret_cast<uint4*>(h);
-        if constexpr (NARROW32) *reinterpret_cast<uint4*>(&st.low[row][part * 8]) = *reinterpret_cast<uint4*>(l);
-        if constexpr (CODES) {
-            alignas(16) int8_t q[16];
-            alignas(16) uint16_t v[16];
-            *reinterpret_cast<uint4*>(q) = qv;
+        *reinterpret_cast<uint4*>(&st.low[row][part * 8]) = *reinterpret_cast<uint4*>(l);
+        *reinterpret_cast<uint4*>(q) = qv;
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = half_bits<BF16>((float)q[i]);
-            uint16_t* dst = &st.wide[row][part * 16];
-            reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<uint4*>(v)[0];
-            reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<uint4*>(v)[1];
-        }
+        for (int i = 0; i < 16; i++) w[i] = half_bits<BF16>((float)q[i]);
+        uint16_t* dst = &st.wide[row][part * 16];
+        reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<uint4*>(w)[0];
+        reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<uint4*>(w)[1];
     };
+    constexpr int AHEAD = OUTER_STAGES - 1;
 #pragma unroll 1
-    for (int s = 0; s < OUTER_STAGES - 1; s++) {
+    for (int s = 0; s < AHEAD; s++) {
         if (s < steps) {
-            fetch(s);
-            put(s);
+            if constexpr (CODES) {
+                fetch(s);
+                put(s);
+            } else {
+                copy(s);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    if constexpr (CODES) {
+        if (AHEAD < steps) fetch(AHEAD);
     }
 #pragma unroll 1
     for (int s = 0; s < steps; s++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(OUTER_STAGES - 2) : "memory");
         __syncthreads();  // stage s is there, and stage s - 1 has been used by every warp
-        const int next = s + OUTER_STAGES - 1;
-        if (next < steps) fetch(next);
+        if constexpr (CODES) {
+            if (s + AHEAD < steps) put(s + AHEAD);
+            if (s + AHEAD + 1 < steps) fetch(s + AHEAD + 1);
+        } else {
+            if (s + AHEAD < steps) copy(s + AHEAD);
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
         const OuterStage& st = ring[s % OUTER_STAGES];
         // A (16 columns x 16 tokens, twice) from token rows: transposed 8 x 8 pieces
@@ -308,7 +339,7 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         for (int j = 0; j < 8; j += 2) {
             if (j * 8 >= ranks) break;
 #pragma unroll
-            for (int low = 0; low < (NARROW32 ? 2 : 1); low++) {
+            for (int low = 0; low < (LOW ? 2 : 1); low++) {
                 uint32_t q[4];  // ranks j * 8 .. + 8, and the next 8
                 const uint32_t pb = (uint32_t)__cvta_generic_to_shared(&(low ? st.low : st.high)[kk + (lane & 15)][j * 8 + (lane >> 4) * 8]);
                 asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -322,32 +353,51 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
                 }
             }
         }
-        if (next < steps) put(next);  // its stage was used last by step s - 1
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    // the second half's sums, through the ring's memory: 64 floats of each of 128 threads
-    float* turn = reinterpret_cast<float*>(ring);
-    if (warp >= 4) {
+    // both halves' sums in the ring's memory, in the output's order (dA: 128 columns a rank, dB: the ranks a column), so that
+    // the CTA writes along the output's rows
+    float* sum = reinterpret_cast<float*>(ring);
+    const int ncols = min(OUTER_COLS, Q.cols - c0);
+    const int pitch = Q.by_rank ? OUTER_RANK + 1 : OUTER_COLS + 4;
 #pragma unroll
-        for (int q = 0; q < 64; q++) turn[q * 128 + (tid & 127)] = acc[q / 32][q / 4 % 8][q % 4];
+    for (int half = 1; half >= 0; half--) {
+        if ((warp >> 2) == half) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (j * 8 >= ranks) break;
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const int cc = m0 + q / 4 * 16 + lane / 4 + (q >> 1 & 1) * 8, k = j * 8 + (lane & 3) * 2 + (q & 1);
+                    float& v = sum[Q.by_rank ? cc * pitch + k : k * pitch + cc];
+                    v = half ? acc[q / 4][j][q % 4] : v + acc[q / 4][j][q % 4];
+                }
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    if (warp >= 4) return;
     const bool whole = chunks == 1;
     const float f = (whole && Q.factor) ? Q.factor[id] : 1.0f;
     const int64_t base = (int64_t)(whole ? id : slot) * P.r * Q.cols;
-#pragma unroll
-    for (int q = 0; q < 64; q++) {
-        const int m = q / 32, j = q / 4 % 8, i = q % 4;
-        const float v = acc[m][j][i] + turn[q * 128 + tid];
-        const int cc = c0 + m0 + m * 16 + lane / 4 + (i >> 1) * 8, k = k0 + j * 8 + (lane & 3) * 2 + (i & 1);
-        if (k >= P.r || j * 8 >= ranks || cc >= Q.cols) continue;
-        const int64_t at = base + (Q.by_rank ? (int64_t)cc * P.r + k : (int64_t)k * Q.cols + cc);
-        if (whole)
-            Q.out[at] = half_bits<BF16>(v * f);
-        else
-            Q.slots[at] = v;
+    // rows of the output's piece, `len` long, `stride` apart; two neighbours a thread where rows start even
+    const int lines = Q.by_rank ? ncols : ranks, len = Q.by_rank ? ranks : ncols;
+    const int64_t stride = Q.by_rank ? P.r : Q.cols, origin = base + (Q.by_rank ? (int64_t)c0 * P.r + k0 : (int64_t)k0 * Q.cols + c0);
+    const bool even = stride % 2 == 0 && len % 2 == 0 && (base & 1) == 0 && (reinterpret_cast<uintptr_t>(Q.out) & 3) == 0;
+    const int per = even ? len / 2 : len;
+    for (int i = tid; i < lines * per; i += 256) {
+        const int line = i / per, e = (i - line * per) * (even ? 2 : 1);
+        const float* v = sum + line * pitch + e;
+        const int64_t at = origin + line * stride + e;
+        if (whole) {
+            if (even)
+                *reinterpret_cast<uint32_t*>(Q.out + at) = (uint32_t)half_bits<BF16>(v[0] * f) | (uint32_t)half_bits<BF16>(v[1] * f) << 16;
+            else
+                Q.out[at] = half_bits<BF16>(v[0] * f);
+        } else {
+            Q.slots[at] = v[0];
+            if (even) Q.slots[at + 1] = v[1];
+        }
     }
 }
 
@@ -470,7 +520,7 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
 }
 
 struct BackwardLayout {
-    size_t expanded = 0, ranked = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
+    size_t expanded = 0, ranked = 0, rest = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
 };
 BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r, bool need_dx) {
     BackwardLayout l;
@@ -485,6 +535,7 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
         partial = std::max(partial, plan_half_gemm(HALF_NN_GROUPED, t, r, w.d_out).partial_bytes);
         l.start = s.take((size_t)(n + 1) * sizeof(int));
         l.order = s.take((size_t)t * sizeof(int));
+        l.rest = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.ranked32 = s.take((size_t)t * r * sizeof(float));
         // the chunk is longer where only one of the two is wanted
         const int chunk = outer_chunk(t, ceil_div(w.d_in, OUTER_COLS) + ceil_div(w.d_out, OUTER_COLS), r);
@@ -657,9 +708,10 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
             g.partial = partial;
             if ((rc = launch_half_gemm(g, plan, st))) return rc;
             f.scale = ad->scale;
-            if (dx) f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
+            f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
             f.lds = ldr;
-            if (da) f.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+            if (da && x) f.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
+            if (da && !x) f.su32 = reinterpret_cast<float*>(ws + l.ranked32);
         }
         if (da || db) {
             f.start = reinterpret_cast<int*>(ws + l.start);
@@ -698,7 +750,14 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         o.a.cols = v.d_in;
         o.a.wide16 = x ? ldx % 8 == 0 && v.d_in % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0
                        : v.d_in % 16 == 0 && (reinterpret_cast<uintptr_t>(x_codes) & 15) == 0;
-        o.a.narrow32 = reinterpret_cast<const float*>(ws + l.ranked32);
+        if (x) {
+            o.a.narrow = reinterpret_cast<const uint16_t*>(ws + l.ranked);
+            o.a.rest = reinterpret_cast<const uint16_t*>(ws + l.rest);
+            o.a.ldn = ldr;
+            o.a.narrow16 = r % 8 == 0;
+        } else {
+            o.a.narrow32 = reinterpret_cast<const float*>(ws + l.ranked32);
+        }
         o.a.out = static_cast<uint16_t*>(da);
         o.a.slots = reinterpret_cast<float*>(ws + l.slots_a);
         o.a.tiles = (int)ceil_div(v.d_in, OUTER_COLS);
@@ -709,6 +768,8 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         o.b.cols = v.d_out;
         o.b.wide16 = v.d_out % 8 == 0;  // the rows start on 16 bytes
         o.b.narrow = static_cast<const uint16_t*>(u);
+        o.b.ldn = r;
+        o.b.narrow16 = r % 8 == 0 && (reinterpret_cast<uintptr_t>(u) & 15) == 0;
         o.b.factor = ad->scale;
         o.b.out = static_cast<uint16_t*>(db);
         o.b.by_rank = 1;
