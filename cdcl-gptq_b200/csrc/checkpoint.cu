@@ -46,104 +46,138 @@ struct Type<CDCLQ_DTYPE_BF16> {
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// The absolute values' largest bits over 8 values: as whole numbers they order like the values, infinities and NaN above.
-__device__ __forceinline__ uint32_t top_bits(const float (&raw)[8]) {
+// Two f32 operations at a time, each rounded on its own.
+struct Pair {
+    float x, y;
+};
+__device__ __forceinline__ uint64_t bits(Pair v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ Pair pair(uint64_t v) { return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))}; }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair(r);
+}
+
+// The absolute values' largest bits over N values: as whole numbers they order like the values, infinities and NaN above.
+template <int N>
+__device__ __forceinline__ uint32_t top_bits(const float (&raw)[N]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(raw[i]) & 0x7fffffffu);
+    for (int i = 0; i < N; i++) m = max(m, __float_as_uint(raw[i]) & 0x7fffffffu);
     return m;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t top_bits(const T (&raw)[8]) {
+template <int N, typename T>
+__device__ __forceinline__ uint32_t top_bits(const T (&raw)[N]) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    for (int i = 0; i < N / 2; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
     return max(m & 0xffffu, m >> 16);
 }
 __device__ __forceinline__ float value_of_bits(uint32_t b, const float*) { return __uint_as_float(b); }
 __device__ __forceinline__ float value_of_bits(uint32_t b, const __half*) { return __half2float(__ushort_as_half((uint16_t)b)); }
 __device__ __forceinline__ float value_of_bits(uint32_t b, const __nv_bfloat16*) { return __uint_as_float(b << 16); }
 
-// 16 lanes to a block of 128 columns, 8 values a lane: one wide load of a 16-bit type.  A CTA has 16 such groups: `across`
-// of them (a power of two) side by side along a row, 16 / across rows; it takes two such sets of rows at a time.
+constexpr int SAVE_LANES = 8, SAVE_VALUES = BLOCK / SAVE_LANES;  // lanes of a block, values of a lane
+constexpr int SAVE_GROUPS = 256 / SAVE_LANES;
+
+// 8 lanes to a block of 128 columns, 16 neighbouring values a lane.  A CTA has 32 such groups: `across` of them (a power of
+// two) side by side along a row, 32 / across rows.
 //
-// Rounding x / s: p = x * (1 / s) is within 127 * 2^-23 of the quotient, so it rounds to the same number unless it lies
-// within 2^-15 of a half; a thread with such a value divides.  Adding 1.5 * 2^23 rounds p to the nearest whole number, ties
-// to even, and leaves it in the sum's low byte.  |p| <= 127 (1 + 2^-22), so no code is out of range.
+// x / s to the nearest whole number of the rounded quotient, ties to even (values of few bits meet ties often: with a block's
+// largest value a power of two, in one of two).  With y = 1 / s rounded, q = x y and its remainder e = x - q s, which one FMA
+// gives exactly, q + e y rounded is the quotient rounded (Markstein, IBM J. Res. Dev. 34, 1990) - as long as nothing
+// underflows: below a scale of 2^-100 a thread divides.  Adding 1.5 * 2^23 rounds to a whole number and leaves it in the
+// sum's low byte; |x / s| <= 127 (1 + 2^-23), so no code is out of range.
 template <int DT, bool WIDE>
-__global__ void __launch_bounds__(256) checkpoint_save_kernel(const typename Type<DT>::T* __restrict__ x, int64_t ldx, int64_t t,
+__global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename Type<DT>::T* __restrict__ x, int64_t ldx, int64_t t,
                                                               int64_t d, int across, int8_t* __restrict__ codes,
                                                               float* __restrict__ scales) {
     typedef typename Type<DT>::T T;
-    constexpr int UNROLL = 2;
+    constexpr int N = SAVE_VALUES;
     constexpr float MAGIC = 12582912.0f;
-    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int lane = threadIdx.x % SAVE_LANES, group = threadIdx.x / SAVE_LANES;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
     const int64_t b = (int64_t)blockIdx.x * across + (group & (across - 1));
-    const int64_t c = b * BLOCK + lane * 8;
-    const int down = 16 / across;
-    const int n = (int)max((int64_t)0, min((int64_t)8, d - c));
-    // every thread of a warp walks the same number of rows (the shuffles need them all)
-    for (int64_t r0 = (int64_t)blockIdx.y * down * UNROLL; r0 < t; r0 += (int64_t)gridDim.y * down * UNROLL) {
-        alignas(16) T raw[UNROLL][8];
-        int64_t row[UNROLL];
+    const int64_t c = b * BLOCK + lane * N;
+    const int down = SAVE_GROUPS / across;
+    const int n = (int)max((int64_t)0, min((int64_t)N, d - c));
+    const int64_t first = (int64_t)blockIdx.y * down + group / across, step = (int64_t)gridDim.y * down;
+    const T* src = x + first * ldx + c;
+    int8_t* dst = codes + first * d + c;
+    float* to = scales + first * nb + b;
+    alignas(16) T next[N];
+    auto load = [&](int m) {
+        if (WIDE) {
 #pragma unroll
-        for (int k = 0; k < UNROLL; k++) {
-            row[k] = r0 + k * down + group / across;
-            const int m = row[k] < t ? n : 0;
-            const T* src = x + row[k] * ldx + c;
-            if (WIDE) {
+            for (int i = 0; i < (int)sizeof(next) / 16; i++)
+                reinterpret_cast<uint4*>(next)[i] = m ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        } else {
 #pragma unroll
-                for (int i = 0; i < (int)sizeof(raw[0]) / 16; i++)
-                    reinterpret_cast<uint4*>(raw[k])[i] = m ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) raw[k][i] = i < m ? src[i] : Type<DT>::down(0.0f);
-            }
+            for (int i = 0; i < N; i++) next[i] = i < m ? src[i] : Type<DT>::down(0.0f);
         }
+        src += step * ldx;
+    };
+    load(first < t ? n : 0);
+    // every thread of a warp walks the same number of rows (the shuffles need them all); the next row is on its way meanwhile
+    for (int64_t r0 = (int64_t)blockIdx.y * down; r0 < t; r0 += step, dst += step * d, to += step * nb) {
+        const int64_t row = r0 + group / across;
+        const int m = row < t ? n : 0;
+        alignas(16) T raw[N];
 #pragma unroll
-        for (int k = 0; k < UNROLL; k++) {
-            uint32_t bits = top_bits(raw[k]);
+        for (int i = 0; i < N; i++) raw[i] = next[i];
+        load(row + step < t ? n : 0);
+        uint32_t most = top_bits(raw);
 #pragma unroll
-            for (int o = 8; o; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-            const float top = value_of_bits(bits, static_cast<const T*>(nullptr));
-            const bool finite = top < INFINITY;
-            const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
-            const bool normal = finite && s >= 1.1754944e-38f;  // 1 / s is then finite
-            const float inv = normal ? __fdiv_rn(1.0f, s) : 0.0f;
-            uint32_t q[8];
-            float near = 0.0f;
+        for (int o = SAVE_LANES / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float top = value_of_bits(most, static_cast<const T*>(nullptr));
+        const bool finite = top < INFINITY;
+        const float s = finite ? __fdiv_rn(top, 127.0f) : __int_as_float(0x7fffffff);
+        const bool normal = finite && s >= 7.8886091e-31f;  // 2^-100
+        const float inv = normal ? __fdiv_rn(1.0f, s) : 0.0f;
+        uint32_t q[N];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float p = normal ? Type<DT>::up(raw[k][i]) * inv : 0.0f;
-                const float m = p + MAGIC;
-                near = fmaxf(near, fabsf(p - (m - MAGIC)));
-                q[i] = __float_as_uint(m);
-            }
-            if (near > 0.5f - 1.0f / 32768.0f || (finite && !normal && s > 0.0f)) {
+        for (int i = 0; i < N; i += 2) {
+            const Pair v = {Type<DT>::up(raw[i]), Type<DT>::up(raw[i + 1])};
+            const Pair p = mul2(v, {inv, inv});
+            const Pair r = add2(fma2(fma2(p, {-s, -s}, v), {inv, inv}, p), {MAGIC, MAGIC});
+            q[i] = __float_as_uint(r.x), q[i + 1] = __float_as_uint(r.y);
+        }
+        if (!normal) {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    q[i] = (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(Type<DT>::up(raw[k][i]), s)), -127.0f), 127.0f);
-            }
-            if (row[k] >= t || n == 0) continue;
-            if (lane == 0) scales[row[k] * nb + b] = s;
-            int8_t* dst = codes + row[k] * d + c;
-            if (WIDE) {
-                const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-                const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
-                *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-            } else {
+            for (int i = 0; i < N; i++)
+                q[i] = finite && s > 0.0f ? (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(Type<DT>::up(raw[i]), s)), -127.0f), 127.0f) : 0u;
+        }
+        if (m == 0) continue;
+        if (lane == 0) *to = s;
+        if (WIDE) {
+            uint32_t w[N / 4];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i < n) dst[i] = (int8_t)q[i];
-            }
+            for (int i = 0; i < N / 4; i++)
+                w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i < m) dst[i] = (int8_t)q[i];
         }
     }
 }
 
 // 16 values a thread; a CTA has `across` (a power of two) threads along a row.  ld: elements from row to row of the output;
-// columns d..ld of it are left as they are.
+// columns d..ld of it are left as they are.  A code's byte, its sign bit turned, in the low byte of 2^23 is the number
+// 2^23 + 128 + code.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
                                                                  int64_t t, int64_t d, int across, typename Type<DT>::T* __restrict__ out,
@@ -158,11 +192,17 @@ __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* _
         const int8_t* src = codes + row * d + c;
         T* dst = out + row * ld + c;
         if (WIDE && c + 16 <= d) {
-            alignas(16) int8_t q[16];
             alignas(16) T r[16];
-            *reinterpret_cast<uint4*>(q) = __ldcs(reinterpret_cast<const uint4*>(src));
+            const uint4 four = __ldcs(reinterpret_cast<const uint4*>(src));
+            const uint32_t w[4] = {four.x ^ 0x80808080u, four.y ^ 0x80808080u, four.z ^ 0x80808080u, four.w ^ 0x80808080u};
 #pragma unroll
-            for (int k = 0; k < 16; k++) r[k] = Type<DT>::down(__fmul_rn((float)q[k], s));
+            for (int k = 0; k < 16; k += 2) {
+                const uint32_t v = w[k / 4];
+                const Pair q = add2({__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4)), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4 + 1))},
+                                    {-8388736.0f, -8388736.0f});
+                const Pair p = mul2(q, {s, s});
+                r[k] = Type<DT>::down(p.x), r[k + 1] = Type<DT>::down(p.y);
+            }
 #pragma unroll
             for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<uint4*>(r)[k];
         } else {
@@ -186,12 +226,12 @@ template <int DT>
 int save(const void* x, int64_t ldx, int64_t t, int64_t d, int8_t* codes, float* scales, cudaStream_t st) {
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * sizeof(T)) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
+                      (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && d % 16 == 0;
     const int64_t nb = ceil_div(d, BLOCK);
-    const int across = power_of_two(nb, 16);
+    const int across = power_of_two(nb, SAVE_GROUPS);
     const int64_t gx = ceil_div(nb, across);
     auto kern = wide ? checkpoint_save_kernel<DT, true> : checkpoint_save_kernel<DT, false>;
-    CDCLQ_LAUNCH(kern, dim3((unsigned)gx, grid_rows(ceil_div(t, 2 * (16 / across)), gx)), 256, 0, st, static_cast<const T*>(x), ldx, t, d,
+    CDCLQ_LAUNCH(kern, dim3((unsigned)gx, grid_rows(ceil_div(t, SAVE_GROUPS / across), gx)), 256, 0, st, static_cast<const T*>(x), ldx, t, d,
                  across, codes, scales);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? 0 : cuda_error(e, "checkpoint_save_kernel launch");
