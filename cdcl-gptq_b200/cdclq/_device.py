@@ -40,46 +40,45 @@ def tensor(x, what, dims, dtype=None, shape=None, device=None):
     return x
 
 
-def on_device_of(position):
-    """Runs an operator with the device of its argument at `position` as the current one."""
+def _tensors(args):
+    for a in args:
+        if isinstance(a, torch.Tensor):
+            yield a
+        elif a is not None:
+            yield from getattr(a, "tensors", ())  # a Checkpoint, a PackedProjection
 
-    def wrap(f):
-        @functools.wraps(f)
-        def g(*args, **kw):
-            x = args[position] if len(args) > position else None
-            if not isinstance(x, torch.Tensor):
-                x = getattr(x, "codes", None)  # a Checkpoint
-            if x is None or not x.is_cuda or x.get_device() == _current_device():
+
+def operator(f):
+    """An operator on the tensors of one CUDA device: runs with the device of its first argument as the current one and on
+    `stream`, a CUDA stream's handle as the library's other calls take it (0: the legacy default stream), or on torch's
+    current stream if None.  Results belong to that stream, as torch's own would."""
+
+    @functools.wraps(f)
+    def g(*args, stream=None, **kw):
+        x = args[0] if args else None
+        if not isinstance(x, torch.Tensor):
+            x = next(_tensors(args), None)
+        if x is None or not x.is_cuda or (stream is None and x.get_device() == _current_device()):
+            return f(*args, **kw)
+        with torch.cuda.device(x.device):
+            if stream is None or stream == current_stream(x):
                 return f(*args, **kw)
-            with torch.cuda.device(x.device):
-                return f(*args, **kw)
+            s = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+            with torch.cuda.stream(s):
+                out = f(*args, **kw)
+            for t in _tensors((*args, *kw.values())):
+                t.record_stream(s)  # their memory is not reused while the stream reads it
+            return out
 
-        return g
-
-    return wrap
-
-
-class Call:
-    """The stream of one call: `stream` as the library's other calls take it (a CUDA stream's handle, 0 for the legacy
-    default stream), or None for torch's current stream.  What a call allocates, and its arguments, stay alive for
-    work on a stream that is not torch's current one: keep() marks them."""
-
-    __slots__ = ("handle", "apart")
-
-    def __init__(self, x, stream):
-        current = _raw_stream(x.get_device())
-        self.apart = stream is not None and stream != current
-        self.handle = stream if self.apart else current
-
-    def keep(self, *tensors):
-        if self.apart:
-            s = torch.cuda.ExternalStream(self.handle) if self.handle else torch.cuda.default_stream()
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(s)
+    return g
 
 
-def rows16(x, call):
+def current_stream(x):
+    """Handle of torch's current stream on x's device."""
+    return _raw_stream(x.get_device())
+
+
+def rows16(x):
     """(x, elements from row to row) of a 2-d 16-bit matrix in the layout the kernels read: columns contiguous, rows
     starting on 16 bytes.  x itself where it has that layout (any such row stride), else a copy."""
     t, d = x.shape
@@ -96,13 +95,10 @@ def rows16(x, call):
     pad = -(-d // 8) * 8
     if ld == pad and x.data_ptr() % 16 == 0:
         return x, ld
-    out = torch.empty((t, pad), dtype=x.dtype, device=x.device)
-    check(lib().cdclq_align_rows_device(x.data_ptr(), t, d, ld, out.data_ptr(), pad, call.handle))
-    call.keep(x, out)
+    out = x.new_empty(t, pad)
+    check(lib().cdclq_align_rows_device(x.data_ptr(), t, d, ld, out.data_ptr(), pad, current_stream(x)))
     return out, pad
 
 
-def workspace(nbytes, like, call):
-    w = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    call.keep(w)
-    return w
+def workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)

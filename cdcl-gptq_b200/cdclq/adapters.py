@@ -14,10 +14,11 @@ adapter holds (a NaN among it) does not reach another.  The calls are asynchrono
 None).
 """
 import ctypes
+import functools
 
 import torch
 
-from ._device import HALF, Call, half_code, on_device_of, refuse, rows16, tensor, workspace
+from ._device import HALF, current_stream, half_code, operator, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 from .abi import CAdapters, CPackedLayer
 from .checkpoint import Checkpoint
@@ -30,12 +31,12 @@ class PackedProjection:
     packed format has them (src/io.rs:244-270), CUDA tensors; gsize: columns of a group.  They are copied into the layout
     and not kept; building synchronises."""
 
-    def __init__(self, qweight, scales, qzeros, perm, gbits, gsize, stream=None):
+    def __init__(self, qweight, scales, qzeros, perm, gbits, gsize):
         tensor(qweight, "qweight", 2, torch.uint8)
         with torch.cuda.device(qweight.device):
-            self._build(qweight, scales, qzeros, perm, gbits, gsize, stream)
+            self._build(qweight, scales, qzeros, perm, gbits, gsize)
 
-    def _build(self, qweight, scales, qzeros, perm, gbits, gsize, stream):
+    def _build(self, qweight, scales, qzeros, perm, gbits, gsize):
         dev = qweight.get_device()
         tensor(perm, "perm", 1, torch.int32, None, dev)
         gb = gbits.cpu().to(torch.uint8).contiguous()
@@ -49,15 +50,16 @@ class PackedProjection:
             refuse("qweight: need %d bytes a row, got %d" % (row_bytes, qweight.shape[1]))
         self._c = CPackedLayer()
         self._ref = ctypes.addressof(self._c)
-        call = Call(qweight, stream)
         need = lib().cdclq_packed_layer_bytes(d_out, d_in, gsize, gb.data_ptr())
         self._layout = torch.empty(max(1, need), dtype=torch.uint8, device=qweight.device)
         qweight, scales, qzeros, perm = (x.contiguous() for x in (qweight, scales, qzeros, perm))
         check(lib().cdclq_packed_layer_build(qweight.data_ptr(), scales.data_ptr(), qzeros.data_ptr(), perm.data_ptr(), d_out,
                                              d_in, gsize, gb.data_ptr(), self._layout.data_ptr(), need, self._ref,
-                                             call.handle))
-        call.keep(self._layout, qweight, scales, qzeros, perm)
+                                             current_stream(qweight)))
         self.d_out, self.d_in, self.device = d_out, d_in, qweight.device
+        # workspace bytes by the sizes of a call
+        self._forward_need = functools.lru_cache(256)(functools.partial(lib().cdclq_projection_forward_workspace, self._ref))
+        self._backward_need = functools.lru_cache(256)(functools.partial(lib().cdclq_projection_backward_workspace, self._ref))
 
     @staticmethod
     def from_tensors(tensors, layer, device="cuda"):
@@ -73,15 +75,19 @@ class PackedProjection:
         return PackedProjection(q, s, z, p, get("gbits"), int(get("gsize").reshape(-1)[0]))
 
     @property
+    def tensors(self):
+        return (self._layout,)
+
+    @property
     def nbytes(self):
         return self._layout.numel()
 
 
-def _matrix(x, cols, call):
+def _matrix(x, cols):
     """The rows of an n x rows x columns tensor, as rows16 gives them."""
     if cols % 8 == 0 and x.is_contiguous() and x.data_ptr() % 16 == 0:
         return x, cols
-    return rows16(x.reshape(-1, cols), call)
+    return rows16(x.reshape(-1, cols))
 
 
 def _refuse_adapters(w, like, a, b, scale, index, t):
@@ -103,7 +109,7 @@ class _Adapters:
 
     __slots__ = ("n", "r", "c", "ref", "held")
 
-    def __init__(self, w, like, a, b, scale, index, t, call):
+    def __init__(self, w, like, a, b, scale, index, t):
         self.n = self.r = 0
         self.ref, self.held = None, ()
         if a is None and b is None and scale is None and index is None:
@@ -119,8 +125,8 @@ class _Adapters:
         self.n, self.r = n, r
         if n == 0:
             return
-        ar, lda = _matrix(a, d_in, call)
-        br, ldb = _matrix(b, r, call)
+        ar, lda = _matrix(a, d_in)
+        br, ldb = _matrix(b, r)
         scale, index = scale.contiguous(), index.contiguous()
         self.held = (a, b, ar, br, scale, index)
         self.c = CAdapters(ar.data_ptr(), br.data_ptr(), lda, ldb, scale.data_ptr(), index.data_ptr(), n, r)
@@ -139,38 +145,35 @@ def _projection(w, x, what, backward):
     return code, x.shape[0]
 
 
-@on_device_of(0)
-def forward(x, w, a=None, b=None, scale=None, index=None, keep=False, stream=None):
+@operator
+def forward(x, w, a=None, b=None, scale=None, index=None, keep=False, *, stream=None):
     """y (t x d_out); with keep also u (t x r), which backward() takes."""
     code, t = _projection(w, x, "x", False)
-    call, L = Call(x, stream), lib()
-    ad = _Adapters(w, x, a, b, scale, index, t, call)
-    y = x.new_empty((t, w.d_out))
-    u = x.new_empty((t, ad.r)) if keep else None
+    L = lib()
+    ad = _Adapters(w, x, a, b, scale, index, t)
+    y = x.new_empty(t, w.d_out)
+    u = x.new_empty(t, ad.r) if keep else None
     if t:
-        xr, ldx = rows16(x, call)
-        need = L.cdclq_projection_forward_workspace(w._ref, t, ad.n, ad.r)
-        ws = workspace(need, x, call)
+        xr, ldx = rows16(x)
+        need = w._forward_need(t, ad.n, ad.r)
+        ws = workspace(need, x)
         check(L.cdclq_projection_forward_device(w._ref, xr.data_ptr(), ldx, code, t, ad.ref, y.data_ptr(), w.d_out,
-                                                u.data_ptr() if keep and ad.n else None, ws.data_ptr(), need, call.handle))
+                                                u.data_ptr() if keep and ad.n else None, ws.data_ptr(), need, current_stream(x)))
         if keep and not ad.n:
             u.zero_()
-        if call.apart:
-            call.keep(x, xr, y, u, w._layout, *ad.held)
     return (y, u) if keep else y
 
 
-@on_device_of(0)
-def backward(dy, x, u, w, a, b, scale, index, need_dx=True, need_da=True, need_db=True, stream=None):
+@operator
+def backward(dy, x, u, w, a, b, scale, index, need_dx=True, need_da=True, need_db=True, *, stream=None):
     """(dx, da, db) for the gradient dy of y; None in the place of one that is not needed.  x: the forward's input or its
     Checkpoint; u: what forward(keep=True) returned."""
     code, t = _projection(w, dy, "dy", True)
-    call, L, dev = Call(dy, stream), lib(), dy.get_device()
-    ad = _Adapters(w, dy, a, b, scale, index, t, call)
-    new = lambda need, shape: dy.new_empty(shape) if need else None  # noqa: E731
-    dx = new(need_dx, (t, w.d_in))
-    da = new(need_da and a is not None, (ad.n, ad.r, w.d_in))
-    db = new(need_db and a is not None, (ad.n, w.d_out, ad.r))
+    L, dev = lib(), dy.get_device()
+    ad = _Adapters(w, dy, a, b, scale, index, t)
+    dx = dy.new_empty(t, w.d_in) if need_dx else None
+    da = dy.new_empty(ad.n, ad.r, w.d_in) if need_da and a is not None else None
+    db = dy.new_empty(ad.n, w.d_out, ad.r) if need_db and a is not None else None
     codes = scales = xr = None
     ldx = 0
     if da is not None:
@@ -185,12 +188,10 @@ def backward(dy, x, u, w, a, b, scale, index, need_dx=True, need_da=True, need_d
     if t == 0:
         return dx, da.zero_() if da is not None else None, db.zero_() if db is not None else None
     at = lambda v: None if v is None else v.data_ptr()  # noqa: E731
-    src, ld = rows16(dy, call)
-    need = L.cdclq_projection_backward_workspace(w._ref, t, ad.n, ad.r, need_dx)
-    ws = workspace(need, dy, call)
+    src, ld = rows16(dy)
+    need = w._backward_need(t, ad.n, ad.r, bool(need_dx))
+    ws = workspace(need, dy)
     check(L.cdclq_projection_backward_device(w._ref, src.data_ptr(), ld, code, t, ad.ref, at(xr), ldx, at(codes), at(scales),
                                              u.data_ptr() if db is not None else None, at(dx), w.d_in, at(da), at(db),
-                                             ws.data_ptr(), need, call.handle))
-    if call.apart:
-        call.keep(dy, src, xr, codes, scales, u if db is not None else None, dx, da, db, w._layout, *ad.held)
+                                             ws.data_ptr(), need, current_stream(dy)))
     return dx, da, db

@@ -11,7 +11,7 @@ The calls are asynchronous on `stream` (torch's current one if None).
 """
 import torch
 
-from ._device import HALF, Call, half_code, on_device_of, refuse, rows16, tensor, workspace
+from ._device import HALF, current_stream, half_code, operator, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 from .io import _dtype_code
 
@@ -37,6 +37,10 @@ class Checkpoint:
         return c
 
     @property
+    def tensors(self):
+        return self.codes, self.scales
+
+    @property
     def shape(self):
         return self.codes.shape
 
@@ -46,38 +50,34 @@ def _code(dt):
     return _dtype_code(torch, dt) if code is None else code
 
 
-@on_device_of(0)
-def save(x, stream=None):
+@operator
+def save(x, *, stream=None):
     if x.dim() != 2 or not x.is_cuda:
         tensor(x, "x", 2)
     code = _code(x.dtype)
     t, d = x.shape
-    call = Call(x, stream)
     ld, step = x.stride()
     if d > 1 and step != 1 or t > 1 and ld < d:
         x, ld = x.contiguous(), d
-    codes = torch.empty((t, d), dtype=torch.int8, device=x.device)
-    scales = torch.empty((t, -(-d // BLOCK)), dtype=torch.float32, device=x.device)
+    codes = torch.empty(t, d, dtype=torch.int8, device=x.device)
+    scales = torch.empty(t, -(-d // BLOCK), dtype=torch.float32, device=x.device)
     check(lib().cdclq_checkpoint_save_device(x.data_ptr(), ld if t > 1 else d, code, t, d, codes.data_ptr(), scales.data_ptr(),
-                                             call.handle))
-    call.keep(x, codes, scales)
+                                             current_stream(x)))
     return Checkpoint._made(codes, scales, x.dtype)
 
 
-@on_device_of(0)
-def restore(c, stream=None):
+@operator
+def restore(c, *, stream=None):
     codes, scales = c.codes, c.scales
     t, d = codes.shape
-    call = Call(codes, stream)
-    out = torch.empty((t, d), dtype=c.dtype, device=codes.device)
+    out = torch.empty(t, d, dtype=c.dtype, device=codes.device)
     check(lib().cdclq_checkpoint_restore_device(codes.data_ptr(), scales.data_ptr(), t, d, out.data_ptr(), d, _code(c.dtype),
-                                                call.handle))
-    call.keep(codes, scales, out)
+                                                current_stream(codes)))
     return out
 
 
-@on_device_of(0)
-def weight_grad(dy, c, stream=None):
+@operator
+def weight_grad(dy, c, *, stream=None):
     """dy^T x^ with the restored values rounded to dy's type, as the operand of the tensor cores."""
     (t, d), codes = c.shape, c.codes
     tensor(dy, "dy", 2, device=codes.get_device())
@@ -86,12 +86,11 @@ def weight_grad(dy, c, stream=None):
     tensor(dy, "dy", 2, shape=(t, n))
     if d == 0 or n == 0:
         refuse("weight_grad: no columns")
-    call, L = Call(dy, stream), lib()
-    dw = dy.new_empty((n, d))
-    src, ld = rows16(dy, call) if t else (dy, n)
+    L = lib()
+    dw = dy.new_empty(n, d)
+    src, ld = rows16(dy) if t else (dy, n)
     need = L.cdclq_checkpoint_weight_grad_workspace(t, d, n)
-    ws = workspace(need, dy, call)
+    ws = workspace(need, dy)
     check(L.cdclq_checkpoint_weight_grad_device(src.data_ptr(), ld, code, codes.data_ptr(), c.scales.data_ptr(), t, d, n,
-                                                dw.data_ptr(), d, ws.data_ptr(), need, call.handle))
-    call.keep(dy, codes, c.scales, dw)
+                                                dw.data_ptr(), d, ws.data_ptr(), need, current_stream(dy)))
     return dw

@@ -15,7 +15,7 @@ if None).
 """
 import torch
 
-from ._device import Call, half_code, on_device_of, refuse, rows16, tensor, workspace
+from ._device import current_stream, half_code, operator, refuse, rows16, tensor, workspace
 from ._lib import check, lib
 
 
@@ -23,53 +23,52 @@ def _head(h, w, target):
     tensor(h, "h", 2)
     code = half_code(h.dtype, "h")
     (t, d), dev = h.shape, h.get_device()
-    tensor(w, "w", 2, h.dtype, (w.shape[0], d) if w.dim() == 2 else (None, d), dev)
-    tensor(target, "target", 1, torch.int64, (t,), dev)
+    tensor(w, "w", 2, h.dtype, None, dev)
     v = w.shape[0]
+    tensor(w, "w", 2, shape=(v, d))
+    tensor(target, "target", 1, torch.int64, (t,), dev)
     if d == 0 or v == 0:
         refuse("w: the head has no rows or no columns")
     return code, t, d, v
 
 
-@on_device_of(0)
-def linear_cross_entropy(h, w, target, stream=None):
+@operator
+def linear_cross_entropy(h, w, target, *, stream=None):
     """(loss, lse), float32, one for each row of h."""
     code, t, d, v = _head(h, w, target)
     loss = torch.empty(t, dtype=torch.float32, device=h.device)
     lse = torch.empty_like(loss)
     if t == 0:
         return loss, lse
-    call, L = Call(h, stream), lib()
+    L = lib()
     target = target.contiguous()
-    hr, ldh = rows16(h, call)
-    wr, ldw = rows16(w, call)
+    hr, ldh = rows16(h)
+    wr, ldw = rows16(w)
     need = L.cdclq_linear_cross_entropy_workspace(t, d, v)
-    ws = workspace(need, h, call)
+    ws = workspace(need, h)
     check(L.cdclq_linear_cross_entropy_device(hr.data_ptr(), ldh, wr.data_ptr(), ldw, code, t, d, v, target.data_ptr(),
-                                              loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, call.handle))
-    call.keep(h, w, target, loss, lse)
+                                              loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, current_stream(h)))
     return loss, lse
 
 
-@on_device_of(0)
-def linear_cross_entropy_backward(h, w, target, lse, dloss, need_dh=True, need_dw=True, stream=None):
+@operator
+def linear_cross_entropy_backward(h, w, target, lse, dloss, need_dh=True, need_dw=True, *, stream=None):
     """(dh, dw) for the gradient dloss of each token's loss; None in the place of one that is not needed."""
     code, t, d, v = _head(h, w, target)
     dev = h.get_device()
     tensor(lse, "lse", 1, torch.float32, (t,), dev)
     tensor(dloss, "dloss", 1, torch.float32, (t,), dev)
-    dh = torch.empty((t, d), dtype=h.dtype, device=h.device) if need_dh else None
-    dw = torch.empty((v, d), dtype=h.dtype, device=h.device) if need_dw else None
+    dh = h.new_empty(t, d) if need_dh else None
+    dw = h.new_empty(v, d) if need_dw else None
     if t == 0 or not (need_dh or need_dw):
         return dh, dw.zero_() if dw is not None else None
-    call, L = Call(h, stream), lib()
+    L = lib()
     target, lse, dloss = target.contiguous(), lse.contiguous(), dloss.contiguous()
-    hr, ldh = rows16(h, call)
-    wr, ldw = rows16(w, call)
+    hr, ldh = rows16(h)
+    wr, ldw = rows16(w)
     need = L.cdclq_linear_cross_entropy_backward_workspace(t, d, v, need_dh, need_dw)
-    ws = workspace(need, h, call)
+    ws = workspace(need, h)
     check(L.cdclq_linear_cross_entropy_backward_device(
         hr.data_ptr(), ldh, wr.data_ptr(), ldw, code, t, d, v, target.data_ptr(), lse.data_ptr(), dloss.data_ptr(),
-        dh.data_ptr() if need_dh else None, d, dw.data_ptr() if need_dw else None, d, ws.data_ptr(), need, call.handle))
-    call.keep(h, w, target, lse, dloss, dh, dw)
+        dh.data_ptr() if need_dh else None, d, dw.data_ptr() if need_dw else None, d, ws.data_ptr(), need, current_stream(h)))
     return dh, dw
