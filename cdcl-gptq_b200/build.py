@@ -22,9 +22,9 @@ OUT = os.path.join(HERE, "cdclq", "libcdclq_cuda.so")
 SOURCES = ["engine.cu", "prep.cu", "gptq.cu", "repair.cu", "repair_bm64.cu", "repair_bm128.cu", "gemm.cu", "pack.cu",
            "syrk.cu", "noalloc.cu", "io.cu", "model_io.cu", "runtime.cu", "model.cu", "half_gemm.cu",
            "half_gemm_bf16.cu", "half_gemm_f16.cu", "loss.cu", "checkpoint.cu",
-           "packed.cu", "adapters.cu"]
+           "packed.cu", "adapters.cu", "rank.cu"]
 HEADERS = ["common.cuh", "gemm_core.cuh", "kernels.h", "repair_core.cuh", "model_io.h", "runtime.h", "tcgen05.cuh",
-           "half_gemm.cuh", "half_gemm.h", "half_gemm_launch.cuh", "packed.h"]
+           "half_gemm.cuh", "half_gemm.h", "half_gemm_launch.cuh", "packed.h", "rank.h", "mma16.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-fmad=false", "-Xcompiler", "-fPIC"]
 

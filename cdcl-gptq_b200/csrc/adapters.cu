@@ -11,11 +11,10 @@
 #include <algorithm>
 #include <exception>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "half_gemm.h"
+#include "mma16.cuh"
 #include "packed.h"
+#include "rank.h"
 
 namespace cdclq {
 
@@ -23,100 +22,6 @@ namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
-
-template <bool BF16>
-__device__ __forceinline__ uint16_t half_bits(float v) {
-    return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-}
-
-template <bool BF16>
-__device__ __forceinline__ float half_value(uint16_t v) {
-    return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
-}
-// v - h, rounded: with h = v rounded, h + rest has twice the significand.  An infinity is all in h.
-template <bool BF16>
-__device__ __forceinline__ uint16_t rest_bits(float v, uint16_t h) {
-    const float high = half_value<BF16>(h);
-    return half_bits<BF16>(fabsf(high) < INFINITY ? v - high : 0.0f);
-}
-
-// Each adapter's tokens in ascending order, one CTA (1024 threads) an adapter: start[i] = tokens of lower adapters.
-__device__ __forceinline__ void token_list(const int* __restrict__ index, int t, int n, int id, int* __restrict__ start,
-                                           int* __restrict__ order) {
-    __shared__ int below[32], mine[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int lower = 0;
-    for (int i = threadIdx.x; i < t; i += 1024) {
-        const int v = index[i];
-        lower += v >= 0 && v < id;
-    }
-    lower = __reduce_add_sync(0xffffffffu, lower);
-    if (lane == 0) below[warp] = lower;
-    __syncthreads();
-    int at = 0;
-    for (int w = 0; w < 32; w++) at += below[w];
-    if (threadIdx.x == 0) start[id] = at;
-    for (int base = 0; base < t; base += 1024) {
-        const int i = base + threadIdx.x;
-        const bool hit = i < t && index[i] == id;
-        const uint32_t m = __ballot_sync(0xffffffffu, hit);
-        if (lane == 0) mine[warp] = __popc(m);
-        __syncthreads();
-        int before = at, all = 0;
-        for (int w = 0; w < 32; w++) {
-            if (w < warp) before += mine[w];
-            all += mine[w];
-        }
-        if (hit) order[before + __popc(m & ((1u << lane) - 1u))] = i;
-        at += all;
-        __syncthreads();
-    }
-    if (id == n - 1 && threadIdx.x == 0) start[n] = at;
-}
-
-struct FinishArgs {
-    const float* partial;  // [split][t][ldp], or null
-    int splits, t, r, ldp;
-    const int* index;
-    int n;
-    const float* scale;
-    uint16_t* u16;         // the sums, rounded, or null
-    int64_t ldu;
-    uint16_t* su16;        // scale of the row's adapter times the sums, rounded, or null
-    uint16_t* rest16;      // what the rounding took off, rounded, or null
-    int64_t lds;
-    float* su32;           // the same, not rounded, [t][r], or null
-    int* start;            // the adapters' token lists, or null
-    int* order;
-};
-
-// The f32 sums of a grouped product, splits in order; and, in its first n CTAs, the token lists that the gradients need.
-template <bool BF16>
-__global__ void __launch_bounds__(1024) rank_finish_kernel(const FinishArgs P) {
-    const int lists = P.start ? P.n : 0;
-    if ((int)blockIdx.x < lists) {
-        token_list(P.index, P.t, P.n, blockIdx.x, P.start, P.order);
-        return;
-    }
-    if (!P.partial) return;
-    const int64_t total = (int64_t)P.t * P.r;
-    for (int64_t i = (blockIdx.x - lists) * (int64_t)1024 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - lists) * 1024) {
-        const int64_t row = i / P.r;
-        const int c = (int)(i - row * P.r);
-        float s = 0.0f;
-#pragma unroll 4
-        for (int k = 0; k < P.splits; k++) s += P.partial[((int64_t)k * P.t + row) * P.ldp + c];
-        if (P.u16) P.u16[row * P.ldu + c] = half_bits<BF16>(s);
-        if (P.su16 || P.su32) {
-            const int id = P.index[row];
-            const float v = (id >= 0 && id < P.n) ? P.scale[id] * s : 0.0f;
-            const uint16_t h = half_bits<BF16>(v);
-            if (P.su16) P.su16[row * P.lds + c] = h;
-            if (P.rest16) P.rest16[row * P.lds + c] = rest_bits<BF16>(v, h);
-            if (P.su32) P.su32[i] = v;
-        }
-    }
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Outer products of an adapter's tokens: out[c][k] = factor * sum_t wide[t][c] narrow[t][k], c over the wide matrix'
@@ -182,30 +87,12 @@ __device__ __forceinline__ bool outer_item(const OuterPair& P, int item, int lan
     return false;
 }
 
-__device__ __forceinline__ void copy16(void* dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
-                 "r"(live ? 16 : 0)
-                 : "memory");
-}
-
 // rows of 128 + 8 and 64 + 8 halves: 16-byte pieces of eight rows fall into different banks
 struct OuterStage {
     uint16_t wide[OUTER_TOK][OUTER_COLS + 8];
     uint16_t high[OUTER_TOK][OUTER_RANK + 8];
     uint16_t low[OUTER_TOK][OUTER_RANK + 8];
 };
-
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // LOW: the narrow factor is high + low.
 template <bool BF16, bool CODES, bool LOW>
@@ -307,14 +194,14 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
                 copy(s);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copy_commit();
     }
     if constexpr (CODES) {
         if (AHEAD < steps) fetch(AHEAD);
     }
 #pragma unroll 1
     for (int s = 0; s < steps; s++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(OUTER_STAGES - 2) : "memory");
+        copy_wait<OUTER_STAGES - 2>();
         __syncthreads();  // stage s is there, and stage s - 1 has been used by every warp
         if constexpr (CODES) {
             if (s + AHEAD < steps) put(s + AHEAD);
@@ -322,30 +209,20 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         } else {
             if (s + AHEAD < steps) copy(s + AHEAD);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copy_commit();
         const OuterStage& st = ring[s % OUTER_STAGES];
         // A (16 columns x 16 tokens, twice) from token rows: transposed 8 x 8 pieces
         uint32_t a[2][4];
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            const uint32_t pa = (uint32_t)__cvta_generic_to_shared(
-                &st.wide[kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + m * 16 + ((lane >> 3) & 1) * 8]);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(a[m][0]), "=r"(a[m][1]), "=r"(a[m][2]), "=r"(a[m][3])
-                         : "r"(pa)
-                         : "memory");
-        }
+        for (int m = 0; m < 2; m++)
+            load_pieces<true>(a[m], &st.wide[kk + (lane & 7) + ((lane >> 4) & 1) * 8][m0 + m * 16 + ((lane >> 3) & 1) * 8]);
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             if (j * 8 >= ranks) break;
 #pragma unroll
             for (int low = 0; low < (LOW ? 2 : 1); low++) {
                 uint32_t q[4];  // ranks j * 8 .. + 8, and the next 8
-                const uint32_t pb = (uint32_t)__cvta_generic_to_shared(&(low ? st.low : st.high)[kk + (lane & 15)][j * 8 + (lane >> 4) * 8]);
-                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                             : "r"(pb)
-                             : "memory");
+                load_pieces<true>(q, &(low ? st.low : st.high)[kk + (lane & 15)][j * 8 + (lane >> 4) * 8]);
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
                     mma16816<BF16>(acc[m][j], a[m], q[0], q[1]);
@@ -354,7 +231,7 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
             }
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    copy_wait<0>();
     __syncthreads();
     // both halves' sums in the ring's memory, in the output's order (dA: 128 columns a rank, dB: the ranks a column), so that
     // the CTA writes along the output's rows
@@ -508,12 +385,8 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
         l.decode = s.take(packed_decode_workspace(w, (int)t, n ? (int)r : 0));
     } else {
         l.expanded = s.take((size_t)w.d_out * ceil_div(w.d_in, 8) * 8 * 2);
-        size_t partial = plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in).partial_bytes;
-        if (n) {
-            l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
-            partial = std::max(partial, plan_half_gemm(HALF_NT_GROUPED, t, r, w.d_in).partial_bytes);
-        }
-        l.partial = s.take(partial);
+        if (n) l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
+        l.partial = s.take(plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in).partial_bytes);
     }
     l.total = s.at;
     return l;
@@ -532,7 +405,6 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
     }
     if (n) {
         l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
-        partial = std::max(partial, plan_half_gemm(HALF_NN_GROUPED, t, r, w.d_out).partial_bytes);
         l.start = s.take((size_t)(n + 1) * sizeof(int));
         l.order = s.take((size_t)t * sizeof(int));
         l.rest = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
@@ -576,22 +448,6 @@ int check_call(const char* what, const cdclq_packed_layer* w, int dtype, size_t 
     return check_fail_word(what);
 }
 
-// The f32 sums of a grouped product (none where g.partial is null), and the adapters' token lists.
-int finish_rank(bool bf16, const HalfGemm& g, const HalfPlan& plan, FinishArgs f, cudaStream_t st) {
-    f.partial = g.partial;
-    f.splits = plan.splits;
-    f.t = (int)g.m, f.r = (int)g.n, f.ldp = (int)(ceil_div(g.n, 4) * 4);
-    f.index = g.index;
-    f.n = g.adapters;
-    const int64_t sums = g.partial ? std::max<int64_t>(1, std::min<int64_t>(ceil_div(g.m * g.n, 1024), sm_count() * 2)) : 0;
-    const unsigned grid = (unsigned)(sums + (f.start ? f.n : 0));
-    if (!grid) return 0;
-    auto kern = bf16 ? rank_finish_kernel<true> : rank_finish_kernel<false>;
-    CDCLQ_LAUNCH(kern, grid, 1024, 0, st, f);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : cuda_error(e, "rank_finish_kernel launch");
-}
-
 }  // namespace
 
 }  // namespace cdclq
@@ -625,24 +481,20 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
     const int64_t ldw = ceil_div(v.d_in, 8) * 8, ldr = ceil_div(r, 8) * 8;
     float* partial = reinterpret_cast<float*>(ws + l.partial);
     if (n) {
-        HalfGemm g{};
-        g.form = HALF_NT_GROUPED;
-        g.bf16 = bf16;
-        g.m = t, g.n = r, g.k = v.d_in;
-        g.a = operand(x, t, v.d_in, ldx);
-        g.x = operand(ad->a, r, v.d_in, ad->lda, n);
-        g.index = ad->index;
-        g.adapters = (int)n;
-        g.partial = partial;
-        const HalfPlan plan = plan_half_gemm(HALF_NT_GROUPED, t, r, v.d_in);
-        if ((rc = launch_half_gemm(g, plan, st))) return rc;
-        FinishArgs f{};
-        f.scale = ad->scale;
-        f.u16 = static_cast<uint16_t*>(u);
-        f.ldu = r;
-        f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
-        f.lds = ldr;
-        if ((rc = finish_rank(bf16, g, plan, f, st))) return rc;
+        RankArgs p{};
+        p.x = static_cast<const uint16_t*>(x);
+        p.ldx = ldx;
+        p.t = (int)t, p.k = v.d_in;
+        p.m = static_cast<const uint16_t*>(ad->a);
+        p.ldm = ad->lda;
+        p.index = ad->index;
+        p.n = (int)n, p.r = (int)r;
+        p.scale = ad->scale;
+        p.u16 = static_cast<uint16_t*>(u);
+        p.ldu = r;
+        p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
+        p.lds = ldr;
+        if ((rc = launch_rank(bf16, false, p, st))) return rc;
     }
     if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;
     HalfGemm g{};
@@ -694,30 +546,24 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
     const int64_t ldw = ceil_div(v.d_in, 8) * 8, ldr = ceil_div(r, 8) * 8;
     float* partial = reinterpret_cast<float*>(ws + l.partial);
     if (n) {
-        HalfGemm g{};
-        g.form = HALF_NN_GROUPED;
-        g.bf16 = bf16;
-        g.m = t, g.n = r, g.k = v.d_out;
-        g.a = operand(dy, t, v.d_out, lddy);
-        g.x = operand(ad->b, v.d_out, r, ad->ldb, n);
-        g.index = ad->index;
-        g.adapters = (int)n;
-        const HalfPlan plan = plan_half_gemm(HALF_NN_GROUPED, t, r, v.d_out);
-        FinishArgs f{};
-        if (dx || da) {
-            g.partial = partial;
-            if ((rc = launch_half_gemm(g, plan, st))) return rc;
-            f.scale = ad->scale;
-            f.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
-            f.lds = ldr;
-            if (da && x) f.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
-            if (da && !x) f.su32 = reinterpret_cast<float*>(ws + l.ranked32);
-        }
+        RankArgs p{};
+        p.x = static_cast<const uint16_t*>(dy);
+        p.ldx = lddy;
+        p.t = (int)t, p.k = v.d_out;
+        p.m = static_cast<const uint16_t*>(ad->b);
+        p.ldm = ad->ldb;
+        p.index = ad->index;
+        p.n = (int)n, p.r = (int)r;
+        p.scale = ad->scale;
+        p.lds = ldr;
+        if (dx || da) p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
+        if (da && x) p.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
+        if (da && !x) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
         if (da || db) {
-            f.start = reinterpret_cast<int*>(ws + l.start);
-            f.order = reinterpret_cast<int*>(ws + l.order);
+            p.start = reinterpret_cast<int*>(ws + l.start);
+            p.order = reinterpret_cast<int*>(ws + l.order);
         }
-        if ((rc = finish_rank(bf16, g, plan, f, st))) return rc;
+        if ((rc = launch_rank(bf16, true, p, st))) return rc;
     }
     if (dx) {
         if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;

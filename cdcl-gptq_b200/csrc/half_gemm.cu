@@ -95,36 +95,28 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Splitting K adds the f32 sums' way out and back, and a launch.
 HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
     const bool store = form != HALF_STATS && form != HALF_GRAD;
-    const bool grouped = form == HALF_NT_GROUPED || form == HALF_NN_GROUPED;
     const int64_t sms = sm_count(), nkb = ceil_div(k, KB);
     HalfPlan p{1, 64, 1, 0};
-    if (grouped) {
-        // a tile's work grows with its adapters: two items to an SM, four K blocks at least for each
-        const int64_t tiles = ceil_div(m, BM) * ceil_div(n, p.bn);
-        p.splits = (int)std::max<int64_t>(1, std::min(2 * sms / tiles, nkb / 4));
-        p.splits = (int)ceil_div(nkb, ceil_div(nkb, p.splits));
-    } else {
-        static const struct { int cg, bn, block, item; } shapes[] = {
-            {2, 512, 1060, 6000}, {2, 256, 630, 3000}, {2, 128, 450, 3000}, {1, 128, 560, 2500}, {1, 64, 430, 2000}};
-        double best = 1e300;
-        for (const auto& s : shapes) {
-            if ((s.bn == 64 && !store) || (s.bn == 512 && form == HALF_STATS)) continue;
-            if (s.cg == 2 && m <= BM) continue;  // the second CTA's rows would be empty
-            const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
-            const int64_t most = store ? std::max<int64_t>(1, std::min(slots / tiles, nkb / 8)) : 1;
-            for (int64_t want = 1; want <= most; want++) {
-                const int64_t per = ceil_div(nkb, want), splits = ceil_div(nkb, per);
-                if (splits != want) continue;
-                double cost = (double)ceil_div(tiles * splits, slots) * ((double)per * s.block + s.item);
-                if (splits > 1) cost += 6000.0 + (splits + 1.0) * m * n * 4.0 / 2000.0;
-                if (cost < best) {
-                    best = cost;
-                    p.cg = s.cg, p.bn = s.bn, p.splits = (int)splits;
-                }
+    static const struct { int cg, bn, block, item; } shapes[] = {
+        {2, 512, 1060, 6000}, {2, 256, 630, 3000}, {2, 128, 450, 3000}, {1, 128, 560, 2500}, {1, 64, 430, 2000}};
+    double best = 1e300;
+    for (const auto& s : shapes) {
+        if ((s.bn == 64 && !store) || (s.bn == 512 && form == HALF_STATS)) continue;
+        if (s.cg == 2 && m <= BM) continue;  // the second CTA's rows would be empty
+        const int64_t tiles = ceil_div(m, s.cg * BM) * ceil_div(n, s.bn), slots = sms / s.cg;
+        const int64_t most = store ? std::max<int64_t>(1, std::min(slots / tiles, nkb / 8)) : 1;
+        for (int64_t want = 1; want <= most; want++) {
+            const int64_t per = ceil_div(nkb, want), splits = ceil_div(nkb, per);
+            if (splits != want) continue;
+            double cost = (double)ceil_div(tiles * splits, slots) * ((double)per * s.block + s.item);
+            if (splits > 1) cost += 6000.0 + (splits + 1.0) * m * n * 4.0 / 2000.0;
+            if (cost < best) {
+                best = cost;
+                p.cg = s.cg, p.bn = s.bn, p.splits = (int)splits;
             }
         }
     }
-    if (p.splits > 1 || grouped) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
+    if (p.splits > 1) p.partial_bytes = (size_t)p.splits * m * (ceil_div(n, 4) * 4) * sizeof(float);
     return p;
 }
 
@@ -165,16 +157,15 @@ __global__ void __launch_bounds__(256) half_gemm_reduce_kernel(const float* __re
 int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     if (g.m <= 0 || g.n <= 0) return 0;
     const bool a_mn = g.form == HALF_TN;
-    const bool b_mn = g.form == HALF_NN || g.form == HALF_TN || g.form == HALF_NN_EXTEND || g.form == HALF_NN_GROUPED;
-    const bool grouped = g.form == HALF_NT_GROUPED || g.form == HALF_NN_GROUPED;
+    const bool b_mn = g.form == HALF_NN || g.form == HALF_TN || g.form == HALF_NN_EXTEND;
     const bool extend = (g.form == HALF_NT_EXTEND || g.form == HALF_NN_EXTEND) && g.adapters > 0;
     if (g.m > 0x7fffff00 || g.n > 0x7fffff00 || g.k > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "half product: too large");
     Maps maps{};
     int rc;
     if ((rc = encode(&maps.a, g.a, g.bf16, false, a_mn ? KB : BM))) return rc;
-    if (!grouped && (rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
+    if ((rc = encode(&maps.b, g.b, g.bf16, false, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
     if (extend && (rc = encode(&maps.u, g.u, g.bf16, false, BM))) return rc;
-    if ((extend || grouped) && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
+    if (extend && (rc = encode(&maps.x, g.x, g.bf16, true, b_mn ? KB : std::min(plan.bn, 256) / plan.cg))) return rc;
     Params p{};
     p.m = (int)g.m;
     p.n = (int)g.n;
@@ -186,7 +177,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.splits = plan.splits;
     p.kb_per_split = (int)ceil_div(p.nkb, plan.splits);
     p.index = g.index;
-    p.adapters = (extend || grouped) ? g.adapters : 0;
+    p.adapters = extend ? g.adapters : 0;
     p.rank = extend ? (int)g.u.cols : 0;
     p.target = g.target;
     p.col0 = g.col0;
@@ -198,7 +189,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.gain = g.gain;
     p.fail = device_fail_word();
     if (!p.fail) return set_error(CDCLQ_ERR_CUDA, "half product: no mapped host memory (is there a CUDA device?)");
-    if (plan.splits > 1 || grouped) {
+    if (plan.splits > 1) {
         p.f32out = g.partial;
         p.ldf = ceil_div(g.n, 4) * 4;
         p.split_stride = g.m * p.ldf;
@@ -212,7 +203,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
         p.alpha = g.alpha;
     }
     rc = g.bf16 ? launch_form<true>(g.form, plan.cg, plan.bn, maps, p, st) : launch_form<false>(g.form, plan.cg, plan.bn, maps, p, st);
-    if (rc || plan.splits == 1 || grouped) return rc;
+    if (rc || plan.splits == 1) return rc;
     const int64_t groups = ceil_div(g.m * p.ldf, 4 * 256);
     const unsigned grid = (unsigned)std::min<int64_t>(groups, (int64_t)sm_count() * 8);
     auto kern = g.bf16 ? half_gemm_reduce_kernel<true> : half_gemm_reduce_kernel<false>;

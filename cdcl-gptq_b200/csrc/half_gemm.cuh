@@ -27,7 +27,6 @@ using namespace tc;
 constexpr int BM = 128;            // tile rows of a CTA = tensor-memory lanes
 constexpr int KB = 64;             // K block: 128 bytes of a 16-bit type
 constexpr int A_BYTES = BM * KB * 2;
-constexpr int GROUP = 4;           // ROWS_GROUPED: adapters of a pass over K
 constexpr int EPI_WARPS = 16;      // four per lane quadrant, each with a quarter of the accumulator's columns
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int TURN_BYTES = 32 * 64;   // one epilogue warp's transposition buffer: 64 bytes of each of its 32 rows
@@ -45,8 +44,7 @@ __host__ __device__ constexpr int b_bytes(int cg, int bn) { return bn / cg * KB 
 // How the adapter of each row (index[m]; none if outside [0, adapters)) takes part.
 enum RowMode {
     ROWS_PLAIN = 0,   // not at all
-    ROWS_EXTEND = 1,  // D[m] += U[m] Bx[index[m]]: further K blocks, whose MMAs write the adapter's own rows only
-    ROWS_GROUPED = 2  // D[m] = A[m] B[index[m]]: one pass over K for each adapter of the tile, for its own rows only
+    ROWS_EXTEND = 1   // D[m] += U[m] Bx[index[m]]: further K blocks, whose MMAs write the adapter's own rows only
 };
 enum Epilogue {
     EPI_STORE = 0,  // a 16-bit matrix, and / or f32 partial sums
@@ -54,9 +52,6 @@ enum Epilogue {
     EPI_GRAD = 2    // (softmax - onehot) * dloss as a 16-bit matrix
 };
 
-__host__ __device__ constexpr int stage_bytes(int cg, int bn, int rows) {
-    return A_BYTES + (rows == ROWS_GROUPED ? GROUP : 1) * b_bytes(cg, bn);
-}
 __host__ __device__ constexpr size_t smem_bytes() {
     return RING_BYTES + EPI_WARPS * TURN_BYTES + 1024 /* alignment */ + 256 /* barriers */;
 }
@@ -156,13 +151,12 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                  const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_x, const Params P) {
     constexpr bool WIDE = BN == 512;
     constexpr int AC = WIDE ? 256 : BN;  // columns of an accumulator
-    constexpr int B_BYTES = b_bytes(CG, BN);
-    constexpr int STAGE_BYTES = stage_bytes(CG, BN, ROWS);
+    constexpr int STAGE_BYTES = A_BYTES + b_bytes(CG, BN);
     constexpr int NS = RING_BYTES / STAGE_BYTES;
     constexpr int BC = AC / CG;  // B's rows of an accumulator in this CTA
     constexpr int HALF_BYTES = BC * KB * 2;
     constexpr uint32_t TMEM_COLS = 2 * AC;
-    static_assert(!WIDE || (CG == 2 && ROWS != ROWS_GROUPED && EPI != EPI_STATS), "tiles of 512 columns");
+    static_assert(!WIDE || (CG == 2 && EPI != EPI_STATS), "tiles of 512 columns");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* turn = base + RING_BYTES;
@@ -202,7 +196,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int ctr = 0;
         bool ok = true;
         // waits for the next stage and, in the first CTA, announces the pair's bytes; returns its address
-        auto stage = [&](uint32_t& bar, uint32_t bytes) -> uint32_t {
+        auto stage = [&](uint32_t& bar) -> uint32_t {
             const int s = ctr % NS;
             if (ctr >= NS && !mbar_wait(&empty[s], ((ctr / NS) - 1) & 1, flag)) {
                 ok = false;
@@ -210,7 +204,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             bar = smem_u32(&full[s]);
             if constexpr (CG == 2) bar = first_cta(bar);
-            if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
+            if (rank == 0) mbar_expect_tx(&full[s], CG * STAGE_BYTES);
             ctr++;
             return ring + s * STAGE_BYTES;
         };
@@ -239,66 +233,47 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             item_coords(P, item, mb, nb, split);
             const int m0 = (mb * CG + rank) * BM, n0 = nb * BN + rank * BC;
             const int kb0 = split * P.kb_per_split, kb1 = min(P.nkb, kb0 + P.kb_per_split);
-            if constexpr (ROWS != ROWS_GROUPED) {
-                if (lane == 0) {
-                    for (int kb = kb0; kb < kb1; kb++) {
-                        uint32_t bar;
-                        const uint32_t st = stage(bar, A_BYTES + B_BYTES);
-                        if (!ok) break;
-                        load_a(st, m0, kb, bar);
+            if (lane == 0) {
+                for (int kb = kb0; kb < kb1; kb++) {
+                    uint32_t bar;
+                    const uint32_t st = stage(bar);
+                    if (!ok) break;
+                    load_a(st, m0, kb, bar);
 #pragma unroll
-                        for (int w = 0; w < BN / AC; w++) {
-                            const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
-                            if constexpr (BMN) {
+                    for (int w = 0; w < BN / AC; w++) {
+                        const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
+                        if constexpr (BMN) {
 #pragma unroll
-                                for (int h = 0; h < BC / 64; h++)
-                                    load2(sb + h * (64 * KB * 2), &map_b, n0 + w * AC + 64 * h, kb * KB, bar);
-                            } else {
-                                load2(sb, &map_b, kb * KB, n0 + w * AC, bar);
-                            }
+                            for (int h = 0; h < BC / 64; h++)
+                                load2(sb + h * (64 * KB * 2), &map_b, n0 + w * AC + 64 * h, kb * KB, bar);
+                        } else {
+                            load2(sb, &map_b, kb * KB, n0 + w * AC, bar);
                         }
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
             }
-            if constexpr (ROWS != ROWS_PLAIN) {
-                if (ROWS == ROWS_EXTEND && split != P.splits - 1) continue;  // the last split extends
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if constexpr (ROWS == ROWS_EXTEND) {
+                if (split != P.splits - 1) continue;  // the last split extends
                 RowAdapters<CG> who;
                 who.load(P, mb * CG * BM, lane);
                 uint32_t off[4 * CG];
-                constexpr int MOST = ROWS == ROWS_GROUPED ? GROUP : 1;
-                int j[MOST];
-                for (j[0] = who.next(off); j[0] != RowAdapters<CG>::NONE && ok; j[0] = who.next(off)) {
-                    int count = 1;
-#pragma unroll
-                    for (int q = 1; q < MOST; q++) {
-                        j[q] = who.next(off);
-                        count += j[q] != RowAdapters<CG>::NONE;
-                    }
+                for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
                     if (lane == 0) {
-                        const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
-                        const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
-                        for (int kb = e0; kb < e1; kb++) {
+                        for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
                             uint32_t bar;
-                            const uint32_t st = stage(bar, A_BYTES + count * B_BYTES);
+                            const uint32_t st = stage(bar);
                             if (!ok) break;
-                            if constexpr (ROWS == ROWS_GROUPED)
-                                load_a(st, m0, kb, bar);
-                            else
-                                load2(st, &map_u, kb * KB, m0, bar);
+                            load2(st, &map_u, kb * KB, m0, bar);
 #pragma unroll
-                            for (int q = 0; q < MOST; q++) {
-                                if (q >= count) break;
+                            for (int w = 0; w < BN / AC; w++) {
+                                const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
+                                if constexpr (BMN) {
 #pragma unroll
-                                for (int w = 0; w < BN / AC; w++) {
-                                    const uint32_t sb = st + A_BYTES + q * B_BYTES + w * HALF_BYTES;
-                                    if constexpr (BMN) {
-#pragma unroll
-                                        for (int h = 0; h < BC / 64; h++)
-                                            load3(sb + h * (64 * KB * 2), &map_x, n0 + w * AC + 64 * h, kb * KB, j[q], bar);
-                                    } else {
-                                        load3(sb, &map_x, kb * KB, n0 + w * AC, j[q], bar);
-                                    }
+                                    for (int h = 0; h < BC / 64; h++)
+                                        load3(sb + h * (64 * KB * 2), &map_x, n0 + w * AC + 64 * h, kb * KB, j, bar);
+                                } else {
+                                    load3(sb, &map_x, kb * KB, n0 + w * AC, j, bar);
                                 }
                             }
                         }
@@ -339,21 +314,22 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // descriptors of the first stage's operands; a stage, a half and a step of 16 further are added to their addresses
         constexpr uint64_t A_STEP = (AMN ? 2048 : 32) >> 4, B_STEP = (BMN ? 2048 : 32) >> 4;
         const uint64_t desc_a = AMN ? smem_desc(ring, 64 * KB * 2, 1024) : smem_desc(ring, 16, 1024);
-        const uint64_t desc_u = smem_desc(ring, 16, 1024);  // the extension's first operand is K-major
+        [[maybe_unused]] const uint64_t desc_u = smem_desc(ring, 16, 1024);  // the extension's first operand is K-major
         const uint64_t desc_b = BMN ? smem_desc(ring + A_BYTES, 64 * KB * 2, 1024) : smem_desc(ring + A_BYTES, 16, 1024);
-        constexpr uint32_t ID = idesc_half(BF16, AMN, BMN, CG * BM, AC), ID_U = idesc_half(BF16, false, BMN, CG * BM, AC);
+        constexpr uint32_t ID = idesc_half(BF16, AMN, BMN, CG * BM, AC);
+        [[maybe_unused]] constexpr uint32_t ID_U = idesc_half(BF16, false, BMN, CG * BM, AC);
         // the four MMAs of a stage's operands into d
         auto multiply = [&](uint32_t d, int s, int half, bool fresh) {
             const uint64_t da = desc_a + (uint64_t)(s * (STAGE_BYTES >> 4)), db = desc_b + (uint64_t)(s * (STAGE_BYTES >> 4) + half * (HALF_BYTES >> 4));
 #pragma unroll
             for (int k = 0; k < KB / 16; k++) mma_half<CG>(d, da + k * A_STEP, db + k * B_STEP, ID, (fresh && k == 0) ? 0u : 1u);
         };
-        // `ks` of them for some rows only; at: 16-byte units from the stage's second operand
-        auto multiply_rows = [&](uint32_t d, int s, int at, bool u, int ks, bool fresh, const uint32_t (&off)[4 * CG]) {
-            const uint64_t da = (u ? desc_u : desc_a) + (uint64_t)(s * (STAGE_BYTES >> 4)), db = desc_b + (uint64_t)(s * (STAGE_BYTES >> 4) + at);
+        // `ks` of them, of the extension, for some rows only
+        [[maybe_unused]] auto extend = [&](uint32_t d, int s, int half, int ks, const uint32_t (&off)[4 * CG]) {
+            const uint64_t da = desc_u + (uint64_t)(s * (STAGE_BYTES >> 4)), db = desc_b + (uint64_t)(s * (STAGE_BYTES >> 4) + half * (HALF_BYTES >> 4));
 #pragma unroll
             for (int k = 0; k < KB / 16; k++)
-                if (k < ks) mma_half_rows(d, da + k * (u ? 2 : A_STEP), db + k * B_STEP, u ? ID_U : ID, (fresh && k == 0) ? 0u : 1u, off);
+                if (k < ks) mma_half_rows(d, da + k * 2, db + k * B_STEP, ID_U, 1u, off);
         };
         // the K blocks k0 .. k1 into accumulator d
         auto plain = [&](uint32_t d, int k0, int k1) {
@@ -420,42 +396,25 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             const uint32_t d = accumulator();
             if (!ok) break;
-            if constexpr (ROWS != ROWS_GROUPED) {
-                if (lane == 0) {
-                    if constexpr (WIDE)
-                        plain_wide(acc, kb0, kb1);
-                    else
-                        plain(d, kb0, kb1);
-                }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (lane == 0) {
+                if constexpr (WIDE)
+                    plain_wide(acc, kb0, kb1);
+                else
+                    plain(d, kb0, kb1);
             }
-            if constexpr (ROWS != ROWS_PLAIN) {
-                if (ROWS == ROWS_GROUPED || split == P.splits - 1) {
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if constexpr (ROWS == ROWS_EXTEND) {
+                if (split == P.splits - 1) {
                     RowAdapters<CG> who;
                     who.load(P, mb * CG * BM, lane);
-                    constexpr int MOST = ROWS == ROWS_GROUPED ? GROUP : 1;
-                    uint32_t off[MOST][4 * CG];
-                    while (ok && who.next(off[0]) != RowAdapters<CG>::NONE) {
-                        int count = 1;
-#pragma unroll
-                        for (int q = 1; q < MOST; q++) count += who.next(off[q]) != RowAdapters<CG>::NONE;
+                    uint32_t off[4 * CG];
+                    while (ok && who.next(off) != RowAdapters<CG>::NONE) {
                         if (lane == 0) {
-                            const int e0 = ROWS == ROWS_GROUPED ? kb0 : 0;
-                            const int e1 = ROWS == ROWS_GROUPED ? kb1 : (P.rank + KB - 1) / KB;
-                            for (int kb = e0; kb < e1; kb++) {
+                            for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
                                 if (!arrived(false)) break;
-                                if constexpr (ROWS == ROWS_GROUPED) {
 #pragma unroll
-                                    for (int q = 0; q < MOST; q++) {
-                                        if (q >= count) break;
-                                        multiply_rows(d, slot, q * (B_BYTES >> 4), false, KB / 16, kb == kb0, off[q]);
-                                    }
-                                } else {
-#pragma unroll
-                                    for (int w = 0; w < BN / AC; w++)
-                                        multiply_rows(d + w * AC, slot, w * (HALF_BYTES >> 4), true,
-                                                      min(KB / 16, (P.rank - kb * KB + 15) / 16), false, off[0]);
-                                }
+                                for (int w = 0; w < BN / AC; w++)
+                                    extend(d + w * AC, slot, w, min(KB / 16, (P.rank - kb * KB + 15) / 16), off);
                                 done();
                             }
                         }
@@ -571,10 +530,6 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             int64_t label = -1;  // relative to this piece's column 0
             bool none = false;
             if constexpr (EPI == EPI_STORE) {
-                if constexpr (ROWS == ROWS_GROUPED) {
-                    const int id = live ? P.index[row] : -1;
-                    none = id < 0 || id >= P.adapters;
-                }
                 if (P.alpha) factor = *P.alpha;
             } else {
                 const int64_t t = live ? P.target[row] : -1;
@@ -625,9 +580,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             if (P.f32out) {
 #pragma unroll
                                 for (int i = 0; i < 4; i++)
-                                    *reinterpret_cast<float4*>(chunk(lane, i)) = (ROWS == ROWS_GROUPED && none)
-                                                                                     ? make_float4(0, 0, 0, 0)
-                                                                                     : make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
+                                    *reinterpret_cast<float4*>(chunk(lane, i)) = make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
                                 __syncwarp();
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {

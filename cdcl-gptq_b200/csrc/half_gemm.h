@@ -20,9 +20,7 @@ enum HalfForm {
     HALF_NN,          // K-major x MN-major, stored
     HALF_TN,          // MN-major x MN-major, stored
     HALF_NT_EXTEND,   // K-major x K-major plus the rows' adapters, stored
-    HALF_NN_EXTEND,   // K-major x MN-major plus the rows' adapters, stored
-    HALF_NT_GROUPED,  // K-major x the row's own K-major operand, the splits' f32 sums left in `partial`
-    HALF_NN_GROUPED   // K-major x the row's own MN-major operand, likewise
+    HALF_NN_EXTEND    // K-major x MN-major plus the rows' adapters, stored
 };
 
 // A 16-bit operand: `rows` x `cols` (cols contiguous), `ld` elements from row to row, `batch` of them `step` elements apart.
@@ -36,8 +34,8 @@ struct HalfGemm {
     HalfForm form;
     bool bf16;
     int64_t m, n, k;
-    HalfOperand a, b;            // b: unused in the grouped forms
-    HalfOperand u, x;            // extension: u (m x rank) times x[adapter]; grouped: x[adapter] is the second operand
+    HalfOperand a, b;
+    HalfOperand u, x;            // extension: u (m x rank) times x[adapter]
     const int* index = nullptr;  // the rows' adapters
     int adapters = 0;
     void* out = nullptr;         // 16-bit, ldo elements from row to row
@@ -54,8 +52,7 @@ struct HalfGemm {
     float* partial = nullptr;    // workspace of the split plan
 };
 
-// Tile (cg CTAs of 128 rows, bn columns) and K splits of a product; partial_bytes of workspace when splits > 1, and for the grouped forms.
-// Split s of row m is at partial + (s * m_total + m) * ld, ld = n rounded up to a multiple of 4.
+// Tile (cg CTAs of 128 rows, bn columns) and K splits of a product; partial_bytes of workspace when splits > 1.
 struct HalfPlan {
     int cg, bn, splits;
     size_t partial_bytes;

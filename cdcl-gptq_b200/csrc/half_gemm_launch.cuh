@@ -36,18 +36,14 @@ static int launch_one(const Maps& maps, const Params& p, cudaStream_t st) {
 
 template <bool BF16, bool AMN, bool BMN, int ROWS, int EPI>
 static int launch_tile(int cg, int bn, const Maps& maps, const Params& p, cudaStream_t st) {
-    if constexpr (ROWS == ROWS_GROUPED) {
-        return launch_one<BF16, AMN, BMN, 1, 64, ROWS, EPI>(maps, p, st);
-    } else {
-        if constexpr (EPI != EPI_STATS) {
-            if (bn == 512) return launch_one<BF16, AMN, BMN, 2, 512, ROWS, EPI>(maps, p, st);
-        }
-        if (cg == 2 && bn == 256) return launch_one<BF16, AMN, BMN, 2, 256, ROWS, EPI>(maps, p, st);
-        if (cg == 2) return launch_one<BF16, AMN, BMN, 2, 128, ROWS, EPI>(maps, p, st);
-        if (bn == 128) return launch_one<BF16, AMN, BMN, 1, 128, ROWS, EPI>(maps, p, st);
-        if constexpr (EPI == EPI_STORE) return launch_one<BF16, AMN, BMN, 1, 64, ROWS, EPI>(maps, p, st);
-        return set_error(CDCLQ_ERR_ARG, "half product: no such tile");
+    if constexpr (EPI != EPI_STATS) {
+        if (bn == 512) return launch_one<BF16, AMN, BMN, 2, 512, ROWS, EPI>(maps, p, st);
     }
+    if (cg == 2 && bn == 256) return launch_one<BF16, AMN, BMN, 2, 256, ROWS, EPI>(maps, p, st);
+    if (cg == 2) return launch_one<BF16, AMN, BMN, 2, 128, ROWS, EPI>(maps, p, st);
+    if (bn == 128) return launch_one<BF16, AMN, BMN, 1, 128, ROWS, EPI>(maps, p, st);
+    if constexpr (EPI == EPI_STORE) return launch_one<BF16, AMN, BMN, 1, 64, ROWS, EPI>(maps, p, st);
+    return set_error(CDCLQ_ERR_ARG, "half product: no such tile");
 }
 
 template <bool BF16>
@@ -59,8 +55,6 @@ int launch_form(HalfForm form, int cg, int bn, const Maps& maps, const Params& p
         case HALF_TN: return launch_tile<BF16, true, true, ROWS_PLAIN, EPI_STORE>(cg, bn, maps, p, st);
         case HALF_NT_EXTEND: return launch_tile<BF16, false, false, ROWS_EXTEND, EPI_STORE>(cg, bn, maps, p, st);
         case HALF_NN_EXTEND: return launch_tile<BF16, false, true, ROWS_EXTEND, EPI_STORE>(cg, bn, maps, p, st);
-        case HALF_NT_GROUPED: return launch_tile<BF16, false, false, ROWS_GROUPED, EPI_STORE>(cg, bn, maps, p, st);
-        case HALF_NN_GROUPED: return launch_tile<BF16, false, true, ROWS_GROUPED, EPI_STORE>(cg, bn, maps, p, st);
     }
     return set_error(CDCLQ_ERR_ARG, "half product: no such form");
 }

@@ -5,10 +5,8 @@
 #include <type_traits>
 #include <vector>
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "half_gemm.h"
+#include "mma16.cuh"
 #include "packed.h"
 #include "tcgen05.cuh"
 
@@ -156,15 +154,6 @@ __global__ void __launch_bounds__(256) packed_grid_kernel(const uint16_t* __rest
         }
         grid[i] = v;
     }
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint16_t half_bits(float v) {
-    return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
-}
-template <bool BF16>
-__device__ __forceinline__ float half_value(uint16_t v) {
-    return BF16 ? __uint_as_float((uint32_t)v << 16) : __half2float(__ushort_as_half(v));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -479,18 +468,6 @@ __global__ void __launch_bounds__(256) packed_tokens_kernel(const PackedView W, 
     xf[i] = tok < t ? make_uint2(a | b << 16, c | d << 16) : make_uint2(0, 0);
 }
 
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
-    if constexpr (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
-}
-
 // One unit of a row tile times NT token tiles.  codes: the unit's words; grid: the tile's, one word for each (group, row).
 template <bool BF16, int BITS, int NT>
 __device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t* codes, const uint32_t* grid, const uint2 (&x)[4][NT],
@@ -509,7 +486,7 @@ __device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t*
 #pragma unroll
             for (int p = 0; p < 4; p++) a[p] = decode_pair<BF16, BITS>(w, ks, p, zero[p & 1]);
 #pragma unroll
-            for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n]);
+            for (int n = 0; n < NT; n++) mma16816<BF16>(part[n], a, x[ks][n].x, x[ks][n].y);
         }
         const float f0 = __half2float(__ushort_as_half((uint16_t)s0)), f1 = __half2float(__ushort_as_half((uint16_t)s1));
 #pragma unroll
@@ -528,7 +505,7 @@ __device__ __forceinline__ void decode_unit(const PackedUnit& u, const uint32_t*
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float part[4] = {};
-                mma16816<BF16>(part, a, x[ks][n]);
+                mma16816<BF16>(part, a, x[ks][n].x, x[ks][n].y);
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[n][i] = fmaf(i < 2 ? f0 : f1, part[i], acc[n][i]);
             }
@@ -565,7 +542,7 @@ __host__ __device__ constexpr int dec_sums(int nt) { return nt * 8 * 17; }
 template <bool BF16, int BITS, int NT>
 __global__ void __launch_bounds__(DEC_THREADS, 1) packed_decode_kernel(const PackedView W, const AdapterArgs ad, const DecodeArgs P) {
     extern __shared__ __align__(128) uint32_t smem[];
-    constexpr int UNITS = dec_units(NT), CHUNK = dec_chunk(NT), TOK = NT * 8;
+    constexpr int UNITS = dec_units(NT), CHUNK = dec_chunk(NT);
     __shared__ uint64_t ready[2];
     __shared__ int flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp % DEC_GROUPS, parity = warp / DEC_GROUPS;
