@@ -80,9 +80,10 @@ __device__ __forceinline__ void token_list(const RankArgs& P, int id) {
     if (id == P.n - 1 && threadIdx.x == 0) P.start[P.n] = at;
 }
 
-// TOKENS: 64, a warp for each 16 of them, or 16, a warp for each 16 of the K block's columns.
-template <bool BF16, bool TRANSPOSED, int TOKENS>
-__global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
+// TOKENS: 64, a warp for each 16 of them, or 16, a warp for each 16 of the K block's columns.  NT: the ranks' tiles of 8, at
+// most; fewer leave registers for a fourth CTA on the SM.
+template <bool BF16, bool TRANSPOSED, int TOKENS, int NT>
+__global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const RankArgs P) {
     extern __shared__ __align__(16) uint16_t ring[];
     __shared__ int id_of[TOKENS], who[TOKENS], found;
     const int products = P.compute ? P.tiles * P.cut : 0;
@@ -112,15 +113,15 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
     const int m0 = TOKENS == 64 ? warp * 16 : 0;
     const int pitch = TRANSPOSED ? P.rp + 8 : X_PITCH, fh = factor_halves(P.rp, TRANSPOSED), sh = stage_halves(TOKENS, P.rp, TRANSPOSED);
     const int mine0 = id_of[m0 + lane / 4], mine1 = id_of[m0 + lane / 4 + 8];
-    float sums[8][4];
+    float sums[NT][4];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
+    for (int j = 0; j < NT; j++)
 #pragma unroll
         for (int i = 0; i < 4; i++) sums[j][i] = 0.0f;
 
     // This thread's copies of a stage: XC pieces of 16 bytes of the tokens, up to FC of each factor.  A whole K block needs only
     // their offsets; the last one, cut short, is looked at piece by piece.
-    constexpr int XC = TOKENS * 8 / THREADS, FC = 4;
+    constexpr int XC = TOKENS * 8 / THREADS, FC = NT / 2;
     const int pieces = TRANSPOSED ? KB * P.rp / 8 : P.rp * 8;  // of a factor
     const uint16_t* x_from[XC];
     bool x_live[XC];
@@ -150,13 +151,13 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
     for (int g0 = 0; g0 < found; g0 += PAIR) {
         const int pair = min(PAIR, found - g0);
         bool use[PAIR];  // some token of this warp has the adapter
-        float acc[PAIR][8][4];
+        float acc[PAIR][NT][4];
 #pragma unroll
         for (int q = 0; q < PAIR; q++) {
             const int j = q < pair ? who[g0 + q] : -1;
             use[q] = __any_sync(0xffffffffu, mine0 == j || mine1 == j);
 #pragma unroll
-            for (int n = 0; n < 8; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[q][n][i] = 0.0f;
         }
@@ -233,8 +234,8 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
                     if (!use[q]) continue;
                     const uint16_t* f = st + TOKENS * X_PITCH + q * fh;
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        if (j * 8 >= P.rp) break;
+                    for (int j = 0; j < NT; j += 2) {
+                        if (NT == 8 && j * 8 >= P.rp) break;
                         uint32_t b[4];
                         if (TRANSPOSED)
                             load_pieces<true>(b, f + (kk + (lane & 15)) * pitch + j * 8 + (lane >> 4) * 8);
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
         for (int q = 0; q < PAIR; q++) {
             const int j = q < pair ? who[g0 + q] : -1;
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
+            for (int n = 0; n < NT; n++) {
                 if (mine0 == j) sums[n][0] = acc[q][n][0], sums[n][1] = acc[q][n][1];
                 if (mine1 == j) sums[n][2] = acc[q][n][2], sums[n][3] = acc[q][n][3];
             }
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
     float* part = reinterpret_cast<float*>(ring);
     constexpr int PITCH = MOST_RANK + 2;
 #pragma unroll
-    for (int n = 0; n < 8; n++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) part[(warp * 16 + lane / 4 + (i >> 1) * 8) * PITCH + n * 8 + (lane & 3) * 2 + (i & 1)] = sums[n][i];
     __syncthreads();
@@ -297,9 +298,9 @@ __global__ void __launch_bounds__(THREADS) rank_kernel(const RankArgs P) {
     }
 }
 
-template <bool BF16, bool TRANSPOSED, int TOKENS>
+template <bool BF16, bool TRANSPOSED, int TOKENS, int NT>
 int launch(const RankArgs& p, cudaStream_t st) {
-    auto kern = rank_kernel<BF16, TRANSPOSED, TOKENS>;
+    auto kern = rank_kernel<BF16, TRANSPOSED, TOKENS, NT>;
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_smem(kern, smem_bytes(TOKENS, MOST_RANK, TRANSPOSED), done, "rank_kernel shared memory")) return rc;
     const int64_t lists = p.start ? ceil_div(p.n, p.cut) * p.cut : 0;
@@ -319,9 +320,14 @@ int launch(const RankArgs& p, cudaStream_t st) {
     return e == cudaSuccess ? 0 : cuda_error(e, "rank_kernel launch");
 }
 
+template <bool BF16, bool TRANSPOSED, int TOKENS>
+int launch_ranks(const RankArgs& p, cudaStream_t st) {
+    if (p.rp == 16) return launch<BF16, TRANSPOSED, TOKENS, 2>(p, st);
+    return p.rp == 32 ? launch<BF16, TRANSPOSED, TOKENS, 4>(p, st) : launch<BF16, TRANSPOSED, TOKENS, 8>(p, st);
+}
 template <bool BF16, bool TRANSPOSED>
 int launch_tokens(const RankArgs& p, bool few, cudaStream_t st) {
-    return few ? launch<BF16, TRANSPOSED, 16>(p, st) : launch<BF16, TRANSPOSED, 64>(p, st);
+    return few ? launch_ranks<BF16, TRANSPOSED, 16>(p, st) : launch_ranks<BF16, TRANSPOSED, 64>(p, st);
 }
 
 }  // namespace
@@ -332,7 +338,7 @@ int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st) {
     // 16 tokens to a cluster where 64 leave SMs idle even with 8 CTAs each; K blocks over as many CTAs as make four to an SM,
     // four blocks at least for each
     const int sms = sm_count(), nkb = (int)ceil_div(p.k, KB);
-    const bool few = ceil_div(p.t, 64) * 8 < 2 * sms;
+    const bool few = ceil_div(p.t, 64) * 8 < sms;
     p.tiles = (int)ceil_div(p.t, few ? 16 : 64);
     p.cut = 1;
     while (p.cut < 8 && (int64_t)p.tiles * p.cut * ceil_div(p.r, MOST_RANK) < 4 * sms && nkb / (p.cut * 2) >= 4) p.cut *= 2;
