@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(256) outer_kernel(const OuterPair P) {
         outer_tile<BF16, CODES, true>(P, P.a, ring, list, count, id, chunks, slot, blockIdx.x, k0);
     else
         outer_tile<BF16, false, false>(P, P.b, ring, list, count, id, chunks, slot, blockIdx.x - P.a.tiles, k0);
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) wait_for_previous();
 }
 
 // The adapters of several chunks: out = factor * (slot 0 + slot 1 + ...), four neighbouring values a thread.
@@ -342,7 +343,8 @@ int outer_chunk(int64_t t, int64_t tiles, int64_t r) {
 // Slots of adapters with several chunks: each such adapter has over `chunk` tokens, so it has fewer than 2 tokens / chunk.
 int64_t outer_slots(int64_t t, int chunk) { return 2 * t / chunk; }
 
-int launch_outer(bool bf16, const OuterPair& p, cudaStream_t st) {
+// beside: the launch before this one is not the one that made its factors or lists.
+int launch_outer(bool bf16, const OuterPair& p, bool beside, cudaStream_t st) {
     // an adapter without tokens still writes its zeros: one item each
     const int64_t items = ceil_div(p.t, p.chunk) + p.n, tiles = p.a.tiles + p.b.tiles;
     if (items > 65535) return set_error(CDCLQ_ERR_ARG, "adapters: too many tokens or adapters for one call");
@@ -353,7 +355,7 @@ int launch_outer(bool bf16, const OuterPair& p, cudaStream_t st) {
     auto kern = bf16 ? (p.a.codes ? outer_kernel<true, true> : outer_kernel<true, false>)
                      : (p.a.codes ? outer_kernel<false, true> : outer_kernel<false, false>);
     if (int rc = allow_smem(kern, smem, done[which], "outer_kernel shared memory")) return rc;
-    CDCLQ_LAUNCH(kern, grid, 256, smem, st, p);
+    if (int rc = launch_after(beside, kern, grid, dim3(256), smem, st, "outer_kernel launch", p)) return rc;
     if (outer_slots(p.t, p.chunk) > 0) {
         const int64_t most = (int64_t)p.r * std::max(p.a.cols, p.b.cols);
         const unsigned gx = (unsigned)std::max<int64_t>(1, std::min<int64_t>(ceil_div(most, 256), sm_count() * 4));
@@ -496,7 +498,7 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         p.lds = ldr;
         if ((rc = launch_rank(bf16, false, p, st))) return rc;
     }
-    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;
+    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, n > 0, st))) return rc;  // beside u's products
     HalfGemm g{};
     g.form = HALF_NT_EXTEND;
     g.bf16 = bf16;
@@ -566,7 +568,7 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         if ((rc = launch_rank(bf16, true, p, st))) return rc;
     }
     if (dx) {
-        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, st))) return rc;
+        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, n > 0, st))) return rc;  // beside v's products
         HalfGemm g{};
         g.form = HALF_NN_EXTEND;
         g.bf16 = bf16;
@@ -623,5 +625,6 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         o.b.tiles = (int)ceil_div(v.d_out, OUTER_COLS);
     }
     o.chunk = outer_chunk(t, o.a.tiles + o.b.tiles, r);
-    return launch_outer(bf16, o, st);
+    // dx's product stands between them, unless its sums were split: then the kernel that joins them does
+    return launch_outer(bf16, o, dx && plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out).splits == 1, st);
 }

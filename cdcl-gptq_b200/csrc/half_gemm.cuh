@@ -169,6 +169,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 2 ? (int)cluster_rank() : 0;
 
+    // a later kernel that needs nothing of this one may take the SMs that run out of tiles
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int s = 0; s < NS; s++) {
             mbar_init(&full[s], 1);

@@ -65,10 +65,10 @@ int64_t half_stats_parts(const HalfPlan& plan, int64_t n);
 // Launches the product (and, when the plan splits K, the pass that adds the splits in order).
 int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st);
 
-// Launches a kernel that may start while the one before it in the stream still runs; it waits for that one's results itself
-// (griddepcontrol.wait).
+// Launches a kernel.  overlap: it may start while the kernel before it in the stream still runs, once that one has let it
+// (griddepcontrol.launch_dependents); what it needs of that one's results it waits for itself (griddepcontrol.wait).
 template <typename... Params, typename... Args>
-int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what, const Args&... args) {
+int launch_after(bool overlap, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what, const Args&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -78,7 +78,7 @@ int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t sm
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = overlap ? 1 : 0;
     g_launches.fetch_add(1, std::memory_order_relaxed);
     cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return e == cudaSuccess ? 0 : cuda_error(e, what);

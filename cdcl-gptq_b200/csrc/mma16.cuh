@@ -53,6 +53,9 @@ __device__ __forceinline__ void load_pieces(uint32_t (&v)[4], const void* p) {
                      : "memory");
 }
 
+// A kernel that ran beside the one before it in the stream ends after it, so that what follows finds both done: one CTA waits.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 16 bytes to shared memory, zeros unless `live` (src is then not read).
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),

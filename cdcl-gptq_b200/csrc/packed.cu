@@ -18,7 +18,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct Sections {
-    size_t unit, column, place, grid, codes, total;
+    size_t unit, column, scatter, grid, codes, total;
 };
 Sections sections(uint64_t d_out, uint64_t d_in, uint64_t groups, uint64_t units, uint64_t tile_words) {
     const uint64_t tiles = (d_out + 15) / 16;
@@ -26,7 +26,7 @@ Sections sections(uint64_t d_out, uint64_t d_in, uint64_t groups, uint64_t units
     size_t at = 0;
     s.unit = at, at += align_up(units * sizeof(PackedUnit));
     s.column = at, at += align_up(units * 64 * sizeof(int));
-    s.place = at, at += align_up(d_in * sizeof(int));
+    s.scatter = at, at += align_up(units * 64 * sizeof(uint32_t));
     s.grid = at, at += align_up(tiles * groups * 16 * sizeof(uint32_t));
     s.codes = at, at += align_up(tiles * tile_words * 32 * sizeof(uint32_t));
     s.total = at;
@@ -122,20 +122,22 @@ __global__ void __launch_bounds__(256) packed_layout_kernel(const uint8_t* __res
     }
 }
 
-// column: permuted place -> original column; place: its inverse.  A perm that is not one raises *bad.
-__global__ void __launch_bounds__(256) packed_columns_kernel(const int* __restrict__ perm, int places, int d_in, int* column, int* place,
-                                                             int* seen, int* bad) {
+// column: permuted place -> original column; scatter: see PackedView.  A perm that is not one raises *bad.
+__global__ void __launch_bounds__(256) packed_columns_kernel(const int* __restrict__ perm, int places, int d_in, int pitch, int* column,
+                                                             uint32_t* scatter, int* seen, int* bad) {
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < places; i += gridDim.x * blockDim.x) {
         const int j = column[i];
-        if (j < 0) continue;
-        const int c = perm[j];
-        if (c < 0 || c >= d_in || atomicAdd(&seen[c], 1)) {
-            *bad = 1;
-            column[i] = -1;
-            continue;
+        int c = -1;
+        if (j >= 0) {
+            c = perm[j];
+            if (c < 0 || c >= d_in || atomicAdd(&seen[c], 1)) {
+                *bad = 1;
+                c = -1;
+            }
+            column[i] = c;
         }
-        column[i] = c;
-        place[c] = i;
+        const int k = i & 15;
+        scatter[(i >> 6) * 64 + ((k & 7) >> 1) * 16 + ((i >> 4) & 3) * 4 + (k >> 3) * 2 + (k & 1)] = 2u * (c >= 0 ? c : pitch - 1);
     }
 }
 
@@ -218,13 +220,15 @@ __device__ __forceinline__ uint32_t decode_pair(const uint32_t (&w)[BITS], int k
     }
 }
 
-// scale * (code - zero point), rounded once: the product of an 11-bit and an 8-bit significand is exact in f32, and f16's
-// own product is that product rounded.
+// scale * (code - zero point) of a pair, rounded once: the product of an 11-bit and an 8-bit significand is exact in f32, and
+// f16's own product is that product rounded.
 template <bool BF16>
 __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) {
     if constexpr (BF16) {
-        const float s = __half2float(__ushort_as_half((uint16_t)scale_f16));
-        __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(d << 16) * s, __uint_as_float(d & 0xffff0000u) * s);
+        const uint32_t s = __float_as_uint(__half2float(__ushort_as_half((uint16_t)scale_f16)));
+        uint64_t p;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"((uint64_t)(d & 0xffff0000u) << 32 | d << 16), "l"((uint64_t)s << 32 | s));
+        __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)(p >> 32)));
         return *reinterpret_cast<uint32_t*>(&r);
     } else {
         const uint32_t ss = scale_f16 | scale_f16 << 16;
@@ -235,13 +239,13 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) 
 
 constexpr int EXPAND_WARPS = 16;
 
-// The unit's codes of one half of the tile's rows, scaled, to the rows' columns; padding goes to column `trash`.
+// The unit's codes of one half of the tile's rows, scaled, to their columns of `row`.
 template <bool BF16, int BITS, bool ALL>
-__device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[BITS], const int2* __restrict__ column,
-                                            const uint32_t* __restrict__ g, int half, bool live, uint16_t* row, uint32_t trash) {
-    int2 c[8];
+__device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[BITS], const uint4* __restrict__ scatter,
+                                            const uint32_t* __restrict__ g, int half, bool live, char* row) {
+    uint4 to[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) c[i] = column[i * 4];
+    for (int i = 0; i < 4; i++) to[i] = scatter[i];
     // the upper rows' codes follow the lower rows' in every plane
     int at = 0;
 #pragma unroll
@@ -251,22 +255,26 @@ __device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[B
         for (int i = 0; i < pb; i++) w[at + i] >>= half * pb;
         at += pb;
     }
-    const bool one = u.group[0] == u.group[3];
-    uint32_t sz = g[(int64_t)u.group[0] * 16], zero = zero_pair<BF16, BITS>(sz);
-#pragma unroll
-    for (int ks = 0; ks < 4; ks++) {
-        if (ks > 0 && !one) {
-            sz = g[(int64_t)u.group[ks] * 16];
-            zero = zero_pair<BF16, BITS>(sz);
+    auto step = [&](int ks, uint32_t sz, uint32_t zero) {
+        const uint32_t lo = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, 0, zero), sz & 0xffffu);
+        const uint32_t hi = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, 2, zero), sz & 0xffffu);
+        if (ALL || live) {
+            *reinterpret_cast<uint16_t*>(row + to[ks].x) = (uint16_t)lo;
+            *reinterpret_cast<uint16_t*>(row + to[ks].y) = (uint16_t)(lo >> 16);
+            *reinterpret_cast<uint16_t*>(row + to[ks].z) = (uint16_t)hi;
+            *reinterpret_cast<uint16_t*>(row + to[ks].w) = (uint16_t)(hi >> 16);
         }
+    };
+    const uint32_t sz = g[(int64_t)u.group[0] * 16];
+    if (u.group[0] == u.group[3]) {
+        const uint32_t zero = zero_pair<BF16, BITS>(sz);
 #pragma unroll
-        for (int hi = 0; hi < 2; hi++) {
-            const uint32_t v = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, hi * 2, zero), sz & 0xffffu);
-            const int2 to = c[ks * 2 + hi];
-            if (ALL || live) {
-                row[min((uint32_t)to.x, trash)] = (uint16_t)v;
-                row[min((uint32_t)to.y, trash)] = (uint16_t)(v >> 16);
-            }
+        for (int ks = 0; ks < 4; ks++) step(ks, sz, zero);
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            const uint32_t s = g[(int64_t)u.group[ks] * 16];
+            step(ks, s, zero_pair<BF16, BITS>(s));
         }
     }
 }
@@ -282,12 +290,11 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = first >> 3, r0 = lane / 4 - (first & 7);
     const bool live = r0 >= 0 && r0 < R;
-    uint16_t* row = rows + (live ? r0 : 0) * ld;
-    const uint32_t trash = ld - 1;
+    char* row = reinterpret_cast<char*>(rows + (live ? r0 : 0) * ld);
     const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
     const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
     const uint32_t* g = grid + half * 8 + lane / 4;
-    const int2* columns = reinterpret_cast<const int2*>(W.column) + (lane & 3);
+    const uint4* scatter = reinterpret_cast<const uint4*>(W.scatter) + (lane & 3) * 4;
     if constexpr (BITS) {
         // the next unit's codes are on their way while this one is decoded
         uint32_t ahead[BITS];
@@ -302,7 +309,7 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
             u = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
 #pragma unroll
             for (int i = 0; i < BITS; i++) ahead[i] = codes[(u.word + i) * 32 + lane];
-            expand_unit<BF16, BITS, ALL>(here, w, columns + ui * 32, g, half, live, row, trash);
+            expand_unit<BF16, BITS, ALL>(here, w, scatter + ui * 16, g, half, live, row);
         }
     } else {
         auto unit = [&](auto width, const PackedUnit& u, int ui) {
@@ -310,7 +317,7 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
             uint32_t w[B];
 #pragma unroll
             for (int i = 0; i < B; i++) w[i] = codes[(u.word + i) * 32 + lane];
-            expand_unit<BF16, B, ALL>(u, w, columns + ui * 32, g, half, live, row, trash);
+            expand_unit<BF16, B, ALL>(u, w, scatter + ui * 16, g, half, live, row);
         };
         for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
             const PackedUnit u = W.unit[ui];
@@ -338,28 +345,28 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
             for (int c = threadIdx.x; c < W.d_in; c += EXPAND_WARPS * 32) dst[c] = src[c];
         }
     }
+    if (blockIdx.x == 0) wait_for_previous();
 }
 
 template <bool BF16, int BITS>
-int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, cudaStream_t st) {
+int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, bool beside, cudaStream_t st) {
     static std::atomic<uint64_t> done_all{0}, done_some{0};
     auto kern = R == 8 ? packed_expand_kernel<BF16, BITS, true> : packed_expand_kernel<BF16, BITS, false>;
     if (int rc = allow_smem(kern, 220 * 1024, R == 8 ? done_all : done_some, "packed_expand_kernel shared memory")) return rc;
-    CDCLQ_LAUNCH(kern, w.tiles * (16 / R), EXPAND_WARPS * 32, (size_t)(R * ld * 2), st, w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? 0 : cuda_error(e, "packed_expand_kernel launch");
+    return launch_after(beside, kern, dim3(w.tiles * (16 / R)), dim3(EXPAND_WARPS * 32), (size_t)(R * ld * 2), st,
+                        "packed_expand_kernel launch", w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
 }
 
 // The widths of configurations that quantize every group alike have a kernel of their own; the others share one that
 // branches by unit.
 template <bool BF16>
-int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, cudaStream_t st) {
+int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, bool beside, cudaStream_t st) {
     switch (w.bits) {
-        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, st);
-        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, st);
-        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, st);
-        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, st);
-        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, st);
+        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, beside, st);
+        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, beside, st);
+        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, beside, st);
+        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, beside, st);
+        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, beside, st);
     }
 }
 
@@ -376,20 +383,19 @@ PackedView packed_view(const cdclq_packed_layer& w) {
     v.bits = (int)w.bits;
     v.unit = reinterpret_cast<const PackedUnit*>(base + s.unit);
     v.column = reinterpret_cast<const int*>(base + s.column);
-    v.place = reinterpret_cast<const int*>(base + s.place);
+    v.scatter = reinterpret_cast<const uint32_t*>(base + s.scatter);
     v.grid = reinterpret_cast<const uint32_t*>(base + s.grid);
     v.codes = reinterpret_cast<const uint32_t*>(base + s.codes);
     return v;
 }
 
-int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, cudaStream_t st) {
-    // rows 4 banks apart (16 bytes past a multiple of 128), whole 16-byte pieces
-    const int64_t ld = ceil_div(w.d_in, 64) * 64 + 8;
+int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, bool beside, cudaStream_t st) {
+    const int64_t ld = expand_pitch(w.d_in);
     int R = 8;
     while (R > 1 && R * ld * 2 > 220 * 1024) R /= 2;
     if (R * ld * 2 > 220 * 1024) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
     const int wide = ldw % 8 == 0 && ldw >= ceil_div(w.d_in, 8) * 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, st) : expand_any<false>(w, R, ld, out, ldw, wide, st);
+    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, beside, st) : expand_any<false>(w, R, ld, out, ldw, wide, beside, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -674,7 +680,7 @@ int decode_tokens(const PackedView& w, const AdapterArgs& ad, DecodeArgs p, cuda
     auto kern = packed_decode_kernel<BF16, BITS, NT>;
     static std::atomic<uint64_t> done{0};
     if (int rc = allow_smem(kern, DEC_SMEM, done, "packed_decode_kernel shared memory")) return rc;
-    return launch_dependent(kern, dim3((unsigned)ceil_div(w.tiles, p.tiles)), dim3(DEC_THREADS), smem, st, "packed_decode_kernel launch",
+    return launch_after(true, kern, dim3((unsigned)ceil_div(w.tiles, p.tiles)), dim3(DEC_THREADS), smem, st, "packed_decode_kernel launch",
                             w, ad, p);
 }
 
@@ -803,7 +809,8 @@ static int build_layer(const uint8_t* qweight, const void* scales_f16, const uin
                      static_cast<const uint16_t*>(scales_f16), qzeros, reinterpret_cast<const uint8_t*>(tmp + o2), v.d_out, v.groups,
                      v.tiles, const_cast<uint32_t*>(v.grid), verdict);
         CDCLQ_LAUNCH(packed_columns_kernel, (unsigned)std::min<int64_t>(most, ceil_div(v.units * 64, 256)), 256, 0, st, perm, v.units * 64,
-                     v.d_in, const_cast<int*>(v.column), const_cast<int*>(v.place), reinterpret_cast<int*>(tmp + o3), verdict);
+                     v.d_in, expand_pitch(v.d_in), const_cast<int*>(v.column), const_cast<uint32_t*>(v.scatter),
+                     reinterpret_cast<int*>(tmp + o3), verdict);
         e = cudaGetLastError();
         if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, verdict, sizeof(int), cudaMemcpyDeviceToHost, st);
     }

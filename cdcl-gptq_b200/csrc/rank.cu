@@ -86,6 +86,7 @@ template <bool BF16, bool TRANSPOSED, int TOKENS, int NT>
 __global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const RankArgs P) {
     extern __shared__ __align__(16) uint16_t ring[];
     __shared__ int id_of[TOKENS], who[TOKENS], found;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int products = P.compute ? P.tiles * P.cut : 0;
     if ((int)blockIdx.x >= products) {
         if (blockIdx.y == 0 && (int)blockIdx.x - products < P.n) token_list(P, blockIdx.x - products);
