@@ -92,8 +92,9 @@ __device__ __forceinline__ float value_of_bits(uint32_t b, const __nv_bfloat16*)
 constexpr int SAVE_LANES = 8, SAVE_VALUES = BLOCK / SAVE_LANES;  // lanes of a block, values of a lane
 constexpr int SAVE_GROUPS = 256 / SAVE_LANES;
 
-// 8 lanes to a block of 128 columns, 16 neighbouring values a lane.  A CTA has 32 such groups: `across` of them (a power of
-// two) side by side along a row, 32 / across rows.
+// 8 lanes to a block of 128 columns, 16 values a lane: neighbouring ones where rows start on 16 bytes (WIDE), else every
+// eighth, so that the lanes' single values lie side by side.  A CTA has 32 such groups: `across` of them (a power of two)
+// along a row, 32 / across rows.
 //
 // x / s to the nearest whole number of the rounded quotient, ties to even (values of few bits meet ties often: with a block's
 // largest value a power of two, in one of two).  With y = 1 / s rounded, q = x y and its remainder e = x - q s, which one FMA
@@ -110,9 +111,10 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
     const int lane = threadIdx.x % SAVE_LANES, group = threadIdx.x / SAVE_LANES;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
     const int64_t b = (int64_t)blockIdx.x * across + (group & (across - 1));
-    const int64_t c = b * BLOCK + lane * N;
+    constexpr int STRIDE = WIDE ? 1 : SAVE_LANES;  // from a lane's value to its next
+    const int64_t c = b * BLOCK + lane * (WIDE ? N : 1);
     const int down = SAVE_GROUPS / across;
-    const int n = (int)max((int64_t)0, min((int64_t)N, d - c));
+    const int n = (int)max((int64_t)0, min((int64_t)N, (d - c + STRIDE - 1) / STRIDE));
     const int64_t first = (int64_t)blockIdx.y * down + group / across, step = (int64_t)gridDim.y * down;
     const T* src = x + first * ldx + c;
     int8_t* dst = codes + first * d + c;
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
                 reinterpret_cast<uint4*>(next)[i] = m ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; i++) next[i] = i < m ? src[i] : Type<DT>::down(0.0f);
+            for (int i = 0; i < N; i++) next[i] = i < m ? __ldcs(src + i * STRIDE) : Type<DT>::down(0.0f);
         }
         src += step * ldx;
     };
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
                 q[i] = finite && s > 0.0f ? (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(Type<DT>::up(raw[i]), s)), -127.0f), 127.0f) : 0u;
         }
         if (m == 0) continue;
-        if (lane == 0) *to = s;
+        if (lane == 0) *to = s;  // lane 0 has the block's first value
         if (WIDE) {
             uint32_t w[N / 4];
 #pragma unroll
@@ -170,12 +172,13 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (i < m) dst[i] = (int8_t)q[i];
+                if (i < m) dst[i * STRIDE] = (int8_t)q[i];
         }
     }
 }
 
-// 16 values a thread; a CTA has `across` (a power of two) threads along a row.  ld: elements from row to row of the output;
+// 16 values a thread; a CTA has `across` (a power of two) threads along a row.  WIDE: neighbouring values; else, for rows that
+// do not start on 16 bytes, every `across`-th (8 <= across <= 32), so that a warp reads and writes along the row.  ld: elements from row to row of the output;
 // columns d..ld of it are left as they are.  A code's byte, its sign bit turned, in the low byte of 2^23 is the number
 // 2^23 + 128 + code.
 template <int DT, bool WIDE>
@@ -184,14 +187,15 @@ __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* _
                                                                  int64_t ld) {
     typedef typename Type<DT>::T T;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
-    const int64_t c = ((int64_t)blockIdx.x * across + (threadIdx.x & (across - 1))) * 16;
+    const int lane = threadIdx.x & (across - 1);
+    const int64_t c = (int64_t)blockIdx.x * across * 16 + lane * (WIDE ? 16 : 1);
     if (c >= d) return;
     const int down = 256 / across;
     for (int64_t row = (int64_t)blockIdx.y * down + threadIdx.x / across; row < t; row += (int64_t)gridDim.y * down) {
-        const float s = scales[row * nb + c / BLOCK];
         const int8_t* src = codes + row * d + c;
         T* dst = out + row * ld + c;
-        if (WIDE && c + 16 <= d) {
+        if constexpr (WIDE) {
+            const float s = scales[row * nb + c / BLOCK];
             alignas(16) T r[16];
             const uint4 four = __ldcs(reinterpret_cast<const uint4*>(src));
             const uint32_t w[4] = {four.x ^ 0x80808080u, four.y ^ 0x80808080u, four.z ^ 0x80808080u, four.w ^ 0x80808080u};
@@ -206,7 +210,14 @@ __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* _
 #pragma unroll
             for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<uint4*>(r)[k];
         } else {
-            for (int k = 0; k < 16 && c + k < d; k++) dst[k] = Type<DT>::down(__fmul_rn((float)src[k], s));
+            const int n = (int)min((int64_t)16, (d - c + across - 1) / across);
+            const float* scale = scales + row * nb + (c - lane) / BLOCK;  // a CTA's first column begins a block
+            int8_t q[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) q[k] = k < n ? __ldcs(src + k * across) : (int8_t)0;
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (k < n) dst[k * across] = Type<DT>::down(__fmul_rn((float)q[k], scale[k * across / BLOCK]));
         }
     }
 }
@@ -242,7 +253,7 @@ int restore(const int8_t* codes, const float* scales, int64_t t, int64_t d, void
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ld * sizeof(T)) % 16 == 0 &&
                       (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && d % 16 == 0;
-    const int across = power_of_two(ceil_div(d, 16), 256);
+    const int across = wide ? power_of_two(ceil_div(d, 16), 256) : std::max(8, power_of_two(ceil_div(d, 16), 32));
     const int64_t gx = ceil_div(d, 16 * across);
     auto kern = wide ? checkpoint_restore_kernel<DT, true> : checkpoint_restore_kernel<DT, false>;
     CDCLQ_LAUNCH(kern, dim3((unsigned)gx, grid_rows(ceil_div(t, 256 / across), gx)), 256, 0, st, codes, scales, t, d, across,
