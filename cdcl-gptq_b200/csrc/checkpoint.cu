@@ -92,8 +92,8 @@ __device__ __forceinline__ float value_of_bits(uint32_t b, const __nv_bfloat16*)
 constexpr int SAVE_LANES = 8, SAVE_VALUES = BLOCK / SAVE_LANES;  // lanes of a block, values of a lane
 constexpr int SAVE_GROUPS = 256 / SAVE_LANES;
 
-// 8 lanes to a block of 128 columns, 16 values a lane: neighbouring ones where rows start on 16 bytes (WIDE), else every
-// eighth, so that the lanes' single values lie side by side.  A CTA has 32 such groups: `across` of them (a power of two)
+// 8 lanes to a block of 128 columns, 16 values a lane: two pieces of eight where x's rows start on 16 bytes and the codes' on
+// 8 (WIDE), else every eighth value, so that the lanes' pieces or values lie side by side.  A CTA has 32 such groups: `across` of them (a power of two)
 // along a row, 32 / across rows.
 //
 // x / s to the nearest whole number of the rounded quotient, ties to even (values of few bits meet ties often: with a block's
@@ -111,10 +111,10 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
     const int lane = threadIdx.x % SAVE_LANES, group = threadIdx.x / SAVE_LANES;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
     const int64_t b = (int64_t)blockIdx.x * across + (group & (across - 1));
-    constexpr int STRIDE = WIDE ? 1 : SAVE_LANES;  // from a lane's value to its next
-    const int64_t c = b * BLOCK + lane * (WIDE ? N : 1);
+    constexpr int PIECE = WIDE ? 8 : 1, STRIDE = SAVE_LANES * PIECE;  // neighbouring values, from a lane's piece to its next
+    const int64_t c = b * BLOCK + lane * PIECE;
     const int down = SAVE_GROUPS / across;
-    const int n = (int)max((int64_t)0, min((int64_t)N, (d - c + STRIDE - 1) / STRIDE));
+    const int n = (int)max((int64_t)0, min((int64_t)(N / PIECE), (d - c + STRIDE - 1) / STRIDE));  // pieces
     const int64_t first = (int64_t)blockIdx.y * down + group / across, step = (int64_t)gridDim.y * down;
     const T* src = x + first * ldx + c;
     int8_t* dst = codes + first * d + c;
@@ -123,8 +123,11 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
     auto load = [&](int m) {
         if (WIDE) {
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(next) / 16; i++)
-                reinterpret_cast<uint4*>(next)[i] = m ? __ldcs(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < (int)sizeof(next) / 16; i++) {
+                constexpr int IN_PIECE = PIECE * (int)sizeof(T) / 16;
+                reinterpret_cast<uint4*>(next)[i] = i / IN_PIECE < m ? __ldcs(reinterpret_cast<const uint4*>(src + i / IN_PIECE * STRIDE) + i % IN_PIECE)
+                                                                     : make_uint4(0, 0, 0, 0);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++) next[i] = i < m ? __ldcs(src + i * STRIDE) : Type<DT>::down(0.0f);
@@ -168,7 +171,9 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
 #pragma unroll
             for (int i = 0; i < N / 4; i++)
                 w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
-            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int i = 0; i < N / PIECE; i++)
+                if (i < m) *reinterpret_cast<uint2*>(dst + i * STRIDE) = make_uint2(w[2 * i], w[2 * i + 1]);
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++)
@@ -177,10 +182,10 @@ __global__ void __launch_bounds__(256, 4) checkpoint_save_kernel(const typename 
     }
 }
 
-// 16 values a thread; a CTA has `across` (a power of two) threads along a row.  WIDE: neighbouring values; else, for rows that
-// do not start on 16 bytes, every `across`-th (8 <= across <= 32), so that a warp reads and writes along the row.  ld: elements from row to row of the output;
-// columns d..ld of it are left as they are.  A code's byte, its sign bit turned, in the low byte of 2^23 is the number
-// 2^23 + 128 + code.
+// 16 values a thread; a CTA has `across` (a power of two) threads along a row.  WIDE: two pieces of eight, where the output's
+// rows start on 16 bytes and the codes' on 8; else single values (8 <= across <= 32).  Either way the threads' pieces lie side
+// by side.  ld: elements from row to row of the output; columns d..ld of it are left as they are.  A code's byte, its sign bit
+// turned, in the low byte of 2^23 is the number 2^23 + 128 + code.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scales,
                                                                  int64_t t, int64_t d, int across, typename Type<DT>::T* __restrict__ out,
@@ -188,27 +193,33 @@ __global__ void __launch_bounds__(256) checkpoint_restore_kernel(const int8_t* _
     typedef typename Type<DT>::T T;
     const int64_t nb = (d + BLOCK - 1) / BLOCK;
     const int lane = threadIdx.x & (across - 1);
-    const int64_t c = (int64_t)blockIdx.x * across * 16 + lane * (WIDE ? 16 : 1);
+    const int64_t c = (int64_t)blockIdx.x * across * 16 + lane * (WIDE ? 8 : 1);
     if (c >= d) return;
     const int down = 256 / across;
+    const bool both = c + across * 8 < d;
     for (int64_t row = (int64_t)blockIdx.y * down + threadIdx.x / across; row < t; row += (int64_t)gridDim.y * down) {
         const int8_t* src = codes + row * d + c;
         T* dst = out + row * ld + c;
         if constexpr (WIDE) {
-            const float s = scales[row * nb + c / BLOCK];
-            alignas(16) T r[16];
-            const uint4 four = __ldcs(reinterpret_cast<const uint4*>(src));
-            const uint32_t w[4] = {four.x ^ 0x80808080u, four.y ^ 0x80808080u, four.z ^ 0x80808080u, four.w ^ 0x80808080u};
+            const float* scale = scales + row * nb;
+            const uint2 w[2] = {__ldcs(reinterpret_cast<const uint2*>(src)), both ? __ldcs(reinterpret_cast<const uint2*>(src + across * 8)) : make_uint2(0, 0)};
+            const float s[2] = {scale[c / BLOCK], both ? scale[(c + across * 8) / BLOCK] : 0.0f};
 #pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-                const uint32_t v = w[k / 4];
-                const Pair q = add2({__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4)), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4 + 1))},
-                                    {-8388736.0f, -8388736.0f});
-                const Pair p = mul2(q, {s, s});
-                r[k] = Type<DT>::down(p.x), r[k + 1] = Type<DT>::down(p.y);
+            for (int i = 0; i < 2; i++) {
+                alignas(16) T r[8];
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    const uint32_t v = (k < 4 ? w[i].x : w[i].y) ^ 0x80808080u;
+                    const Pair q = add2({__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4)), __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7540 + k % 4 + 1))},
+                                        {-8388736.0f, -8388736.0f});
+                    const Pair p = mul2(q, {s[i], s[i]});
+                    r[k] = Type<DT>::down(p.x), r[k + 1] = Type<DT>::down(p.y);
+                }
+                if (i == 0 || both) {
+#pragma unroll
+                    for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(dst + i * across * 8)[k] = reinterpret_cast<uint4*>(r)[k];
+                }
             }
-#pragma unroll
-            for (int k = 0; k < (int)sizeof(r) / 16; k++) reinterpret_cast<uint4*>(dst)[k] = reinterpret_cast<uint4*>(r)[k];
         } else {
             const int n = (int)min((int64_t)16, (d - c + across - 1) / across);
             const float* scale = scales + row * nb + (c - lane) / BLOCK;  // a CTA's first column begins a block
@@ -237,7 +248,7 @@ template <int DT>
 int save(const void* x, int64_t ldx, int64_t t, int64_t d, int8_t* codes, float* scales, cudaStream_t st) {
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * sizeof(T)) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && d % 16 == 0;
+                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
     const int64_t nb = ceil_div(d, BLOCK);
     const int across = power_of_two(nb, SAVE_GROUPS);
     const int64_t gx = ceil_div(nb, across);
@@ -252,7 +263,7 @@ template <int DT>
 int restore(const int8_t* codes, const float* scales, int64_t t, int64_t d, void* out, int64_t ld, cudaStream_t st) {
     typedef typename Type<DT>::T T;
     const bool wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && (ld * sizeof(T)) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(codes) & 15) == 0 && d % 16 == 0;
+                      (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && d % 8 == 0;
     const int across = wide ? power_of_two(ceil_div(d, 16), 256) : std::max(8, power_of_two(ceil_div(d, 16), 32));
     const int64_t gx = ceil_div(d, 16 * across);
     auto kern = wide ? checkpoint_restore_kernel<DT, true> : checkpoint_restore_kernel<DT, false>;
