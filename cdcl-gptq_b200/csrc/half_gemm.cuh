@@ -104,6 +104,27 @@ __device__ __forceinline__ uint16_t pack1(float a) {
         return __half_as_ushort(__float2half_rn(a));
 }
 
+// 2^v; results below 2^-126 are 0, nothing beside a sum of 1 or more or in a gradient of 16 bits.
+__device__ __forceinline__ float exp2_normal(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// (v - ref) * factor, two at a time, each operation rounded: the difference of near numbers stays exact.
+__device__ __forceinline__ void scale_off(float (&v)[16], float ref, float factor) {
+    uint64_t minus, by;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(minus) : "f"(-ref));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(by) : "f"(factor));
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        uint64_t x;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(v[i]), "f"(v[i + 1]));
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(minus));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(by));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(x));
+    }
+}
+
 // Item -> (row block, column block, split): splits outermost; bands of BAND row blocks, column block by column block.
 __device__ __forceinline__ void item_coords(const Params& P, int item, int& mb, int& nb, int& split) {
     split = item / P.ntiles;
@@ -479,51 +500,66 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             const int row0 = (mb * CG + rank) * BM + quad * 32, row = row0 + lane;
             const bool live = row < P.m;
             if constexpr (EPI == EPI_STATS) {
-                float z[COLS];
                 const int64_t t = live ? P.target[row] : -1;
-                const int64_t label = (t >= 0 && t < P.vocab) ? t - P.col0 : -1;  // relative to this piece's column 0
                 const int chunks = (P.nkb + STATS_KB - 1) / STATS_KB;
+                const int c0 = nb * BN + part * COLS, cols = min(COLS, P.n - c0);
+                // the label's place among the thread's columns, -1 where it is not
+                const int at = (t >= P.col0 + c0 && t < P.col0 + c0 + cols && t < P.vocab) ? (int)(t - P.col0 - c0) : -1;
+                float top = -INFINITY, sum = 0.0f;
+                float z[COLS];
+#pragma unroll
+                for (int i = 0; i < COLS; i++) z[i] = 0.0f;
                 for (int c = 0; c < chunks; c++, acc++) {
                     if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
                         ok = false;
                         break;
                     }
                     fence_after();
+                    if (c + 1 < chunks) {
 #pragma unroll
-                    for (int q = 0; q < COLS; q += 16) {
-                        float v[16];
-                        tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), v);
+                        for (int q = 0; q < COLS; q += 16) {
+                            float v[16];
+                            tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), v);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) z[q + i] = c ? z[q + i] + v[i] : v[i];
+                            for (int i = 0; i < 16; i++) z[q + i] += v[i];
+                        }
+                    } else {
+                        // the logits are complete, 16 columns at a time: exp2((v - top) log2 e), the sum so far brought to the new
+                        // maximum; a row of -inf alone keeps sum 0
+                        constexpr float L2E = 1.4426950408889634f;
+#pragma unroll
+                        for (int q = 0; q < COLS; q += 16) {
+                            float v[16];
+                            tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), v);
+                            float most = top;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) v[i] += z[q + i];
+                            if (cols < COLS) {
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (q + i >= cols) v[i] = -INFINITY;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++) most = fmaxf(most, v[i]);
+                            if (at >= q && at < q + 16) {
+                                float own = 0.0f;
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    if (q + i == at) own = v[i];
+                                P.label_logit[row] = own;
+                            }
+                            const float ref = most == -INFINITY ? 0.0f : most;
+                            scale_off(v, ref, L2E);
+                            float some = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) some += exp2_normal(v[i]);
+                            sum = sum * exp2_normal((top - ref) * L2E) + some;
+                            top = most;
+                        }
                     }
                     release(acc & 1);
                 }
                 if (!ok) break;
-                const int c0 = nb * BN + part * COLS, cols = min(COLS, P.n - c0);
-                float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < COLS; i++) {
-                    if (i >= cols) z[i] = -INFINITY;
-                    top = fmaxf(top, z[i]);
-                }
-                // exp2((z - top) log2 e); a row of -inf alone keeps sum 0
-                constexpr float L2E = 1.4426950408889634f;
-                const float ref = top == -INFINITY ? 0.0f : top;
-                const int64_t at = label - c0;
-#pragma unroll
-                for (int q = 0; q < COLS; q += 16) {
-                    if (at >= q && at < q + 16 && at < cols) {
-                        float own = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (q + i == at) own = z[q + i];
-                        P.label_logit[row] = own;
-                    }
-                    float some = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) some += exp2f((z[q + i] - ref) * L2E);
-                    sum += some;
-                }
                 if (live) P.stats[(int64_t)(nb * STATS_PARTS + part) * P.m + row] = make_float2(top, sum);
                 continue;
             }
@@ -622,9 +658,10 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     if constexpr (EPI == EPI_GRAD) {
                         constexpr float L2E = 1.4426950408889634f;
                         const int c0 = first_col + q, at = (label >= c0 && label < c0 + 16) ? (int)(label - c0) : -1;
+                        scale_off(z, lse, L2E);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            float p = exp2f((z[i] - lse) * L2E);
+                            float p = exp2_normal(z[i]);
                             if (i == at) p -= 1.0f;
                             z[i] = none ? 0.0f : p * dl;
                         }

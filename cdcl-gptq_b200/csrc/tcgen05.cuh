@@ -84,8 +84,10 @@ __device__ __forceinline__ uint32_t first_cta(uint32_t local) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(local));
     return a;
 }
+// For arrivals after reads of tensor memory alone, which have completed by then: release at cluster scope would also wait for
+// every global store of the warp on its way.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
