@@ -378,7 +378,7 @@ struct Space {
 };
 
 struct ForwardLayout {
-    size_t expanded = 0, ranked = 0, partial = 0, decode = 0, total = 0;
+    size_t expanded = 0, ranked = 0, lists = 0, partial = 0, decode = 0, total = 0;
 };
 ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r) {
     ForwardLayout l;
@@ -387,15 +387,17 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
         l.decode = s.take(packed_decode_workspace(w, (int)t, n ? (int)r : 0));
     } else {
         l.expanded = s.take((size_t)w.d_out * ceil_div(w.d_in, 8) * 8 * 2);
+        const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in);
         if (n) l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
-        l.partial = s.take(plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in).partial_bytes);
+        if (n) l.lists = s.take(row_lists_bytes(plan, t));
+        l.partial = s.take(plan.partial_bytes);
     }
     l.total = s.at;
     return l;
 }
 
 struct BackwardLayout {
-    size_t expanded = 0, ranked = 0, rest = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
+    size_t expanded = 0, ranked = 0, lists = 0, rest = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
 };
 BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r, bool need_dx) {
     BackwardLayout l;
@@ -403,7 +405,9 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
     size_t partial = 0;
     if (need_dx) {
         l.expanded = s.take((size_t)w.d_out * ceil_div(w.d_in, 8) * 8 * 2);
-        partial = plan_half_gemm(HALF_NN_EXTEND, t, w.d_in, w.d_out).partial_bytes;
+        const HalfPlan plan = plan_half_gemm(HALF_NN_EXTEND, t, w.d_in, w.d_out);
+        if (n) l.lists = s.take(row_lists_bytes(plan, t));
+        partial = plan.partial_bytes;
     }
     if (n) {
         l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
@@ -498,7 +502,9 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         p.lds = ldr;
         if ((rc = launch_rank(bf16, false, p, st))) return rc;
     }
-    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, n > 0, st))) return rc;  // beside u's products
+    const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, v.d_out, v.d_in);
+    const RowLists lists = n ? row_lists(plan, ad->index, t, n, ws + l.lists) : RowLists();
+    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, n > 0, st))) return rc;  // beside u's products
     HalfGemm g{};
     g.form = HALF_NT_EXTEND;
     g.bf16 = bf16;
@@ -508,13 +514,12 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
     if (n) {
         g.u = operand(ws + l.ranked, t, r, ldr);
         g.x = operand(ad->b, v.d_out, r, ad->ldb, n);
-        g.index = ad->index;
-        g.adapters = (int)n;
+        g.lists = lists.out;
     }
     g.out = y;
     g.ldo = ldy;
     g.partial = partial;
-    return launch_half_gemm(g, plan_half_gemm(HALF_NT_EXTEND, t, v.d_out, v.d_in), st);
+    return launch_half_gemm(g, plan, st);
 }
 
 extern "C" size_t cdclq_projection_backward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r, int need_dx) {
@@ -567,8 +572,10 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         }
         if ((rc = launch_rank(bf16, true, p, st))) return rc;
     }
+    const HalfPlan plan = plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out);
     if (dx) {
-        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, n > 0, st))) return rc;  // beside v's products
+        const RowLists lists = n ? row_lists(plan, ad->index, t, n, ws + l.lists) : RowLists();
+        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, n > 0, st))) return rc;  // beside v's products
         HalfGemm g{};
         g.form = HALF_NN_EXTEND;
         g.bf16 = bf16;
@@ -578,13 +585,12 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         if (n) {
             g.u = operand(ws + l.ranked, t, r, ldr);
             g.x = operand(ad->a, r, v.d_in, ad->lda, n);
-            g.index = ad->index;
-            g.adapters = (int)n;
+            g.lists = lists.out;
         }
         g.out = dx;
         g.ldo = lddx;
         g.partial = partial;
-        if ((rc = launch_half_gemm(g, plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out), st))) return rc;
+        if ((rc = launch_half_gemm(g, plan, st))) return rc;
     }
     if (!n || !(da || db)) return 0;
     OuterPair o{};
@@ -626,5 +632,5 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
     }
     o.chunk = outer_chunk(t, o.a.tiles + o.b.tiles, r);
     // dx's product stands between them, unless its sums were split: then the kernel that joins them does
-    return launch_outer(bf16, o, dx && plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out).splits == 1, st);
+    return launch_outer(bf16, o, dx && plan.splits == 1, st);
 }

@@ -122,6 +122,19 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k) {
 
 int64_t half_stats_parts(const HalfPlan& plan, int64_t n) { return STATS_PARTS * ceil_div(n, plan.bn); }
 
+RowLists row_lists(const HalfPlan& plan, const int* index, int64_t m, int64_t adapters, void* out) {
+    RowLists l;
+    l.index = index;
+    l.m = (int)m, l.adapters = (int)adapters;
+    l.rows = plan.cg * BM;
+    l.tiles = (int)ceil_div(m, l.rows);
+    l.out = static_cast<uint32_t*>(out);
+    return l;
+}
+size_t row_lists_bytes(const HalfPlan& plan, int64_t m) {
+    return (size_t)ceil_div(m, plan.cg * BM) * row_list_words(plan.cg * BM) * sizeof(uint32_t);
+}
+
 // out = alpha * (f32in + partial[0] + partial[1] + ...), splits in order; also or instead as f32.
 template <bool BF16>
 __global__ void __launch_bounds__(256) half_gemm_reduce_kernel(const float* __restrict__ partial, int splits, int64_t m, int64_t n,
@@ -158,7 +171,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     if (g.m <= 0 || g.n <= 0) return 0;
     const bool a_mn = g.form == HALF_TN;
     const bool b_mn = g.form == HALF_NN || g.form == HALF_TN || g.form == HALF_NN_EXTEND;
-    const bool extend = (g.form == HALF_NT_EXTEND || g.form == HALF_NN_EXTEND) && g.adapters > 0;
+    const bool extend = (g.form == HALF_NT_EXTEND || g.form == HALF_NN_EXTEND) && g.lists;
     if (g.m > 0x7fffff00 || g.n > 0x7fffff00 || g.k > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "half product: too large");
     Maps maps{};
     int rc;
@@ -176,8 +189,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.ntiles = p.tiles_m * p.tiles_n;
     p.splits = plan.splits;
     p.kb_per_split = (int)ceil_div(p.nkb, plan.splits);
-    p.index = g.index;
-    p.adapters = extend ? g.adapters : 0;
+    p.lists = extend ? g.lists : nullptr;
     p.rank = extend ? (int)g.u.cols : 0;
     p.target = g.target;
     p.col0 = g.col0;

@@ -41,7 +41,11 @@ constexpr int STATS_KB = 16;
 
 __host__ __device__ constexpr int b_bytes(int cg, int bn) { return bn / cg * KB * 2; }
 
-// How the adapter of each row (index[m]; none if outside [0, adapters)) takes part.
+// The adapters of a tile's rows (R = 128 or 256), in words: their number, padding to 4, R places for their ids, R places for
+// R / 32 words each that have a bit for every row that is not the adapter's.
+__host__ __device__ constexpr int row_list_words(int R) { return 4 + R + R * (R / 32); }
+
+// How the adapter of each row (none if outside [0, adapters)) takes part.
 enum RowMode {
     ROWS_PLAIN = 0,   // not at all
     ROWS_EXTEND = 1   // D[m] += U[m] Bx[index[m]]: further K blocks, whose MMAs write the adapter's own rows only
@@ -62,9 +66,8 @@ struct Params {
     int m, n, nkb;             // rows, columns, K blocks
     int tiles_m, tiles_n, ntiles;
     int splits, kb_per_split;  // the K blocks of a tile, over several items
-    // rows' adapters
-    const int* index;
-    int adapters;
+    // rows' adapters (see RowLists): null where there are none
+    const uint32_t* lists;
     int rank;                  // ROWS_EXTEND: depth of the extension
     // EPI_STORE
     void* out;                 // 16-bit, or null
@@ -137,34 +140,6 @@ __device__ __forceinline__ void item_coords(const Params& P, int item, int& mb, 
     mb = band * BAND + t - nb * rows;
 }
 
-// The adapters of a tile's 128 CG rows, lowest first; a warp holds 4 CG rows in each lane.
-template <int CG>
-struct RowAdapters {
-    static constexpr int NONE = 0x7fffffff;
-    int id[4 * CG];
-    __device__ __forceinline__ void load(const Params& P, int m0, int lane) {
-#pragma unroll
-        for (int q = 0; q < 4 * CG; q++) {
-            const int row = m0 + 32 * q + lane;
-            const int v = (row < P.m && P.adapters > 0) ? P.index[row] : -1;
-            id[q] = (v >= 0 && v < P.adapters) ? v : NONE;
-        }
-    }
-    // the next adapter and the lanes that are not its rows; NONE after the last
-    __device__ __forceinline__ int next(uint32_t (&off)[4 * CG]) {
-        int least = id[0];
-#pragma unroll
-        for (int q = 1; q < 4 * CG; q++) least = min(least, id[q]);
-        const int cur = __reduce_min_sync(0xffffffffu, least);
-#pragma unroll
-        for (int q = 0; q < 4 * CG; q++) {
-            const bool mine = id[q] == cur;
-            off[q] = ~__ballot_sync(0xffffffffu, mine);
-            if (mine) id[q] = NONE;
-        }
-        return cur;
-    }
-};
 
 template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -215,7 +190,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const uint32_t ring = smem_u32(base);
 
     if (warp == EPI_WARPS) {
-        // ---------------- TMA producer: the whole warp walks the items, lane 0 waits and issues
+        // ---------------- TMA producer: one thread waits and issues (a loop that takes the whole warp along, to share a word of it
+        // now and then, pays 200 clocks for each)
         int ctr = 0;
         bool ok = true;
         // waits for the next stage and, in the first CTA, announces the pair's bytes; returns its address
@@ -251,57 +227,50 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 load2(dst, &map_a, kb * KB, m0, bar);
             }
         };
-        for (int item = first; item < items && ok; item += step) {
+        for (int item = lane == 0 ? first : items; item < items && ok; item += step) {
             int mb, nb, split;
             item_coords(P, item, mb, nb, split);
             const int m0 = (mb * CG + rank) * BM, n0 = nb * BN + rank * BC;
             const int kb0 = split * P.kb_per_split, kb1 = min(P.nkb, kb0 + P.kb_per_split);
-            if (lane == 0) {
-                for (int kb = kb0; kb < kb1; kb++) {
-                    uint32_t bar;
-                    const uint32_t st = stage(bar);
-                    if (!ok) break;
-                    load_a(st, m0, kb, bar);
+            for (int kb = kb0; kb < kb1; kb++) {
+                uint32_t bar;
+                const uint32_t st = stage(bar);
+                if (!ok) break;
+                load_a(st, m0, kb, bar);
 #pragma unroll
-                    for (int w = 0; w < BN / AC; w++) {
-                        const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
-                        if constexpr (BMN) {
+                for (int w = 0; w < BN / AC; w++) {
+                    const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
+                    if constexpr (BMN) {
 #pragma unroll
-                            for (int h = 0; h < BC / 64; h++)
-                                load2(sb + h * (64 * KB * 2), &map_b, n0 + w * AC + 64 * h, kb * KB, bar);
-                        } else {
-                            load2(sb, &map_b, kb * KB, n0 + w * AC, bar);
-                        }
+                        for (int h = 0; h < BC / 64; h++) load2(sb + h * (64 * KB * 2), &map_b, n0 + w * AC + 64 * h, kb * KB, bar);
+                    } else {
+                        load2(sb, &map_b, kb * KB, n0 + w * AC, bar);
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
             if constexpr (ROWS == ROWS_EXTEND) {
-                if (split != P.splits - 1) continue;  // the last split extends
-                RowAdapters<CG> who;
-                who.load(P, mb * CG * BM, lane);
-                uint32_t off[4 * CG];
-                for (int j = who.next(off); j != RowAdapters<CG>::NONE && ok; j = who.next(off)) {
-                    if (lane == 0) {
-                        for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
-                            uint32_t bar;
-                            const uint32_t st = stage(bar);
-                            if (!ok) break;
-                            load2(st, &map_u, kb * KB, m0, bar);
+                if (split != P.splits - 1 || !P.lists) continue;  // the last split extends
+                const uint32_t* list = P.lists + (int64_t)mb * row_list_words(CG * BM);
+                const int count = (int)list[0];
+                for (int e = 0; e < count && ok; e++) {
+                    const int j = (int)list[4 + e];
+                    for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
+                        uint32_t bar;
+                        const uint32_t st = stage(bar);
+                        if (!ok) break;
+                        load2(st, &map_u, kb * KB, m0, bar);
 #pragma unroll
-                            for (int w = 0; w < BN / AC; w++) {
-                                const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
-                                if constexpr (BMN) {
+                        for (int w = 0; w < BN / AC; w++) {
+                            const uint32_t sb = st + A_BYTES + w * HALF_BYTES;
+                            if constexpr (BMN) {
 #pragma unroll
-                                    for (int h = 0; h < BC / 64; h++)
-                                        load3(sb + h * (64 * KB * 2), &map_x, n0 + w * AC + 64 * h, kb * KB, j, bar);
-                                } else {
-                                    load3(sb, &map_x, kb * KB, n0 + w * AC, j, bar);
-                                }
+                                for (int h = 0; h < BC / 64; h++)
+                                    load3(sb + h * (64 * KB * 2), &map_x, n0 + w * AC + 64 * h, kb * KB, j, bar);
+                            } else {
+                                load3(sb, &map_x, kb * KB, n0 + w * AC, j, bar);
                             }
                         }
                     }
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
                 }
             }
         }
@@ -310,10 +279,11 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (lane == 0)
             for (int k = (ctr > NS ? ctr - NS : 0); k < ctr; k++)
                 if (!mbar_wait(&empty[k % NS], (k / NS) & 1, flag) && rank == 0) mbar_wait(&full[k % NS], (k / NS) & 1, flag);
+        __syncwarp();
     } else if (warp == EPI_WARPS + 1) {
-        // ---------------- MMA issuer, of the pair's first CTA
+        // ---------------- MMA issuer, one thread of the pair's first CTA
         int acc = 0;
-        bool ok = rank == 0;
+        bool ok = rank == 0 && lane == 0;
         int slot = 0;        // of the next stage
         uint32_t phase = 0;  // parity of its barrier
         // the next stage's operands are there (false: the wait ran out); a look at the barrier may have shown it already
@@ -332,7 +302,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         auto done = [&]() -> bool {
             mma_commit<CG>(&empty[slot]);
             advance(slot, phase);
-            return mbar_try(&full[slot], phase);
+            return mbar_test(&full[slot], phase);
         };
         // descriptors of the first stage's operands; a stage, a half and a step of 16 further are added to their addresses
         constexpr uint64_t A_STEP = (AMN ? 2048 : 32) >> 4, B_STEP = (BMN ? 2048 : 32) >> 4;
@@ -391,16 +361,13 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // accumulator `acc & 1` (of a tile of 512: the first half), once its last contents have been read
         auto accumulator = [&]() -> uint32_t {
             const int b = WIDE ? 0 : acc & 1, use = WIDE ? acc : acc / 2;
-            if (lane == 0 && use > 0 && !mbar_wait(&acce[b], (use - 1) & 1, flag)) ok = false;
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (use > 0 && !mbar_wait(&acce[b], (use - 1) & 1, flag)) ok = false;
             fence_after();
             return tmem_base + (uint32_t)(b * AC);
         };
         auto finished = [&]() {
-            if (lane == 0) {
-                mma_commit<CG>(&accf[WIDE ? 0 : acc & 1]);  // the accumulator is complete (or tracks what was issued)
-                if (WIDE) mma_commit<CG>(&accf[1]);
-            }
+            mma_commit<CG>(&accf[WIDE ? 0 : acc & 1]);  // the accumulator is complete (or tracks what was issued)
+            if (WIDE) mma_commit<CG>(&accf[1]);
             acc++;
         };
         for (int item = first; item < items && ok; item += step) {
@@ -411,37 +378,33 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 for (int c0 = kb0; c0 < kb1 && ok; c0 += STATS_KB) {
                     const uint32_t d = accumulator();
                     if (!ok) break;
-                    if (lane == 0) plain(d, c0, min(kb1, c0 + STATS_KB));
-                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    plain(d, c0, min(kb1, c0 + STATS_KB));
                     finished();
                 }
                 continue;
             }
             const uint32_t d = accumulator();
             if (!ok) break;
-            if (lane == 0) {
-                if constexpr (WIDE)
-                    plain_wide(acc, kb0, kb1);
-                else
-                    plain(d, kb0, kb1);
-            }
-            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if constexpr (WIDE)
+                plain_wide(acc, kb0, kb1);
+            else
+                plain(d, kb0, kb1);
             if constexpr (ROWS == ROWS_EXTEND) {
-                if (split == P.splits - 1) {
-                    RowAdapters<CG> who;
-                    who.load(P, mb * CG * BM, lane);
-                    uint32_t off[4 * CG];
-                    while (ok && who.next(off) != RowAdapters<CG>::NONE) {
-                        if (lane == 0) {
-                            for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
-                                if (!arrived(false)) break;
+                if (split == P.splits - 1 && P.lists) {
+                    const uint32_t* list = P.lists + (int64_t)mb * row_list_words(CG * BM);
+                    const int count = (int)list[0];
+                    const uint4* masks = reinterpret_cast<const uint4*>(list + 4 + CG * BM);
+                    for (int e = 0; e < count && ok; e++) {
+                        uint32_t off[4 * CG];
 #pragma unroll
-                                for (int w = 0; w < BN / AC; w++)
-                                    extend(d + w * AC, slot, w, min(KB / 16, (P.rank - kb * KB + 15) / 16), off);
-                                done();
-                            }
+                        for (int q = 0; q < CG; q++) *reinterpret_cast<uint4*>(off + 4 * q) = masks[e * CG + q];
+                        for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
+                            if (!arrived(false)) break;
+#pragma unroll
+                            for (int w = 0; w < BN / AC; w++)
+                                extend(d + w * AC, slot, w, min(KB / 16, (P.rank - kb * KB + 15) / 16), off);
+                            done();
                         }
-                        ok = __shfl_sync(0xffffffffu, ok, 0);
                     }
                 }
             }
@@ -454,6 +417,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             else
                 mbar_wait(&accf[(acc - 1) & 1], ((acc - 1) / 2) & 1, flag);
         }
+        __syncwarp();
     } else {
         // ---------------- epilogue: lanes 32 * (warp % 4) .., quarter warp / 4 of the accumulator's columns
         constexpr int COLS = AC / 4;  // a thread's: 64, 32 or 16 of one row

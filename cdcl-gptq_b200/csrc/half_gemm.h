@@ -36,8 +36,7 @@ struct HalfGemm {
     int64_t m, n, k;
     HalfOperand a, b;
     HalfOperand u, x;            // extension: u (m x rank) times x[adapter]
-    const int* index = nullptr;  // the rows' adapters
-    int adapters = 0;
+    const uint32_t* lists = nullptr;  // the adapters of each tile's rows (RowLists), or null: no extension
     void* out = nullptr;         // 16-bit, ldo elements from row to row
     int64_t ldo = 0;
     float* f32out = nullptr;     // f32, ldf elements from row to row
@@ -61,6 +60,16 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);
 
 // (maximum, sum) pairs that the statistics form leaves for each row.
 int64_t half_stats_parts(const HalfPlan& plan, int64_t n);
+
+// The adapters of the rows of each of the plan's tiles, for the extended forms; words of them for m rows.
+struct RowLists {
+    const int* index = nullptr;  // [m], none if outside [0, adapters)
+    int m = 0, adapters = 0;
+    int rows = 0, tiles = 0;     // rows of a tile, tiles
+    uint32_t* out = nullptr;
+};
+RowLists row_lists(const HalfPlan& plan, const int* index, int64_t m, int64_t adapters, void* out);
+size_t row_lists_bytes(const HalfPlan& plan, int64_t m);
 
 // Launches the product (and, when the plan splits K, the pass that adds the splits in order).
 int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st);

@@ -238,6 +238,7 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) 
 }
 
 constexpr int EXPAND_WARPS = 16;
+constexpr size_t EXPAND_LIST_BYTES = (512 + EXPAND_WARPS) * sizeof(int);  // of a tile's list of adapters
 
 // The unit's codes of one half of the tile's rows, scaled, to their columns of `row`.
 template <bool BF16, int BITS, bool ALL>
@@ -279,14 +280,53 @@ __device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[B
     }
 }
 
+// The adapters of the rows of one tile, in order of their first rows (see row_list_words).  Small integers at a CTA's leisure
+// while others expand the weight: of the product's loop it would be the longest part, 2000 clocks an adapter.
+__device__ void build_row_list(const RowLists& L, int tile, int* ids) {
+    const int R = L.rows, i = threadIdx.x, row = tile * R + i, lane = i & 31;
+    int* place = ids + 256;   // of an adapter's first row
+    int* before = ids + 512;  // first rows of each warp
+    uint32_t* out = L.out + (int64_t)tile * (4 + R + R * (R / 32));
+    int id = i < R && row < L.m ? L.index[row] : -1;
+    if (id >= L.adapters) id = -1;
+    if (i < R) ids[i] = id;
+    __syncthreads();
+    int first = i;
+    if (i < R && id >= 0)
+        for (int j = R - 1; j >= 0; j--)
+            if (ids[j] == id) first = j;
+    const bool leads = i < R && id >= 0 && first == i;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+    if (lane == 0) before[i >> 5] = __popc(leaders);
+    __syncthreads();
+    int at = __popc(leaders & ((1u << lane) - 1u)), count = 0;
+    for (int w = 0; w < R / 32; w++) {
+        if (w < (i >> 5)) at += before[w];
+        count += before[w];
+    }
+    if (leads) place[i] = at, out[4 + at] = id;
+    if (i == 0) out[0] = count;
+    uint32_t* mask = out + 4 + R;
+    for (int k = i; k < count * (R / 32); k += blockDim.x) mask[k] = 0xffffffffu;
+    __syncthreads();
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    if (i < R && id >= 0 && lane == __ffs(same) - 1) mask[place[first] * (R / 32) + (i >> 5)] = ~same;
+}
+
 // A CTA expands `R` of a tile's 16 rows (R = 8, ALL, unless the rows do not fit): warps decode unit by unit into rows in
 // shared memory, at their original columns, and the CTA writes whole rows out.  BITS: the width of every group, or 0 where
 // they differ.  Bound by the 16-bit rows written and by issuing the scattered 2-byte stores, rows being four banks apart.
 template <bool BF16, int BITS, bool ALL>
 __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, int R, int ld, uint16_t* __restrict__ out,
-                                                                          int64_t ldw, int wide) {
+                                                                          int64_t ldw, int wide, const RowLists lists) {
     extern __shared__ __align__(16) uint16_t rows[];
-    const int parts = 16 / R, tile = blockIdx.x / parts, first = (blockIdx.x % parts) * R;  // rows first .. first + R of the tile
+    if ((int)blockIdx.x < lists.tiles) {
+        build_row_list(lists, blockIdx.x, reinterpret_cast<int*>(rows));
+        if (blockIdx.x == 0) wait_for_previous();
+        return;
+    }
+    const int here = blockIdx.x - lists.tiles;
+    const int parts = 16 / R, tile = here / parts, first = (here % parts) * R;  // rows first .. first + R of the tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = first >> 3, r0 = lane / 4 - (first & 7);
     const bool live = r0 >= 0 && r0 < R;
@@ -349,24 +389,27 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
 }
 
 template <bool BF16, int BITS>
-int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, bool beside, cudaStream_t st) {
+int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, const RowLists& lists,
+           bool beside, cudaStream_t st) {
     static std::atomic<uint64_t> done_all{0}, done_some{0};
     auto kern = R == 8 ? packed_expand_kernel<BF16, BITS, true> : packed_expand_kernel<BF16, BITS, false>;
     if (int rc = allow_smem(kern, 220 * 1024, R == 8 ? done_all : done_some, "packed_expand_kernel shared memory")) return rc;
-    return launch_after(beside, kern, dim3(w.tiles * (16 / R)), dim3(EXPAND_WARPS * 32), (size_t)(R * ld * 2), st,
-                        "packed_expand_kernel launch", w, R, (int)ld, static_cast<uint16_t*>(out), ldw, wide);
+    return launch_after(beside, kern, dim3(lists.tiles + w.tiles * (16 / R)), dim3(EXPAND_WARPS * 32),
+                        std::max((size_t)(R * ld * 2), EXPAND_LIST_BYTES), st, "packed_expand_kernel launch", w, R, (int)ld,
+                        static_cast<uint16_t*>(out), ldw, wide, lists);
 }
 
 // The widths of configurations that quantize every group alike have a kernel of their own; the others share one that
 // branches by unit.
 template <bool BF16>
-int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, bool beside, cudaStream_t st) {
+int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, const RowLists& lists,
+           bool beside, cudaStream_t st) {
     switch (w.bits) {
-        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, beside, st);
-        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, beside, st);
-        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, beside, st);
-        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, beside, st);
-        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, beside, st);
+        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, lists, beside, st);
+        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, lists, beside, st);
+        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, lists, beside, st);
+        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, lists, beside, st);
+        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, lists, beside, st);
     }
 }
 
@@ -389,13 +432,13 @@ PackedView packed_view(const cdclq_packed_layer& w) {
     return v;
 }
 
-int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, bool beside, cudaStream_t st) {
+int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
     const int64_t ld = expand_pitch(w.d_in);
     int R = 8;
     while (R > 1 && R * ld * 2 > 220 * 1024) R /= 2;
     if (R * ld * 2 > 220 * 1024) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
     const int wide = ldw % 8 == 0 && ldw >= ceil_div(w.d_in, 8) * 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, beside, st) : expand_any<false>(w, R, ld, out, ldw, wide, beside, st);
+    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, lists, beside, st) : expand_any<false>(w, R, ld, out, ldw, wide, lists, beside, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

@@ -8,6 +8,7 @@
 
 #include "cdclq.h"
 #include "common.cuh"
+#include "half_gemm.h"
 
 namespace cdclq {
 
@@ -43,7 +44,8 @@ inline int expand_pitch(int d_in) { return (d_in + 63) / 64 * 64 + 8; }
 
 // W (d_out x d_in, original column order, ldw elements from row to row) rounded once to f16 or bf16.  beside: the launch before
 // it in the stream neither writes what it reads nor reads what it writes, so that they may run side by side.
-int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, bool beside, cudaStream_t st);
+// lists: built along the way, by CTAs of their own.
+int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st);
 
 // Largest number of tokens of the single-token form.
 constexpr int DECODE_TOKENS = 32;

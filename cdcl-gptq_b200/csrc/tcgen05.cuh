@@ -38,6 +38,16 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Whether the phase is complete, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait for the completion of the phase with the given parity; false (and the CTA's flag set) on timeout.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* flag) {
     for (int it = 0; it < WAIT_LIMIT; it++) {
