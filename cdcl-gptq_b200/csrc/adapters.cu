@@ -54,7 +54,7 @@ struct OuterArgs {
 struct OuterPair {
     OuterArgs a, b;
     int r, n, t, chunk;
-    const int* start;          // [n + 1]
+    const int* start;          // [n + 1] and more
     const int* order;
 };
 
@@ -378,7 +378,7 @@ struct Space {
 };
 
 struct ForwardLayout {
-    size_t expanded = 0, ranked = 0, lists = 0, partial = 0, decode = 0, total = 0;
+    size_t expanded = 0, ranked = 0, lists = 0, start = 0, order = 0, partial = 0, decode = 0, total = 0;
 };
 ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r) {
     ForwardLayout l;
@@ -390,6 +390,8 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
         const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in);
         if (n) l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         if (n) l.lists = s.take(row_lists_bytes(plan, t));
+        if (n) l.start = s.take((size_t)(n + 2) * sizeof(int));
+        if (n) l.order = s.take((size_t)t * sizeof(int));
         l.partial = s.take(plan.partial_bytes);
     }
     l.total = s.at;
@@ -411,7 +413,7 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
     }
     if (n) {
         l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
-        l.start = s.take((size_t)(n + 1) * sizeof(int));
+        l.start = s.take((size_t)(n + 2) * sizeof(int));
         l.order = s.take((size_t)t * sizeof(int));
         l.rest = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.ranked32 = s.take((size_t)t * r * sizeof(float));
@@ -500,6 +502,8 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         p.ldu = r;
         p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
         p.lds = ldr;
+        p.start = reinterpret_cast<int*>(ws + l.start);
+        p.order = reinterpret_cast<int*>(ws + l.order);
         if ((rc = launch_rank(bf16, false, p, st))) return rc;
     }
     const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, v.d_out, v.d_in);
@@ -566,10 +570,8 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         if (dx || da) p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
         if (da && x) p.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
         if (da && !x) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
-        if (da || db) {
-            p.start = reinterpret_cast<int*>(ws + l.start);
-            p.order = reinterpret_cast<int*>(ws + l.order);
-        }
+        p.start = reinterpret_cast<int*>(ws + l.start);
+        p.order = reinterpret_cast<int*>(ws + l.order);
         if ((rc = launch_rank(bf16, true, p, st))) return rc;
     }
     const HalfPlan plan = plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out);

@@ -24,10 +24,10 @@ struct RankArgs {
     uint16_t* rest16;       // what that rounding took off, rounded, [t][lds], or null
     int64_t lds;
     float* su32;            // scale p, [t][r], or null
-    int* start;             // [n + 1]: the adapters' token lists, wanted where not null; each one's first place in
-    int* order;             // [t]: ascending tokens, adapter by adapter
+    int* start;             // [n + 2], written: the adapters' token lists (and that of the tokens without), each one's first place in
+    int* order;             // [t], written: ascending tokens, adapter by adapter
     // the launch's own
-    int tiles, cut, rp, compute;
+    int groups, cut, rp;
 };
 int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st);
 
