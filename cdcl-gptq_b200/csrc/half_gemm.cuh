@@ -66,6 +66,7 @@ struct Params {
     int m, n, nkb;             // rows, columns, K blocks
     int tiles_m, tiles_n, ntiles;
     int splits, kb_per_split;  // the K blocks of a tile, over several items
+    int stage_bytes;           // that the copies of a K block bring, to all CTAs of the tile
     // rows' adapters (see RowLists): null where there are none
     const uint32_t* lists;
     int rank;                  // ROWS_EXTEND: depth of the extension
@@ -203,7 +204,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             bar = smem_u32(&full[s]);
             if constexpr (CG == 2) bar = first_cta(bar);
-            if (rank == 0) mbar_expect_tx(&full[s], CG * STAGE_BYTES);
+            if (rank == 0) mbar_expect_tx(&full[s], (uint32_t)P.stage_bytes);
             ctr++;
             return ring + s * STAGE_BYTES;
         };
