@@ -303,6 +303,33 @@ def test_gradient_against_differences(gpu, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t,n,kind", [(300, 300, "each its own"), (300, 200, "random"), (1290, 129, "random"), (1290, 700, "random"),
+                                      (640, 3, "none"), (640, 1, "all"), (256, 4, "in turn")])
+def test_adapters_among_a_tile_of_tokens(gpu, t, n, kind):
+    """Tiles whose tokens have an adapter each, all the same, or none; more adapters than a CTA's threads."""
+    import torch
+    from cdclq import adapters as A
+
+    packed, w = layer(72, 88, [4], 32, t + n)
+    p = A.PackedProjection(*packed)
+    a, b, scale = bank(n, 4, 88, 72, "f16", 1)
+    x, index = tokens(t, 88, n, "f16", 3)
+    if kind == "none":
+        index = torch.full_like(index, n)
+    elif kind == "all":
+        index = torch.zeros_like(index)
+    elif kind != "random":
+        index = (torch.arange(t, device="cuda") % n).int()
+    y, u = A.forward(x, p, a, b, scale, index, keep=True)
+    check_forward(y, u, x, w, a, b, scale, index, "f16")
+    dy, _ = tokens(t, 72, n, "f16", 4)
+    got = A.backward(dy, x, u, p, a, b, scale, index)
+    check_backward(got, dy, x.double(), u, w, a, b, scale, index, "f16", False)
+    again = A.backward(dy, x, u, p, a, b, scale, index)
+    assert all(bool((g == h).all()) for g, h in zip(got, again))
+
+
+@pytest.mark.gpu
 def test_a_quantized_layer(gpu):
     """From quantize_layer through the packed tensors: the projection of unit vectors is the dequantized weight."""
     import torch

@@ -58,6 +58,39 @@ def test_save_and_restore(gpu, t, d, name):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("t,d", [(70, 4099), (33, 1004), (2000, 301), (40, 520)])
+def test_rows_that_start_anywhere(gpu, t, d, name):
+    """Codes and values do not depend on where the rows start: padded and shifted inputs, codes that begin on any byte."""
+    import torch
+    from cdclq import checkpoint as C
+
+    g = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.randn(t, d, generator=g, device="cuda").to(dtype_of(torch, name))
+    pad = torch.zeros(t, -(-d // 128) * 128, dtype=torch.float64, device="cuda")
+    pad[:, :d] = x.double()
+    top = pad.reshape(t, -1, 128).abs().amax(2)
+    want = C.save(x)
+    s = want.scales.double()
+    assert float((s - top / 127).abs().max()) <= 2.0 ** -24 * float(top.max())
+    full = s.repeat_interleave(128, 1)[:, :d]
+    assert bool(((want.codes.double() * full - x.double()).abs() <= full * (0.5 + 2.0 ** -15)).all())
+    back = C.restore(want)
+    exact = (want.codes.float() * want.scales.repeat_interleave(128, 1)[:, :d]).to(x.dtype)
+    assert bool((back == exact).all())
+    wide = torch.zeros(t, d + 5, dtype=x.dtype, device="cuda")
+    for first in (0, 1, 5):
+        part = wide[:, first:first + d]
+        part.copy_(x)
+        c = C.save(part)
+        assert bool((c.codes == want.codes).all()) and bool((c.scales == want.scales).all())
+    held = torch.empty(t * d + 3, dtype=torch.int8, device="cuda")
+    moved = held[3:].view(t, d)
+    moved.copy_(want.codes)
+    assert bool((C.restore(C.Checkpoint(moved, want.scales, x.dtype)) == back).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16", "f32"])
 def test_ties_zeros_and_non_finite_blocks(gpu, name):
     import torch
     from cdclq import checkpoint as C
