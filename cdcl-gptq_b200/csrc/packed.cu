@@ -18,7 +18,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct Sections {
-    size_t unit, column, scatter, grid, codes, total;
+    size_t unit, column, place, grid, codes, total;
 };
 Sections sections(uint64_t d_out, uint64_t d_in, uint64_t groups, uint64_t units, uint64_t tile_words) {
     const uint64_t tiles = (d_out + 15) / 16;
@@ -26,7 +26,7 @@ Sections sections(uint64_t d_out, uint64_t d_in, uint64_t groups, uint64_t units
     size_t at = 0;
     s.unit = at, at += align_up(units * sizeof(PackedUnit));
     s.column = at, at += align_up(units * 64 * sizeof(int));
-    s.scatter = at, at += align_up(units * 64 * sizeof(uint32_t));
+    s.place = at, at += align_up((d_in + 3) / 4 * 4 * sizeof(uint32_t));
     s.grid = at, at += align_up(tiles * groups * 16 * sizeof(uint32_t));
     s.codes = at, at += align_up(tiles * tile_words * 32 * sizeof(uint32_t));
     s.total = at;
@@ -122,9 +122,9 @@ __global__ void __launch_bounds__(256) packed_layout_kernel(const uint8_t* __res
     }
 }
 
-// column: permuted place -> original column; scatter: see PackedView.  A perm that is not one raises *bad.
-__global__ void __launch_bounds__(256) packed_columns_kernel(const int* __restrict__ perm, int places, int d_in, int pitch, int* column,
-                                                             uint32_t* scatter, int* seen, int* bad) {
+// column: permuted place -> original column; place: its inverse.  A perm that is not one raises *bad.
+__global__ void __launch_bounds__(256) packed_columns_kernel(const int* __restrict__ perm, int places, int d_in, int* column,
+                                                             uint32_t* place, int* seen, int* bad) {
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < places; i += gridDim.x * blockDim.x) {
         const int j = column[i];
         int c = -1;
@@ -135,9 +135,8 @@ __global__ void __launch_bounds__(256) packed_columns_kernel(const int* __restri
                 c = -1;
             }
             column[i] = c;
+            if (c >= 0) place[c] = i;
         }
-        const int k = i & 15;
-        scatter[(i >> 6) * 64 + ((k & 7) >> 1) * 16 + ((i >> 4) & 3) * 4 + (k >> 3) * 2 + (k & 1)] = 2u * (c >= 0 ? c : pitch - 1);
     }
 }
 
@@ -238,43 +237,41 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t d, uint32_t scale_f16) 
 }
 
 constexpr int EXPAND_WARPS = 16;
+constexpr size_t EXPAND_SMEM = 220 * 1024;
 constexpr size_t EXPAND_LIST_BYTES = (512 + EXPAND_WARPS) * sizeof(int);  // of a tile's list of adapters
 
-// The unit's codes of one half of the tile's rows, scaled, to their columns of `row`.
-template <bool BF16, int BITS, bool ALL>
-__device__ __forceinline__ void expand_unit(const PackedUnit& u, uint32_t (&w)[BITS], const uint4* __restrict__ scatter,
-                                            const uint32_t* __restrict__ g, int half, bool live, char* row) {
-    uint4 to[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) to[i] = scatter[i];
+// The unit's codes of one half of the tile's rows, scaled, to their places; sz: the first k-step's grid word, `at`: the lane's
+// row of its first place of the unit.
+template <bool BF16, int BITS, int R>
+__device__ __forceinline__ void expand_unit(const uint16_t (&group)[4], uint32_t (&w)[BITS], const uint32_t* __restrict__ g,
+                                            uint32_t sz, int half, bool live, uint16_t* at) {
     // the upper rows' codes follow the lower rows' in every plane
-    int at = 0;
+    int word = 0;
 #pragma unroll
     for (int plane = 0; plane < 3; plane++) {
         const int pb = plane_bits(BITS, plane);
 #pragma unroll
-        for (int i = 0; i < pb; i++) w[at + i] >>= half * pb;
-        at += pb;
+        for (int i = 0; i < pb; i++) w[word + i] >>= half * pb;
+        word += pb;
     }
     auto step = [&](int ks, uint32_t sz, uint32_t zero) {
         const uint32_t lo = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, 0, zero), sz & 0xffffu);
         const uint32_t hi = scaled_pair<BF16>(decode_pair<BF16, BITS>(w, ks, 2, zero), sz & 0xffffu);
-        if (ALL || live) {
-            *reinterpret_cast<uint16_t*>(row + to[ks].x) = (uint16_t)lo;
-            *reinterpret_cast<uint16_t*>(row + to[ks].y) = (uint16_t)(lo >> 16);
-            *reinterpret_cast<uint16_t*>(row + to[ks].z) = (uint16_t)hi;
-            *reinterpret_cast<uint16_t*>(row + to[ks].w) = (uint16_t)(hi >> 16);
+        if (R == 8 || live) {
+            at[(ks * 16 + 0) * R] = (uint16_t)lo;
+            at[(ks * 16 + 1) * R] = (uint16_t)(lo >> 16);
+            at[(ks * 16 + 8) * R] = (uint16_t)hi;
+            at[(ks * 16 + 9) * R] = (uint16_t)(hi >> 16);
         }
     };
-    const uint32_t sz = g[(int64_t)u.group[0] * 16];
-    if (u.group[0] == u.group[3]) {
+    if (group[0] == group[3]) {
         const uint32_t zero = zero_pair<BF16, BITS>(sz);
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) step(ks, sz, zero);
     } else {
 #pragma unroll
         for (int ks = 0; ks < 4; ks++) {
-            const uint32_t s = g[(int64_t)u.group[ks] * 16];
+            const uint32_t s = ks ? g[(int64_t)group[ks] * 16] : sz;
             step(ks, s, zero_pair<BF16, BITS>(s));
         }
     }
@@ -313,54 +310,78 @@ __device__ void build_row_list(const RowLists& L, int tile, int* ids) {
     if (i < R && id >= 0 && lane == __ffs(same) - 1) mask[place[first] * (R / 32) + (i >> 5)] = ~same;
 }
 
-// A CTA expands `R` of a tile's 16 rows (R = 8, ALL, unless the rows do not fit): warps decode unit by unit into rows in
-// shared memory, at their original columns, and the CTA writes whole rows out.  BITS: the width of every group, or 0 where
-// they differ.  Bound by the 16-bit rows written and by issuing the scattered 2-byte stores, rows being four banks apart.
-template <bool BF16, int BITS, bool ALL>
-__global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, int R, int ld, uint16_t* __restrict__ out,
-                                                                          int64_t ldw, int wide, const RowLists lists) {
-    extern __shared__ __align__(16) uint16_t rows[];
+// R values of neighbouring rows at one place.
+template <int R>
+struct Rows;
+template <>
+struct Rows<8> { typedef uint4 T; };
+template <>
+struct Rows<4> { typedef uint2 T; };
+template <>
+struct Rows<2> { typedef uint32_t T; };
+template <>
+struct Rows<1> { typedef uint16_t T; };
+
+// A CTA expands R of a tile's 16 rows (8, unless they do not fit).  Warps decode unit by unit into shared memory, the R rows'
+// values of a place side by side: no two lanes meet in a bank, and addresses are constants.  Then every thread gathers four
+// neighbouring columns, a place of R values at once, and the warps write along the rows.  BITS: the width of every group, or 0
+// where they differ.
+template <bool BF16, int BITS, int R>
+__global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, uint16_t* __restrict__ out, int64_t ldw,
+                                                                          const RowLists lists) {
+    extern __shared__ __align__(16) uint16_t places[];
     if ((int)blockIdx.x < lists.tiles) {
-        build_row_list(lists, blockIdx.x, reinterpret_cast<int*>(rows));
+        build_row_list(lists, blockIdx.x, reinterpret_cast<int*>(places));
         if (blockIdx.x == 0) wait_for_previous();
         return;
     }
-    const int here = blockIdx.x - lists.tiles;
-    const int parts = 16 / R, tile = here / parts, first = (here % parts) * R;  // rows first .. first + R of the tile
+    constexpr int PARTS = 16 / R;
+    const int here = blockIdx.x - lists.tiles, tile = here / PARTS, first = here % PARTS * R;  // rows first .. first + R of the tile
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = first >> 3, r0 = lane / 4 - (first & 7);
     const bool live = r0 >= 0 && r0 < R;
-    char* row = reinterpret_cast<char*>(rows + (live ? r0 : 0) * ld);
-    const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32;
-    const uint32_t* grid = W.grid + (int64_t)tile * W.groups * 16;
-    const uint32_t* g = grid + half * 8 + lane / 4;
-    const uint4* scatter = reinterpret_cast<const uint4*>(W.scatter) + (lane & 3) * 4;
+    uint16_t* mine = places + (lane & 3) * 2 * R + (live ? r0 : 0);
+    const uint32_t* codes = W.codes + (int64_t)tile * W.tile_words * 32 + lane;
+    const uint32_t* g = W.grid + (int64_t)tile * W.groups * 16 + half * 8 + lane / 4;
     if constexpr (BITS) {
-        // the next unit's codes are on their way while this one is decoded
-        uint32_t ahead[BITS];
-        PackedUnit u = W.unit[min(warp, W.units - 1)];
+        // the next unit's codes and scale, and the groups of the one after it, are on their way while this one is decoded; units
+        // of one width follow one another
+        const int last = W.units - 1;
+        uint32_t ahead[BITS], sz_ahead;
+        uint2 group_ahead;
+        auto groups = [&](int ui) { return *reinterpret_cast<const uint2*>(W.unit[min(ui, last)].group); };
+        uint2 group_next = groups(warp);
 #pragma unroll
-        for (int i = 0; i < BITS; i++) ahead[i] = codes[(u.word + i) * 32 + lane];
-        for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
-            const PackedUnit here = u;
+        for (int i = 0; i < BITS; i++) ahead[i] = codes[(min(warp, last) * BITS + i) * 32];
+        group_ahead = groups(warp + EXPAND_WARPS);
+        sz_ahead = g[(int64_t)(group_next.x & 0xffffu) * 16];
+        for (int ui = warp; ui <= last; ui += EXPAND_WARPS) {
             uint32_t w[BITS];
+            alignas(8) uint16_t group[4];
+            *reinterpret_cast<uint2*>(group) = group_next;
+            const uint32_t sz = sz_ahead;
 #pragma unroll
             for (int i = 0; i < BITS; i++) w[i] = ahead[i];
-            u = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
+            const int next = min(ui + EXPAND_WARPS, last) * BITS;
 #pragma unroll
-            for (int i = 0; i < BITS; i++) ahead[i] = codes[(u.word + i) * 32 + lane];
-            expand_unit<BF16, BITS, ALL>(here, w, scatter + ui * 16, g, half, live, row);
+            for (int i = 0; i < BITS; i++) ahead[i] = codes[(next + i) * 32];
+            group_next = group_ahead;
+            sz_ahead = g[(int64_t)(group_next.x & 0xffffu) * 16];
+            group_ahead = groups(ui + 2 * EXPAND_WARPS);
+            expand_unit<BF16, BITS, R>(group, w, g, sz, half, live, mine + (int64_t)ui * 64 * R);
         }
     } else {
         auto unit = [&](auto width, const PackedUnit& u, int ui) {
             constexpr int B = decltype(width)::value;
             uint32_t w[B];
 #pragma unroll
-            for (int i = 0; i < B; i++) w[i] = codes[(u.word + i) * 32 + lane];
-            expand_unit<BF16, B, ALL>(u, w, scatter + ui * 16, g, half, live, row);
+            for (int i = 0; i < B; i++) w[i] = codes[(u.word + i) * 32];
+            expand_unit<BF16, B, R>(u.group, w, g, g[(int64_t)u.group[0] * 16], half, live, mine + (int64_t)ui * 64 * R);
         };
+        PackedUnit after = W.unit[min(warp, W.units - 1)];
         for (int ui = warp; ui < W.units; ui += EXPAND_WARPS) {
-            const PackedUnit u = W.unit[ui];
+            const PackedUnit u = after;
+            after = W.unit[min(ui + EXPAND_WARPS, W.units - 1)];
             switch (u.bits) {
                 case 2: unit(std::integral_constant<int, 2>(), u, ui); break;
                 case 3: unit(std::integral_constant<int, 3>(), u, ui); break;
@@ -374,42 +395,48 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
     }
     __syncthreads();
     const int rows_here = min(R, W.d_out - tile * 16 - first);
-    for (int r = 0; r < rows_here; r++) {
-        uint16_t* dst = out + ((int64_t)tile * 16 + first + r) * ldw;
-        const uint16_t* src = rows + r * ld;
-        if (wide) {  // ldw is d_in rounded up to 8; what lies past d_in is written along
-#pragma unroll 4
-            for (int c = threadIdx.x * 8; c < W.d_in; c += EXPAND_WARPS * 32 * 8)
-                *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-        } else {
-            for (int c = threadIdx.x; c < W.d_in; c += EXPAND_WARPS * 32) dst[c] = src[c];
-        }
+    uint16_t* dst = out + ((int64_t)tile * 16 + first) * ldw;
+    for (int c = threadIdx.x * 4; c < W.d_in; c += EXPAND_WARPS * 32 * 4) {
+        typedef typename Rows<R>::T T;
+        const uint4 p = *reinterpret_cast<const uint4*>(W.place + c);
+        alignas(16) T v[4] = {reinterpret_cast<const T*>(places)[p.x], reinterpret_cast<const T*>(places)[p.y],
+                              reinterpret_cast<const T*>(places)[p.z], reinterpret_cast<const T*>(places)[p.w]};
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(v);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (r < rows_here)
+                *reinterpret_cast<uint2*>(dst + r * ldw + c) =
+                    make_uint2((uint32_t)h[r] | (uint32_t)h[R + r] << 16, (uint32_t)h[2 * R + r] | (uint32_t)h[3 * R + r] << 16);
     }
     if (blockIdx.x == 0) wait_for_previous();
 }
 
-template <bool BF16, int BITS>
-int expand(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, const RowLists& lists,
-           bool beside, cudaStream_t st) {
-    static std::atomic<uint64_t> done_all{0}, done_some{0};
-    auto kern = R == 8 ? packed_expand_kernel<BF16, BITS, true> : packed_expand_kernel<BF16, BITS, false>;
-    if (int rc = allow_smem(kern, 220 * 1024, R == 8 ? done_all : done_some, "packed_expand_kernel shared memory")) return rc;
+template <bool BF16, int BITS, int R>
+int expand(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    auto kern = packed_expand_kernel<BF16, BITS, R>;
+    if (int rc = allow_smem(kern, EXPAND_SMEM, done, "packed_expand_kernel shared memory")) return rc;
     return launch_after(beside, kern, dim3(lists.tiles + w.tiles * (16 / R)), dim3(EXPAND_WARPS * 32),
-                        std::max((size_t)(R * ld * 2), EXPAND_LIST_BYTES), st, "packed_expand_kernel launch", w, R, (int)ld,
-                        static_cast<uint16_t*>(out), ldw, wide, lists);
+                        std::max((size_t)w.units * 64 * R * 2, EXPAND_LIST_BYTES), st, "packed_expand_kernel launch", w,
+                        static_cast<uint16_t*>(out), ldw, lists);
 }
 
-// The widths of configurations that quantize every group alike have a kernel of their own; the others share one that
-// branches by unit.
+// The widths of configurations that quantize every group alike have a kernel of their own; the others, and rows too long for
+// eight of them, share those that branch by unit.
 template <bool BF16>
-int expand_any(const PackedView& w, int R, int64_t ld, void* out, int64_t ldw, int wide, const RowLists& lists,
-           bool beside, cudaStream_t st) {
+int expand_any(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
+    const size_t row = (size_t)w.units * 64 * 2;
+    if (row > EXPAND_SMEM) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
+    if (row * 8 > EXPAND_SMEM) {
+        if (row * 4 <= EXPAND_SMEM) return expand<BF16, 0, 4>(w, out, ldw, lists, beside, st);
+        return row * 2 <= EXPAND_SMEM ? expand<BF16, 0, 2>(w, out, ldw, lists, beside, st) : expand<BF16, 0, 1>(w, out, ldw, lists, beside, st);
+    }
     switch (w.bits) {
-        case 2: return expand<BF16, 2>(w, R, ld, out, ldw, wide, lists, beside, st);
-        case 3: return expand<BF16, 3>(w, R, ld, out, ldw, wide, lists, beside, st);
-        case 4: return expand<BF16, 4>(w, R, ld, out, ldw, wide, lists, beside, st);
-        case 8: return expand<BF16, 8>(w, R, ld, out, ldw, wide, lists, beside, st);
-        default: return expand<BF16, 0>(w, R, ld, out, ldw, wide, lists, beside, st);
+        case 2: return expand<BF16, 2, 8>(w, out, ldw, lists, beside, st);
+        case 3: return expand<BF16, 3, 8>(w, out, ldw, lists, beside, st);
+        case 4: return expand<BF16, 4, 8>(w, out, ldw, lists, beside, st);
+        case 8: return expand<BF16, 8, 8>(w, out, ldw, lists, beside, st);
+        default: return expand<BF16, 0, 8>(w, out, ldw, lists, beside, st);
     }
 }
 
@@ -426,19 +453,14 @@ PackedView packed_view(const cdclq_packed_layer& w) {
     v.bits = (int)w.bits;
     v.unit = reinterpret_cast<const PackedUnit*>(base + s.unit);
     v.column = reinterpret_cast<const int*>(base + s.column);
-    v.scatter = reinterpret_cast<const uint32_t*>(base + s.scatter);
+    v.place = reinterpret_cast<const uint32_t*>(base + s.place);
     v.grid = reinterpret_cast<const uint32_t*>(base + s.grid);
     v.codes = reinterpret_cast<const uint32_t*>(base + s.codes);
     return v;
 }
 
 int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
-    const int64_t ld = expand_pitch(w.d_in);
-    int R = 8;
-    while (R > 1 && R * ld * 2 > 220 * 1024) R /= 2;
-    if (R * ld * 2 > 220 * 1024) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
-    const int wide = ldw % 8 == 0 && ldw >= ceil_div(w.d_in, 8) * 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    return bf16 ? expand_any<true>(w, R, ld, out, ldw, wide, lists, beside, st) : expand_any<false>(w, R, ld, out, ldw, wide, lists, beside, st);
+    return bf16 ? expand_any<true>(w, out, ldw, lists, beside, st) : expand_any<false>(w, out, ldw, lists, beside, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -838,6 +860,7 @@ static int build_layer(const uint8_t* qweight, const void* scales_f16, const uin
     cudaError_t e = cudaMemcpyAsync(tmp, group_bit.data(), ng * 8, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaMemcpyAsync(tmp + o1, unit_of.data(), unit_of.size() * 4, cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaMemcpyAsync(tmp + o2, gbits, ng, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaMemsetAsync(const_cast<uint32_t*>(v.place), 0, (d_in + 3) / 4 * 4 * sizeof(uint32_t), st);
     if (e == cudaSuccess) e = cudaMemsetAsync(tmp + o3, 0, o4 - o3 + 256, st);
     if (e == cudaSuccess) e = cudaMemcpyAsync(const_cast<PackedUnit*>(v.unit), unit.data(), unit.size() * sizeof(PackedUnit), cudaMemcpyHostToDevice, st);
     if (e == cudaSuccess) e = cudaMemcpyAsync(const_cast<int*>(v.column), column.data(), column.size() * 4, cudaMemcpyHostToDevice, st);
@@ -852,7 +875,7 @@ static int build_layer(const uint8_t* qweight, const void* scales_f16, const uin
                      static_cast<const uint16_t*>(scales_f16), qzeros, reinterpret_cast<const uint8_t*>(tmp + o2), v.d_out, v.groups,
                      v.tiles, const_cast<uint32_t*>(v.grid), verdict);
         CDCLQ_LAUNCH(packed_columns_kernel, (unsigned)std::min<int64_t>(most, ceil_div(v.units * 64, 256)), 256, 0, st, perm, v.units * 64,
-                     v.d_in, expand_pitch(v.d_in), const_cast<int*>(v.column), const_cast<uint32_t*>(v.scatter),
+                     v.d_in, const_cast<int*>(v.column), const_cast<uint32_t*>(v.place),
                      reinterpret_cast<int*>(tmp + o3), verdict);
         e = cudaGetLastError();
         if (e == cudaSuccess) e = cudaMemcpyAsync(&bad, verdict, sizeof(int), cudaMemcpyDeviceToHost, st);

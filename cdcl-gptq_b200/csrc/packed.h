@@ -30,8 +30,7 @@ struct PackedView {
     int bits;                  // the width of every group, 0 where they differ
     const PackedUnit* unit;    // [units]
     const int* column;         // [64 * units]: original column of a padded place, -1 for padding
-    const uint32_t* scatter;   // [units][4][16]: for lane l % 4, the bytes from a row's start to the column of each of its 16
-                               // codes of a row (k-step by k-step, columns 0, 1, 8, 9), padding past the row's end
+    const uint32_t* place;     // [d_in, rounded up to 4 with zeros]: padded place of an original column
     const uint32_t* grid;      // [tiles][groups][16]: f16 scale in the low half, zero point in the high half
     const uint32_t* codes;     // [tiles][32 * tile_words]
 };
@@ -39,10 +38,8 @@ struct PackedView {
 // Points into the layout buffer of `w`.
 PackedView packed_view(const cdclq_packed_layer& w);
 
-// Halves of a row in the expansion's shared memory: rows four banks apart (16 bytes past a multiple of 128), with room past d_in.
-inline int expand_pitch(int d_in) { return (d_in + 63) / 64 * 64 + 8; }
-
-// W (d_out x d_in, original column order, ldw elements from row to row) rounded once to f16 or bf16.  beside: the launch before
+// W (d_out x d_in, original column order, ldw elements from row to row: d_in rounded up to 8, rows on 16 bytes; what lies past
+// d_in holds anything) rounded once to f16 or bf16.  beside: the launch before
 // it in the stream neither writes what it reads nor reads what it writes, so that they may run side by side.
 // lists: built along the way, by CTAs of their own.
 int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st);
