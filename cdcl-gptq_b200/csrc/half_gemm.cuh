@@ -14,6 +14,10 @@
 // a finished accumulator into registers and work on it while the next MMAs run.  Tensor memory holds two accumulators of
 // up to 256 columns: two tiles' in turn, or the halves of a tile of 512, where the next tile's first MMAs go to the half
 // that is free first.
+// Bound by the tensor cores, and over milliseconds by the power limit.  Measured: 4096 x 4096 x 4096 in bf16 with 8 adapters
+// of rank 32, 103 us (1.34 PFLOP/s, 82 % of what a library product of bf16 gives in a burst); the three products of a training
+// step of 8191 x 32000 x 2048 in f16, 1.18-1.23 PFLOP/s (86-90 % of the library's lasting rate).  With 57 rows it reads its
+// other operand, 206 MB, at 5.0 TB/s (76 % of a copy): 393 tiles make 2.7 rounds over 148 SMs.
 #pragma once
 
 #include "common.cuh"
@@ -30,7 +34,7 @@ constexpr int A_BYTES = BM * KB * 2;
 constexpr int EPI_WARPS = 16;      // four per lane quadrant, each with a quarter of the accumulator's columns
 constexpr int THREADS = (EPI_WARPS + 2) * 32;
 constexpr int TURN_BYTES = 32 * 64;   // one epilogue warp's transposition buffer: 64 bytes of each of its 32 rows
-constexpr int RING_BYTES = 192 * 1024;
+constexpr int RING_BYTES = 192 * 1024;  // deep enough: eight stages of 57 rows of A, in place of six of 128, gave the same time
 constexpr int LEAD = 2;            // tiles of 512: stages whose MMAs go to the first half before the second half's
 constexpr int BAND = 16;           // row blocks per band of the tile order: a wave's operands stay in L2
 

@@ -4,6 +4,9 @@
 // ranks; each CTA a share of k.  The tokens' rows, gathered by the list, and the factor's pass through a ring in shared memory
 // once; the cluster's CTAs add up one another's sums, each for its share of the tokens, in order, and write the results.
 // Bound by reading the tokens (r products for each value read): mma.sync keeps up with memory at any rank of up to 64.
+// 4096 tokens of 4096 values, 8 adapters of rank 32: 18 us (1.8 TB/s) beside the weight's expansion, after 4 us of sorting;
+// 4100, 6 of rank 64: 34 us.  Tokens as they come, one pass over them for every two adapters of a tile, took 28 and 49 us, and
+// 76 us for 3005 tokens of 8256 values and 32 adapters of rank 64 (now 40); it saved the sorting, 2 us for 333 tokens.
 #include <algorithm>
 #include <atomic>
 
