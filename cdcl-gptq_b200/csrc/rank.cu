@@ -20,7 +20,7 @@ namespace cdclq {
 
 namespace {
 
-constexpr int THREADS = 128, LIST_THREADS = 512, KB = 64, STAGES = 4, MOST_RANK = 64;
+constexpr int THREADS = 128, LIST_THREADS = 512, KB = 64, STAGES = 4, MOST_RANK = 64, MOST_CUT = 8;
 constexpr int X_PITCH = KB + 8;  // halves: 16-byte pieces of eight rows fall into different banks
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -274,8 +274,11 @@ __global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const Ra
     for (int i = tid; i < rows * ranks; i += THREADS) {
         const int row = first + i / ranks, c = i % ranks;
         const uint32_t at = tc::smem_u32(part + row * PITCH + c);
-        float s = 0.0f;
-        for (int q = 0; q < P.cut; q++) s += tc::cluster_load(at, q);
+        float v8[MOST_CUT], s = 0.0f;  // all on their way at once
+#pragma unroll
+        for (int q = 0; q < MOST_CUT; q++) v8[q] = q < P.cut ? tc::cluster_load(at, q) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < MOST_CUT; q++) s += v8[q];
         const int64_t t = token[row], k = r0 + c;
         if (P.u16) P.u16[t * P.ldu + k] = half_bits<BF16>(s);
         if (P.su16 || P.su32) {
@@ -333,7 +336,7 @@ int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st) {
     if (e != cudaSuccess) return cuda_error(e, "token_list_kernel launch");
     if (!p.u16 && !p.su16 && !p.su32) return 0;
     // Each adapter (and those without) may leave one group that is not full.  16 tokens to a cluster where 64 leave SMs idle
-    // even with 8 CTAs each; K blocks over as many CTAs as make four to an SM, four blocks at least for each.
+    // even with 8 CTAs each; K blocks over as many CTAs as run at once, four blocks at least for each.
     const int64_t sms = sm_count(), nkb = ceil_div(p.k, KB);
     auto most = [&](int64_t tokens) { return p.t / tokens + std::min<int64_t>(p.n + 1, p.t); };
     auto likely = [&](int64_t tokens) { return ceil_div(p.t, tokens) + std::min<int64_t>(p.n, p.t / tokens); };
@@ -341,7 +344,8 @@ int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st) {
     const int tokens = few ? 16 : 64;
     p.groups = (int)most(tokens);
     p.cut = 1;
-    while (p.cut < 8 && likely(tokens) * p.cut * ceil_div(p.r, MOST_RANK) < 4 * sms && nkb / (p.cut * 2) >= 4) p.cut *= 2;
+    const int64_t at_once = (p.r > 32 ? 3 : 4) * sms;
+    while (p.cut < MOST_CUT && likely(tokens) * p.cut * 2 * ceil_div(p.r, MOST_RANK) <= at_once && nkb / (p.cut * 2) >= 4) p.cut *= 2;
     p.rp = (int)ceil_div(std::min(p.r, MOST_RANK), 16) * 16;
     if (bf16) return transposed ? launch_tokens<true, true>(p, few, st) : launch_tokens<true, false>(p, few, st);
     return transposed ? launch_tokens<false, true>(p, few, st) : launch_tokens<false, false>(p, few, st);
