@@ -31,8 +31,8 @@ size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 // a checkpoint's codes through registers) and transposed into fragments by ldmatrix; what lies past the chunk is zero.
 // v is f32: it enters as the sum of two 16-bit numbers, so that dA is rounded where it is written and nowhere before.
 // Bound by reading `wide`: the rank is small, so mma.sync keeps up with memory.  4100 tokens, x and dy of 4096 columns, rank 64
-// in f16: 41 us alone (67 MB, 1.6 TB/s: at rank 64 the fragments' loads from shared memory take their share), all but 25 of them
-// beside the last tiles of dx's product; a second kernel of 8 us adds the chunks.
+// in f16: 41 us alone (67 MB, 1.6 TB/s: at rank 64 the fragments' loads from shared memory take their share); it starts on the
+// SMs that dx's product leaves first.  A second kernel of 8 us adds the chunks.
 constexpr int OUTER_COLS = 128, OUTER_TOK = 32, OUTER_MOST = 1024, OUTER_RANK = 64, OUTER_STAGES = 4;
 
 struct OuterArgs {

@@ -45,3 +45,40 @@ def test_training_teaches_what_serving_gives(gpu):
     losses, (before, after) = tune.demo(steps=40)
     assert np.isfinite(losses).all() and losses[-1] < 0.5 * losses[0]
     assert after > before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 12, 90])
+def test_a_captured_step_gives_the_same(gpu, t):
+    """A decode step and a training step in a CUDA graph, replayed on new inputs: the same bits as calls."""
+    import torch
+
+    from cdclq import adapters as A
+    from cdclq import tune
+    from test_gpu_adapters import bank, layer, tokens
+
+    packed, _ = layer(96, 136, [4], 64, 3)
+    w = A.PackedProjection(*packed)
+    a, b, scale = bank(3, 8, 136, 96, "bf16", 1)
+    x, index = tokens(t, 136, 3, "bf16", 2)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    head = (torch.randn(300, 96, generator=g, device="cuda") / 10).bfloat16()
+    target = torch.randint(0, 300, (t,), generator=g, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        tune.step(w, head, x, target, a, b, scale, index)
+        A.forward(x, w, a, b, scale, index)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = A.forward(x, w, a, b, scale, index)
+        value, grads = tune.step(w, head, x, target, a, b, scale, index)
+    other, others = tokens(t, 136, 3, "bf16", 9)
+    x.copy_(other)
+    index.copy_(others)
+    graph.replay()
+    want = A.forward(x, w, a, b, scale, index)
+    v, wg = tune.step(w, head, x, target, a, b, scale, index)
+    assert bool((y == want).all()) and bool(value == v)
+    assert all(bool((grads[k] == wg[k]).all()) for k in ("dx", "da", "db"))
