@@ -90,7 +90,7 @@ struct Params {
     float* label_logit;        // [m]
     const float* lse;          // [m]
     const float* dloss;        // [m]
-    const float* gain;         // power of two on the gradient, or null
+    const float* gain;         // on the gradient
     int* fail;                 // host word, set when a wait ran out
 };
 
@@ -545,7 +545,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     label = t - P.col0;
                     lse = P.lse[row];
                     dl = P.dloss[row];
-                    if (P.gain) dl *= *P.gain;
+                    dl *= *P.gain;
                 }
             }
             const int rows = min(32, P.m - row0);

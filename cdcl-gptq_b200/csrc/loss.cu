@@ -6,7 +6,9 @@
 // Forward: the product's epilogue keeps each row's running maximum and sum of exponentials over the tile's columns and
 // picks the label's logit; a small kernel joins the tiles.  Backward: the logits are computed again, a piece of the
 // vocabulary at a time; the epilogue turns a piece into g, rounded once to the inputs' type as the operand of the two
-// gradient products (f16 under a power-of-two gain, which keeps its small probabilities), dh is summed over the pieces
+// gradient products under a gain that makes the largest |dloss| 2^13, taken off again where dh and dW are written: a label's
+// entry, of nearly that size in every row, is then not rounded where all tokens weigh alike (as 1 / t it was off by up to
+// 2^-9 in bf16, for all rows alike, and so were the gradients), and f16 keeps small probabilities.  dh is summed over the pieces
 // in f32.  Memory does not grow with the vocabulary beyond GRAD_BYTES for g.
 //
 // Bound by the tensor cores: 2 t d v operations forward, 4 or 6 backward; with few tokens by reading W.  Forward and
@@ -84,7 +86,7 @@ loss_join_kernel(const float2* __restrict__ stats, int parts, int t, int64_t voc
     }
 }
 
-// gain[0] = the power of two that brings the largest finite |dloss| of a labelled token to 2^13..2^14, gain[1] = 1 / it.
+// gain[0] = 2^13 / the largest finite |dloss| of a labelled token, gain[1] = 1 / it; powers of two where that leaves the range.
 __global__ void __launch_bounds__(1024) loss_gain_kernel(const float* __restrict__ dloss, const int64_t* __restrict__ target,
                                                          int t, int64_t vocab, float* gain) {
     __shared__ float part[32];
@@ -98,11 +100,10 @@ __global__ void __launch_bounds__(1024) loss_gain_kernel(const float* __restrict
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 32; w++) top = fmaxf(top, part[w]);
-        int e = 0;
-        if (top > 0.0f) frexpf(top, &e);  // top < 2^e
-        e = min(max(14 - e, -100), 100);
-        gain[0] = ldexpf(1.0f, e);
-        gain[1] = ldexpf(1.0f, -e);
+        const bool normal = top > 7.8886091e-31f && top < 1.2676506e30f;  // 2^-100, 2^100
+        const float g = top == 0.0f ? 1.0f : top < 1.0f ? 1.2676506e30f : 7.8886091e-31f;
+        gain[0] = normal ? 8192.0f / top : g;
+        gain[1] = normal ? top * (1.0f / 8192.0f) : 1.0f / g;
     }
 }
 
@@ -260,8 +261,8 @@ extern "C" int cdclq_linear_cross_entropy_backward_device(const void* h, size_t 
         return set_error(CDCLQ_ERR_ARG, "linear_cross_entropy_backward: the workspace is too small");
     char* ws = static_cast<char*>(workspace);
     const bool bf16 = dtype == CDCLQ_DTYPE_BF16;
-    float* gain = bf16 ? nullptr : reinterpret_cast<float*>(ws + l.gain);
-    if (gain) CDCLQ_LAUNCH(loss_gain_kernel, 1, 1024, 0, st, dloss, target, (int)t, (int64_t)v, gain);
+    float* gain = reinterpret_cast<float*>(ws + l.gain);
+    CDCLQ_LAUNCH(loss_gain_kernel, 1, 1024, 0, st, dloss, target, (int)t, (int64_t)v, gain);
     const int64_t d8 = ceil_div(d, 8);
     if (dw) {
         const int64_t blocks = ceil_div((int64_t)t * d8, 256);
@@ -305,7 +306,7 @@ extern "C" int cdclq_linear_cross_entropy_backward_device(const void* h, size_t 
             } else {
                 q.out = dh;
                 q.ldo = lddh;
-                q.alpha = gain ? gain + 1 : nullptr;
+                q.alpha = gain + 1;
             }
             q.partial = reinterpret_cast<float*>(ws + l.partial);
             if ((rc = launch_half_gemm(q, plan_half_gemm(HALF_NN, t, d, cols), st))) return rc;
@@ -319,7 +320,7 @@ extern "C" int cdclq_linear_cross_entropy_backward_device(const void* h, size_t 
             q.b = operand(ws + l.rows, t, d, d8 * 8);
             q.out = static_cast<char*>(dw) + v0 * lddw * 2;
             q.ldo = lddw;
-            q.alpha = gain ? gain + 1 : nullptr;
+            q.alpha = gain + 1;
             q.partial = reinterpret_cast<float*>(ws + l.partial);
             if ((rc = launch_half_gemm(q, plan_half_gemm(HALF_TN, cols, d, t), st))) return rc;
         }

@@ -150,6 +150,29 @@ def test_strides_and_rows_off_16_bytes(gpu):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("t", [13, 51, 205])
+def test_a_mean_is_as_exact_as_its_output(gpu, t, name):
+    """dloss = 1 / t, whose rounding would fall on every label's entry alike.  With labels of small probability these entries
+    make up half of each row of g and are exact; the others' roundings are random among thousands.  What is left is the
+    outputs' own rounding: u / sqrt(3) of the norm at most, and 10 % of it for the rest."""
+    import torch
+    from cdclq import loss as L
+
+    h, w, target, _ = head(t, 264, 6000, name, t)
+    dloss = torch.full((t,), 1.0 / t, device="cuda")
+    target = torch.where(target < 0, torch.zeros_like(target), target % 6000)
+    _, lse = L.linear_cross_entropy(h, w, target)
+    dh, dw = L.linear_cross_entropy_backward(h, w, target, lse, dloss)
+    g = torch.softmax(h.double() @ w.double().t(), 1)
+    g[torch.arange(t, device="cuda"), target] -= 1
+    g /= t
+    for got, want in ((dh, g @ w.double()), (dw, g.t() @ h.double())):
+        off = (got.double() - want).norm() / want.norm()
+        assert float(off) <= 1.1 * U[name] / 3 ** 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
 def test_tokens_without_a_label_reach_nothing(gpu, name):
     """NaN and infinities in h, lse and dloss of unlabelled tokens; labels beyond the vocabulary count as none."""
     import torch
