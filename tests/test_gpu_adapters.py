@@ -330,6 +330,24 @@ def test_adapters_among_a_tile_of_tokens(gpu, t, n, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("t,d_in,gbits,group", [(40, 14000, [4], 128), (40, 20000, [4], 128), (3, 20000, [3, 8], 96), (33, 40004, [3, 8], 100),
+                                                (35, 60001, [2], 0)])
+def test_long_rows(gpu, t, d_in, gbits, group, name):
+    """Rows of which eight, four, two or one fit a CTA's shared memory."""
+    from cdclq import adapters as A
+
+    packed, w = layer(21, d_in, gbits, group, d_in)
+    p = A.PackedProjection(*packed)
+    a, b, scale = bank(2, 8, d_in, 21, name, 1)
+    x, index = tokens(t, d_in, 2, name, 3)
+    y, u = A.forward(x, p, a, b, scale, index, keep=True)
+    check_forward(y, u, x, w, a, b, scale, index, name)
+    dy, _ = tokens(t, 21, 2, name, 4)
+    check_backward(A.backward(dy, x, u, p, a, b, scale, index), dy, x.double(), u, w, a, b, scale, index, name, False)
+
+
+@pytest.mark.gpu
 def test_a_quantized_layer(gpu):
     """From quantize_layer through the packed tensors: the projection of unit vectors is the dequantized weight."""
     import torch
