@@ -12,8 +12,8 @@
 // in f32.  Memory does not grow with the vocabulary beyond GRAD_BYTES for g.
 //
 // Bound by the tensor cores: 2 t d v operations forward, 4 or 6 backward; with few tokens by reading W.  Forward and
-// backward, 2048 tokens x 32000 words of 4096 in bf16, no dW: 1.05 ms (1.53 PFLOP/s in a burst, 1.29 under the power limit);
-// 8191 x 32000 of 2048 in f16, all gradients: 3.35 ms (1.28 PFLOP/s; 1.17 under the limit).
+// backward, 2048 tokens x 32000 words of 4096 in bf16, no dW: 1.04 ms (1.54 PFLOP/s in a burst, 1.28 under the power limit);
+// 8191 x 32000 of 2048 in f16, all gradients: 3.28 ms (1.31 PFLOP/s; 1.17 under the limit).
 // Forward of 57 tokens x 50257 words of 2048 in bf16: 50 us.  With words of 232 the exponentials and additions of the
 // epilogue take most of the time (4069 x 68034: 185 us, 1.5 T logits a second).
 #include <algorithm>
