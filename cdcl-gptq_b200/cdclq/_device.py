@@ -49,15 +49,15 @@ def _tensors(args):
 
 
 def operator(f):
-    """An operator on the tensors of one CUDA device: runs with the device of its first argument as the current one and on
-    `stream`, a CUDA stream's handle as the library's other calls take it (0: the legacy default stream), or on torch's
-    current stream if None.  Results belong to that stream, as torch's own would."""
+    """An operator on the tensors of one CUDA device: runs with the device of its first tensor, by position or by name, as the
+    current one and on `stream`, a CUDA stream's handle as the library's other calls take it (0: the legacy default stream),
+    or on torch's current stream if None.  Results belong to that stream, as torch's own would."""
 
     @functools.wraps(f)
     def g(*args, stream=None, **kw):
         x = args[0] if args else None
         if not isinstance(x, torch.Tensor):
-            x = next(_tensors(args), None)
+            x = next(_tensors((*args, *kw.values())), None)
         if x is None or not x.is_cuda or (stream is None and x.get_device() == _current_device()):
             return f(*args, **kw)
         with torch.cuda.device(x.device):
