@@ -137,8 +137,9 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         uint16_t* low = &st.low[row][part * 8];
         if (Q.narrow16 && (in <= 0 || in == 8)) {
             const bool live = tok >= 0 && in > 0;
-            copy16(high, live ? Q.narrow + at : Q.wide, live);
-            if constexpr (LOW) copy16(low, live ? Q.rest + at : Q.wide, live);
+            // an address that is not read is on 16 bytes all the same, as `wide` may not be
+            copy16(high, live ? Q.narrow + at : Q.narrow, live);
+            if constexpr (LOW) copy16(low, live ? Q.rest + at : Q.rest, live);
         } else {
             for (int i = 0; i < 8; i++) {
                 high[i] = (tok >= 0 && i < in) ? Q.narrow[at + i] : (uint16_t)0;
