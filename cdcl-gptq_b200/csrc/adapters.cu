@@ -29,7 +29,8 @@ size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 // 64 ranks, one adapter, a chunk of its tokens.  An adapter of one chunk writes its result; the chunks of others go to f32
 // slots that a second kernel adds in order.  Tokens are gathered by list into a ring in shared memory (asynchronous copies;
 // a checkpoint's codes through registers) and transposed into fragments by ldmatrix; what lies past the chunk is zero.
-// v is f32: it enters as the sum of two 16-bit numbers, so that dA is rounded where it is written and nowhere before.
+// v is f32: it enters as the sum of two 16-bit numbers, in bf16 off by 2^-17 of it at most, so that dA's rounding is the one of
+// its output.
 // Bound by reading `wide`: the rank is small, so mma.sync keeps up with memory.  4100 tokens, x and dy of 4096 columns, rank 64
 // in f16: 41 us alone (67 MB, 1.6 TB/s: at rank 64 the fragments' loads from shared memory take their share); it starts on the
 // SMs that dx's product leaves first.  A second kernel of 8 us adds the chunks.
@@ -96,10 +97,13 @@ struct OuterStage {
     uint16_t low[OUTER_TOK][OUTER_RANK + 8];
 };
 
-// LOW: the narrow factor is high + low.
+// LOW: the narrow factor is high + low.  A checkpoint's codes and its v meet as bf16 whatever the type: codes are exact in it,
+// and v times a block's scale keeps 16 bits however small or large it is.  (As f16 the pair ends at 2^-24: with v of 3e-6 da was
+// off by a quarter of its norm.)
 template <bool BF16, bool CODES, bool LOW>
 __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& Q, OuterStage* ring, const int* list, int count, int id,
                                            int chunks, int slot, int tile, int k0) {
+    constexpr bool AS_BF16 = BF16 || CODES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c0 = tile * OUTER_COLS, ranks = min(OUTER_RANK, P.r - k0);
     const int steps = (count + OUTER_TOK - 1) / OUTER_TOK;
@@ -174,14 +178,14 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         alignas(16) int8_t q[16];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            h[i] = half_bits<BF16>(nv[i]);
-            l[i] = rest_bits<BF16>(nv[i], h[i]);
+            h[i] = half_bits<AS_BF16>(nv[i]);
+            l[i] = rest_bits<AS_BF16>(nv[i], h[i]);
         }
         *reinterpret_cast<uint4*>(&st.high[row][part * 8]) = *reinterpret_cast<uint4*>(h);
         *reinterpret_cast<uint4*>(&st.low[row][part * 8]) = *reinterpret_cast<uint4*>(l);
         *reinterpret_cast<uint4*>(q) = qv;
 #pragma unroll
-        for (int i = 0; i < 16; i++) w[i] = half_bits<BF16>((float)q[i]);
+        for (int i = 0; i < 16; i++) w[i] = half_bits<AS_BF16>((float)q[i]);
         uint16_t* dst = &st.wide[row][part * 16];
         reinterpret_cast<uint4*>(dst)[0] = reinterpret_cast<uint4*>(w)[0];
         reinterpret_cast<uint4*>(dst)[1] = reinterpret_cast<uint4*>(w)[1];
@@ -228,8 +232,8 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
                 load_pieces<true>(q, &(low ? st.low : st.high)[kk + (lane & 15)][j * 8 + (lane >> 4) * 8]);
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
-                    mma16816<BF16>(acc[m][j], a[m], q[0], q[1]);
-                    mma16816<BF16>(acc[m][j + 1], a[m], q[2], q[3]);
+                    mma16816<AS_BF16>(acc[m][j], a[m], q[0], q[1]);
+                    mma16816<AS_BF16>(acc[m][j + 1], a[m], q[2], q[3]);
                 }
             }
         }

@@ -1,8 +1,12 @@
-"""Adapters' gradients from inputs that start anywhere."""
+"""Adapters whose factors or gradients are small or large for their type, and inputs that start anywhere.
+
+u = 2^-8 (bf16), 2^-11 (f16) is one rounding to nearest.  Of a gradient da whose elements are each rounded once, that is at most
+u / sqrt(3) of its norm (and 2^-25 an element below f16's normal range); 20 % more stand for what is rounded before it.
+"""
 import pytest
 
 import conftest  # noqa: F401  (import paths)
-from test_gpu_adapters import bank, layer, tokens
+from test_gpu_adapters import U, bank, layer, own, tokens
 
 
 def gradients(t, d_in, d_out, n, r, name, sizes, seed=3):
@@ -13,6 +17,50 @@ def gradients(t, d_in, d_out, n, r, name, sizes, seed=3):
     dy, _ = tokens(t, d_out, n, name, seed + 2)
     b = (b.double() * r ** 0.5 * sizes[1]).to(b.dtype)
     return packed, w, a, b, scale, (x.double() * sizes[2]).to(x.dtype), (dy.double() * sizes[0]).to(dy.dtype), index
+
+
+def check_da(got, dy, x, b, scale, index, name):
+    import torch
+
+    want = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
+    for i in range(b.shape[0]):
+        rows = own(index, i)
+        want[i] = (scale[i].double() * (dy[rows].double() @ b[i].double())).t() @ x[rows].double()
+    assert float(want.abs().max()) < 60000 and float(want.norm()) > 0
+    off = float((got.double() - want).norm())
+    assert off <= 1.2 * U[name] / 3 ** 0.5 * float(want.norm()) + 2.0 ** -25 * want.numel() ** 0.5, off / float(want.norm())
+
+
+SIZES = [(1, 1, 1), (1e-3, 1e-2, 1), (1e-3, 1e-3, 1), (1e-3, 1e-4, 1), (1e-2, 1e-4, 0.05), (1e-2, 1e-2, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", SIZES)
+@pytest.mark.parametrize("t,r", [(2048, 16), (333, 24)])
+def test_a_gradient_of_a_from_a_checkpoint(gpu, t, r, sizes, name):
+    """Freshly started adapters have a small b, a mean's dy is small: neither costs da bits."""
+    from cdclq import adapters as A
+    from cdclq import checkpoint as C
+
+    packed, w, a, b, scale, x, dy, index = gradients(t, 264, 1024, 2, r, name, sizes)
+    c = C.save(x)
+    da = A.backward(dy, c, None, A.PackedProjection(*packed), a, b, scale, index, need_dx=False, need_db=False)[1]
+    check_da(da, dy, c.codes.double() * c.scales.double().repeat_interleave(128, 1)[:, :264], b, scale, index, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_a_gradient_of_a_from_a_checkpoint_of_large_v(gpu, name):
+    """v past f16's range, x small: da is far inside it."""
+    from cdclq import adapters as A
+    from cdclq import checkpoint as C
+
+    packed, w, a, b, scale, x, dy, index = gradients(700, 136, 1024, 2, 8, name, (100, 60, 1e-3))
+    x[:, 1::2] = 0  # a zero code beside them
+    c = C.save(x)
+    da = A.backward(dy, c, None, A.PackedProjection(*packed), a, b, scale, index, need_dx=False, need_db=False)[1]
+    check_da(da, dy, c.codes.double() * c.scales.double().repeat_interleave(128, 1)[:, :136], b, scale, index, name)
 
 
 @pytest.mark.gpu
