@@ -29,8 +29,9 @@ size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 // 64 ranks, one adapter, a chunk of its tokens.  An adapter of one chunk writes its result; the chunks of others go to f32
 // slots that a second kernel adds in order.  Tokens are gathered by list into a ring in shared memory (asynchronous copies;
 // a checkpoint's codes through registers) and transposed into fragments by ldmatrix; what lies past the chunk is zero.
-// v is f32: it enters as the sum of two 16-bit numbers, in bf16 off by 2^-17 of it at most, so that dA's rounding is the one of
-// its output.
+// v is f32: it enters as the sum of two 16-bit numbers, so that dA's rounding is the one of its output: in bf16 off by 2^-17 of
+// it at most; in f16, whose pairs end at 2^-24 and 2^16, under a gain that makes the adapter's largest |v| about 2^13 and comes
+// off the sums (without it v of 3e-6 cost dA 5e-3 of its norm, v past 65504 everything): off by 2^-22, or 2^-38 of the largest.
 // Bound by reading `wide`: the rank is small, so mma.sync keeps up with memory.  4100 tokens, x and dy of 4096 columns, rank 64
 // in f16: 41 us alone (67 MB, 1.6 TB/s: at rank 64 the fragments' loads from shared memory take their share); it starts on the
 // SMs that dx's product leaves first.  A second kernel of 8 us adds the chunks.
@@ -46,6 +47,7 @@ struct OuterArgs {
     const uint16_t* narrow;    // [t][ldn] 16-bit, and
     const uint16_t* rest;      // what is added to it, or null; with codes both are null:
     const float* narrow32;     // [t][r]
+    const uint32_t* top;       // [n]: of the gain that narrow and rest have in f16 (rank_gain)
     int64_t ldn;
     int narrow16;              // its rows can be read 16 bytes at a time
     const float* factor;       // [n] or null
@@ -103,7 +105,7 @@ struct OuterStage {
 template <bool BF16, bool CODES, bool LOW>
 __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& Q, OuterStage* ring, const int* list, int count, int id,
                                            int chunks, int slot, int tile, int k0) {
-    constexpr bool AS_BF16 = BF16 || CODES;
+    constexpr bool AS_BF16 = BF16 || CODES, GAIN = LOW && !AS_BF16;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c0 = tile * OUTER_COLS, ranks = min(OUTER_RANK, P.r - k0);
     const int steps = (count + OUTER_TOK - 1) / OUTER_TOK;
@@ -262,7 +264,7 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
         __syncthreads();
     }
     const bool whole = chunks == 1;
-    const float f = (whole && Q.factor) ? Q.factor[id] : 1.0f;
+    const float f = GAIN ? 1.0f / rank_gain(Q.top[id]) : (whole && Q.factor) ? Q.factor[id] : 1.0f;
     const int64_t base = (int64_t)(whole ? id : slot) * P.r * Q.cols;
     // rows of the output's piece, `len` long, `stride` apart; two neighbours a thread where rows start even
     const int lines = Q.by_rank ? ncols : ranks, len = Q.by_rank ? ranks : ncols;
@@ -279,8 +281,8 @@ __device__ __forceinline__ void outer_tile(const OuterPair& P, const OuterArgs& 
             else
                 Q.out[at] = half_bits<BF16>(v[0] * f);
         } else {
-            Q.slots[at] = v[0];
-            if (even) Q.slots[at + 1] = v[1];
+            Q.slots[at] = v[0] * f;
+            if (even) Q.slots[at + 1] = v[1] * f;
         }
     }
 }
@@ -408,7 +410,7 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
 }
 
 struct BackwardLayout {
-    size_t expanded = 0, ranked = 0, lists = 0, rest = 0, ranked32 = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
+    size_t expanded = 0, ranked = 0, lists = 0, high = 0, rest = 0, ranked32 = 0, top = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
 };
 BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r, bool need_dx) {
     BackwardLayout l;
@@ -424,8 +426,10 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
         l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.start = s.take((size_t)(n + 2) * sizeof(int));
         l.order = s.take((size_t)t * sizeof(int));
+        l.high = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.rest = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.ranked32 = s.take((size_t)t * r * sizeof(float));
+        l.top = s.take((size_t)n * sizeof(uint32_t));
         // the chunk is longer where only one of the two is wanted
         const int chunk = outer_chunk(t, ceil_div(w.d_in, OUTER_COLS) + ceil_div(w.d_out, OUTER_COLS), r);
         const size_t slots = (size_t)outer_slots(t, std::min(chunk, outer_chunk(t, ceil_div(std::min(w.d_in, w.d_out), OUTER_COLS), r)));
@@ -517,7 +521,7 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
     }
     const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, v.d_out, v.d_in);
     const RowLists lists = n ? row_lists(plan, ad->index, t, n, ws + l.lists) : RowLists();
-    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, n > 0, st))) return rc;  // beside u's products
+    if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, RankSplit(), n > 0, st))) return rc;  // beside u's products
     HalfGemm g{};
     g.form = HALF_NT_EXTEND;
     g.bf16 = bf16;
@@ -565,6 +569,7 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
     const bool bf16 = dtype == CDCLQ_DTYPE_BF16;
     const int64_t ldw = ceil_div(v.d_in, 8) * 8, ldr = ceil_div(r, 8) * 8;
     float* partial = reinterpret_cast<float*>(ws + l.partial);
+    RankSplit split;  // dA's v in f16
     if (n) {
         RankArgs p{};
         p.x = static_cast<const uint16_t*>(dy);
@@ -577,16 +582,24 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         p.scale = ad->scale;
         p.lds = ldr;
         if (dx || da) p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
-        if (da && x) p.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
-        if (da && !x) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+        if (da && x && bf16) p.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
+        if (da && (!x || !bf16)) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+        if (da && x && !bf16) {
+            p.top = reinterpret_cast<uint32_t*>(ws + l.top);
+            split.v = p.su32, split.top = p.top, split.index = ad->index;
+            split.t = (int)t, split.n = (int)n, split.r = (int)r;
+            split.high = reinterpret_cast<uint16_t*>(ws + l.high), split.low = reinterpret_cast<uint16_t*>(ws + l.rest);
+            split.ld = ldr;
+        }
         p.start = reinterpret_cast<int*>(ws + l.start);
         p.order = reinterpret_cast<int*>(ws + l.order);
         if ((rc = launch_rank(bf16, true, p, st))) return rc;
+        if (!dx && split.v && (rc = launch_rank_split(split, st))) return rc;
     }
     const HalfPlan plan = plan_half_gemm(HALF_NN_EXTEND, t, v.d_in, v.d_out);
     if (dx) {
         const RowLists lists = n ? row_lists(plan, ad->index, t, n, ws + l.lists) : RowLists();
-        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, n > 0, st))) return rc;  // beside v's products
+        if ((rc = launch_packed_expand(v, bf16, ws + l.expanded, ldw, lists, split, n > 0, st))) return rc;  // beside v's products
         HalfGemm g{};
         g.form = HALF_NN_EXTEND;
         g.bf16 = bf16;
@@ -616,7 +629,8 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         o.a.wide16 = x ? ldx % 8 == 0 && v.d_in % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0
                        : v.d_in % 16 == 0 && (reinterpret_cast<uintptr_t>(x_codes) & 15) == 0;
         if (x) {
-            o.a.narrow = reinterpret_cast<const uint16_t*>(ws + l.ranked);
+            o.a.narrow = split.v ? split.high : reinterpret_cast<const uint16_t*>(ws + l.ranked);
+            o.a.top = split.top;
             o.a.rest = reinterpret_cast<const uint16_t*>(ws + l.rest);
             o.a.ldn = ldr;
             o.a.narrow16 = r % 8 == 0;

@@ -330,11 +330,16 @@ struct Rows<1> { typedef uint16_t T; };
 // which decoding waits for the codes and writing for the whole row: latency, not a unit that is full.
 template <bool BF16, int BITS, int R>
 __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const PackedView W, uint16_t* __restrict__ out, int64_t ldw,
-                                                                          const RowLists lists) {
+                                                                          const RowLists lists, const RankSplit split) {
     extern __shared__ __align__(16) uint16_t places[];
     if ((int)blockIdx.x < lists.tiles) {
         build_row_list(lists, blockIdx.x, reinterpret_cast<int*>(places));
         if (blockIdx.x == 0) wait_for_previous();
+        return;
+    }
+    if ((int)(gridDim.x - blockIdx.x) <= split.ctas) {
+        wait_for_previous();
+        rank_split(split, gridDim.x - 1 - blockIdx.x);
         return;
     }
     constexpr int PARTS = 16 / R;
@@ -414,31 +419,31 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) packed_expand_kernel(const 
 }
 
 template <bool BF16, int BITS, int R>
-int expand(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
+int expand(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, const RankSplit& split, bool beside, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     auto kern = packed_expand_kernel<BF16, BITS, R>;
     if (int rc = allow_smem(kern, EXPAND_SMEM, done, "packed_expand_kernel shared memory")) return rc;
-    return launch_after(beside, kern, dim3(lists.tiles + w.tiles * (16 / R)), dim3(EXPAND_WARPS * 32),
+    return launch_after(beside, kern, dim3(lists.tiles + w.tiles * (16 / R) + split.ctas), dim3(EXPAND_WARPS * 32),
                         std::max((size_t)w.units * 64 * R * 2, EXPAND_LIST_BYTES), st, "packed_expand_kernel launch", w,
-                        static_cast<uint16_t*>(out), ldw, lists);
+                        static_cast<uint16_t*>(out), ldw, lists, split);
 }
 
 // The widths of configurations that quantize every group alike have a kernel of their own; the others, and rows too long for
 // eight of them, share those that branch by unit.
 template <bool BF16>
-int expand_any(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
+int expand_any(const PackedView& w, void* out, int64_t ldw, const RowLists& lists, const RankSplit& split, bool beside, cudaStream_t st) {
     const size_t row = (size_t)w.units * 64 * 2;
     if (row > EXPAND_SMEM) return set_error(CDCLQ_ERR_ARG, "packed layer: a row of over 112000 columns cannot be expanded");
     if (row * 8 > EXPAND_SMEM) {
-        if (row * 4 <= EXPAND_SMEM) return expand<BF16, 0, 4>(w, out, ldw, lists, beside, st);
-        return row * 2 <= EXPAND_SMEM ? expand<BF16, 0, 2>(w, out, ldw, lists, beside, st) : expand<BF16, 0, 1>(w, out, ldw, lists, beside, st);
+        if (row * 4 <= EXPAND_SMEM) return expand<BF16, 0, 4>(w, out, ldw, lists, split, beside, st);
+        return row * 2 <= EXPAND_SMEM ? expand<BF16, 0, 2>(w, out, ldw, lists, split, beside, st) : expand<BF16, 0, 1>(w, out, ldw, lists, split, beside, st);
     }
     switch (w.bits) {
-        case 2: return expand<BF16, 2, 8>(w, out, ldw, lists, beside, st);
-        case 3: return expand<BF16, 3, 8>(w, out, ldw, lists, beside, st);
-        case 4: return expand<BF16, 4, 8>(w, out, ldw, lists, beside, st);
-        case 8: return expand<BF16, 8, 8>(w, out, ldw, lists, beside, st);
-        default: return expand<BF16, 0, 8>(w, out, ldw, lists, beside, st);
+        case 2: return expand<BF16, 2, 8>(w, out, ldw, lists, split, beside, st);
+        case 3: return expand<BF16, 3, 8>(w, out, ldw, lists, split, beside, st);
+        case 4: return expand<BF16, 4, 8>(w, out, ldw, lists, split, beside, st);
+        case 8: return expand<BF16, 8, 8>(w, out, ldw, lists, split, beside, st);
+        default: return expand<BF16, 0, 8>(w, out, ldw, lists, split, beside, st);
     }
 }
 
@@ -461,8 +466,10 @@ PackedView packed_view(const cdclq_packed_layer& w) {
     return v;
 }
 
-int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st) {
-    return bf16 ? expand_any<true>(w, out, ldw, lists, beside, st) : expand_any<false>(w, out, ldw, lists, beside, st);
+int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, RankSplit split, bool beside,
+                         cudaStream_t st) {
+    if (split.v) split.ctas = rank_split_ctas(split, EXPAND_WARPS * 32);
+    return bf16 ? expand_any<true>(w, out, ldw, lists, split, beside, st) : expand_any<false>(w, out, ldw, lists, split, beside, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

@@ -9,6 +9,7 @@
 #include "cdclq.h"
 #include "common.cuh"
 #include "half_gemm.h"
+#include "rank.h"
 
 namespace cdclq {
 
@@ -41,8 +42,9 @@ PackedView packed_view(const cdclq_packed_layer& w);
 // W (d_out x d_in, original column order, ldw elements from row to row: d_in rounded up to 8, rows on 16 bytes; what lies past
 // d_in holds anything) rounded once to f16 or bf16.  beside: the launch before
 // it in the stream neither writes what it reads nor reads what it writes, so that they may run side by side.
-// lists: built along the way, by CTAs of their own.
-int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, bool beside, cudaStream_t st);
+// lists: built along the way, by CTAs of their own; split: done by others, once the launch before it has ended.
+int launch_packed_expand(const PackedView& w, bool bf16, void* out, int64_t ldw, const RowLists& lists, RankSplit split, bool beside,
+                         cudaStream_t st);
 
 // Largest number of tokens of the single-token form.  It costs a pass over the codes for every 32 tokens, the expanded form one
 // expansion: 2048 x 2048 in 3 bits 12.3 us for 32 tokens and 28 us for 33, 4096 x 4096 in 4 bits 20.6 and 38 us, 11008 x 4096

@@ -36,7 +36,8 @@ size_t smem_bytes(int tokens, int rp, bool transposed) {
 }
 
 // A CTA for each adapter and one for the tokens without: its tokens, ascending, after those of lower adapters.
-__global__ void __launch_bounds__(LIST_THREADS) token_list_kernel(const int* __restrict__ index, int t, int n, int* start, int* order) {
+__global__ void __launch_bounds__(LIST_THREADS) token_list_kernel(const int* __restrict__ index, int t, int n, int* start, int* order,
+                                                                  uint32_t* top) {
     constexpr int WARPS = LIST_THREADS / 32;
     __shared__ int below[WARPS], mine[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(LIST_THREADS) token_list_kernel(const int* __r
     if (threadIdx.x == 0) {
         start[id] = at;
         if (id == n) start[n + 1] = t;
+        if (top && id < n) top[id] = 0;
     }
     for (int base = 0; base < t; base += 4 * LIST_THREADS) {
         // four neighbouring tokens a thread
@@ -271,6 +273,7 @@ __global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const Ra
     }
     if (P.cut > 1) tc::cluster_sync();
     const int share = (TOKENS + P.cut - 1) / P.cut, first = rank * share, rows = min(share, count - first);
+    uint32_t most = 0;
     for (int i = tid; i < rows * ranks; i += THREADS) {
         const int row = first + i / ranks, c = i % ranks;
         const uint32_t at = tc::smem_u32(part + row * PITCH + c);
@@ -283,11 +286,17 @@ __global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const Ra
         if (P.u16) P.u16[t * P.ldu + k] = half_bits<BF16>(s);
         if (P.su16 || P.su32) {
             const float v = bare ? 0.0f : P.scale[id] * s;
+            const uint32_t size = __float_as_uint(fabsf(v));
+            if (size < 0x7f800000u) most = max(most, size);
             const uint16_t h = half_bits<BF16>(v);
             if (P.su16) P.su16[t * P.lds + k] = h;
             if (P.rest16) P.rest16[t * P.lds + k] = rest_bits<BF16>(v, h);
             if (P.su32) P.su32[t * P.r + k] = v;
         }
+    }
+    if (P.top && !bare) {  // a maximum does not depend on the order
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && most) atomicMax(P.top + id, most);
     }
     if (P.cut > 1) {
         __syncwarp();
@@ -328,10 +337,23 @@ int launch_tokens(const RankArgs& p, bool few, cudaStream_t st) {
     return few ? launch_ranks<BF16, TRANSPOSED, 16>(p, st) : launch_ranks<BF16, TRANSPOSED, 64>(p, st);
 }
 
+__global__ void __launch_bounds__(256) rank_split_kernel(const RankSplit S) { rank_split(S, blockIdx.x); }
+
 }  // namespace
 
+int rank_split_ctas(const RankSplit& s, int threads) {
+    return (int)std::min<int64_t>(ceil_div((int64_t)s.t * (s.ld / 8), threads), 2 * sm_count());
+}
+
+int launch_rank_split(RankSplit s, cudaStream_t st) {
+    s.ctas = rank_split_ctas(s, 256);
+    CDCLQ_LAUNCH(rank_split_kernel, (unsigned)s.ctas, 256, 0, st, s);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : cuda_error(e, "rank_split_kernel launch");
+}
+
 int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st) {
-    CDCLQ_LAUNCH(token_list_kernel, (unsigned)(p.n + 1), LIST_THREADS, 0, st, p.index, p.t, p.n, p.start, p.order);
+    CDCLQ_LAUNCH(token_list_kernel, (unsigned)(p.n + 1), LIST_THREADS, 0, st, p.index, p.t, p.n, p.start, p.order, p.top);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_error(e, "token_list_kernel launch");
     if (!p.u16 && !p.su16 && !p.su32) return 0;

@@ -65,6 +65,36 @@ def test_a_gradient_of_a_from_a_checkpoint_of_large_v(gpu, name):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", SIZES + [(100, 60, 1e-3)])
+@pytest.mark.parametrize("t,d_in,r", [(2048, 264, 16), (333, 264, 24), (150, 131, 70)])
+def test_a_gradient_of_a_from_x_in_full(gpu, t, d_in, r, sizes, name):
+    from cdclq import adapters as A
+
+    packed, w, a, b, scale, x, dy, index = gradients(t, d_in, 1024, 2, r, name, sizes)
+    da = A.backward(dy, x, None, A.PackedProjection(*packed), a, b, scale, index, need_dx=False, need_db=False)[1]
+    check_da(da, dy, x, b, scale, index, name)
+
+
+@pytest.mark.gpu
+def test_gradients_of_unlike_tokens_and_adapters(gpu):
+    """One adapter's v is 2^20 times another's, a third has none but infinities: each has its own bits."""
+    import torch
+
+    from cdclq import adapters as A
+
+    packed, w, a, b, scale, x, dy, index = gradients(900, 136, 512, 4, 16, "f16", (1, 1, 1))
+    b[0] /= 1024
+    dy[index == 0] /= 1024
+    dy[index == 3] = float("inf")
+    p = A.PackedProjection(*packed)
+    da = A.backward(dy, x, None, p, a, b, scale, index, need_dx=False, need_db=False)[1]
+    for i in range(3):
+        check_da(da[i:i + 1], dy, x, b[i:i + 1], scale[i:i + 1], torch.where(index == i, 0, -1), "f16")
+    assert not bool(da[3].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["bf16", "f16"])
 @pytest.mark.parametrize("first", [1, 3, 8])
 @pytest.mark.parametrize("t,d_in,r", [(45, 64, 8), (300, 200, 16), (70, 133, 72)])
 def test_x_that_starts_anywhere(gpu, t, d_in, r, first, name):
