@@ -6,7 +6,8 @@
 // A few tokens (packed.cu): the codes are read once, W is never formed.  More tokens: W is expanded once to 16 bits, which
 // stays in L2 for the layers of a model, and multiplied on the tensor cores; the adapters ride in the same accumulators as
 // further K blocks, whose MMAs write only the tensor-memory lanes of the adapter's own tokens.  So a request never meets
-// another one's adapter, not even as a product with zero: a NaN in one adapter or one request stays there.
+// another one's adapter, not even as a product with zero: a NaN in one adapter or one request stays there.  In f16 what of s_i u_t
+// or v_t is past 65504 stays f32 and meets its factor in the product's epilogue, so that y and dx are as large as they are.
 // dA and dB gather the adapter's tokens by a list, for the same reason.
 #include <algorithm>
 #include <exception>
@@ -389,7 +390,7 @@ struct Space {
 };
 
 struct ForwardLayout {
-    size_t expanded = 0, ranked = 0, lists = 0, start = 0, order = 0, partial = 0, decode = 0, total = 0;
+    size_t expanded = 0, ranked = 0, ranked32 = 0, past = 0, lists = 0, start = 0, order = 0, partial = 0, decode = 0, total = 0;
 };
 ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r) {
     ForwardLayout l;
@@ -400,6 +401,8 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
         l.expanded = s.take((size_t)w.d_out * ceil_div(w.d_in, 8) * 8 * 2);
         const HalfPlan plan = plan_half_gemm(HALF_NT_EXTEND, t, w.d_out, w.d_in);
         if (n) l.ranked = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
+        if (n) l.ranked32 = s.take((size_t)t * r * sizeof(float));
+        if (n) l.past = s.take((size_t)t * sizeof(int));
         if (n) l.lists = s.take(row_lists_bytes(plan, t));
         if (n) l.start = s.take((size_t)(n + 2) * sizeof(int));
         if (n) l.order = s.take((size_t)t * sizeof(int));
@@ -410,7 +413,7 @@ ForwardLayout forward_layout(const PackedView& w, int64_t t, int64_t n, int64_t 
 }
 
 struct BackwardLayout {
-    size_t expanded = 0, ranked = 0, lists = 0, high = 0, rest = 0, ranked32 = 0, top = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
+    size_t expanded = 0, ranked = 0, lists = 0, high = 0, rest = 0, ranked32 = 0, past = 0, top = 0, partial = 0, start = 0, order = 0, slots_a = 0, slots_b = 0, total = 0;
 };
 BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_t r, bool need_dx) {
     BackwardLayout l;
@@ -429,6 +432,7 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
         l.high = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.rest = s.take((size_t)t * ceil_div(r, 8) * 8 * 2);
         l.ranked32 = s.take((size_t)t * r * sizeof(float));
+        l.past = s.take((size_t)t * sizeof(int));
         l.top = s.take((size_t)n * sizeof(uint32_t));
         // the chunk is longer where only one of the two is wanted
         const int chunk = outer_chunk(t, ceil_div(w.d_in, OUTER_COLS) + ceil_div(w.d_out, OUTER_COLS), r);
@@ -450,6 +454,16 @@ HalfOperand operand(const void* p, int64_t rows, int64_t cols, int64_t ld, int64
     o.batch = batch;
     o.step = batch > 1 ? rows * ld : 0;
     return o;
+}
+
+FarRows far_rows(const void* past, const int* index, const void* u32, const HalfOperand& x) {
+    FarRows f;
+    f.past = static_cast<const int*>(past);
+    f.index = index;
+    f.u = static_cast<const float*>(u32);
+    f.x = static_cast<const uint16_t*>(x.p);
+    f.ld = x.ld, f.step = x.step;
+    return f;
 }
 
 bool aligned(const void* p, size_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
@@ -515,6 +529,10 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         p.ldu = r;
         p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
         p.lds = ldr;
+        if (!bf16) {
+            p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+            p.past = reinterpret_cast<int*>(ws + l.past);
+        }
         p.start = reinterpret_cast<int*>(ws + l.start);
         p.order = reinterpret_cast<int*>(ws + l.order);
         if ((rc = launch_rank(bf16, false, p, st))) return rc;
@@ -532,6 +550,7 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
         g.u = operand(ws + l.ranked, t, r, ldr);
         g.x = operand(ad->b, v.d_out, r, ad->ldb, n);
         g.lists = lists.out;
+        if (!bf16) g.far = far_rows(ws + l.past, ad->index, ws + l.ranked32, g.x);
     }
     g.out = y;
     g.ldo = ldy;
@@ -583,7 +602,8 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
         p.lds = ldr;
         if (dx || da) p.su16 = reinterpret_cast<uint16_t*>(ws + l.ranked);
         if (da && x && bf16) p.rest16 = reinterpret_cast<uint16_t*>(ws + l.rest);
-        if (da && (!x || !bf16)) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+        if ((da && !x) || ((dx || da) && !bf16)) p.su32 = reinterpret_cast<float*>(ws + l.ranked32);
+        if (dx && !bf16) p.past = reinterpret_cast<int*>(ws + l.past);
         if (da && x && !bf16) {
             p.top = reinterpret_cast<uint32_t*>(ws + l.top);
             split.v = p.su32, split.top = p.top, split.index = ad->index;
@@ -610,6 +630,7 @@ extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, con
             g.u = operand(ws + l.ranked, t, r, ldr);
             g.x = operand(ad->a, r, v.d_in, ad->lda, n);
             g.lists = lists.out;
+            if (!bf16) g.far = far_rows(ws + l.past, ad->index, ws + l.ranked32, g.x);
         }
         g.out = dx;
         g.ldo = lddx;

@@ -195,6 +195,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     p.kb_per_split = (int)ceil_div(p.nkb, plan.splits);
     p.lists = extend ? g.lists : nullptr;
     p.rank = extend ? (int)g.u.cols : 0;
+    if (extend) p.far = g.far;
     p.target = g.target;
     p.col0 = g.col0;
     p.vocab = g.vocab;

@@ -21,6 +21,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "half_gemm.h"
 #include "tcgen05.cuh"
 
 namespace cdclq {
@@ -74,6 +75,7 @@ struct Params {
     // rows' adapters (see RowLists): null where there are none
     const uint32_t* lists;
     int rank;                  // ROWS_EXTEND: depth of the extension
+    FarRows far;
     // EPI_STORE
     void* out;                 // 16-bit, or null
     int64_t ldo;
@@ -145,6 +147,20 @@ __device__ __forceinline__ void item_coords(const Params& P, int item, int& mb, 
     mb = band * BAND + t - nb * rows;
 }
 
+
+// The part of a row's extension whose factors are past f16's range, in f32, to 16 of its columns.  Few rows ever have one: a function
+// of its own keeps it out of the epilogue's registers.
+template <bool BMN>
+__device__ __noinline__ void add_far(const FarRows far, int rank, int n, int row, int col, float* z) {
+    const float* u = far.u + (int64_t)row * rank;
+    const uint16_t* x = far.x + far.index[row] * far.step + col * (BMN ? (int64_t)1 : far.ld);
+    for (int k = 0; k < rank; k++) {
+        const float v = u[k];
+        if (!(fabsf(v) >= 65520.0f && fabsf(v) < INFINITY)) continue;  // what rounds to an infinity
+        for (int i = 0; i < 16 && col + i < n; i++)
+            z[i] = fmaf(v, __half2float(__ushort_as_half(x[BMN ? k * far.ld + i : i * far.ld + k])), z[i]);
+    }
+}
 
 template <bool BF16, bool AMN, bool BMN, int CG, int BN, int ROWS, int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -549,6 +565,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 }
             }
             const int rows = min(32, P.m - row0);
+            bool far = false;  // whether the row has factors that U lacks
+            if constexpr (!BF16 && ROWS == ROWS_EXTEND) far = live && P.far.past && split == P.splits - 1 && P.far.past[row];
             // waits for the accumulator of the tile's half `w` (or the whole tile)
             auto complete = [&]() -> bool {
                 if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) ok = false;
@@ -556,8 +574,8 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 return ok;
             };
             if constexpr (EPI == EPI_STORE) {
-                if (P.f32in || P.f32out) {
-                    // f32 sums, 16 columns at a time
+                if (P.f32in || P.f32out || __any_sync(0xffffffffu, far)) {
+                    // f32 sums (or what of them is to be added to), 16 columns at a time
 #pragma unroll 1
                     for (int w = 0; w < BN / AC; w++, acc++) {
                         if (!complete()) break;
@@ -567,6 +585,17 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             tmem_ld16(mine + (uint32_t)((acc & 1) * AC + q), z);
                             const int c0 = nb * BN + w * AC + part * COLS + q, cols = min(16, P.n - c0);
                             if (cols <= 0 || rows <= 0) continue;
+                            if constexpr (!BF16 && ROWS == ROWS_EXTEND) {
+                                if (far) {
+                                    float some[16];
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) some[i] = z[i];
+                                    add_far<BMN>(P.far, P.rank, P.n, row, c0, some);
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) z[i] = some[i];
+                                }
+                                __syncwarp();
+                            }
                             if (P.f32in) {
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {

@@ -30,6 +30,15 @@ struct HalfOperand {
     int64_t rows = 0, cols = 0, ld = 0, batch = 1, step = 0;
 };
 
+// What u lacks of the rows' factors in f16 (see RankArgs::past): past null: nothing.
+struct FarRows {
+    const int* past = nullptr;   // [m]
+    const int* index = nullptr;  // [m]
+    const float* u = nullptr;    // [m][rank]
+    const uint16_t* x = nullptr; // as the operand x
+    int64_t ld = 0, step = 0;
+};
+
 struct HalfGemm {
     HalfForm form;
     bool bf16;
@@ -37,6 +46,7 @@ struct HalfGemm {
     HalfOperand a, b;
     HalfOperand u, x;            // extension: u (m x rank) times x[adapter]
     const uint32_t* lists = nullptr;  // the adapters of each tile's rows (RowLists), or null: no extension
+    FarRows far;
     void* out = nullptr;         // 16-bit, ldo elements from row to row
     int64_t ldo = 0;
     float* f32out = nullptr;     // f32, ldf elements from row to row

@@ -37,7 +37,7 @@ size_t smem_bytes(int tokens, int rp, bool transposed) {
 
 // A CTA for each adapter and one for the tokens without: its tokens, ascending, after those of lower adapters.
 __global__ void __launch_bounds__(LIST_THREADS) token_list_kernel(const int* __restrict__ index, int t, int n, int* start, int* order,
-                                                                  uint32_t* top) {
+                                                                  int* past, uint32_t* top) {
     constexpr int WARPS = LIST_THREADS / 32;
     __shared__ int below[WARPS], mine[WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -84,7 +84,11 @@ __global__ void __launch_bounds__(LIST_THREADS) token_list_kernel(const int* __r
         }
 #pragma unroll
         for (int q = 0; q < 4; q++)
-            if (which >> q & 1) order[place++] = base + threadIdx.x * 4 + q;
+            if (which >> q & 1) {
+                const int i = base + threadIdx.x * 4 + q;
+                order[place++] = i;
+                if (past) past[i] = 0;
+            }
         at += all;
         __syncthreads();
     }
@@ -288,7 +292,8 @@ __global__ void __launch_bounds__(THREADS, NT == 8 ? 3 : 4) rank_kernel(const Ra
             const float v = bare ? 0.0f : P.scale[id] * s;
             const uint32_t size = __float_as_uint(fabsf(v));
             if (size < 0x7f800000u) most = max(most, size);
-            const uint16_t h = half_bits<BF16>(v);
+            uint16_t h = half_bits<BF16>(v);
+            if (!BF16 && P.past && (h & 0x7fffu) == 0x7c00u && size < 0x7f800000u) h = 0, P.past[t] = 1;
             if (P.su16) P.su16[t * P.lds + k] = h;
             if (P.rest16) P.rest16[t * P.lds + k] = rest_bits<BF16>(v, h);
             if (P.su32) P.su32[t * P.r + k] = v;
@@ -353,7 +358,7 @@ int launch_rank_split(RankSplit s, cudaStream_t st) {
 }
 
 int launch_rank(bool bf16, bool transposed, RankArgs p, cudaStream_t st) {
-    CDCLQ_LAUNCH(token_list_kernel, (unsigned)(p.n + 1), LIST_THREADS, 0, st, p.index, p.t, p.n, p.start, p.order, p.top);
+    CDCLQ_LAUNCH(token_list_kernel, (unsigned)(p.n + 1), LIST_THREADS, 0, st, p.index, p.t, p.n, p.start, p.order, p.past, p.top);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_error(e, "token_list_kernel launch");
     if (!p.u16 && !p.su16 && !p.su32) return 0;

@@ -23,6 +23,8 @@ struct RankArgs {
     uint16_t* u16;          // p, rounded, [t][ldu], or null
     int64_t ldu;
     uint16_t* su16;         // scale p, rounded, [t][lds], or null
+    int* past;              // [t], written, or null: whether some of the token's scale p are past f16, which are then 0 in su16 and
+                            // in su32 alone (an infinity or a NaN is in both)
     uint16_t* rest16;       // what that rounding took off, rounded, [t][lds], or null
     int64_t lds;
     float* su32;            // scale p, [t][r], or null

@@ -6,7 +6,7 @@ u / sqrt(3) of its norm (and 2^-25 an element below f16's normal range); 20 % mo
 import pytest
 
 import conftest  # noqa: F401  (import paths)
-from test_gpu_adapters import U, bank, layer, own, tokens
+from test_gpu_adapters import U, acc, bank, layer, own, tokens, within
 
 
 def gradients(t, d_in, d_out, n, r, name, sizes, seed=3):
@@ -91,6 +91,68 @@ def test_gradients_of_unlike_tokens_and_adapters(gpu):
     for i in range(3):
         check_da(da[i:i + 1], dy, x, b[i:i + 1], scale[i:i + 1], torch.where(index == i, 0, -1), "f16")
     assert not bool(da[3].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,d_in,d_out,n,r", [(40, 512, 64, 3, 16), (300, 328, 515, 4, 100), (333, 2048, 256, 3, 8), (2100, 264, 1100, 3, 16),
+                                              (129, 130, 77, 3, 5)])
+def test_u_past_the_range_of_float16(gpu, t, d_in, d_out, n, r):
+    """scale u is past 65504 for some tokens of some adapters, u and y are not.  Bounds as the forward pass has them elsewhere."""
+    import torch
+
+    from cdclq import adapters as A
+    from test_gpu_adapters import check_forward, want_forward
+
+    packed, w = layer(d_out, d_in, [4], 64, t)
+    p = A.PackedProjection(*packed)
+    a, b, scale = bank(n, r, d_in, d_out, "f16", t)
+    x, index = tokens(t, d_in, n, "f16", t + 1)
+    scale[1] = 64.0
+    b[1] = (b[1].double() / 4096).half()
+    loud = torch.arange(t, device="cuda") % 3 == 0
+    x[loud] = (x[loud].double() * 2000).half()
+    wy, wu = want_forward(x, w, a, b, scale, index)[:2]
+    assert float(wy.abs().max()) < 60000 and float(wu.abs().max()) < 60000
+    assert float(wu[index == 1].abs().max()) * 64 > 70000
+    y, u = A.forward(x, p, a, b, scale, index, keep=True)
+    check_forward(y, u, x, w, a, b, scale, index, "f16")
+    few = slice(0, 30)  # the same tokens, few at a time
+    y2 = A.forward(x[few], p, a, b, scale, index[few])
+    assert bool(y2.isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,d_in,d_out,n,r", [(40, 64, 512, 3, 16), (300, 515, 328, 4, 100), (333, 256, 2048, 3, 8), (2100, 1100, 264, 3, 16)])
+def test_v_past_the_range_of_float16(gpu, t, d_in, d_out, n, r):
+    """v under a loss scale is past 65504 for some tokens of one adapter, dx is not.  dx: the rounding of the weight and of v (u
+    each, v's where it is inside the range), f32 sums, the output's own."""
+    import torch
+
+    from cdclq import adapters as A
+
+    packed, w = layer(d_out, d_in, [4], 64, t)
+    p = A.PackedProjection(*packed)
+    a, b, scale = bank(n, r, d_in, d_out, "f16", t)
+    x, index = tokens(t, d_in, n, "f16", t + 1)
+    dy, _ = tokens(t, d_out, n, "f16", t + 2)
+    scale[1] = 40.0
+    a[1] = (a[1].double() / 1024).half()
+    b[1] = (b[1].double() * 4).half()
+    loud = torch.arange(t, device="cuda") % 3 == 0
+    dy[loud] = (dy[loud].double() * 500).half()
+    uu, e, tiny = U["f16"], acc(d_out, r), 2.0 ** -25
+    dd, ad = dy.double(), dy.double().abs()
+    dx, bound = dd @ w, (uu + 2 * e) * (ad @ w.abs()) + 4 * tiny * ad.sum(1, keepdim=True) + tiny
+    for i in range(n):
+        rows = own(index, i)
+        s, ai, bi = scale[i].double(), a[i].double(), b[i].double()
+        v = s * (dd[rows] @ bi)
+        assert (float(v.abs().max()) > 70000) == (i == 1)
+        dx[rows] += v @ ai
+        bound[rows] += (s * (ad[rows] @ bi.abs())) @ ai.abs() * (uu + 3 * e) + 4 * tiny * ai.abs().sum(0)
+    assert float(dx.abs().max()) < 60000
+    got = A.backward(dy, None, None, p, a, b, scale, index, need_da=False, need_db=False)[0]
+    within(got, dx, bound + uu * dx.abs(), "dx")
 
 
 @pytest.mark.gpu
