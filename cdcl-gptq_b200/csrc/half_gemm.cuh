@@ -510,7 +510,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         }
                     } else {
                         // the logits are complete, 16 columns at a time: exp2((v - top) log2 e), the sum so far brought to the new
-                        // maximum; a row of -inf alone keeps sum 0
+                        // maximum; a row of -inf alone keeps sum 0, one with +inf gets the sum inf (nothing is taken off an infinite maximum)
                         constexpr float L2E = 1.4426950408889634f;
 #pragma unroll
                         for (int q = 0; q < COLS; q += 16) {
@@ -533,7 +533,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                     if (q + i == at) own = v[i];
                                 P.label_logit[row] = own;
                             }
-                            const float ref = most == -INFINITY ? 0.0f : most;
+                            const float ref = fabsf(most) == INFINITY ? 0.0f : most;
                             scale_off(v, ref, L2E);
                             float some = 0.0f;
 #pragma unroll

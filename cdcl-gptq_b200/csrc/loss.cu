@@ -32,7 +32,7 @@ size_t align_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Joins the (maximum, sum) pairs of a row's column tiles: JOIN_ROWS rows to a CTA, a row's threads each with every (threads to
 // a row)-th pair; the maximum of all first, so that a pair costs one exponential.  A pair's maximum is -inf where its logits
-// all are; its sum is then 0, or NaN with a NaN among them.
+// all are; its sum is then 0, or NaN with a NaN among them.  Where it is +inf the sum is inf, or NaN, and lse with it.
 template <int JOIN_ROWS>
 __global__ void __launch_bounds__(JOIN_THREADS)
 loss_join_kernel(const float2* __restrict__ stats, int parts, int t, int64_t vocab, const int64_t* __restrict__ target,
@@ -66,7 +66,7 @@ loss_join_kernel(const float2* __restrict__ stats, int parts, int t, int64_t voc
         }
     }
     top = over_row(top, [](float a, float b) { return fmaxf(a, b); });
-    const float ref = top == -INFINITY ? 0.0f : top;
+    const float ref = fabsf(top) == INFINITY ? 0.0f : top;
     if (row < t) {
         for (int p = ty; p < parts; p += BATCH * STEP) {
             float2 v[BATCH];
