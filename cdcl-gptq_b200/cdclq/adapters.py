@@ -28,8 +28,8 @@ class PackedProjection:
     """A packed layer on the GPU, laid out for products with activations: `.d_out` x `.d_in`.
 
     qweight u8 [d_out, row_bytes], scales f16 and qzeros u8 [d_out, groups], perm i32 [d_in] and gbits u8 [groups] as the
-    packed format has them (src/io.rs:244-270), CUDA tensors; gsize: columns of a group.  They are copied into the layout
-    and not kept; building synchronises."""
+    packed format has them (src/io.rs:244-270), CUDA tensors; gsize: columns of a group, 0 for one group of all.  They are
+    copied into the layout and not kept; building synchronises."""
 
     def __init__(self, qweight, scales, qzeros, perm, gbits, gsize):
         tensor(qweight, "qweight", 2, torch.uint8)
@@ -41,7 +41,8 @@ class PackedProjection:
         tensor(perm, "perm", 1, torch.int32, None, dev)
         gb = gbits.cpu().to(torch.uint8).contiguous()
         d_out, d_in, ng, gsize = qweight.shape[0], perm.shape[0], gb.numel(), int(gsize)
-        if gsize <= 0 or gb.dim() != 1 or ng != -(-d_in // min(gsize, max(d_in, 1))):
+        gsize = gsize or max(d_in, 1)
+        if gsize < 0 or gb.dim() != 1 or ng != -(-d_in // min(gsize, max(d_in, 1))):
             refuse("gbits: need one width for each group of %d of %d columns, got %d" % (gsize, d_in, ng))
         tensor(scales, "scales", 2, torch.float16, (d_out, ng), dev)
         tensor(qzeros, "qzeros", 2, torch.uint8, (d_out, ng), dev)

@@ -817,9 +817,9 @@ using namespace cdclq;
 static int plan_layer(size_t d_out, size_t d_in, size_t group, const uint8_t* gbits, cdclq_packed_layer* w,
                       std::vector<PackedUnit>* unit, std::vector<int>* column) {
     if (!gbits || !w) return set_error(CDCLQ_ERR_ARG, "packed layer: null pointer");
-    if (!d_out || !d_in || !group) return set_error(CDCLQ_ERR_ARG, "packed layer: d_out, d_in and the group size must be > 0");
+    if (!d_out || !d_in) return set_error(CDCLQ_ERR_ARG, "packed layer: d_out and d_in must be > 0");
     if (d_out > 0x7ffffff0 || d_in > (1u << 24)) return set_error(CDCLQ_ERR_ARG, "packed layer: too large");
-    const size_t g = group < d_in ? group : d_in;
+    const size_t g = group && group < d_in ? group : d_in;
     if ((d_in + g - 1) / g > 65535) return set_error(CDCLQ_ERR_ARG, "packed layer: more than 65535 column groups");
     uint64_t units = 0, words = 0;
     int most = 0, least = 0;
