@@ -389,10 +389,12 @@ int cdclq_align_rows_device(const void* src, size_t rows, size_t cols, size_t ld
 
 /* x (t x d, any CDCLQ_DTYPE_*, ldx elements from row to row) as 8-bit codes (t x d) under one f32 scale for 128 columns
  * of a row (t x ceil(d / 128)): scale = max |x| / 127, code = x / scale to the nearest whole number.  A block with a
- * NaN or an infinity gets the scale NaN. */
+ * NaN or an infinity gets the scale NaN.  A scale below f32's normal range is a multiple of 2^-149, so that code * scale is
+ * within scale / 2 of x, or within 127 * 2^-150 where that is more. */
 int cdclq_checkpoint_save_device(const void* x, size_t ldx, int dtype, size_t t, size_t d, int8_t* codes, float* scales,
                                  void* stream);
-/* code * scale, rounded once to dtype. */
+/* code * scale, rounded once to dtype; in f32 the scale FLT_MAX / 127, rounded up, counts as the number below it, so that finite
+ * values come back finite. */
 int cdclq_checkpoint_restore_device(const int8_t* codes, const float* scales, size_t t, size_t d, void* out, size_t ldo,
                                     int dtype, void* stream);
 /* dw (n x d) = dy^T x^ from the codes of x (t x d) and dy (t x n, f16 or bf16, rows start on 16 bytes); the restored
