@@ -70,6 +70,7 @@ SIGNATURES = {
     "cdclq_dequantize_packed": (I32, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p,
                                       ctypes.POINTER(ctypes.c_uint64)]),
     "cdclq_operator_status": (I32, []),
+    "cdclq_operator_word": (P, [I32]),
     "cdclq_linear_cross_entropy_workspace": (SZ, [SZ, SZ, SZ]),
     "cdclq_linear_cross_entropy_device": (I32, [P, SZ, P, SZ, I32, SZ, SZ, SZ, P, P, P, P, SZ, P]),
     "cdclq_linear_cross_entropy_backward_workspace": (SZ, [SZ, SZ, SZ, I32, I32]),

@@ -5,9 +5,10 @@
     dw = weight_grad(dy, c)        dy: t x n, float16 or bfloat16; dw = dy^T x^, n x d, dy's type
 
 A block of 128 columns of a row shares the scale s = max |x| / 127 (float32); a value is kept as the nearest whole
-multiple of it (ties to even), so it comes back within s / 2, or within 1e-43 where that is more (blocks whose largest value is
-below 1e-41: under half of 127 times the smallest number they come back as zeros).  A block of finite values comes back
-finite, one of zeros as zeros; one that holds a NaN or an infinity comes back as NaN.  A checkpoint takes d + 4 ceil(d / 128) bytes a row: 52 % of a 16-bit matrix.
+multiple of it (ties to even), so it comes back within s / 2, or within 1e-43 where that is more (blocks whose largest
+value is below 3e-41; below 9e-44 they come back as zeros).  A block of finite values comes back finite, one of zeros as
+zeros; one that holds a NaN or an infinity comes back as NaN.  A checkpoint takes d + 4 ceil(d / 128) bytes a row: 52 % of
+a 16-bit matrix.
 The calls are asynchronous on `stream` (torch's current one if None).
 """
 import torch

@@ -328,6 +328,7 @@ extern "C" int cdclq_checkpoint_save_device(const void* x, size_t ldx, int dtype
     if (!t || !d) return 0;
     if (!x || !codes || !scales) return set_error(CDCLQ_ERR_ARG, "checkpoint_save: null pointer");
     if (ldx < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_save: rows overlap");
+    if (int rc = check_fail_word("checkpoint_save")) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == CDCLQ_DTYPE_F32) return save<CDCLQ_DTYPE_F32>(x, ldx, t, d, codes, scales, st);
     if (dtype == CDCLQ_DTYPE_F16) return save<CDCLQ_DTYPE_F16>(x, ldx, t, d, codes, scales, st);
@@ -340,6 +341,7 @@ extern "C" int cdclq_checkpoint_restore_device(const int8_t* codes, const float*
     if (!t || !d) return 0;
     if (!codes || !scales || !out) return set_error(CDCLQ_ERR_ARG, "checkpoint_restore: null pointer");
     if (ldo < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_restore: rows overlap");
+    if (int rc = check_fail_word("checkpoint_restore")) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (dtype == CDCLQ_DTYPE_F32) return restore<CDCLQ_DTYPE_F32>(codes, scales, t, d, out, ldo, st);
     return restore_half(dtype == CDCLQ_DTYPE_BF16, codes, scales, t, d, out, ldo, st);

@@ -22,32 +22,36 @@ int sm_count() {
     return sms;
 }
 
-// One word of mapped host memory: the host reads it without a synchronisation.
-static int* fail_word_host() {
-    static int* word = nullptr;
+// A word of mapped host memory for each device: the host reads it without a synchronisation.
+constexpr int FAIL_DEVICES = 64;
+static int* fail_word_host(int device) {
+    static int* words = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
         void* p = nullptr;
-        if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
-            word = static_cast<int*>(p);
-            *word = 0;
+        if (cudaHostAlloc(&p, FAIL_DEVICES * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
+            words = static_cast<int*>(p);
+            std::fill(words, words + FAIL_DEVICES, 0);
         } else {
             cudaGetLastError();
         }
     });
-    return word;
+    return words && device >= 0 && device < FAIL_DEVICES ? words + device : nullptr;
 }
 
-// Unified addressing: the word has the same address on every device.
-int* device_fail_word() { return fail_word_host(); }
+// Unified addressing: the words have the same addresses on every device.
+int* device_fail_word() {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+    return fail_word_host(dev);
+}
 
 int check_fail_word(const char* what) {
-    int* h = fail_word_host();
+    int* h = device_fail_word();
     if (!h) return set_error(CDCLQ_ERR_CUDA, std::string(what) + ": no mapped host memory (is there a CUDA device?)");
-    if (*(volatile int*)h) {
-        *(volatile int*)h = 0;
-        return set_error(CDCLQ_ERR_CUDA, std::string(what) + ": a pipeline wait of an earlier launch timed out (its outputs are incomplete)");
-    }
+    if (*(volatile int*)h && __atomic_exchange_n(h, 0, __ATOMIC_RELAXED))
+        return set_error(CDCLQ_ERR_CUDA, std::string(what) + ": a pipeline wait of an earlier launch on this device timed out (its outputs "
+                                                             "are incomplete); this call has not run");
     return 0;
 }
 
@@ -236,6 +240,8 @@ using namespace cdclq;
 
 extern "C" int cdclq_operator_status(void) { return check_fail_word("operator"); }
 
+extern "C" int* cdclq_operator_word(int device) { return fail_word_host(device); }
+
 namespace cdclq {
 __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t cols, int64_t lds,
                                                          uint16_t* __restrict__ dst, int64_t ldd) {
@@ -249,6 +255,7 @@ __global__ void __launch_bounds__(256) align_rows_kernel(const uint16_t* __restr
 extern "C" int cdclq_align_rows_device(const void* src, size_t rows, size_t cols, size_t lds, void* dst, size_t ldd, void* stream) {
     if (!rows || !cols) return 0;
     if (!src || !dst || lds < cols || ldd < cols) return set_error(CDCLQ_ERR_ARG, "align_rows: null pointer, or rows overlap");
+    if (int rc = check_fail_word("align_rows")) return rc;
     const int64_t blocks = ceil_div((int64_t)rows * (int64_t)ldd, 256);
     CDCLQ_LAUNCH(align_rows_kernel, (unsigned)std::min<int64_t>(blocks, sm_count() * 16), 256, 0, static_cast<cudaStream_t>(stream),
                  static_cast<const uint16_t*>(src), (int64_t)rows, (int64_t)cols, (int64_t)lds, static_cast<uint16_t*>(dst),

@@ -119,9 +119,9 @@ int allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done, const c
 
 // Number of SMs of the current device.
 int sm_count();
-// Device pointer of the host word that a kernel sets when one of its bounded waits ran out; null on failure.
+// The current device's host word that a kernel sets when one of its bounded waits ran out; null on failure.
 int* device_fail_word();
-// CDCLQ_OK, or the error left by an earlier launch whose wait ran out (reported once).
+// CDCLQ_OK, or the error left by an earlier launch on the current device whose wait ran out (reported once).
 int check_fail_word(const char* what);
 
 }  // namespace cdclq

@@ -358,11 +358,17 @@ int cdclq_unpack_dequant(const uint8_t* packed, size_t d_out, size_t n, size_t g
 /* No counterpart in the reference.  The operators below are asynchronous on `stream`, take device pointers and a
  * workspace of the size their `_workspace` function gives (it may be reused by the next call on the same stream),
  * and can be captured into a CUDA graph once each has run on the device.  A kernel whose bounded pipeline wait ran
- * out ends without finishing its outputs; the next of these calls, or cdclq_operator_status, reports it
- * (CDCLQ_ERR_CUDA). */
+ * out ends without finishing its outputs and sets its device's word.  The next of these calls that has work for that
+ * device (whichever thread or stream it comes from; cdclq_packed_layer_build is not one of them), or
+ * cdclq_operator_status, clears the word and returns CDCLQ_ERR_CUDA; that call has not run and may be repeated.  With
+ * several streams on a device, look at the word after synchronising each. */
 
-/* CDCLQ_OK, or the error that an earlier operator left (reported once).  Synchronise first for a verdict on it. */
+/* CDCLQ_OK, or the error that an earlier operator left on the current device (reported once).  Synchronise first for
+ * a verdict on it. */
 int cdclq_operator_status(void);
+/* The word of a device (0..63; the runtime's numbers): not 0 while an error waits to be reported.  In host memory, for a
+ * program that watches it without a call; NULL for other numbers or without CUDA. */
+int* cdclq_operator_word(int device);
 
 /* Softmax cross entropy of a linear head over v classes, without its logits z = h w^T:
  *   lse[i] = log sum_c exp z[i][c],   loss[i] = lse[i] - z[i][target[i]]
