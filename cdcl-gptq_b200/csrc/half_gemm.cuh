@@ -495,7 +495,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                 for (int i = 0; i < COLS; i++) z[i] = 0.0f;
                 for (int c = 0; c < chunks; c++, acc++) {
-                    if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) {
+                    if (!mbar_wait_warp(&accf[acc & 1], (acc / 2) & 1, flag)) {
                         ok = false;
                         break;
                     }
@@ -569,7 +569,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if constexpr (!BF16 && ROWS == ROWS_EXTEND) far = live && P.far.past && split == P.splits - 1 && P.far.past[row];
             // waits for the accumulator of the tile's half `w` (or the whole tile)
             auto complete = [&]() -> bool {
-                if (!mbar_wait(&accf[acc & 1], (acc / 2) & 1, flag)) ok = false;
+                if (!mbar_wait_warp(&accf[acc & 1], (acc / 2) & 1, flag)) ok = false;
                 fence_after();
                 return ok;
             };

@@ -669,9 +669,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) packed_decode_kernel(const Pac
 #pragma unroll
                 for (int k = 0; k < NT; k++)
                     x[q][ks][k] = u0 + q < W.units ? P.xf[((int64_t)((u0 + q) * 4 + ks) * NT + k) * 32 + lane] : make_uint2(0, 0);
-        if (!mbar_wait(&ready[f & 1], (f >> 1) & 1, &flag)) break;
+        const bool there = mbar_wait_warp(&ready[f & 1], (f >> 1) & 1, &flag);
         const uint32_t w0 = word_of(c * CHUNK);
-        for (int tl = parity; tl < n; tl += DEC_WARPS / DEC_GROUPS) {
+        for (int tl = there ? parity : n; tl < n; tl += DEC_WARPS / DEC_GROUPS) {
             const uint32_t* codes = smem + (f & 1) * slot_words + tl * tile_words;
             const uint32_t* g = grid + (t0 + tl) * W.groups * 16;
             float acc[NT][4];
@@ -704,7 +704,16 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) packed_decode_kernel(const Pac
 #pragma unroll
                 for (int i = 0; i < 4; i++) mine[(k * 8 + (i & 1)) * 17 + (i >> 1) * 8] = acc[k][i];
         }
-        __syncthreads();  // the slot is free, the sums are there
+        // the slot is free, the sums are there; where a wait ran out all leave together, the copies on their way first (bounded)
+        if (__syncthreads_or(!there)) {
+            if (threadIdx.x == 0) {
+                int own = 0;
+                mbar_wait(&ready[f & 1], (f >> 1) & 1, &own);
+                if (f + 1 < fills) mbar_wait(&ready[(f + 1) & 1], ((f + 1) >> 1) & 1, &own);
+            }
+            __syncthreads();
+            break;
+        }
         if (threadIdx.x == 0 && f + 2 < fills) fetch(f + 2, 0);
         if (c + 1 < chunks) continue;
         for (int i = threadIdx.x; i < n * 16 * P.t; i += DEC_THREADS) {

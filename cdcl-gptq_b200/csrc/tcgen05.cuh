@@ -58,6 +58,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, int* fla
     return false;
 }
 
+// The same by a whole warp, whose lanes go on together whatever each of them saw: the instructions after it want all of them.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, int* flag) {
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, flag));
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
