@@ -40,6 +40,14 @@ def tensor(x, what, dims, dtype=None, shape=None, device=None):
     return x
 
 
+def refuse_autograd(what, *inputs):
+    """Refuses inputs that autograd would follow: it cannot see through the library's kernels, and their gradients would be
+    lost without a word."""
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
+        refuse("%s: an input requires a gradient, which comes from %s, not from autograd: call it under torch.no_grad() or "
+               "with detached tensors" % (what, "linear_cross_entropy_backward()" if what == "linear_cross_entropy" else "backward()"))
+
+
 def _tensors(args):
     for a in args:
         if isinstance(a, torch.Tensor):

@@ -18,7 +18,7 @@ import functools
 
 import torch
 
-from ._device import HALF, current_stream, half_code, operator, refuse, rows16, tensor, workspace
+from ._device import HALF, current_stream, half_code, operator, refuse, refuse_autograd, rows16, tensor, workspace
 from ._lib import check, lib
 from .abi import CAdapters, CPackedLayer
 from .checkpoint import Checkpoint
@@ -148,8 +148,9 @@ def _projection(w, x, what, backward):
 
 @operator
 def forward(x, w, a=None, b=None, scale=None, index=None, keep=False, *, stream=None):
-    """y (t x d_out); with keep also u (t x r), which backward() takes."""
+    """y (t x d_out); with keep also u (t x r), which backward() takes.  Inputs that autograd would follow are refused."""
     code, t = _projection(w, x, "x", False)
+    refuse_autograd("forward", x, a, b, scale)
     L = lib()
     ad = _Adapters(w, x, a, b, scale, index, t)
     y = x.new_empty(t, w.d_out)

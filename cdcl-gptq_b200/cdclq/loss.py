@@ -15,7 +15,7 @@ if None).
 """
 import torch
 
-from ._device import current_stream, half_code, operator, refuse, rows16, tensor, workspace
+from ._device import current_stream, half_code, operator, refuse, refuse_autograd, rows16, tensor, workspace
 from ._lib import check, lib
 
 
@@ -34,8 +34,9 @@ def _head(h, w, target):
 
 @operator
 def linear_cross_entropy(h, w, target, *, stream=None):
-    """(loss, lse), float32, one for each row of h."""
+    """(loss, lse), float32, one for each row of h.  Inputs that autograd would follow are refused."""
     code, t, d, v = _head(h, w, target)
+    refuse_autograd("linear_cross_entropy", h, w)
     loss = torch.empty(t, dtype=torch.float32, device=h.device)
     lse = torch.empty_like(loss)
     if t == 0:

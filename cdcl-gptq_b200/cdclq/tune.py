@@ -18,6 +18,7 @@ import torch
 from . import adapters, checkpoint, loss
 
 
+@torch.no_grad()
 def step(w, head, x, target, a, b, scale, index, need_head=False, loss_scale=1.0):
     """The mean loss over the labelled tokens of head(w(x)), a 0-d tensor, and loss_scale times its gradients by name."""
     y, u = adapters.forward(x, w, a, b, scale, index, keep=True)
@@ -30,6 +31,7 @@ def step(w, head, x, target, a, b, scale, index, need_head=False, loss_scale=1.0
     return (each * share).sum(), {"da": da, "db": db, "dx": dx, "dhead": dhead}
 
 
+@torch.no_grad()
 def serve(w, head, x, a, b, scale, index):
     """The logits (t x v) of a few tokens, each with its own adapter."""
     return adapters.forward(x, w, a, b, scale, index) @ head.t()
