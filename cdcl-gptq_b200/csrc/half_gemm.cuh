@@ -46,10 +46,6 @@ constexpr int STATS_KB = 16;
 
 __host__ __device__ constexpr int b_bytes(int cg, int bn) { return bn / cg * KB * 2; }
 
-// The adapters of a tile's rows (R = 128 or 256), in words: their number, padding to 4, R places for their ids, R places for
-// R / 32 words each that have a bit for every row that is not the adapter's.
-__host__ __device__ constexpr int row_list_words(int R) { return 4 + R + R * (R / 32); }
-
 // How the adapter of each row (none if outside [0, adapters)) takes part.
 enum RowMode {
     ROWS_PLAIN = 0,   // not at all
@@ -274,7 +270,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const uint32_t* list = P.lists + (int64_t)mb * row_list_words(CG * BM);
                 const int count = (int)list[0];
                 for (int e = 0; e < count && ok; e++) {
-                    const int j = (int)list[4 + e];
+                    const int j = (int)list[ROW_LIST_IDS + e];
                     for (int kb = 0; kb < (P.rank + KB - 1) / KB; kb++) {
                         uint32_t bar;
                         const uint32_t st = stage(bar);
@@ -414,7 +410,7 @@ half_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (split == P.splits - 1 && P.lists) {
                     const uint32_t* list = P.lists + (int64_t)mb * row_list_words(CG * BM);
                     const int count = (int)list[0];
-                    const uint4* masks = reinterpret_cast<const uint4*>(list + 4 + CG * BM);
+                    const uint4* masks = reinterpret_cast<const uint4*>(list + row_list_masks(CG * BM));
                     for (int e = 0; e < count && ok; e++) {
                         uint32_t off[4 * CG];
 #pragma unroll

@@ -71,6 +71,12 @@ HalfPlan plan_half_gemm(HalfForm form, int64_t m, int64_t n, int64_t k);
 // (maximum, sum) pairs that the statistics form leaves for each row.
 int64_t half_stats_parts(const HalfPlan& plan, int64_t n);
 
+// The list of a tile's rows (R = 128 or 256), in words: the number of their adapters, padding to 4, R places for the adapters' ids,
+// R places for R / 32 words each that have a bit for every row that is not the adapter's.
+constexpr int ROW_LIST_IDS = 4;
+__host__ __device__ constexpr int row_list_masks(int R) { return ROW_LIST_IDS + R; }
+__host__ __device__ constexpr int row_list_words(int R) { return row_list_masks(R) + R * (R / 32); }
+
 // The adapters of the rows of each of the plan's tiles, for the extended forms; words of them for m rows.
 struct RowLists {
     const int* index = nullptr;  // [m], none if outside [0, adapters)

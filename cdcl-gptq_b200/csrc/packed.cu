@@ -283,7 +283,7 @@ __device__ void build_row_list(const RowLists& L, int tile, int* ids) {
     const int R = L.rows, i = threadIdx.x, row = tile * R + i, lane = i & 31;
     int* place = ids + 256;   // of an adapter's first row
     int* before = ids + 512;  // first rows of each warp
-    uint32_t* out = L.out + (int64_t)tile * (4 + R + R * (R / 32));
+    uint32_t* out = L.out + (int64_t)tile * row_list_words(R);
     int id = i < R && row < L.m ? L.index[row] : -1;
     if (id >= L.adapters) id = -1;
     if (i < R) ids[i] = id;
@@ -301,9 +301,9 @@ __device__ void build_row_list(const RowLists& L, int tile, int* ids) {
         if (w < (i >> 5)) at += before[w];
         count += before[w];
     }
-    if (leads) place[i] = at, out[4 + at] = id;
+    if (leads) place[i] = at, out[ROW_LIST_IDS + at] = id;
     if (i == 0) out[0] = count;
-    uint32_t* mask = out + 4 + R;
+    uint32_t* mask = out + row_list_masks(R);
     for (int k = i; k < count * (R / 32); k += blockDim.x) mask[k] = 0xffffffffu;
     __syncthreads();
     const uint32_t same = __match_any_sync(0xffffffffu, id);
