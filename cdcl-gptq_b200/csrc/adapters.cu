@@ -434,7 +434,7 @@ BackwardLayout backward_layout(const PackedView& w, int64_t t, int64_t n, int64_
         l.ranked32 = s.take((size_t)t * r * sizeof(float));
         l.past = s.take((size_t)t * sizeof(int));
         l.top = s.take((size_t)n * sizeof(uint32_t));
-        // the chunk is longer where only one of the two is wanted
+        // fewer column tiles, where only one of the two is wanted, may shorten the chunk and so make more slots
         const int chunk = outer_chunk(t, ceil_div(w.d_in, OUTER_COLS) + ceil_div(w.d_out, OUTER_COLS), r);
         const size_t slots = (size_t)outer_slots(t, std::min(chunk, outer_chunk(t, ceil_div(std::min(w.d_in, w.d_out), OUTER_COLS), r)));
         l.slots_a = s.take(slots * r * w.d_in * sizeof(float));

@@ -380,7 +380,8 @@ int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, const void* w, 
                                       size_t workspace_bytes, void* stream);
 /* Its gradient for dloss (f32, one for each token), from the forward's lse:
  *   g[i][c] = (exp(z[i][c] - lse[i]) - [c = target[i]]) dloss[i]   (0 without a label),  dh = g w,  dw = g^T h
- * dh (t x d) and dw (v x d) have the inputs' type; either may be NULL.  What a token without a label holds in h,
+ * dh (t x d) and dw (v x d) have the inputs' type; either may be NULL.  g is rounded to it as an operand, under a gain
+ * that brings the largest |dloss| to 2^13; sums are f32.  What a token without a label holds in h,
  * lse and dloss reaches neither. */
 size_t cdclq_linear_cross_entropy_backward_workspace(size_t t, size_t d, size_t v, int need_dh, int need_dw);
 int cdclq_linear_cross_entropy_backward_device(const void* h, size_t ldh, const void* w, size_t ldw, int dtype, size_t t,
@@ -442,14 +443,17 @@ typedef struct cdclq_adapters {
 } cdclq_adapters;
 
 /* y (t x d_out) = x W^T + scale_i (x A_i^T) B_i^T for the adapter i of each token; u (t x r, may be NULL) = x A_i^T, 0
- * without one, for the backward pass.  x: t x d_in, f16 or bf16, rows on 16 bytes.  ad may be NULL. */
+ * without one, for the backward pass.  x: t x d_in, f16 or bf16, rows on 16 bytes.  ad may be NULL.  Sums are f32.  Up to
+ * 32 tokens W is multiplied as its codes and scales; above, W and scale_i x A_i^T are first rounded to x's type (in f16
+ * what of the latter is past 65504 stays f32). */
 size_t cdclq_projection_forward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r);
 int cdclq_projection_forward_device(const cdclq_packed_layer* w, const void* x, size_t ldx, int dtype, size_t t,
                                     const cdclq_adapters* ad, void* y, size_t ldy, void* u, void* workspace,
                                     size_t workspace_bytes, void* stream);
 /* The gradient for dy (t x d_out): v = scale_i dy B_i, dx (t x d_in) = dy W + v A_i, da (n x r x d_in) = sum over the
  * adapter's tokens of v^T x, db (n x d_out x r) = scale_i sum dy^T u.  x is needed for da: in full, or (x NULL) as the
- * checkpoint x_codes, x_scales.  u is needed for db.  dx, da and db may be NULL. */
+ * checkpoint x_codes, x_scales.  u is needed for db.  dx, da and db may be NULL.  For dx W and v are first rounded to dy's
+ * type (in f16 what of v is past 65504 stays f32); for da v enters as two 16-bit parts. */
 size_t cdclq_projection_backward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r, int need_dx);
 int cdclq_projection_backward_device(const cdclq_packed_layer* w, const void* dy, size_t lddy, int dtype, size_t t,
                                      const cdclq_adapters* ad, const void* x, size_t ldx, const int8_t* x_codes,
