@@ -468,14 +468,21 @@ FarRows far_rows(const void* past, const int* index, const void* u32, const Half
 
 bool aligned(const void* p, size_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
+constexpr size_t MOST_ADAPTERS = 32767, MOST_RANK = 4096;
+
+// Whether a call of these sizes is refused: it has no workspace.
+bool refused(const cdclq_packed_layer* w, size_t t, size_t n, size_t r) {
+    return !w || !t || !w->d_out || !w->d_in || t > MOST_SIZE || n > MOST_ADAPTERS || (n && (!r || r > MOST_RANK));
+}
+
 int check_call(const char* what, const cdclq_packed_layer* w, int dtype, size_t t, const cdclq_adapters* ad) {
     const std::string s(what);
     if (!w || !w->layout || !w->d_out || !w->d_in) return set_error(CDCLQ_ERR_ARG, s + ": no packed layer");
     if (dtype != CDCLQ_DTYPE_F16 && dtype != CDCLQ_DTYPE_BF16) return set_error(CDCLQ_ERR_ARG, s + ": dtype must be f16 or bf16");
-    if (t > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, s + ": too many tokens");
+    if (t > MOST_SIZE) return set_error(CDCLQ_ERR_ARG, s + ": too many tokens");
     if (ad && ad->n) {
         if (!ad->r) return set_error(CDCLQ_ERR_ARG, s + ": the adapters' rank must be > 0");
-        if (ad->n > 32767 || ad->r > 4096) return set_error(CDCLQ_ERR_ARG, s + ": too many adapters, or too high a rank");
+        if (ad->n > MOST_ADAPTERS || ad->r > MOST_RANK) return set_error(CDCLQ_ERR_ARG, s + ": too many adapters, or too high a rank");
         if (!ad->a || !ad->b || !ad->scale || (t && !ad->index)) return set_error(CDCLQ_ERR_ARG, s + ": null pointer");
         if (ad->lda < w->d_in || ad->ldb < ad->r || !aligned(ad->a, ad->lda) || !aligned(ad->b, ad->ldb))
             return set_error(CDCLQ_ERR_ARG, s + ": rows of a and b must start on 16 bytes and not overlap");
@@ -490,8 +497,8 @@ int check_call(const char* what, const cdclq_packed_layer* w, int dtype, size_t 
 using namespace cdclq;
 
 extern "C" size_t cdclq_projection_forward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r) {
-    if (!w || !t) return 0;
-    return forward_layout(packed_view(*w), t, n, r).total;
+    if (refused(w, t, n, r)) return 0;
+    return forward_layout(packed_view(*w), t, n, n ? r : 0).total;
 }
 
 extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, const void* x, size_t ldx, int dtype, size_t t,
@@ -559,8 +566,8 @@ extern "C" int cdclq_projection_forward_device(const cdclq_packed_layer* w, cons
 }
 
 extern "C" size_t cdclq_projection_backward_workspace(const cdclq_packed_layer* w, size_t t, size_t n, size_t r, int need_dx) {
-    if (!w || !t) return 0;
-    return backward_layout(packed_view(*w), t, n, r, need_dx != 0).total;
+    if (refused(w, t, n, r)) return 0;
+    return backward_layout(packed_view(*w), t, n, n ? r : 0, need_dx != 0).total;
 }
 
 extern "C" int cdclq_projection_backward_device(const cdclq_packed_layer* w, const void* dy, size_t lddy, int dtype, size_t t,

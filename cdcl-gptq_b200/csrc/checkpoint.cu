@@ -348,7 +348,8 @@ extern "C" int cdclq_checkpoint_restore_device(const int8_t* codes, const float*
 }
 
 extern "C" size_t cdclq_checkpoint_weight_grad_workspace(size_t t, size_t d, size_t n) {
-    return t && d && n ? grad_layout(t, d, n).total : 0;
+    if (!t || !d || !n || t > MOST_SIZE || d > MOST_SIZE || n > MOST_SIZE) return 0;
+    return grad_layout(t, d, n).total;
 }
 
 extern "C" int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, int dtype, const int8_t* codes, const float* scales,
@@ -358,7 +359,7 @@ extern "C" int cdclq_checkpoint_weight_grad_device(const void* dy, size_t lddy, 
         return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: dtype must be f16 or bf16");
     if (!d || !n) return 0;
     if (!dw || lddw < d) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: null pointer, or rows overlap");
-    if (t > 0x7fffff00 || d > 0x7fffff00 || n > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: too large");
+    if (t > MOST_SIZE || d > MOST_SIZE || n > MOST_SIZE) return set_error(CDCLQ_ERR_ARG, "checkpoint_weight_grad: too large");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!t) {
         CDCLQ_CUDA_TRY(cudaMemset2DAsync(dw, lddw * 2, 0, d * 2, n, st));

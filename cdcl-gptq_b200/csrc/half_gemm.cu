@@ -176,7 +176,7 @@ int launch_half_gemm(const HalfGemm& g, const HalfPlan& plan, cudaStream_t st) {
     const bool a_mn = g.form == HALF_TN;
     const bool b_mn = g.form == HALF_NN || g.form == HALF_TN || g.form == HALF_NN_EXTEND;
     const bool extend = (g.form == HALF_NT_EXTEND || g.form == HALF_NN_EXTEND) && g.lists;
-    if (g.m > 0x7fffff00 || g.n > 0x7fffff00 || g.k > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, "half product: too large");
+    if (g.m > (int64_t)MOST_SIZE || g.n > (int64_t)MOST_SIZE || g.k > (int64_t)MOST_SIZE) return set_error(CDCLQ_ERR_ARG, "half product: too large");
     Maps maps{};
     int rc;
     // Where one CTA has all rows, copies bring no others; what the tile's other rows come to is never stored.  (2 tokens x 50292

@@ -39,6 +39,9 @@ struct FarRows {
     int64_t ld = 0, step = 0;
 };
 
+// The product's rows, columns and depth: a tile more is still an int.
+constexpr size_t MOST_SIZE = 0x7fffff00;
+
 struct HalfGemm {
     HalfForm form;
     bool bf16;

@@ -177,7 +177,7 @@ int check_head(const char* what, const void* h, size_t ldh, const void* w, size_
     const std::string s(what);
     if (dtype != CDCLQ_DTYPE_F16 && dtype != CDCLQ_DTYPE_BF16) return set_error(CDCLQ_ERR_ARG, s + ": dtype must be f16 or bf16");
     if (d == 0 || v == 0) return set_error(CDCLQ_ERR_ARG, s + ": the head has no rows or no columns");
-    if (t > 0x7fffff00 || d > 0x7fffff00 || v > 0x7fffff00) return set_error(CDCLQ_ERR_ARG, s + ": too large");
+    if (t > MOST_SIZE || d > MOST_SIZE || v > MOST_SIZE) return set_error(CDCLQ_ERR_ARG, s + ": too large");
     if (t && (!h || !w)) return set_error(CDCLQ_ERR_ARG, s + ": null pointer");
     if (ldh < d || ldw < d) return set_error(CDCLQ_ERR_ARG, s + ": rows overlap");
     if (t && ((ldh % 8) || (ldw % 8) || (reinterpret_cast<uintptr_t>(h) & 15) || (reinterpret_cast<uintptr_t>(w) & 15)))
@@ -201,7 +201,7 @@ HalfOperand operand(const void* p, int64_t rows, int64_t cols, int64_t ld) {
 using namespace cdclq;
 
 extern "C" size_t cdclq_linear_cross_entropy_workspace(size_t t, size_t d, size_t v) {
-    if (!t || !d || !v) return 0;
+    if (!t || !d || !v || t > MOST_SIZE || d > MOST_SIZE || v > MOST_SIZE) return 0;
     return align_up(sizeof(float2) * half_stats_parts(plan_half_gemm(HALF_STATS, t, v, d), v) * t) + align_up(sizeof(float) * t);
 }
 
@@ -237,7 +237,7 @@ extern "C" int cdclq_linear_cross_entropy_device(const void* h, size_t ldh, cons
 }
 
 extern "C" size_t cdclq_linear_cross_entropy_backward_workspace(size_t t, size_t d, size_t v, int need_dh, int need_dw) {
-    if (!t || !d || !v) return 0;
+    if (!t || !d || !v || t > MOST_SIZE || d > MOST_SIZE || v > MOST_SIZE) return 0;
     return backward_layout(t, d, v, need_dh != 0, need_dw != 0).total;
 }
 

@@ -356,8 +356,8 @@ int cdclq_unpack_dequant(const uint8_t* packed, size_t d_out, size_t n, size_t g
 /* ---- after the quantization: loss of a linear head ---------------------------------------------------- */
 
 /* No counterpart in the reference.  The operators below are asynchronous on `stream`, take device pointers and a
- * workspace of the size their `_workspace` function gives (it may be reused by the next call on the same stream),
- * and can be captured into a CUDA graph once each has run on the device.  A kernel whose bounded pipeline wait ran
+ * workspace of the size their `_workspace` function gives (0 for sizes that the call refuses; it may be reused by the
+ * next call on the same stream), and can be captured into a CUDA graph once each has run on the device.  A kernel whose bounded pipeline wait ran
  * out ends without finishing its outputs and sets its device's word.  The next of these calls that has work for that
  * device (whichever thread or stream it comes from; cdclq_packed_layer_build is not one of them), or
  * cdclq_operator_status, clears the word and returns CDCLQ_ERR_CUDA; that call has not run and may be repeated.  With
