@@ -45,6 +45,8 @@ class PackedProjection:
     def _build(self, qweight, scales, qzeros, perm, gbits, gsize):
         dev = qweight.get_device()
         tensor(perm, "perm", 1, torch.int32, None, dev)
+        if not isinstance(gbits, torch.Tensor):
+            refuse("gbits: need a tensor, got %s" % type(gbits).__name__)
         gb = gbits.cpu().to(torch.uint8).contiguous()
         d_out, d_in, ng, gsize = qweight.shape[0], perm.shape[0], gb.numel(), int(gsize)
         gsize = gsize or max(d_in, 1)
@@ -122,7 +124,8 @@ class _Adapters:
         if a is None and b is None and scale is None and index is None:
             return
         dev, dt = like.get_device(), like.dtype
-        if a is None or b is None or scale is None or index is None or a.dim() != 3:
+        T = torch.Tensor
+        if not (isinstance(a, T) and isinstance(b, T) and isinstance(scale, T) and isinstance(index, T)) or a.dim() != 3:
             _refuse_adapters(w, like, a, b, scale, index, t)
         n, r, d_in = a.shape
         if not (d_in == w.d_in and r and b.shape == (n, w.d_out, r) and scale.shape == (n,) and index.shape == (t,) and a.dtype is dt
@@ -144,6 +147,8 @@ def _projection(w, x, what, backward):
     if not isinstance(w, PackedProjection):
         refuse("w: need a PackedProjection")
     cols = w.d_out if backward else w.d_in
+    if not isinstance(x, torch.Tensor):
+        tensor(x, what, 2)
     code = HALF.get(x.dtype)
     if code is None or x.get_device() != w.device.index or x.dim() != 2 or x.shape[1] != cols:
         tensor(x, what, 2, device=w.device.index)

@@ -47,6 +47,11 @@ class Checkpoint:
         return self.codes.shape
 
 
+def _held(c):
+    if not isinstance(c, Checkpoint):
+        refuse("c: need a Checkpoint, got %s" % type(c).__name__)
+
+
 def _code(dt):
     code = HALF.get(dt)
     return _dtype_code(torch, dt) if code is None else code
@@ -54,7 +59,7 @@ def _code(dt):
 
 @operator
 def save(x, *, stream=None):
-    if x.dim() != 2 or not x.is_cuda:
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda:
         tensor(x, "x", 2)
     code = _code(x.dtype)
     t, d = x.shape
@@ -70,6 +75,7 @@ def save(x, *, stream=None):
 
 @operator
 def restore(c, *, stream=None):
+    _held(c)
     codes, scales = c.codes, c.scales
     t, d = codes.shape
     out = torch.empty(t, d, dtype=c.dtype, device=codes.device)
@@ -81,6 +87,7 @@ def restore(c, *, stream=None):
 @operator
 def weight_grad(dy, c, *, stream=None):
     """dy^T x^ with the restored values rounded to dy's type, as the operand of the tensor cores."""
+    _held(c)
     (t, d), codes = c.shape, c.codes
     tensor(dy, "dy", 2, device=codes.get_device())
     code = half_code(dy.dtype, "dy")

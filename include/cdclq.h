@@ -357,11 +357,11 @@ int cdclq_unpack_dequant(const uint8_t* packed, size_t d_out, size_t n, size_t g
 
 /* No counterpart in the reference.  The operators below are asynchronous on `stream`, take device pointers and a
  * workspace of the size their `_workspace` function gives (0 for sizes that the call refuses; it may be reused by the
- * next call on the same stream), and can be captured into a CUDA graph once each has run on the device.  A kernel whose bounded pipeline wait ran
- * out ends without finishing its outputs and sets its device's word.  The next of these calls that has work for that
- * device (whichever thread or stream it comes from; cdclq_packed_layer_build is not one of them), or
- * cdclq_operator_status, clears the word and returns CDCLQ_ERR_CUDA; that call has not run and may be repeated.  With
- * several streams on a device, look at the word after synchronising each. */
+ * next call on the same stream), and can be captured into a CUDA graph once each has run on the device.  A kernel
+ * whose bounded pipeline wait ran out ends without finishing its outputs and sets its device's word.  The next of these
+ * calls that has work for that device (whichever thread or stream it comes from; cdclq_packed_layer_build is not one
+ * of them), or cdclq_operator_status, clears the word and returns CDCLQ_ERR_CUDA; that call has not run and may be
+ * repeated.  With several streams on a device, look at the word after synchronising each. */
 
 /* CDCLQ_OK, or the error that an earlier operator left on the current device (reported once).  Synchronise first for
  * a verdict on it. */
