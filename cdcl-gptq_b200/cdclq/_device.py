@@ -45,9 +45,11 @@ def tensor(x, what, dims, dtype=None, shape=None, device=None):
 def refuse_autograd(what, *inputs):
     """Refuses inputs that autograd would follow: it cannot see through the library's kernels, and their gradients would be
     lost without a word."""
-    if torch.is_grad_enabled() and any(getattr(x, "requires_grad", False) for x in inputs):
-        refuse("%s: an input requires a gradient, which comes from %s, not from autograd: call it under torch.no_grad() or "
-               "with detached tensors" % (what, "linear_cross_entropy_backward()" if what == "linear_cross_entropy" else "backward()"))
+    if torch.is_grad_enabled():
+        for x in inputs:
+            if x is not None and x.requires_grad:
+                refuse("%s: an input requires a gradient, which comes from %s(), not from autograd: call it under torch.no_grad() "
+                       "or with detached tensors" % (what, "linear_cross_entropy_backward" if what == "linear_cross_entropy" else "backward"))
 
 
 def _tensors(args):
@@ -68,7 +70,7 @@ def operator(f):
         x = args[0] if args else None
         if not isinstance(x, torch.Tensor):
             x = next(_tensors((*args, *kw.values())), None)
-        if x is None or not getattr(x, "is_cuda", False) or (stream is None and x.get_device() == _current_device()):
+        if x is None or not x.is_cuda or (stream is None and x.get_device() == _current_device()):
             return f(*args, **kw)
         with torch.cuda.device(x.device):
             if stream is None or stream == current_stream(x):

@@ -124,13 +124,14 @@ class _Adapters:
         if a is None and b is None and scale is None and index is None:
             return
         dev, dt = like.get_device(), like.dtype
-        T = torch.Tensor
-        if not (isinstance(a, T) and isinstance(b, T) and isinstance(scale, T) and isinstance(index, T)) or a.dim() != 3:
-            _refuse_adapters(w, like, a, b, scale, index, t)
-        n, r, d_in = a.shape
-        if not (d_in == w.d_in and r and b.shape == (n, w.d_out, r) and scale.shape == (n,) and index.shape == (t,) and a.dtype is dt
-                and b.dtype is dt and scale.dtype is torch.float32 and index.dtype is torch.int32 and a.get_device() == dev
-                and b.get_device() == dev and scale.get_device() == dev and index.get_device() == dev):
+        try:
+            n, r, d_in = a.shape
+            fit = (d_in == w.d_in and r and b.shape == (n, w.d_out, r) and scale.shape == (n,) and index.shape == (t,) and a.dtype is dt
+                   and b.dtype is dt and scale.dtype is torch.float32 and index.dtype is torch.int32 and a.get_device() == dev
+                   and b.get_device() == dev and scale.get_device() == dev and index.get_device() == dev)
+        except (AttributeError, ValueError):  # no tensor, or one of other dimensions
+            fit = False
+        if not fit:
             _refuse_adapters(w, like, a, b, scale, index, t)
         self.n, self.r = n, r
         if n == 0:
@@ -161,9 +162,9 @@ def _projection(w, x, what, backward):
 def forward(x, w, a=None, b=None, scale=None, index=None, keep=False, *, stream=None):
     """y (t x d_out); with keep also u (t x r), which backward() takes.  Inputs that autograd would follow are refused."""
     code, t = _projection(w, x, "x", False)
-    refuse_autograd("forward", x, a, b, scale)
     L = lib()
     ad = _Adapters(w, x, a, b, scale, index, t)
+    refuse_autograd("forward", x, a, b, scale)
     y = x.new_empty(t, w.d_out)
     u = x.new_empty(t, ad.r) if keep else None
     if t:
